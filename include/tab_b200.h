@@ -282,6 +282,85 @@ int tab_residual_threshold_launch(float* y, const float* residual, float* ths, d
                                   float scale, int N, long long per_image, tab_stream_t stream);
 
 /*
+ * ---- 8-bit floats in blocks of 128 -----------------------------------------------------------------------------------------
+ * A dense layer's operands in 8 bits: values of 8-bit floats (TAB_E4M3, largest 448, or TAB_E5M2, largest 57344) and for each
+ * block of 128 of them one scale, a power of two held as the byte e + 127 (e8m0, the byte 255 is NaN).  No counterpart in the
+ * reference, whose operands are ternary or binary.
+ */
+enum { TAB_FP32 = 0, TAB_BF16 = 1, TAB_FP16 = 2 };     /* types of values */
+enum { TAB_E4M3 = 0, TAB_E5M2 = 1 };                   /* formats of 8-bit floats */
+
+/*
+ * x [M][K] of `type`, row pitch ldx elements -> blocks.  s = 2^e with the least e >= -127 for which max|x| <= F * 2^e over the finite
+ * values of the block, F the format's largest value (e = 0 where they are all zero); q = x / s rounded to nearest, ties to even.
+ * NaN stays NaN; an infinity becomes NaN in e4m3, which has none, and stays one in e5m2; neither touches the other values of its block.
+ *   square == 0   blocks of 128 consecutive values of a row: q [M][K], pitch ldq bytes, s [M][ceil(K/128)]; and, unless qt is NULL,
+ *                 from the same reading of x, blocks of 128 consecutive values of a column: qt [K][M], pitch ldqt, st [K][ceil(M/128)].
+ *   square == 1   blocks of 128 x 128: q [M][K], s [ceil(M/128)][ceil(K/128)] and / or their transposes qt [K][M],
+ *                 st [ceil(K/128)][ceil(M/128)] (either pair may be NULL).
+ * The last block of an axis may be short.  Bytes between rows are not written.
+ */
+int tab_quantize_blocks_launch(const void* x, int type, long long ldx, long long M, int K, int format, int square,
+                               void* q, long long ldq, uint8_t* s, void* qt, long long ldqt, uint8_t* st, tab_stream_t stream);
+
+/*
+ * y[m][n] = sum over k of a[m][k] sa(m, k/128) b[n][k] sb(n, k/128), accumulated in fp32 and rounded once to `type`.
+ * a [M][K], b [N][K] as tab_quantize_blocks_launch writes them: 16-byte aligned, pitches lda, ldb bytes, multiples of 16 (of which a
+ * single row needs none).  The scale of (row, block) is at as[(row / a_share) * a_row + block * a_block]; share is 1 (blocks of a
+ * row) or 128 (squares).  y [M][N], row pitch ldy elements.  tcgen05 kind::mxf8f6f4 applies the scales; waits inside the kernel are
+ * bounded as described at tab_device_status (codes 31-39).  K == 0 gives zeros.
+ */
+int tab_matmul_blocks_launch(const void* a, int a_format, long long lda, const uint8_t* as, int a_share, long long a_row, long long a_block,
+                             const void* b, int b_format, long long ldb, const uint8_t* bs, int b_share, long long b_row, long long b_block,
+                             void* y, int type, long long ldy, int M, int N, int K, tab_stream_t stream);
+/* Name, tile and split of the kernel the calling thread's most recent tab_matmul_blocks_launch launched ("none" before the first). */
+const char* tab_last_matmul_kernel(void);
+
+/*
+ * ---- the residual stream between two blocks ------------------------------------------------------------------------------------
+ *   u = norm(y) * w1 + b1      the norm behind a block; u = y without w1
+ *   r = alpha * x + gate * u   the residual stream, kept in the type of y; without x the first term, without a gate its factor is left out
+ *   h = norm(r) * w2 + b2      the norm before the next block, of r as it is kept; as values of that type or, with q, as blocks of 128
+ * norm(v) = v / sqrt(mean(v^2) + eps) (TAB_NORM_RMS) or (v - mean(v)) / sqrt(var(v) + eps) (TAB_NORM_LAYER), over the C elements of a row.
+ * NULL where absent: x, w1, b1, gate, w2, b2, r, h, q (with s), stats; shifts b1, b2 belong to TAB_NORM_LAYER.  Pitches are in elements (bytes for q).  C <= 16384.
+ * stats: float [M][4], kept for the backward pass.  Sums and statistics are fp32.
+ */
+enum { TAB_GATE_NONE = 0, TAB_GATE_TOKEN = 1, TAB_GATE_CHANNEL = 2, TAB_GATE_FULL = 3 };   /* gate: -, [M] (pitch ldg), [C], [M][C] */
+enum { TAB_NORM_RMS = 0, TAB_NORM_LAYER = 1 };
+typedef struct {
+    const void *y, *x, *w1, *b1, *w2, *b2, *gate;
+    long long ldy, ldx, ldg;
+    int type;                    /* of y, x, r, h */
+    int ptype, gtype;            /* of w1, b1, w2, b2; of the gate */
+    int gkind, layer;            /* TAB_GATE_*; TAB_NORM_* */
+    float alpha, eps;
+    int C;
+    long long M;
+    void *r, *h, *q;
+    uint8_t* s;                  /* [M][ceil(C/128)] */
+    long long ldr, ldh, ldq;
+    int format;                  /* of q */
+    float* stats;
+} tab_norm_t;
+int tab_residual_norm_launch(const tab_norm_t* args, tab_stream_t stream);
+
+/*
+ * Gradients of r and h (gr, gh; either may be NULL) to those of y, x, the gate, the weights and the shifts, each NULL where it is not
+ * wanted.  f: the forward arguments with its stats and, where it has w2, the r it kept; dgate has the gate's shape (rows without gaps) and type,
+ * dw1, db1, dw2, db2 the weights' type.  partial: tab_residual_norm_workspace_bytes(M, C) bytes, 32-byte aligned, needed where a
+ * sum over rows is wanted (weights, shifts, channel gate).  Two launches; the sums' order is fixed, so the same inputs give the same bits.
+ */
+typedef struct {
+    tab_norm_t f;
+    const void *gr, *gh;
+    void *dy, *dx, *dgate, *dw1, *db1, *dw2, *db2;
+    long long ldgr, ldgh, lddy, lddx;
+    float* partial;
+} tab_norm_backward_t;
+size_t tab_residual_norm_workspace_bytes(long long M, int C);
+int tab_residual_norm_backward_launch(const tab_norm_backward_t* args, tab_stream_t stream);
+
+/*
  * Register-only micro-benchmark of the pipes used by the convolution, for roofline
  * denominators: runs `iters` rounds on a grid that fills the device and writes elapsed-independent
  * checksums to `sink` (at least tab_pipe_probe_sink_bytes() bytes).  kind: 0 = 32-bit POPC,

@@ -6,7 +6,7 @@ inputs, implemented over the C ABI in ``include/tab_b200.h``.  torch is used for
 streams only; all arithmetic happens in the library's CUDA kernels.
 """
 from .ops import (Quantize, Conv2d, TAB_Quantize, TAB_Conv2d, Conv2dFused, conv2d_packed, conv_out_size,  # noqa: F401
-                  residual_threshold)
+                  residual_threshold, quantize_blocks, quantize_blocks2d, matmul_blocks, residual_norm)
 
 __all__ = ["Quantize", "Conv2d", "TAB_Quantize", "TAB_Conv2d", "Conv2dFused", "conv2d_packed", "conv_out_size",
-           "residual_threshold"]
+           "residual_threshold", "quantize_blocks", "quantize_blocks2d", "matmul_blocks", "residual_norm"]

@@ -3,6 +3,7 @@
 // excepted, which exists to synchronise).
 #include "tab_kernels.cuh"
 #include "umma_common.cuh"
+#include "blocks_common.cuh"
 
 namespace tab {
 
@@ -72,7 +73,7 @@ const char* tab_error_string(int code) {
 
 int tab_last_cuda_error(void) { return g_last_cuda_error; }
 
-int tab_version(void) { return 200; }
+int tab_version(void) { return 300; }
 
 int tab_device_status(void) { return umma_status_read_and_clear(); }
 
@@ -393,6 +394,117 @@ int tab_quantize_i16_launch(const int16_t* x, const float* ths, int64_t* qx, int
     if (misaligned(x, 1) || misaligned(ths, 3) || misaligned(qx, 7)) return TAB_E_ALIGNMENT;
     if ((long long)H * W >= (1LL << 31)) return TAB_E_TOO_LARGE;
     return quantize_dispatch(x, ths, qx, nullptr, bitwidth == 1 ? 1 : 2, N, H, W, C, reinterpret_cast<cudaStream_t>(stream), nullptr, true);
+}
+
+// ---- 8-bit blocks and the residual stream ---------------------------------------------------------------------------------------
+
+static bool type_ok(int type) { return type == TAB_FP32 || type == TAB_BF16 || type == TAB_FP16; }
+static bool format_ok(int format) { return format == TAB_E4M3 || format == TAB_E5M2; }
+
+int tab_quantize_blocks_launch(const void* x, int type, long long ldx, long long M, int K, int format, int square,
+                               void* q, long long ldq, uint8_t* s, void* qt, long long ldqt, uint8_t* st, tab_stream_t stream) {
+    if (!type_ok(type) || !format_ok(format) || (square != 0 && square != 1) || M < 0 || K < 0) return TAB_E_BAD_ARGUMENT;
+    if (M == 0 || K == 0) return TAB_OK;
+    if (!x || (!square && !q) || (!q && !qt) || (q && !s) || (qt && !st)) return TAB_E_NULL_POINTER;
+    if ((M > 1 && (ldx < K || (q && ldq < K))) || (qt && K > 1 && ldqt < M)) return TAB_E_BAD_ARGUMENT;
+    if (misaligned(x, (uintptr_t)type_bytes(type) - 1)) return TAB_E_ALIGNMENT;
+    // pitches of single rows are of no account; beyond 2^31 rows or 2^40 elements between two of them the index arithmetic ends
+    if (M >= (1LL << 31) || (M > 1 && (ldx >= (1LL << 40) || ldq >= (1LL << 40))) || (K > 1 && ldqt >= (1LL << 40))) return TAB_E_TOO_LARGE;
+    QuantBlocksParams p = {x, M > 1 ? ldx : 0, M, K, format, static_cast<uint8_t*>(q), M > 1 ? ldq : 0, q ? s : nullptr,
+                           static_cast<uint8_t*>(qt), K > 1 ? ldqt : 0, qt ? st : nullptr};
+    return quantize_blocks_dispatch(p, type, square == 1, reinterpret_cast<cudaStream_t>(stream));
+}
+
+int tab_matmul_blocks_launch(const void* a, int a_format, long long lda, const uint8_t* as, int a_share, long long a_row, long long a_block,
+                             const void* b, int b_format, long long ldb, const uint8_t* bs, int b_share, long long b_row, long long b_block,
+                             void* y, int type, long long ldy, int M, int N, int K, tab_stream_t stream) {
+    if (!type_ok(type) || !format_ok(a_format) || !format_ok(b_format) || M < 0 || N < 0 || K < 0) return TAB_E_BAD_ARGUMENT;
+    if ((a_share != 1 && a_share != 128) || (b_share != 1 && b_share != 128)) return TAB_E_BAD_ARGUMENT;
+    if (M == 0 || N == 0) return TAB_OK;
+    if (M == 1) { lda = ((long long)K + 15) / 16 * 16; ldy = N; }
+    if (N == 1) ldb = ((long long)K + 15) / 16 * 16;
+    if (lda < K || ldb < K || ldy < N) return TAB_E_BAD_ARGUMENT;
+    if (!y) return TAB_E_NULL_POINTER;
+    const size_t size = (size_t)type_bytes(type);
+    if (misaligned(y, size - 1)) return TAB_E_ALIGNMENT;
+    if (ldy >= (1LL << 40)) return TAB_E_TOO_LARGE;
+    cudaStream_t stm = reinterpret_cast<cudaStream_t>(stream);
+    if (K == 0) {
+        cudaError_t e = cudaMemset2DAsync(y, (size_t)ldy * size, 0, (size_t)N * size, (size_t)M, stm);
+        return e == cudaSuccess ? TAB_OK : record_cuda_error(e);
+    }
+    if (!a || !b || !as || !bs) return TAB_E_NULL_POINTER;
+    if (misaligned(a, 15) || misaligned(b, 15) || lda % 16 || ldb % 16) return TAB_E_ALIGNMENT;
+    if (lda >= (1LL << 40) || ldb >= (1LL << 40) || K > 0x7FFFFF00 || M > 0x7FFFFF00 || N > 0x7FFFFF00) return TAB_E_TOO_LARGE;
+    MatmulBlocksParams p = {{static_cast<const uint8_t*>(a), lda, as, a_row, a_block, a_share == 128 ? 7 : 0, M, a_format},
+                            {static_cast<const uint8_t*>(b), ldb, bs, b_row, b_block, b_share == 128 ? 7 : 0, N, b_format}, y, ldy, type, K};
+    return matmul_blocks_dispatch(p, stm);
+}
+
+const char* tab_last_matmul_kernel(void) { return matmul_blocks_last_kernel(); }
+
+// Checks of the forward arguments that both passes share.
+static int norm_args_ok(const tab_norm_t& p) {
+    if (!type_ok(p.type) || !type_ok(p.ptype) || !type_ok(p.gtype) || p.gkind < TAB_GATE_NONE || p.gkind > TAB_GATE_FULL || (p.layer != 0 && p.layer != 1) ||
+        p.M < 0 || p.C < 0 || (p.layer == TAB_NORM_RMS && (p.b1 || p.b2))) return TAB_E_BAD_ARGUMENT;
+    if (p.C > NORM_MAX || p.M >= (1LL << 31)) return TAB_E_TOO_LARGE;
+    return TAB_OK;
+}
+static bool odd_address(const void* p, int type) { return misaligned(p, (uintptr_t)type_bytes(type) - 1); }
+
+int tab_residual_norm_launch(const tab_norm_t* args, tab_stream_t stream) {
+    if (!args) return TAB_E_NULL_POINTER;
+    tab_norm_t p = *args;
+    const int rc = norm_args_ok(p);
+    if (rc != TAB_OK) return rc;
+    if (p.M == 0 || p.C == 0) return TAB_OK;
+    if (p.gkind == TAB_GATE_NONE) p.gate = nullptr;
+    if (!p.y || (p.gkind != TAB_GATE_NONE && !p.gate) || (p.q && !p.s) || ((p.h || p.q) && !p.w2)) return TAB_E_NULL_POINTER;
+    if (p.q && !format_ok(p.format)) return TAB_E_BAD_ARGUMENT;
+    if (p.M > 1 && (p.ldy < p.C || (p.x && p.ldx < p.C) || (p.r && p.ldr < p.C) || (p.h && p.ldh < p.C) || (p.q && p.ldq < p.C) ||
+                    (p.gkind == TAB_GATE_FULL && p.ldg < p.C) || (p.gkind == TAB_GATE_TOKEN && p.ldg < 0))) return TAB_E_BAD_ARGUMENT;
+    if (odd_address(p.y, p.type) || odd_address(p.x, p.type) || odd_address(p.r, p.type) || odd_address(p.h, p.type) || odd_address(p.w1, p.ptype) ||
+        odd_address(p.b1, p.ptype) || odd_address(p.w2, p.ptype) || odd_address(p.b2, p.ptype) || odd_address(p.gate, p.gtype) || misaligned(p.stats, 15))
+        return TAB_E_ALIGNMENT;
+    if (!p.w1) p.b1 = nullptr;
+    if (!p.w2) p.b2 = nullptr;
+    return residual_norm_dispatch(p, p.type, reinterpret_cast<cudaStream_t>(stream));
+}
+
+size_t tab_residual_norm_workspace_bytes(long long M, int C) { return M < 1 || C < 1 || C > NORM_MAX ? 0 : residual_norm_partial_bytes(M, C); }
+
+int tab_residual_norm_backward_launch(const tab_norm_backward_t* args, tab_stream_t stream) {
+    if (!args) return TAB_E_NULL_POINTER;
+    tab_norm_backward_t b = *args;
+    tab_norm_t& p = b.f;
+    const int rc = norm_args_ok(p);
+    if (rc != TAB_OK) return rc;
+    cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+    if (p.C == 0) return TAB_OK;
+    if (p.gkind == TAB_GATE_NONE) { p.gate = nullptr; b.dgate = nullptr; }
+    if (!p.w1) { b.dw1 = b.db1 = nullptr; p.b1 = nullptr; }
+    if (!p.w2) { b.dw2 = b.db2 = nullptr; b.gh = nullptr; }
+    if (p.layer == TAB_NORM_RMS && (b.db1 || b.db2)) return TAB_E_BAD_ARGUMENT;
+    if (p.M == 0) {                                                        // sums over no rows
+        const struct { void* p; int type; } outs[5] = {{b.dw1, p.ptype}, {b.db1, p.ptype}, {b.dw2, p.ptype}, {b.db2, p.ptype}, {p.gkind == TAB_GATE_CHANNEL ? b.dgate : nullptr, p.gtype}};
+        for (const auto& o : outs) {
+            if (!o.p) continue;
+            cudaError_t e = cudaMemsetAsync(o.p, 0, (size_t)p.C * type_bytes(o.type), s);
+            if (e != cudaSuccess) return record_cuda_error(e);
+        }
+        return TAB_OK;
+    }
+    const bool want_u = p.w1 || p.gkind != TAB_GATE_NONE, sums = b.dw1 || b.db1 || b.dw2 || b.db2 || (p.gkind == TAB_GATE_CHANNEL && b.dgate);
+    if ((want_u && !p.y) || (p.gkind != TAB_GATE_NONE && !p.gate) || (b.gh && !p.r) || ((p.w1 || b.gh) && !p.stats)) return TAB_E_NULL_POINTER;
+    if (sums && !b.partial) return TAB_E_WORKSPACE;
+    if (misaligned(b.partial, 31)) return TAB_E_WORKSPACE;
+    if (p.M > 1 && ((want_u && p.ldy < p.C) || (b.gh && (p.ldr < p.C || b.ldgh < p.C)) || (b.gr && b.ldgr < p.C) || (b.dy && b.lddy < p.C) || (b.dx && b.lddx < p.C) ||
+                    (p.gkind == TAB_GATE_FULL && p.ldg < p.C) || (p.gkind == TAB_GATE_TOKEN && p.ldg < 0))) return TAB_E_BAD_ARGUMENT;
+    if (odd_address(p.y, p.type) || odd_address(p.r, p.type) || odd_address(b.gr, p.type) || odd_address(b.gh, p.type) || odd_address(b.dy, p.type) || odd_address(b.dx, p.type) ||
+        odd_address(p.w1, p.ptype) || odd_address(p.b1, p.ptype) || odd_address(p.w2, p.ptype) || odd_address(p.gate, p.gtype) || odd_address(b.dgate, p.gtype) ||
+        odd_address(b.dw1, p.ptype) || odd_address(b.db1, p.ptype) || odd_address(b.dw2, p.ptype) || odd_address(b.db2, p.ptype) || misaligned(p.stats, 15))
+        return TAB_E_ALIGNMENT;
+    return residual_norm_backward_dispatch(b, p.type, s);
 }
 
 }  // extern "C"

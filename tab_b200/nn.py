@@ -188,3 +188,111 @@ class TABConv2d(torch.nn.Module):
     def extra_repr(self):
         return "%s, C=%d, KN=%d, kernel=%dx%d, padding=%s, stride=%s" % (
             TYPE_NAMES[self.conv_type], self.C, self.KN, self.KH, self.KW, self.padding, self.stride)
+
+
+# ---- dense layers in 8 bits and the residual stream between blocks ------------------------------------------------------
+
+def _even_rows(g):
+    """A gradient as autograd hands it over (expanded, transposed, ...) with the rows the operators take."""
+    try:
+        ops._rows(g, "grad")
+        return g
+    except RuntimeError:
+        return g.contiguous()
+
+
+class _BlockLinear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, out_dtype, grad_dtype):
+        need_x, need_w = ctx.needs_input_grad[:2]
+        x = _even_rows(x)
+        xq = ops.quantize_blocks(x, columns=need_w)
+        wq = ops.quantize_blocks2d(weight, transposed=need_x)
+        ctx.shape, ctx.types, ctx.grad_dtype = x.shape, (x.dtype, weight.dtype), grad_dtype
+        ctx.save_for_backward(*(xq[2:] if need_w else (None, None)), *(wq[2:] if need_x else (None, None)))
+        return ops.matmul_blocks(*xq[:2], *wq[:2], out_dtype=out_dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        xt, xts, wt, wts = ctx.saved_tensors
+        g = ops.quantize_blocks(_even_rows(grad), ctx.grad_dtype, columns=xt is not None)
+        dx = None if wt is None else ops.matmul_blocks(*g[:2], wt, wts, out_dtype=ctx.types[0])
+        dw = None if xt is None else ops.matmul_blocks(*g[2:], xt, xts, out_dtype=ctx.types[1])
+        return dx, dw, None, None
+
+
+def block_linear(x, weight, out_dtype=None, grad_dtype=torch.float8_e4m3fn):
+    """``x`` ``[..., K]`` times ``weight`` ``[N, K]`` transposed, for training: both are rounded to 8-bit floats in blocks of 128 (``x`` along its
+    rows, ``weight`` in squares of 128 x 128) and multiplied by ``ops.matmul_blocks``; the result is ``[..., N]`` in ``out_dtype`` (``x``'s type).
+
+    Its gradients are products of the same kind, with the gradient ``g`` of the result rounded to ``grad_dtype``: ``g`` (along its rows) times the
+    rounded weights for ``x``, and ``g`` and ``x`` (both along their columns, i.e. over the rows that this product sums) for ``weight``, in the
+    types of ``x`` and ``weight``.  The rounding itself counts as the identity.  For the backward pass 8-bit copies are kept, not ``x`` and ``weight``."""
+    return _BlockLinear.apply(x, weight, x.dtype if out_dtype is None else out_dtype, grad_dtype)
+
+
+class BlockLinear(torch.nn.Module):
+    """A dense layer with weights prepared once for serving: 8-bit floats ``Wq`` ``[N, K]`` and a scale for each square of 128 x 128.
+    ``forward(x)`` quantises ``x`` ``[..., K]`` along its rows and multiplies; ``forward(q, s)`` takes what ``ops.quantize_blocks`` or
+    ``ops.residual_norm(..., quantize=...)`` made.  Inference only; ``block_linear`` is the form with gradients."""
+
+    def __init__(self, Wq, Ws, out_dtype=torch.bfloat16):
+        super().__init__()
+        if Wq.dim() != 2 or Ws.dim() != 2 or int(Ws.shape[1]) != -(-int(Wq.shape[1]) // 128):
+            raise ValueError("Wq must be [N, K] and Ws [ceil(N/128) or N, ceil(K/128)]")
+        self.N, self.K = (int(v) for v in Wq.shape)
+        self.out_dtype = out_dtype
+        self.register_buffer("Wq", Wq)
+        self.register_buffer("Ws", Ws)
+
+    @classmethod
+    def from_float(cls, weight, dtype=torch.float8_e4m3fn, out_dtype=torch.bfloat16):
+        """``weight``: CUDA tensor ``[N, K]``, fp32, bf16 or fp16."""
+        return cls(*ops.quantize_blocks2d(weight.detach(), dtype), out_dtype=out_dtype)
+
+    def forward(self, x, scales=None):
+        if int(x.shape[-1]) != self.K:
+            raise ValueError("x must be [..., %d]" % self.K)
+        if scales is None:
+            x, scales = ops.quantize_blocks(x)
+        return ops.matmul_blocks(x, scales, self.Wq, self.Ws, self.out_dtype)
+
+    def extra_repr(self):
+        return "K=%d, N=%d, %s -> %s" % (self.K, self.N, self.Wq.dtype, self.out_dtype)
+
+
+_NORM_TENSORS = ("y", "residual", "pre_weight", "pre_bias", "post_weight", "post_bias", "gate")
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps):
+        y = _even_rows(y)
+        residual = None if residual is None else _even_rows(residual)
+        (r, h), stats = ops._residual_norm(y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps, stats=True)
+        ctx.set_materialize_grads(False)
+        ctx.has_residual, ctx.args = residual is not None, (residual_scale, kind, eps)
+        plain = r is y
+        ctx.plain = plain
+        ctx.save_for_backward(y, None if plain else r, stats, pre_weight, pre_bias, post_weight, post_bias, gate)
+        return (None if plain else r), h
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gr, gh):
+        y, r, stats, *weights = ctx.saved_tensors
+        wanted = {n for n, need in zip(_NORM_TENSORS, ctx.needs_input_grad) if need}
+        if (gr is None and gh is None) or not wanted:
+            return (None,) * 10
+        gr, gh = (None if g is None else _even_rows(g) for g in (gr, gh))
+        out = ops.residual_norm_backward(gr, gh, y, y if ctx.plain else r, stats, ctx.has_residual, *weights, *ctx.args, wanted)
+        return tuple(out.get(n) for n in _NORM_TENSORS) + (None, None, None)
+
+
+def residual_norm(y, residual=None, pre_weight=None, pre_bias=None, post_weight=None, post_bias=None, gate=None, residual_scale=1.0,
+                  kind="rms", eps=1e-6):
+    """``ops.residual_norm`` with gradients: returns ``(r, h)``.  Gradients go to ``y``, ``residual``, the weights, the biases and the gate;
+    that of a weight or of a gate ``[C]`` is summed over the rows in a fixed order, so that the same inputs give the same bits."""
+    r, h = _ResidualNorm.apply(y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps)
+    return (y if r is None else r), h

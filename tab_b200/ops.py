@@ -39,7 +39,7 @@ def _try(name, *args):
     if not host:
         return None
     try:
-        return getattr(host, name)(*args)
+        return getattr(host, name, lambda *_: None)(*args)
     except TypeError:
         return None
 
@@ -412,3 +412,269 @@ def Conv2dFused(X, QW, thresholds, btn, type, padding1, padding2, stride1, strid
                                        float(threshold_scale) if threshold_scale is not None else 0.0, st)
         _cabi.check(rc, "tab_conv2d_chain_launch")
     return Y, nxt
+
+
+# ---- 8-bit floats in blocks of 128 ----------------------------------------------------------------------------------
+
+_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_FORMATS = {torch.float8_e4m3fn: 0, torch.float8_e5m2: 1}
+
+
+def _blocks(n):
+    return -(-n // 128)
+
+
+def _on_device(t, name, device, types, what):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise RuntimeError("%s must be a CUDA tensor" % name)
+    if t.dtype not in types:
+        raise RuntimeError("%s must be %s, not %s" % (name, what, t.dtype))
+    if device is not None and t.device != device:
+        raise RuntimeError("%s must be on %s" % (name, device))
+
+
+def _rows(t, name):
+    """``(rows, row length, pitch)`` of a tensor whose leading dimensions are one axis of evenly spaced rows without gaps in them."""
+    if t.dim() == 0:
+        raise RuntimeError("%s must have at least one dimension" % name)
+    K = int(t.shape[-1])
+    M = t[..., 0].numel() if K else int(torch.Size(t.shape[:-1]).numel())
+    if M == 0 or K == 0:
+        return M, K, K
+    if K > 1 and t.stride(-1) != 1:
+        raise RuntimeError("%s must have contiguous rows" % name)
+    try:
+        two = t.view(M, K)
+    except RuntimeError:
+        raise RuntimeError("%s must have evenly spaced rows" % name) from None
+    pitch = two.stride(0) if M > 1 else K
+    if pitch < K:
+        raise RuntimeError("%s must not have overlapping rows" % name)
+    return M, K, pitch
+
+
+def _new_blocks(shape, rows, n, dtype, device):
+    """8-bit values ``shape`` (``rows`` x ``n``), every row starting on 16 bytes."""
+    pitch = -(-n // 16) * 16
+    held = torch.empty((rows, pitch), dtype=torch.uint8, device=device).view(dtype)
+    return held[:, :n].view(shape)
+
+
+def _format(dtype):
+    if dtype not in _FORMATS:
+        raise RuntimeError("dtype must be torch.float8_e4m3fn or torch.float8_e5m2")
+    return _FORMATS[dtype]
+
+
+def quantize_blocks(x, dtype=torch.float8_e4m3fn, columns=False):
+    """``x`` ``[..., K]`` (fp32, bf16 or fp16; evenly spaced rows) -> ``(q, s)``: 8-bit floats ``[..., K]`` and a power-of-two scale
+    for each 128 consecutive values of a row, ``[..., ceil(K/128)]`` ``torch.float8_e8m0fnu``; ``q * s`` is what they stand for.
+
+    ``s = 2**e`` with the least ``e >= -127`` for which the largest finite magnitude of the block is at most ``F * 2**e`` (``F``: 448 for
+    e4m3, 57344 for e5m2); ``q`` is ``x / s`` rounded to nearest even.  NaN stays NaN; infinities become NaN in e4m3.
+
+    ``columns``: also ``(qt, st)``, from the same reading of ``x``: its transpose ``[K, rows]`` with blocks along the rows of ``x``,
+    ``st`` ``[K, ceil(rows/128)]`` - what a product that sums over the rows takes (the gradient of a dense layer's weights).
+
+    Rows of ``q`` and ``qt`` start on 16 bytes, as ``matmul_blocks`` wants them."""
+    done = _try("quantize_blocks", x, dtype, columns)
+    if done is not None:
+        return done
+    fmt = _format(dtype)
+    _on_device(x, "x", None, _TYPES, "float32, bfloat16 or float16")
+    M, K, ldx = _rows(x, "x")
+    with torch.cuda.device(x.device):
+        q = _new_blocks(tuple(x.shape), M, K, dtype, x.device)
+        s = torch.empty((*x.shape[:-1], _blocks(K)), dtype=torch.float8_e8m0fnu, device=x.device)
+        qt = _new_blocks((K, M), K, M, dtype, x.device) if columns else None
+        st = torch.empty((K, _blocks(M)), dtype=torch.float8_e8m0fnu, device=x.device) if columns else None
+        rc = _cabi.lib().tab_quantize_blocks_launch(x.data_ptr(), _TYPES[x.dtype], ldx, M, K, fmt, 0, q.data_ptr(), -(-K // 16) * 16, s.data_ptr(),
+                                                    qt.data_ptr() if columns else None, -(-M // 16) * 16, st.data_ptr() if columns else None,
+                                                    _stream_ptr(x.device))
+    _cabi.check(rc, "tab_quantize_blocks_launch")
+    return (q, s, qt, st) if columns else (q, s)
+
+
+def quantize_blocks2d(w, dtype=torch.float8_e4m3fn, transposed=False):
+    """``w`` ``[N, K]`` -> ``(q, s)`` with one scale for each square of 128 x 128: ``q`` ``[N, K]``, ``s`` ``[ceil(N/128), ceil(K/128)]``.
+    ``transposed``: also ``(qt, st)``, the same values as ``[K, N]`` and the same scales as ``[ceil(K/128), ceil(N/128)]``.
+    Values and scales as ``quantize_blocks`` chooses them."""
+    done = _try("quantize_blocks2d", w, dtype, transposed)
+    if done is not None:
+        return done
+    fmt = _format(dtype)
+    _on_device(w, "w", None, _TYPES, "float32, bfloat16 or float16")
+    if w.dim() != 2:
+        raise RuntimeError("w must be [N, K]")
+    M, K, ldx = _rows(w, "w")
+    with torch.cuda.device(w.device):
+        q = _new_blocks((M, K), M, K, dtype, w.device)
+        s = torch.empty((_blocks(M), _blocks(K)), dtype=torch.float8_e8m0fnu, device=w.device)
+        qt = _new_blocks((K, M), K, M, dtype, w.device) if transposed else None
+        st = torch.empty((_blocks(K), _blocks(M)), dtype=torch.float8_e8m0fnu, device=w.device) if transposed else None
+        rc = _cabi.lib().tab_quantize_blocks_launch(w.data_ptr(), _TYPES[w.dtype], ldx, M, K, fmt, 1, q.data_ptr(), -(-K // 16) * 16, s.data_ptr(),
+                                                    qt.data_ptr() if transposed else None, -(-M // 16) * 16, st.data_ptr() if transposed else None,
+                                                    _stream_ptr(w.device))
+    _cabi.check(rc, "tab_quantize_blocks_launch")
+    return (q, s, qt, st) if transposed else (q, s)
+
+
+def _operand(q, s, name, device):
+    """What ``tab_matmul_blocks_launch`` takes of an operand: ``(pointer, format, pitch, scales, rows to a scale, scale strides), rows, K``."""
+    _on_device(q, name, device, _FORMATS, "8-bit floats (quantize_blocks)")
+    _on_device(s, name + "_scales", q.device, (torch.float8_e8m0fnu,), "torch.float8_e8m0fnu")
+    M, K, ld = _rows(q, name)
+    KB = _blocks(K)
+    if s.dim() == 0 or int(s.shape[-1]) != KB:
+        raise RuntimeError("%s_scales must be [..., %d]: one for each 128 of %d values" % (name, KB, K))
+    R = int(torch.Size(s.shape[:-1]).numel())
+    if R not in (M, _blocks(M)):
+        raise RuntimeError("%s_scales has %d rows, expected %d (a scale for each row) or %d (for each 128 rows)" % (name, R, M, _blocks(M)))
+    if s.numel() and s.dim() != 2:
+        try:
+            s = s.view(R, KB)
+        except RuntimeError:
+            raise RuntimeError("%s_scales must have evenly spaced rows" % name) from None
+    if M > 1 and K and (ld % 16 or q.data_ptr() % 16):
+        raise RuntimeError("%s must have rows that start on 16 bytes, as quantize_blocks makes them" % name)
+    strides = s.stride() if s.numel() else (0, 0)
+    return (q.data_ptr(), _FORMATS[q.dtype], ld, s.data_ptr(), 1 if R == M else 128, strides[0], strides[1]), M, K
+
+
+def matmul_blocks(a, a_scales, b, b_scales, out_dtype=torch.bfloat16):
+    """``y[..., n] = sum_k a[..., k] * b[n, k]`` of what ``a`` ``[..., K]`` and ``b`` ``[N, K]`` stand for: 8-bit floats (either format on
+    either side) with scales for each 128 of a row (``quantize_blocks``) or for each square of 128 x 128 (``quantize_blocks2d``; one row
+    of scales for each 128 rows of values).  Sums in fp32, rounded once to ``out_dtype`` (fp32, bf16 or fp16)."""
+    done = _try("matmul_blocks", a, a_scales, b, b_scales, out_dtype)
+    if done is not None:
+        return done
+    if out_dtype not in _TYPES:
+        raise RuntimeError("out_dtype must be torch.float32, torch.bfloat16 or torch.float16")
+    (pa, M, K), (pb, N, KB) = _operand(a, a_scales, "a", None), _operand(b, b_scales, "b", a.device)
+    if b.dim() != 2 or KB != K:
+        raise RuntimeError("b must be [N, %d]" % K)
+    with torch.cuda.device(a.device):
+        y = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=a.device)
+        rc = _cabi.lib().tab_matmul_blocks_launch(*pa, *pb, y.data_ptr(), _TYPES[out_dtype], N, M, N, K, _stream_ptr(a.device))
+    _cabi.check(rc, "tab_matmul_blocks_launch")
+    return y
+
+
+# ---- the residual stream between two blocks --------------------------------------------------------------------------
+
+_KINDS = {"rms": 0, "layer": 1}
+
+
+def _norm_args(y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps):
+    """``NormArgs`` of the inputs, checked, and the tensors' shapes: ``(args, rows, row length)``."""
+    if kind not in _KINDS:
+        raise RuntimeError("kind must be 'rms' or 'layer'")
+    _on_device(y, "y", None, _TYPES, "float32, bfloat16 or float16")
+    M, C, ldy = _rows(y, "y")
+    a = _cabi.NormArgs(y=y.data_ptr(), ldy=ldy, type=_TYPES[y.dtype], layer=_KINDS[kind], alpha=float(residual_scale), eps=float(eps), M=M, C=C)
+    if residual is not None:
+        _on_device(residual, "residual", y.device, (y.dtype,), str(y.dtype))
+        if residual.shape != y.shape:
+            raise RuntimeError("residual must have the shape of y")
+        a.x, a.ldx = residual.data_ptr(), _rows(residual, "residual")[2]
+    weights = {"w1": ("post_weight", post_weight), "b1": ("post_bias", post_bias), "w2": ("pre_weight", pre_weight), "b2": ("pre_bias", pre_bias)}
+    types = {t.dtype for _, t in weights.values() if isinstance(t, torch.Tensor)}
+    for field, (name, t) in weights.items():
+        if t is None:
+            continue
+        _on_device(t, name, y.device, (torch.float32, y.dtype), "float32 or of y's type")
+        if tuple(t.shape) != (C,) or not t.is_contiguous():
+            raise RuntimeError("%s must be a contiguous vector of %d" % (name, C))
+        if len(types) > 1:
+            raise RuntimeError("weights and biases must have one type")
+        setattr(a, field, t.data_ptr())
+        a.ptype = _TYPES[t.dtype]
+    if (pre_bias is not None and pre_weight is None) or (post_bias is not None and post_weight is None):
+        raise RuntimeError("a bias comes with the weight of its norm")
+    if kind == "rms" and (pre_bias is not None or post_bias is not None):
+        raise RuntimeError("a norm of kind 'rms' has no bias")
+    if gate is not None:
+        _on_device(gate, "gate", y.device, (torch.float32, y.dtype), "float32 or of y's type")
+        a.gtype, a.gate = _TYPES[gate.dtype], gate.data_ptr()
+        if tuple(gate.shape) == (C,) and gate.dim() == 1 and (gate.is_contiguous() or C == 1):
+            a.gkind = 2
+        elif tuple(gate.shape) == (*y.shape[:-1], 1):
+            a.gkind, a.ldg = 1, _rows(gate, "gate")[2]
+        elif gate.shape == y.shape:
+            a.gkind, a.ldg = 3, _rows(gate, "gate")[2]
+        else:
+            raise RuntimeError("gate must be [%d] (contiguous), %s or %s" % (C, (*y.shape[:-1], 1), tuple(y.shape)))
+    return a, M, C
+
+
+def residual_norm(y, residual=None, pre_weight=None, pre_bias=None, post_weight=None, post_bias=None, gate=None, residual_scale=1.0,
+                  kind="rms", eps=1e-6, quantize=None):
+    """What lies between two blocks of a residual network, in one pass: with ``y`` ``[..., C]`` a block's result,
+
+        u = norm(y) * post_weight + post_bias          (``y`` itself without ``post_weight``)
+        r = residual_scale * residual + gate * u       (either factor and the residual may be absent), kept in the type of ``y``
+        h = norm(r) * pre_weight + pre_bias            (what the next block is given; ``None`` without ``pre_weight``)
+
+    Returns ``(r, h)``, or with ``quantize`` (``torch.float8_e4m3fn`` or ``torch.float8_e5m2``) ``(r, q, s)``: ``h`` as ``quantize_blocks`` would
+    give it from fp32, for ``matmul_blocks``.  Without residual, post norm and gate, ``r`` is ``y``.
+    ``kind``: ``"rms"``, v / sqrt(mean(v^2) + eps), or ``"layer"``, (v - mean) / sqrt(var + eps), which alone takes biases.
+    ``gate``: ``[C]``, one for each row (``[..., 1]``), or of ``y``'s shape.  Weights and gate are fp32 or of ``y``'s type.  C <= 16384.
+    ``tab_b200.nn.residual_norm`` is the differentiable form."""
+    done = _try("residual_norm", y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps, quantize)
+    if done is not None:
+        return done
+    return _residual_norm(y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps, quantize)[0]
+
+
+def _residual_norm(y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps, quantize=None, stats=False):
+    """``residual_norm``'s results and, with ``stats``, what the backward pass takes of the statistics."""
+    a, M, C = _norm_args(y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps)
+    if quantize is not None:
+        a.format = _format(quantize)
+        if pre_weight is None:
+            raise RuntimeError("quantize needs pre_weight (the norm whose result is quantised)")
+    plain = residual is None and post_weight is None and gate is None
+    with torch.cuda.device(y.device):
+        r = y if plain else torch.empty(y.shape, dtype=y.dtype, device=y.device)
+        h = s = None
+        if not plain:
+            a.r, a.ldr = r.data_ptr(), C
+        if quantize is not None:
+            h = _new_blocks(tuple(y.shape), M, C, quantize, y.device)
+            s = torch.empty((*y.shape[:-1], _blocks(C)), dtype=torch.float8_e8m0fnu, device=y.device)
+            a.q, a.ldq, a.s = h.data_ptr(), -(-C // 16) * 16, s.data_ptr()
+        elif pre_weight is not None:
+            h = torch.empty(y.shape, dtype=y.dtype, device=y.device)
+            a.h, a.ldh = h.data_ptr(), C
+        st = torch.empty((M, 4), dtype=torch.float32, device=y.device) if stats else None
+        if stats:
+            a.stats = st.data_ptr()
+        rc = _cabi.lib().tab_residual_norm_launch(ctypes.byref(a), _stream_ptr(y.device))
+    _cabi.check(rc, "tab_residual_norm_launch")
+    return ((r, h) if quantize is None else (r, h, s)), st
+
+
+def residual_norm_backward(grad_r, grad_h, y, r, stats, has_residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps, wanted):
+    """Gradients of ``residual_norm`` for those of ``r`` and ``h`` (either may be ``None``), from the kept ``y``, ``r`` and statistics.  ``wanted``: names
+    among y, residual, gate, pre_weight, pre_bias, post_weight, post_bias; returns a dict of those that the arguments have."""
+    a, M, C = _norm_args(y, None, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps)
+    b = _cabi.NormBackwardArgs()
+    a.r, a.ldr, a.stats = r.data_ptr(), _rows(r, "r")[2], stats.data_ptr()
+    b.f = a
+    for field, g in (("gr", grad_r), ("gh", grad_h)):
+        if g is not None:
+            setattr(b, field, g.data_ptr())
+            setattr(b, "ld" + field, _rows(g, "grad")[2])
+    out = {}
+    with torch.cuda.device(y.device):
+        for name, field, like in (("y", "dy", y), ("residual", "dx", y if has_residual else None), ("gate", "dgate", gate), ("pre_weight", "dw2", pre_weight),
+                                  ("pre_bias", "db2", pre_bias), ("post_weight", "dw1", post_weight), ("post_bias", "db1", post_bias)):
+            if name in wanted and like is not None:
+                out[name] = t = torch.empty(like.shape, dtype=like.dtype, device=y.device)
+                setattr(b, field, t.data_ptr())
+        b.lddy = b.lddx = C
+        partial = torch.empty((_cabi.lib().tab_residual_norm_workspace_bytes(M, C) // 4,), dtype=torch.float32, device=y.device)
+        b.partial = partial.data_ptr()
+        rc = _cabi.lib().tab_residual_norm_backward_launch(ctypes.byref(b), _stream_ptr(y.device))
+    _cabi.check(rc, "tab_residual_norm_backward_launch")
+    return out

@@ -1,0 +1,338 @@
+"""8-bit block quantisers and the block-scaled product: what is refused (no GPU), and the results against 64-bit references."""
+import numpy as np
+import pytest
+import torch
+
+import blocks_ref as ref
+import tab_b200 as TAB
+from tab_b200 import _cabi, nn as tab_nn
+
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+F8 = {f: v[0] for f, v in ref.FORMATS.items()}
+BASE = 1 << 20                                                      # a made-up, aligned address: nothing follows it
+
+
+def np_bytes(t):
+    return t.contiguous().view(torch.uint8).cpu().numpy()
+
+
+# ---- refusals, on the CPU ---------------------------------------------------------------------------------------------
+
+def quantize_args(**over):
+    a = dict(x=BASE, type=1, ldx=256, M=4, K=256, format=0, square=0, q=BASE, ldq=256, s=BASE, qt=None, ldqt=0, st=None)
+    a.update(over)
+    return [*a.values(), None]
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(type=3), -1), (dict(type=-1), -1), (dict(format=2), -1), (dict(square=2), -1), (dict(M=-1), -1), (dict(K=-1), -1),
+    (dict(M=0), 0), (dict(K=0), 0), (dict(x=None), -2), (dict(q=None), -2), (dict(s=None), -2), (dict(qt=BASE, ldqt=16), -2),
+    (dict(square=1, q=None, s=None), -2), (dict(ldx=255), -1), (dict(ldq=255), -1), (dict(qt=BASE, st=BASE, ldqt=3), -1),
+    (dict(x=BASE + 1), -6), (dict(type=0, x=BASE + 2), -6), (dict(M=1 << 31), -5), (dict(ldx=1 << 40), -5),
+])
+def test_quantize_blocks_refuses(over, code):
+    assert _cabi.lib().tab_quantize_blocks_launch(*quantize_args(**over)) == code
+
+
+def matmul_args(**over):
+    a = dict(a=BASE, af=0, lda=256, as_=BASE, ash=1, ar=2, ab=1, b=BASE, bf=0, ldb=256, bs=BASE, bsh=128, br=2, bb=1, y=BASE, type=1, ldy=64, M=4, N=64, K=256)
+    a.update(over)
+    return [*a.values(), None]
+
+
+@pytest.mark.parametrize("over, code", [
+    (dict(af=2), -1), (dict(bf=-1), -1), (dict(type=4), -1), (dict(ash=2), -1), (dict(bsh=0), -1), (dict(M=-1), -1), (dict(N=-1), -1), (dict(K=-1), -1),
+    (dict(M=0), 0), (dict(N=0), 0), (dict(lda=255), -1), (dict(ldb=128), -1), (dict(ldy=63), -1), (dict(a=None), -2), (dict(b=None), -2), (dict(as_=None), -2),
+    (dict(bs=None), -2), (dict(y=None), -2), (dict(a=BASE + 8), -6), (dict(b=BASE + 1), -6), (dict(lda=264), -6), (dict(ldb=257), -6), (dict(y=BASE + 1), -6),
+    (dict(type=0, y=BASE + 2), -6), (dict(ldy=1 << 40), -5), (dict(lda=1 << 40), -5), (dict(K=2 ** 31 - 1, lda=1 << 32, ldb=1 << 32), -5),
+])
+def test_matmul_blocks_refuses(over, code):
+    assert _cabi.lib().tab_matmul_blocks_launch(*matmul_args(**over)) == code
+
+
+def test_operators_refuse_host_tensors():
+    x = torch.zeros(2, 128)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        TAB.quantize_blocks(x)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        TAB.quantize_blocks2d(x)
+    with pytest.raises(RuntimeError, match="CUDA tensor"):
+        TAB.matmul_blocks(x, x, x, x)
+    with pytest.raises(RuntimeError, match="float8"):
+        TAB.quantize_blocks(x, torch.int8)
+    with pytest.raises(ValueError, match="Wq"):
+        tab_nn.BlockLinear(torch.zeros(2, 128), torch.zeros(1, 2))
+
+
+def test_row_layouts():
+    """What counts as evenly spaced rows (the arithmetic that hands pitches to the kernels)."""
+    rows = TAB.ops._rows
+    t = torch.zeros(6, 5, 40)
+    assert rows(t, "t") == (30, 40, 40)
+    assert rows(t[:, 0], "t") == (6, 40, 200)
+    assert rows(t[..., :7], "t") == (30, 7, 40)
+    assert rows(t[0, 0], "t") == (1, 40, 40)
+    assert rows(t[:0], "t")[0] == 0 and rows(t[..., :0], "t")[1] == 0
+    assert rows(torch.zeros(0, 0), "t")[:2] == (0, 0)
+    for bad in (t[:, :3], t[..., ::2], t.transpose(0, 1), t[:1, :1].expand(3, 1, 40), torch.zeros(())):
+        with pytest.raises(RuntimeError):
+            rows(bad, "t")
+    for shape in ((3, 7), (2, 3, 7), (7,), (3, 32), (2, 2, 32), (0, 7), (4, 0)):
+        q = TAB.ops._new_blocks(shape, int(np.prod(shape[:-1])), shape[-1], torch.float8_e4m3fn, "cpu")
+        assert tuple(q.shape) == shape and (q.numel() == 0 or q.dim() == 1 or rows(q, "q")[2] % 16 == 0)
+
+
+# ---- quantisers -------------------------------------------------------------------------------------------------------
+
+def spread(seed, M, K, dtype):
+    """Values over many magnitudes: blocks of large, small, subnormal and zero values, ties between neighbours, the types' ends."""
+    rng = np.random.default_rng(seed)
+    x = rng.standard_normal((M, K)) * 2.0 ** rng.integers(-20, 8, (M, 1)) * 2.0 ** rng.integers(-6, 7, (1, K))
+    x[rng.random((M, K)) < 0.1] = 0
+    t = torch.from_numpy(x).to(dtype)
+    if M > 3 and K > 3:
+        t[1, :] = 0
+        t[2, :min(K, 128)] = torch.linspace(-448, 448, min(K, 128)).to(dtype)
+        t[3, ::3] = torch.finfo(dtype).max
+        t[M - 1, :] = torch.finfo(dtype).tiny / 4
+        t[0, K // 2] = -0.0
+    return t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("format", F8)
+@pytest.mark.parametrize("M, K", [(1, 1), (1, 128), (3, 127), (16, 129), (128, 128), (130, 300), (257, 64), (5, 2100), (300, 1000)])
+def test_quantize_blocks(cuda, type, format, M, K):
+    x = spread(M * 1000 + K, M, K, TYPES[type])
+    v = x.double().numpy()
+    want, ws = ref.quantize(v, format)
+    want_t, wst = ref.quantize(v.T.copy(), format)
+    xd = x.to(cuda)
+    q, s = TAB.quantize_blocks(xd, F8[format])
+    assert q.shape == (M, K) and s.shape == (M, -(-K // 128)) and (M == 1 or q.stride(0) % 16 == 0)
+    assert np.array_equal(np_bytes(s), ws) and ref.same_bytes(np_bytes(q), want, format)
+    q, s, qt, st = TAB.quantize_blocks(xd, F8[format], columns=True)
+    assert np.array_equal(np_bytes(s), ws) and ref.same_bytes(np_bytes(q), want, format)
+    assert np.array_equal(np_bytes(st), wst) and ref.same_bytes(np_bytes(qt), want_t, format)
+    want, ws = ref.quantize(v, format, square=True)
+    q, s, qt, st = TAB.quantize_blocks2d(xd, F8[format], transposed=True)
+    assert np.array_equal(np_bytes(s), ws) and ref.same_bytes(np_bytes(q), want, format)
+    assert np.array_equal(np_bytes(st), ws.T) and ref.same_bytes(np_bytes(qt), want.T, format)
+    q, s = TAB.quantize_blocks2d(xd, F8[format])
+    assert np.array_equal(np_bytes(s), ws) and ref.same_bytes(np_bytes(q), want, format)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("format", F8)
+@pytest.mark.parametrize("type", TYPES)
+def test_quantize_blocks_non_finite(cuda, type, format):
+    x = spread(5, 40, 260, TYPES[type])
+    x[4, 7], x[4, 200], x[5, :] = float("nan"), float("inf"), float("-inf")
+    x[6, 130:256] = float("nan")
+    v = x.double().numpy()
+    q, s, qt, st = TAB.quantize_blocks(x.to(cuda), F8[format], columns=True)
+    for got, gs, want in ((q, s, v), (qt, st, v.T.copy())):
+        wq, ws = ref.quantize(want, format)
+        assert np.array_equal(np_bytes(gs), ws) and ref.same_bytes(np_bytes(got), wq, format)
+
+
+@pytest.mark.gpu
+def test_quantize_blocks_strided_and_bounded(cuda):
+    """Slices with a row pitch and odd starts; bytes behind the rows and behind the last row stay as they are."""
+    big = spread(9, 70, 700, torch.bfloat16).to(cuda)
+    for cut in (big[3:60, 5:402], big[::2, 16:272], big.view(10, 7, 700)[:, 2]):
+        q, s = TAB.quantize_blocks(cut)
+        wq, ws = ref.quantize(cut.double().cpu().numpy(), "e4m3")
+        assert np.array_equal(np_bytes(s), ws) and ref.same_bytes(np_bytes(q), wq, "e4m3")
+    l, x = _cabi.lib(), big[:9, :200].contiguous()
+    for qt in (None, torch.full((202, 16), 0xAA, dtype=torch.uint8, device=cuda)):
+        q, s, st = (torch.full(z, 0xAA, dtype=torch.uint8, device=cuda) for z in ((11, 208), (11, 2), (202, 1)))
+        assert l.tab_quantize_blocks_launch(x.data_ptr(), 1, 200, 9, 200, 0, 0, q.data_ptr(), 208, s.data_ptr(), qt.data_ptr() if qt is not None else None, 16,
+                                            st.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        wq, ws = ref.quantize(x.double().cpu().numpy(), "e4m3")
+        assert np.array_equal(q[:9, :200].cpu().numpy(), wq) and np.array_equal(s[:9].cpu().numpy(), ws)
+        assert bool((q[:, 200:] == 0xAA).all()) and bool((q[9:] == 0xAA).all()) and bool((s[9:] == 0xAA).all())
+        if qt is not None:
+            assert bool((qt[:, 9:] == 0xAA).all()) and bool((qt[200:] == 0xAA).all()) and bool((st[200:] == 0xAA).all())
+
+
+# ---- product ----------------------------------------------------------------------------------------------------------
+
+def random_blocks(rng, rows, K, format, squares, whole):
+    """Bytes and scale bytes; whole: small whole numbers under scales 1, 2, 4, whose products and sums fp32 holds exactly."""
+    R, KB = (-(-rows // 128) if squares else rows), -(-K // 128)
+    if whole:
+        table = ref.decode(format)
+        numbers = np.array([int(np.flatnonzero(table == v)[0]) for v in (-3.0, -2.0, -1.0, 0.0, 1.0, 2.0, 3.0, 4.0)], np.uint8)
+        return numbers[rng.integers(0, 8, (rows, K))], (127 + rng.integers(0, 3, (R, KB))).astype(np.uint8)
+    q = rng.integers(0, 256, (rows, K)).astype(np.uint8)
+    bad = ~np.isfinite(ref.decode(format))[q]
+    q[bad] = 0x31
+    return q, (127 + rng.integers(-9, 10, (R, KB))).astype(np.uint8)
+
+
+def device_blocks(cuda, q, s, format):
+    rows, K = q.shape
+    held = torch.full((rows, -(-K // 16) * 16), 0x55, dtype=torch.uint8, device=cuda)        # what lies behind the rows must not count
+    held[:, :K] = torch.from_numpy(q).to(cuda)
+    return held.view(F8[format])[:, :K], torch.from_numpy(s).to(cuda).view(torch.float8_e8m0fnu)
+
+
+SIZES = [(1, 1, 1), (1, 128, 128), (1, 256, 1024), (2, 130, 96), (5, 512, 4096), (16, 100, 640), (17, 1000, 1040), (33, 64, 513), (64, 384, 256), (100, 129, 300),
+         (128, 128, 127), (129, 257, 1000), (200, 2048, 512), (256, 256, 2048), (300, 300, 100), (513, 777, 1411), (1024, 512, 384), (40, 1024, 6000), (257, 1, 4100), (1, 5, 30000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("squares", [(False, True), (False, False), (True, True)])
+@pytest.mark.parametrize("M, N, K", SIZES)
+def test_matmul_blocks_exact(cuda, M, N, K, squares):
+    """Whole numbers: |product| <= 4 * 4 * 4 * 4, sums of 30000 of them stay below 2^24, so every order of additions gives the same."""
+    rng = np.random.default_rng(M + 3 * N + 7 * K)
+    fa, fb = ("e4m3", "e5m2") if K % 2 else ("e4m3", "e4m3")
+    a, b = random_blocks(rng, M, K, fa, squares[0], True), random_blocks(rng, N, K, fb, squares[1], True)
+    want = ref.values(*a, fa) @ ref.values(*b, fb).T
+    y = TAB.matmul_blocks(*device_blocks(cuda, *a, fa), *device_blocks(cuda, *b, fb), out_dtype=torch.float32)
+    assert y.shape == (M, N) and np.array_equal(y.cpu().numpy(), want)
+    assert _cabi.lib().tab_device_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("formats", [("e4m3", "e4m3"), ("e5m2", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e5m2")])
+@pytest.mark.parametrize("type", TYPES)
+@pytest.mark.parametrize("M, N, K", [(1, 300, 1000), (31, 129, 640), (150, 260, 1411), (300, 520, 2048)])
+def test_matmul_blocks(cuda, M, N, K, type, formats):
+    """Any bytes and scales.  Products are exact in fp32; K additions, each off by at most 2^-23 of the running sum of magnitudes, then
+    one rounding to the result's type (half its eps of the result; fp16 below 2^-14 in steps of 2^-24)."""
+    rng = np.random.default_rng(M + N + K)
+    fa, fb = formats
+    a, b = random_blocks(rng, M, K, fa, False, False), random_blocks(rng, N, K, fb, True, False)
+    va, vb = ref.values(*a, fa), ref.values(*b, fb)
+    if type == "fp16":                                              # keep within the type: scale rows of a down by a power of two
+        shift = int(np.ceil(np.log2(np.abs(va) @ np.abs(vb).T).max())) - 15
+        a = (a[0], (a[1].astype(int) - max(shift, 0)).astype(np.uint8))
+        va = ref.values(*a, fa)
+    want, size = va @ vb.T, np.abs(va) @ np.abs(vb).T
+    y = TAB.matmul_blocks(*device_blocks(cuda, *a, fa), *device_blocks(cuda, *b, fb), out_dtype=TYPES[type]).double().cpu().numpy()
+    eps = torch.finfo(TYPES[type]).eps / 2
+    bound = size * K * 2.0 ** -23 * (1 + eps) + np.abs(want) * eps + (2.0 ** -25 if type == "fp16" else 0)
+    assert np.all(np.abs(y - want) <= bound)
+
+
+@pytest.mark.gpu
+def test_matmul_blocks_non_finite(cuda):
+    """A NaN or an infinity reaches the results of its own row and column only."""
+    rng = np.random.default_rng(3)
+    a, b = random_blocks(rng, 140, 300, "e5m2", False, True), random_blocks(rng, 200, 300, "e4m3", True, True)
+    want = ref.values(*a, "e5m2") @ ref.values(*b, "e4m3").T
+    a[0][7, 200], a[0][139, 0], b[0][150, 299] = 0x7F, 0x7E, 0x7F
+    y = TAB.matmul_blocks(*device_blocks(cuda, *a, "e5m2"), *device_blocks(cuda, *b, "e4m3"), out_dtype=torch.float32).cpu().numpy()
+    hit = np.zeros_like(want, bool)
+    hit[7], hit[139], hit[:, 150] = True, True, True
+    assert np.isnan(y[hit]).all() and np.array_equal(y[~hit], want[~hit])
+
+
+@pytest.mark.gpu
+def test_matmul_blocks_layouts(cuda):
+    """Leading dimensions, scales of any strides, slices of operands, an empty sum, empty results, bytes behind the result."""
+    rng = np.random.default_rng(4)
+    a, b = random_blocks(rng, 60, 512, "e4m3", False, True), random_blocks(rng, 300, 512, "e4m3", True, True)
+    want = ref.values(*a, "e4m3") @ ref.values(*b, "e4m3").T
+    (qa, sa), (qb, sb) = device_blocks(cuda, *a, "e4m3"), device_blocks(cuda, *b, "e4m3")
+    y = TAB.matmul_blocks(qa.view(3, 20, 512), sa.view(3, 20, 4), qb, sb, out_dtype=torch.float32)
+    assert y.shape == (3, 20, 300) and np.array_equal(y.cpu().numpy().reshape(60, 300), want)
+    turned = sa.view(torch.uint8).t().contiguous().t().view(torch.float8_e8m0fnu)
+    wide = torch.zeros(3, 9, dtype=torch.uint8, device=cuda)
+    wide[:, 1::2] = sb.view(torch.uint8)
+    y = TAB.matmul_blocks(qa, turned, qb, wide[:, 1::2].view(torch.float8_e8m0fnu), out_dtype=torch.float32)
+    assert np.array_equal(y.cpu().numpy(), want)
+    part = ref.values(*a, "e4m3")[10:50, 128:400] @ ref.values(*b, "e4m3")[128:256, 128:400].T
+    y = TAB.matmul_blocks(qa[10:50, 128:400], sa[10:50, 1:4], qb[128:256, 128:400], sb[1:2, 1:4], out_dtype=torch.float32)
+    assert np.array_equal(y.cpu().numpy(), part)
+    empty = TAB.matmul_blocks(qa[:, :0], sa[:, :0], qb[:, :0], sb[:, :0])
+    assert empty.shape == (60, 300) and not empty.any()
+    assert TAB.matmul_blocks(qa[:0], sa[:0], qb, sb).shape == (0, 300) and TAB.matmul_blocks(qa, sa, qb[:0], sb[:0]).shape == (60, 0)
+    l = _cabi.lib()
+    for M, N in ((60, 299), (3, 200), (1, 77)):
+        out = torch.full((M + 1, 304), 7.0, device=cuda)
+        assert l.tab_matmul_blocks_launch(qa.data_ptr(), 0, 512, sa.data_ptr(), 1, 4, 1, qb.data_ptr(), 0, 512, sb.data_ptr(), 128, 4, 1, out.data_ptr(), 0, 304, M, N, 512,
+                                          torch.cuda.current_stream().cuda_stream) == 0
+        assert np.array_equal(out[:M, :N].cpu().numpy(), want[:M, :N]) and bool((out[:, N:] == 7).all()) and bool((out[M:] == 7).all())
+
+
+@pytest.mark.gpu
+def test_matmul_blocks_argument_errors(cuda):
+    q, s = TAB.quantize_blocks(torch.randn(4, 256, device=cuda))
+    w, ws = TAB.quantize_blocks2d(torch.randn(300, 256, device=cuda))
+    for args, words in [((q, s[:, :1], w, ws), "a_scales"), ((q, s[:3], w, ws), "a_scales has 3"), ((q, s, w, ws[:2]), "b_scales has 2"), ((q, s.float(), w, ws), "e8m0"),
+                        ((q, s, w[:, :128], ws[:, :1]), "b must be"), ((q[:, 1:129], s[:, :1], w[:, :128], ws[:, :1]), "16 bytes"), ((q.float(), s, w, ws), "8-bit")]:
+        with pytest.raises(RuntimeError, match=words):
+            TAB.matmul_blocks(*args)
+    with pytest.raises(RuntimeError, match="out_dtype"):
+        TAB.matmul_blocks(q, s, w, ws, out_dtype=torch.float64)
+    with pytest.raises(RuntimeError, match="float32, bfloat16 or float16"):
+        TAB.quantize_blocks(torch.zeros(2, 2, device=cuda, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="contiguous rows"):
+        TAB.quantize_blocks(torch.zeros(4, 8, device=cuda).t())
+
+
+# ---- dense layers -----------------------------------------------------------------------------------------------------
+
+def layer_reference(x, w, g, grad_format):
+    """block_linear's result and gradients in float64."""
+    v = lambda t, f="e4m3", square=False: ref.values(*ref.quantize(t, f, square), f)
+    wv = v(w, square=True)
+    return v(x) @ wv.T, v(g, grad_format) @ wv, v(g.T.copy(), grad_format) @ v(x.T.copy()).T
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("grad_format", F8)
+@pytest.mark.parametrize("M, N, K, type, wtype", [(1, 16, 40, "bf16", "fp32"), (70, 200, 129, "fp32", "fp32"), (260, 128, 384, "bf16", "bf16"), (130, 513, 256, "fp16", "fp32")])
+def test_block_linear_gradients(cuda, M, N, K, type, wtype, grad_format):
+    gen = torch.Generator().manual_seed(M)
+    x, w = torch.randn(M, K, generator=gen).to(TYPES[type]), (torch.randn(N, K, generator=gen) / K ** 0.5).to(TYPES[wtype])
+    g = torch.randn(M, N, generator=gen).to(TYPES[type])
+    want = layer_reference(x.double().numpy(), w.double().numpy(), g.double().numpy(), grad_format)
+    xd, wd = x.to(cuda).requires_grad_(), w.to(cuda).requires_grad_()
+    y = tab_nn.block_linear(xd, wd, grad_dtype=F8[grad_format])
+    y.backward(g.to(cuda))
+    for got, wanted, terms, t in ((y, want[0], K, type), (xd.grad, want[1], N, type), (wd.grad, want[2], M, wtype)):
+        got = got.detach().double().cpu().numpy()
+        # additions as in test_matmul_blocks; the magnitudes that are summed are at most sqrt(terms) times their norm, here bounded by the largest value
+        bound = np.abs(wanted).max() * 8 * terms ** 0.5 * terms * 2.0 ** -23 + np.abs(wanted) * torch.finfo(TYPES[t]).eps / 2 + 2.0 ** -25
+        assert got.shape == wanted.shape and np.all(np.abs(got - wanted) <= bound)
+    # only what is asked for
+    assert torch.equal(torch.autograd.grad(tab_nn.block_linear(xd, w.to(cuda), grad_dtype=F8[grad_format]), xd, g.to(cuda))[0], xd.grad)
+    assert torch.equal(torch.autograd.grad(tab_nn.block_linear(x.to(cuda), wd, grad_dtype=F8[grad_format]), wd, g.to(cuda))[0], wd.grad)
+
+
+@pytest.mark.gpu
+def test_block_linear_odd_gradients(cuda):
+    """Gradients that autograd hands over expanded or transposed, leading dimensions, no rows at all."""
+    w = torch.randn(96, 64, device=cuda)
+    x = torch.randn(3, 5, 64, device=cuda, requires_grad=True)
+    dx, = torch.autograd.grad(tab_nn.block_linear(x, w).sum(), x)
+    full, = torch.autograd.grad(tab_nn.block_linear(x, w), x, torch.ones(3, 5, 96, device=cuda))
+    assert dx.shape == x.shape and torch.equal(dx, full)
+    g = torch.randn(96, 5, 3, device=cuda)
+    a, = torch.autograd.grad(tab_nn.block_linear(x, w), x, g.permute(2, 1, 0))
+    b, = torch.autograd.grad(tab_nn.block_linear(x, w), x, g.permute(2, 1, 0).contiguous())
+    assert torch.equal(a, b)
+    e, wl = torch.zeros(0, 64, device=cuda, requires_grad=True), w.clone().requires_grad_()
+    y = tab_nn.block_linear(e, wl)
+    dx, dw = torch.autograd.grad(y, (e, wl), torch.zeros(0, 96, device=cuda))
+    assert y.shape == (0, 96) and dx.shape == (0, 64) and not dw.any()
+
+
+@pytest.mark.gpu
+def test_block_linear_module(cuda):
+    w, x = torch.randn(200, 300, device=cuda), torch.randn(2, 9, 300, device=cuda, dtype=torch.bfloat16)
+    m = tab_nn.BlockLinear.from_float(w)
+    q, s = TAB.quantize_blocks(x)
+    want = TAB.matmul_blocks(q, s, m.Wq, m.Ws)
+    assert torch.equal(m(x), want) and torch.equal(m(q, s), want) and torch.equal(tab_nn.block_linear(x, w), want)
+    other = tab_nn.BlockLinear.from_float(torch.zeros(200, 300, device=cuda))
+    other.load_state_dict(m.state_dict())
+    assert torch.equal(other(x), want)
+    with pytest.raises(ValueError, match="300"):
+        m(x[..., :128])
