@@ -7,6 +7,7 @@
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include "../../include/tab_b200.h"
 
 namespace {
@@ -197,6 +198,336 @@ py::object layer(const Tensor& X, const Tensor& W8, int type, int p1, int p2, in
     return Y.defined() ? py::cast(Y) : py::none();
 }
 
+// ---- 8-bit blocks and the residual stream ---------------------------------------------------------------------------------------
+int type_of(const Tensor& t) {
+    const auto s = t.scalar_type();
+    return s == at::kFloat ? TAB_FP32 : s == at::kBFloat16 ? TAB_BF16 : s == at::kHalf ? TAB_FP16 : -1;
+}
+int type_of(at::ScalarType s) { return s == at::kFloat ? TAB_FP32 : s == at::kBFloat16 ? TAB_BF16 : s == at::kHalf ? TAB_FP16 : -1; }
+int format_of(at::ScalarType s) { return s == at::kFloat8_e4m3fn ? TAB_E4M3 : s == at::kFloat8_e5m2 ? TAB_E5M2 : -1; }
+bool on_cuda(const Tensor& t) { return t.defined() && t.is_cuda(); }
+int64_t blocks(int64_t n) { return (n + 127) / 128; }
+
+// Leading dimensions that are one axis of evenly spaced rows without gaps in them, none of them empty.
+struct Rows {
+    int64_t M = 1, K = 0, pitch = 0;
+    bool of(const Tensor& t) {
+        const int64_t d = t.dim();
+        if (d == 0 || t.numel() == 0) return false;
+        const auto sizes = t.sizes(), strides = t.strides();
+        K = sizes[d - 1];
+        if (K > 1 && strides[d - 1] != 1) return false;
+        pitch = K;
+        int64_t step = 0;                                                  // stride that the next (outer) dimension must have
+        for (int64_t i = d - 2; i >= 0; i--) {
+            if (sizes[i] == 1) continue;
+            if (step == 0) pitch = strides[i];
+            else if (strides[i] != step) return false;
+            step = strides[i] * sizes[i];
+            M *= sizes[i];
+        }
+        return pitch >= K && M < (1LL << 31) && K < (1LL << 31) - 256;
+    }
+};
+
+// 8-bit values of `shape` (rows x n), every row starting on 16 bytes; the pitch.
+Tensor new_blocks(const Tensor& like, at::IntArrayRef shape, int64_t rows, int64_t n, at::ScalarType dtype) {
+    const int64_t pitch = (n + 15) / 16 * 16;
+    if (pitch == n) return make(like, shape, dtype);
+    Tensor held = make(like, {rows, pitch}, dtype);
+    std::vector<int64_t> strides(shape.size());
+    int64_t step = pitch;
+    for (int64_t i = (int64_t)shape.size() - 1; i >= 0; i--) {
+        if (i == (int64_t)shape.size() - 1) { strides[i] = 1; continue; }
+        strides[i] = step;
+        step *= shape[i];
+    }
+    return held.as_strided(shape, strides);
+}
+std::vector<int64_t> with_last(const Tensor& t, int64_t n) {
+    std::vector<int64_t> s(t.sizes().begin(), t.sizes().end());
+    s.back() = n;
+    return s;
+}
+
+struct Quantized { Tensor q, s, qt, st; };
+bool quantize_any(const Tensor& x, at::ScalarType dtype, bool both, bool square, Quantized& o) {
+    Rows r;
+    const int format = format_of(dtype);
+    if (!on_cuda(x) || type_of(x) < 0 || format < 0 || (square && x.dim() != 2) || !r.of(x)) return false;
+    const c10::cuda::CUDAGuard guard(x.device());
+    o.q = new_blocks(x, x.sizes(), r.M, r.K, dtype);
+    o.s = square ? make(x, {blocks(r.M), blocks(r.K)}, at::kFloat8_e8m0fnu) : make(x, with_last(x, blocks(r.K)), at::kFloat8_e8m0fnu);
+    if (both) {
+        o.qt = new_blocks(x, {r.K, r.M}, r.K, r.M, dtype);
+        o.st = make(x, {square ? blocks(r.K) : r.K, blocks(r.M)}, at::kFloat8_e8m0fnu);
+    }
+    return tab_quantize_blocks_launch(x.data_ptr(), type_of(x), r.pitch, r.M, (int)r.K, format, square, o.q.data_ptr(), (r.K + 15) / 16 * 16,
+                                      static_cast<uint8_t*>(o.s.data_ptr()), both ? o.qt.data_ptr() : nullptr, (r.M + 15) / 16 * 16,
+                                      both ? static_cast<uint8_t*>(o.st.data_ptr()) : nullptr, stream_of(x)) == TAB_OK;
+}
+py::object quantized(const Tensor& x, at::ScalarType dtype, bool both, bool square) {
+    Quantized o;
+    bool ok;
+    {
+        py::gil_scoped_release nogil;
+        ok = quantize_any(x, dtype, both, square, o);
+    }
+    if (!ok) return py::none();
+    return both ? py::make_tuple(o.q, o.s, o.qt, o.st) : py::make_tuple(o.q, o.s);
+}
+py::object quantize_blocks(const Tensor& x, at::ScalarType dtype, bool columns) { return quantized(x, dtype, columns, false); }
+py::object quantize_blocks2d(const Tensor& w, at::ScalarType dtype, bool transposed) { return quantized(w, dtype, transposed, true); }
+
+struct Operand {
+    Rows r;
+    int share = 1;
+    int64_t sr = 0, sk = 0;
+    bool of(const Tensor& q, const Tensor& s) {
+        if (!on_cuda(q) || !on_cuda(s) || s.device() != q.device() || format_of(q.scalar_type()) < 0 || s.scalar_type() != at::kFloat8_e8m0fnu || !r.of(q)) return false;
+        if (s.dim() == 0 || s.size(-1) != blocks(r.K)) return false;
+        if (s.dim() == 2) {
+            sr = s.stride(0); sk = s.stride(1);
+        } else if (s.is_contiguous()) {
+            sr = blocks(r.K); sk = 1;
+        } else {
+            return false;
+        }
+        const int64_t rows = s.numel() / blocks(r.K);
+        if (rows != r.M && rows != blocks(r.M)) return false;
+        share = rows == r.M ? 1 : 128;
+        return true;
+    }
+};
+bool matmul_any(const Tensor& a, const Tensor& as, const Tensor& b, const Tensor& bs, at::ScalarType dtype, Tensor& y) {
+    Operand A, B;
+    const int type = type_of(dtype);
+    if (type < 0 || !A.of(a, as) || !B.of(b, bs) || b.dim() != 2 || A.r.K != B.r.K || a.device() != b.device()) return false;
+    const c10::cuda::CUDAGuard guard(a.device());
+    y = make(a, with_last(a, B.r.M), dtype);
+    return tab_matmul_blocks_launch(a.data_ptr(), format_of(a.scalar_type()), A.r.pitch, static_cast<const uint8_t*>(as.data_ptr()), A.share, A.sr, A.sk,
+                                    b.data_ptr(), format_of(b.scalar_type()), B.r.pitch, static_cast<const uint8_t*>(bs.data_ptr()), B.share, B.sr, B.sk,
+                                    y.data_ptr(), type, B.r.M, (int)A.r.M, (int)B.r.M, (int)A.r.K, stream_of(a)) == TAB_OK;
+}
+py::object matmul_blocks(const Tensor& a, const Tensor& as, const Tensor& b, const Tensor& bs, at::ScalarType dtype) {
+    Tensor y;
+    bool ok;
+    {
+        py::gil_scoped_release nogil;
+        ok = matmul_any(a, as, b, bs, dtype, y);
+    }
+    return ok ? py::cast(y) : py::none();
+}
+
+// Gradients of gradients are refused when somebody asks for them, not before.
+void differentiable_once(torch::autograd::variable_list& grads) {
+    if (!at::GradMode::is_enabled()) return;
+    auto error = std::make_shared<torch::autograd::DelayedError>("tab_b200: this operator is differentiable once", 1);
+    for (auto& g : grads)
+        if (g.defined()) g = (*error)({g.detach().requires_grad_()})[0];
+}
+Tensor even_rows(const Tensor& g) {
+    Rows r;
+    return !g.defined() || g.numel() == 0 || r.of(g) ? g : g.contiguous();
+}
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+// nn.block_linear; x and weight have passed quantize_any's conditions, so that only an error of the CUDA runtime is left to report.
+struct BlockLinear : torch::autograd::Function<BlockLinear> {
+    static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, int64_t out_type, int64_t grad_type, bool need_x, bool need_w) {
+        Quantized xq, wq;
+        Tensor y;
+        TORCH_CHECK(quantize_any(x, at::kFloat8_e4m3fn, need_w, false, xq) && quantize_any(weight, at::kFloat8_e4m3fn, need_x, true, wq) &&
+                        matmul_any(xq.q, xq.s, wq.q, wq.s, (at::ScalarType)out_type, y),
+                    "block_linear: a launch failed [cudaError ", tab_last_cuda_error(), ", status ", tab_device_status(), "]");
+        ctx->save_for_backward({xq.qt, xq.st, wq.qt, wq.st});
+        ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), (int64_t)weight.scalar_type(), grad_type};
+        return y;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto saved = ctx->get_saved_variables();
+        const auto types = ctx->saved_data["types"].toIntVector();
+        variable_list out(6);
+        const bool need_w = saved[0].defined(), need_x = saved[2].defined();
+        if (!grads[0].defined() || (!need_x && !need_w)) return out;
+        const Tensor g = even_rows(grads[0].detach());
+        Quantized q;
+        bool ok = quantize_any(g, (at::ScalarType)types[2], need_w, false, q);
+        if (ok && need_x) ok = matmul_any(q.q, q.s, saved[2], saved[3], (at::ScalarType)types[0], out[0]);
+        if (ok && need_w) ok = matmul_any(q.qt, q.st, saved[0], saved[1], (at::ScalarType)types[1], out[1]);
+        TORCH_CHECK(ok, "block_linear: a launch of the backward pass failed [cudaError ", tab_last_cuda_error(), "]");
+        differentiable_once(out);
+        return out;
+    }
+};
+py::object block_linear(const Tensor& x, const Tensor& weight, at::ScalarType out_type, at::ScalarType grad_type) {
+    Tensor y;
+    {
+        py::gil_scoped_release nogil;
+        Rows r, w;
+        if (on_cuda(x) && on_cuda(weight) && x.device() == weight.device() && type_of(x) >= 0 && type_of(weight) >= 0 && type_of(out_type) >= 0 && format_of(grad_type) >= 0 &&
+            weight.dim() == 2 && r.of(x) && w.of(weight) && r.K == w.K) {
+            const bool grad = at::GradMode::is_enabled();
+            y = BlockLinear::apply(x, weight, (int64_t)out_type, (int64_t)grad_type, grad && x.requires_grad(), grad && weight.requires_grad());
+        }
+    }
+    return y.defined() ? py::cast(y) : py::none();
+}
+
+// The inputs of residual_norm as the C ABI takes them; false for anything the interpreter's body has to look at.
+struct Norm {
+    tab_norm_t a = {};
+    Rows r;
+    bool of(const Tensor& y, const Tensor& x, const Tensor& w2, const Tensor& b2, const Tensor& w1, const Tensor& b1, const Tensor& gate, double alpha, int64_t layer, double eps) {
+        if (!on_cuda(y) || type_of(y) < 0 || layer < 0 || layer > 1 || !r.of(y)) return false;
+        a.y = y.data_ptr(); a.ldy = r.pitch; a.type = type_of(y); a.layer = (int)layer; a.alpha = (float)alpha; a.eps = (float)eps; a.M = r.M; a.C = (int)r.K;
+        Rows q;
+        if (x.defined()) {
+            if (!x.is_cuda() || x.device() != y.device() || x.scalar_type() != y.scalar_type() || x.sizes() != y.sizes() || !q.of(x)) return false;
+            a.x = x.data_ptr(); a.ldx = q.pitch;
+        }
+        int ptype = -1;
+        const struct { const Tensor& t; const void** p; } weights[4] = {{w1, &a.w1}, {b1, &a.b1}, {w2, &a.w2}, {b2, &a.b2}};
+        for (const auto& w : weights) {
+            if (!w.t.defined()) continue;
+            const int type = type_of(w.t);
+            if (!w.t.is_cuda() || w.t.device() != y.device() || (type != TAB_FP32 && type != a.type) || w.t.dim() != 1 || w.t.size(0) != r.K || !w.t.is_contiguous() ||
+                (ptype >= 0 && ptype != type)) return false;
+            *w.p = w.t.data_ptr();
+            a.ptype = ptype = type;
+        }
+        if ((a.b1 && !a.w1) || (a.b2 && !a.w2) || (!layer && (a.b1 || a.b2))) return false;
+        if (gate.defined()) {
+            a.gtype = type_of(gate);
+            if (!gate.is_cuda() || gate.device() != y.device() || (a.gtype != TAB_FP32 && a.gtype != a.type)) return false;
+            a.gate = gate.data_ptr();
+            if (gate.dim() == 1 && gate.size(0) == r.K && (gate.is_contiguous() || r.K == 1)) {
+                a.gkind = TAB_GATE_CHANNEL;
+            } else if (gate.dim() == y.dim() && gate.sizes().slice(0, y.dim() - 1) == y.sizes().slice(0, y.dim() - 1) && (gate.size(-1) == 1 || gate.size(-1) == r.K)) {
+                Rows g;
+                if (!g.of(gate)) return false;
+                a.gkind = gate.size(-1) == 1 ? TAB_GATE_TOKEN : TAB_GATE_FULL;
+                a.ldg = g.pitch;
+            } else {
+                return false;
+            }
+        }
+        return true;
+    }
+    bool plain() const { return !a.x && !a.w1 && !a.gate; }                // r is y
+};
+// r (undefined where it is y), h or its blocks, statistics where asked for.
+bool norm_any(Norm& n, const Tensor& y, c10::optional<at::ScalarType> quantize, bool stats, Tensor& r, Tensor& h, Tensor& s, Tensor& st) {
+    const c10::cuda::CUDAGuard guard(y.device());
+    if (!n.plain()) { r = make(y, y.sizes(), y.scalar_type()); n.a.r = r.data_ptr(); n.a.ldr = n.r.K; }
+    if (quantize.has_value()) {
+        n.a.format = format_of(*quantize);
+        if (n.a.format < 0 || !n.a.w2) return false;
+        h = new_blocks(y, y.sizes(), n.r.M, n.r.K, *quantize);
+        s = make(y, with_last(y, blocks(n.r.K)), at::kFloat8_e8m0fnu);
+        n.a.q = h.data_ptr(); n.a.ldq = (n.r.K + 15) / 16 * 16; n.a.s = static_cast<uint8_t*>(s.data_ptr());
+    } else if (n.a.w2) {
+        h = make(y, y.sizes(), y.scalar_type());
+        n.a.h = h.data_ptr(); n.a.ldh = n.r.K;
+    }
+    if (stats) { st = make(y, {n.r.M, 4}, at::kFloat); n.a.stats = st.data_ptr<float>(); }
+    return tab_residual_norm_launch(&n.a, stream_of(y)) == TAB_OK;
+}
+const Tensor& given(const OptTensor& t) {
+    static const Tensor none;
+    return t.has_value() ? *t : none;
+}
+py::object residual_norm(const Tensor& y, const OptTensor& x, const OptTensor& w2, const OptTensor& b2, const OptTensor& w1, const OptTensor& b1, const OptTensor& gate, double alpha,
+                         const std::string& kind, double eps, c10::optional<at::ScalarType> quantize) {
+    Norm n;
+    Tensor r, h, s, st;
+    bool ok;
+    {
+        py::gil_scoped_release nogil;
+        ok = (kind == "rms" || kind == "layer") && n.of(y, given(x), given(w2), given(b2), given(w1), given(b1), given(gate), alpha, kind == "layer", eps) &&
+             norm_any(n, y, quantize, false, r, h, s, st);
+    }
+    if (!ok) return py::none();
+    py::object first = n.plain() ? py::cast(y) : py::cast(r), second = h.defined() ? py::cast(h) : py::none();
+    return quantize.has_value() ? py::make_tuple(first, second, s) : py::make_tuple(first, second);
+}
+
+// nn.residual_norm.  Returns r, then h, those that there are.
+struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
+    static variable_list forward(AutogradContext* ctx, const Tensor& y, const OptTensor& ox, const OptTensor& ow2, const OptTensor& ob2, const OptTensor& ow1, const OptTensor& ob1,
+                                 const OptTensor& ogate, double alpha, int64_t layer, double eps) {
+        const Tensor &x = given(ox), &w2 = given(ow2), &b2 = given(ob2), &w1 = given(ow1), &b1 = given(ob1), &gate = given(ogate);
+        Norm n;
+        Tensor r, h, s, st;
+        TORCH_CHECK(n.of(y, x, w2, b2, w1, b1, gate, alpha, layer, eps) && norm_any(n, y, c10::nullopt, true, r, h, s, st),
+                    "residual_norm: the launch failed [cudaError ", tab_last_cuda_error(), "]");
+        ctx->set_materialize_grads(false);
+        ctx->save_for_backward({y, n.plain() ? Tensor() : r, st, w2, b2, w1, b1, gate});
+        ctx->saved_data["residual"] = x.defined();
+        ctx->saved_data["alpha"] = alpha; ctx->saved_data["layer"] = layer; ctx->saved_data["eps"] = eps;
+        variable_list out;
+        if (r.defined()) out.push_back(r);
+        if (h.defined()) out.push_back(h);
+        return out;
+    }
+    static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        const auto v = ctx->get_saved_variables();
+        const Tensor &y = v[0], &r = v[1], &st = v[2], &w2 = v[3], &b2 = v[4], &w1 = v[5], &b1 = v[6], &gate = v[7];
+        const bool plain = !r.defined(), residual = ctx->saved_data["residual"].toBool();
+        variable_list out(10);
+        const Tensor gr = plain ? Tensor() : even_rows(grads[0].defined() ? grads[0].detach() : grads[0]);
+        const Tensor gh = w2.defined() ? even_rows(grads.back().defined() ? grads.back().detach() : grads.back()) : Tensor();
+        if (!gr.defined() && !gh.defined()) return out;
+        Norm n;
+        bool ok = n.of(y, Tensor(), w2, b2, w1, b1, gate, ctx->saved_data["alpha"].toDouble(), ctx->saved_data["layer"].toInt(), ctx->saved_data["eps"].toDouble());
+        if (ok) {
+            const c10::cuda::CUDAGuard guard(y.device());
+            tab_norm_backward_t b = {};
+            Rows q;
+            n.a.r = const_cast<void*>(static_cast<const void*>((plain ? y : r).data_ptr()));
+            n.a.ldr = plain ? n.r.pitch : n.r.K;
+            n.a.stats = st.data_ptr<float>();
+            b.f = n.a;
+            if (gr.defined()) { ok = ok && q.of(gr); b.gr = gr.data_ptr(); b.ldgr = q.pitch; }
+            q = Rows();
+            if (gh.defined()) { ok = ok && q.of(gh); b.gh = gh.data_ptr(); b.ldgh = q.pitch; }
+            const struct { const Tensor& like; void** p; } grads_of[7] = {{y, &b.dy}, {residual ? y : st, &b.dx}, {w2, &b.dw2}, {b2, &b.db2}, {w1, &b.dw1}, {b1, &b.db1}, {gate, &b.dgate}};
+            bool sums = false;
+            size_t input = 0;                                              // autograd numbers the tensors that there are
+            for (size_t i = 0; i < 7; i++) {
+                if (!grads_of[i].like.defined() || (i == 1 && !residual) || !ctx->needs_input_grad(input++)) continue;
+                out[i] = make(grads_of[i].like, grads_of[i].like.sizes(), grads_of[i].like.scalar_type());
+                *grads_of[i].p = out[i].data_ptr();
+                sums = sums || i > 1;
+            }
+            b.lddy = b.lddx = n.r.K;
+            Tensor partial;
+            if (sums) { partial = make(y, {(int64_t)(tab_residual_norm_workspace_bytes(n.r.M, (int)n.r.K) / 4)}, at::kFloat); b.partial = partial.data_ptr<float>(); }
+            ok = ok && tab_residual_norm_backward_launch(&b, stream_of(y)) == TAB_OK;
+        }
+        TORCH_CHECK(ok, "residual_norm: a launch of the backward pass failed [cudaError ", tab_last_cuda_error(), "]");
+        differentiable_once(out);
+        return out;
+    }
+};
+py::object residual_norm_grad(const Tensor& y, const OptTensor& x, const OptTensor& w2, const OptTensor& b2, const OptTensor& w1, const OptTensor& b1, const OptTensor& gate, double alpha,
+                              const std::string& kind, double eps) {
+    Norm n;
+    variable_list out;
+    bool ok;
+    {
+        py::gil_scoped_release nogil;
+        ok = (kind == "rms" || kind == "layer") && n.of(y, given(x), given(w2), given(b2), given(w1), given(b1), given(gate), alpha, kind == "layer", eps) && (n.a.w2 || !n.plain()) &&
+             n.r.K <= 16384;
+        if (ok) out = ResidualNorm::apply(y, x, w2, b2, w1, b1, gate, alpha, (int64_t)(kind == "layer"), eps);
+    }
+    if (!ok) return py::none();
+    py::object r = n.plain() ? py::cast(y) : py::cast(out[0]), h = n.a.w2 ? py::cast(out.back()) : py::none();
+    return py::make_tuple(r, h);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -206,4 +537,10 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("layer", &layer);
     m.def("pack_weights", &pack_weights);
     m.def("conv2d_packed4", &conv2d_packed4);
+    m.def("quantize_blocks", &quantize_blocks);
+    m.def("quantize_blocks2d", &quantize_blocks2d);
+    m.def("matmul_blocks", &matmul_blocks);
+    m.def("residual_norm", &residual_norm);
+    m.def("block_linear", &block_linear);
+    m.def("residual_norm_grad", &residual_norm_grad);
 }

@@ -201,6 +201,14 @@ def _even_rows(g):
         return g.contiguous()
 
 
+def _differentiable_once(grads):
+    """Gradients of gradients are refused when somebody asks for them, not before."""
+    if not torch.is_grad_enabled():
+        return grads
+    error = torch._C._functions.DelayedError(b"tab_b200: this operator is differentiable once", 1)
+    return tuple(None if g is None else error(g.detach().requires_grad_()) for g in grads)
+
+
 class _BlockLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, out_dtype, grad_dtype):
@@ -213,13 +221,12 @@ class _BlockLinear(torch.autograd.Function):
         return ops.matmul_blocks(*xq[:2], *wq[:2], out_dtype=out_dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
         xt, xts, wt, wts = ctx.saved_tensors
-        g = ops.quantize_blocks(_even_rows(grad), ctx.grad_dtype, columns=xt is not None)
+        g = ops.quantize_blocks(_even_rows(grad.detach()), ctx.grad_dtype, columns=xt is not None)
         dx = None if wt is None else ops.matmul_blocks(*g[:2], wt, wts, out_dtype=ctx.types[0])
         dw = None if xt is None else ops.matmul_blocks(*g[2:], xt, xts, out_dtype=ctx.types[1])
-        return dx, dw, None, None
+        return *_differentiable_once((dx, dw)), None, None
 
 
 def block_linear(x, weight, out_dtype=None, grad_dtype=torch.float8_e4m3fn):
@@ -229,7 +236,9 @@ def block_linear(x, weight, out_dtype=None, grad_dtype=torch.float8_e4m3fn):
     Its gradients are products of the same kind, with the gradient ``g`` of the result rounded to ``grad_dtype``: ``g`` (along its rows) times the
     rounded weights for ``x``, and ``g`` and ``x`` (both along their columns, i.e. over the rows that this product sums) for ``weight``, in the
     types of ``x`` and ``weight``.  The rounding itself counts as the identity.  For the backward pass 8-bit copies are kept, not ``x`` and ``weight``."""
-    return _BlockLinear.apply(x, weight, x.dtype if out_dtype is None else out_dtype, grad_dtype)
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    y = ops._try("block_linear", x, weight, out_dtype, grad_dtype)
+    return _BlockLinear.apply(x, weight, out_dtype, grad_dtype) if y is None else y
 
 
 class BlockLinear(torch.nn.Module):
@@ -279,20 +288,22 @@ class _ResidualNorm(torch.autograd.Function):
         return (None if plain else r), h
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, gr, gh):
         y, r, stats, *weights = ctx.saved_tensors
         wanted = {n for n, need in zip(_NORM_TENSORS, ctx.needs_input_grad) if need}
         if (gr is None and gh is None) or not wanted:
             return (None,) * 10
-        gr, gh = (None if g is None else _even_rows(g) for g in (gr, gh))
+        gr, gh = (None if g is None else _even_rows(g.detach()) for g in (gr, gh))
         out = ops.residual_norm_backward(gr, gh, y, y if ctx.plain else r, stats, ctx.has_residual, *weights, *ctx.args, wanted)
-        return tuple(out.get(n) for n in _NORM_TENSORS) + (None, None, None)
+        return *_differentiable_once(tuple(out.get(n) for n in _NORM_TENSORS)), None, None, None
 
 
 def residual_norm(y, residual=None, pre_weight=None, pre_bias=None, post_weight=None, post_bias=None, gate=None, residual_scale=1.0,
                   kind="rms", eps=1e-6):
     """``ops.residual_norm`` with gradients: returns ``(r, h)``.  Gradients go to ``y``, ``residual``, the weights, the biases and the gate;
     that of a weight or of a gate ``[C]`` is summed over the rows in a fixed order, so that the same inputs give the same bits."""
+    done = ops._try("residual_norm_grad", y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps)
+    if done is not None:
+        return done
     r, h = _ResidualNorm.apply(y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps)
     return (y if r is None else r), h

@@ -336,3 +336,40 @@ def test_block_linear_module(cuda):
     assert torch.equal(other(x), want)
     with pytest.raises(ValueError, match="300"):
         m(x[..., :128])
+
+
+@pytest.mark.gpu
+def test_both_bodies_agree(cuda, monkeypatch):
+    """The native bodies and those behind them (taken where the extension is missing): the same bits, values and gradients."""
+    x, w = torch.randn(3, 45, 300, device=cuda, dtype=torch.bfloat16), torch.randn(130, 300, device=cuda)
+    p, gate = torch.rand(300, device=cuda), torch.rand(3, 45, 1, device=cuda)
+
+    def everything():
+        out = [*TAB.quantize_blocks(x, columns=True), *TAB.quantize_blocks2d(w, torch.float8_e5m2, transposed=True)]
+        out += [TAB.matmul_blocks(*out[:2], *out[4:6]), *TAB.residual_norm(x, x, pre_weight=p, post_weight=p, gate=gate, quantize=torch.float8_e4m3fn)]
+        for plain in (False, True):
+            leaves = [t.clone().requires_grad_() for t in (x, w, p, gate)]
+            r, h = tab_nn.residual_norm(leaves[0], pre_weight=leaves[2]) if plain else tab_nn.residual_norm(leaves[0], x, pre_weight=leaves[2], post_weight=p, gate=leaves[3], residual_scale=0.5)
+            y = tab_nn.block_linear(h, leaves[1])
+            grads = torch.autograd.grad((y, r), leaves[:3 if plain else 4], (torch.ones_like(y), torch.ones_like(r)))
+            out += [y.detach(), *grads]
+        return [t.view(torch.uint8) if t.dtype.itemsize == 1 else t for t in out]
+
+    if not TAB.ops._host():
+        pytest.fail("the native bodies are not built")
+    native = everything()
+    monkeypatch.setattr(TAB.ops, "_native", False)
+    for a, b in zip(native, everything()):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_second_derivatives_are_refused(cuda, monkeypatch, native):
+    if not native:
+        monkeypatch.setattr(TAB.ops, "_native", False)
+    x, w, p = (torch.randn(*s, device=cuda, requires_grad=True) for s in ((4, 128), (16, 128), (128,)))
+    for y in (tab_nn.block_linear(x, w), tab_nn.residual_norm(x, pre_weight=p)[1]):
+        g, = torch.autograd.grad(y.sum(), x, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable"):
+            g.sum().backward()
