@@ -308,7 +308,7 @@ int tab_quantize_blocks_launch(const void* x, int type, long long ldx, long long
  * a [M][K], b [N][K] as tab_quantize_blocks_launch writes them: 16-byte aligned, pitches lda, ldb bytes, multiples of 16 (of which a
  * single row needs none).  The scale of (row, block) is at as[(row / a_share) * a_row + block * a_block]; share is 1 (blocks of a
  * row) or 128 (squares).  y [M][N], row pitch ldy elements.  tcgen05 kind::mxf8f6f4 applies the scales; waits inside the kernel are
- * bounded as described at tab_device_status (codes 31-39).  K == 0 gives zeros.
+ * bounded as described at tab_device_status (codes 31-41), which the sum's length must not outlast: K <= 2^24.  K == 0 gives zeros.
  */
 int tab_matmul_blocks_launch(const void* a, int a_format, long long lda, const uint8_t* as, int a_share, long long a_row, long long a_block,
                              const void* b, int b_format, long long ldb, const uint8_t* bs, int b_share, long long b_row, long long b_block,

@@ -435,7 +435,7 @@ int tab_matmul_blocks_launch(const void* a, int a_format, long long lda, const u
     }
     if (!a || !b || !as || !bs) return TAB_E_NULL_POINTER;
     if (misaligned(a, 15) || misaligned(b, 15) || lda % 16 || ldb % 16) return TAB_E_ALIGNMENT;
-    if (lda >= (1LL << 40) || ldb >= (1LL << 40) || K > 0x7FFFFF00 || M > 0x7FFFFF00 || N > 0x7FFFFF00) return TAB_E_TOO_LARGE;
+    if (lda >= (1LL << 40) || ldb >= (1LL << 40) || K > (1 << 24) || M > 0x7FFFFF00 || N > 0x7FFFFF00) return TAB_E_TOO_LARGE;
     MatmulBlocksParams p = {{static_cast<const uint8_t*>(a), lda, as, a_row, a_block, a_share == 128 ? 7 : 0, M, a_format},
                             {static_cast<const uint8_t*>(b), ldb, bs, b_row, b_block, b_share == 128 ? 7 : 0, N, b_format}, y, ldy, type, K};
     return matmul_blocks_dispatch(p, stm);

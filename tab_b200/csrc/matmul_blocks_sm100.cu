@@ -41,22 +41,48 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-// Scale words (4 blocks from kb on, 127 = 2^0 where there is no block or row) of rows lane, lane + 32, lane + 64, lane + 96 of the 128
-// from row0 on.  Only blocks below kb1 are read.
-__device__ __forceinline__ uint4 load_scales(const BlocksOperand& o, int row0, int kb, int kb1, int lane) {
-    uint32_t w[4];
+// The scales of 16 blocks from kb on (127 = 2^0 where there is no block or row) of row lane, lane + 32, lane + 64 or lane + 96 of the 128
+// from row0 on, four blocks to a word.  Only blocks below kb1 are read.  A load from memory takes longer than the MMAs of four blocks
+// when the operands' copies fill the memory system, so 16 blocks are asked for at a time, as one vector where the layout allows.
+// packed: 16 or 4 scales of a row, from a multiple of so many on, are one aligned vector or word; 1: bytes of any stride.
+__device__ __forceinline__ int scale_packing(const BlocksOperand& o, int kb0) {
+    if (o.sk != 1) return 1;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(o.s) | (uintptr_t)o.sr | (uintptr_t)kb0;
+    return (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 1;
+}
+__device__ __forceinline__ void load_scales(const BlocksOperand& o, int packed, int row0, int kb, int kb1, int lane, uint4 (&w)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         if (i > 0 && o.shift) { w[i] = w[0]; continue; }                   // one scale for all 128 rows
         const int row = row0 + i * 32 + lane;
-        const bool in = (o.shift ? row0 : row) < o.rows;
+        w[i] = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
+        if ((o.shift ? row0 : row) >= o.rows) continue;
         const uint8_t* s = o.s + (long long)(o.shift ? row0 >> o.shift : row) * o.sr + (long long)kb * o.sk;
-        uint32_t v = 0;
+        if (packed == 16 && kb + 16 <= kb1) {
+            w[i] = *reinterpret_cast<const uint4*>(s);
+            continue;
+        }
+        uint32_t v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) v |= (in && kb + j < kb1 ? (uint32_t)s[j * o.sk] : 127u) << (8 * j);
-        w[i] = v;
+        for (int j = 0; j < 4; j++) {
+            v[j] = 0x7F7F7F7Fu;
+            if (packed >= 4 && kb + 4 * j + 4 <= kb1) {
+                v[j] = reinterpret_cast<const uint32_t*>(s)[j];
+            } else if (kb + 4 * j < kb1) {
+                v[j] = 0;
+#pragma unroll
+                for (int b = 0; b < 4; b++) v[j] |= (kb + 4 * j + b < kb1 ? (uint32_t)s[(4 * j + b) * o.sk] : 127u) << (8 * b);
+            }
+        }
+        w[i] = make_uint4(v[0], v[1], v[2], v[3]);
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// Word j of the four vectors, as the tensor memory wants it.
+__device__ __forceinline__ void store_scales(uint32_t at, const uint4 (&w)[4], int j) {
+    if (j == 0) sts_v4(at, w[0].x, w[1].x, w[2].x, w[3].x);
+    else if (j == 1) sts_v4(at, w[0].y, w[1].y, w[2].y, w[3].y);
+    else if (j == 2) sts_v4(at, w[0].z, w[1].z, w[2].z, w[3].z);
+    else sts_v4(at, w[0].w, w[1].w, w[2].w, w[3].w);
 }
 
 // 32 accumulators of a row (columns c0 .. c0+31 of ncols) to row-major memory.
@@ -159,25 +185,35 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
         }
         (void)dead;
     } else if (warp == 2) {
-        const int groups = (kb1 - kb0 + 3) / 4;
-        uint4 wr, wc[CG];
-        auto fetch = [&](int q) {
-            wr = load_scales(R, r0, kb0 + 4 * q, kb1, lane);
+        const int rpack = scale_packing(R, kb0), cpack = scale_packing(C, kb0);
+        uint4 w[1 + CG][4];
+        auto fetch = [&](int kb) {
+            load_scales(R, rpack, r0, kb, kb1, lane, w[0]);
 #pragma unroll
-            for (int i = 0; i < CG; i++) wc[i] = load_scales(C, c0 + 128 * i, kb0 + 4 * q, kb1, lane);
+            for (int i = 0; i < CG; i++) load_scales(C, cpack, c0 + 128 * i, kb, kb1, lane, w[1 + i]);
         };
-        if (groups > 0) fetch(0);
-        for (int q = 0; q < groups; q++) {
-            const int slot = q % SF_SLOTS;
-            if (q >= SF_SLOTS && !mbar_wait_warp(sfEmpty + 8 * slot, (q / SF_SLOTS - 1) & 1)) { expire(34); break; }
-            const uint32_t at = sSF + slot * SFB + lane * 16;
-            sts_v4(at, wr.x, wr.y, wr.z, wr.w);
+        if (kb0 < kb1) fetch(kb0);
+        bool dead = false;
+        int q = 0;
+        for (int kb = kb0; kb < kb1 && !dead; kb += 16) {
+            uint4 now[1 + CG][4];
 #pragma unroll
-            for (int i = 0; i < CG; i++) sts_v4(at + 512 * (1 + i), wc[i].x, wc[i].y, wc[i].z, wc[i].w);
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(sfFull + 8 * slot);
-            if (q + 1 < groups) fetch(q + 1);
+            for (int i = 0; i < 1 + CG; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) now[i][k] = w[i][k];
+            if (kb + 16 < kb1) fetch(kb + 16);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (kb + 4 * j >= kb1 || dead) continue;
+                const int slot = q % SF_SLOTS;
+                if (q >= SF_SLOTS && !mbar_wait_warp(sfEmpty + 8 * slot, (q / SF_SLOTS - 1) & 1)) { expire(34); dead = true; continue; }
+#pragma unroll
+                for (int i = 0; i < 1 + CG; i++) store_scales(sSF + slot * SFB + lane * 16 + 512 * i, now[i], j);
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(sfFull + 8 * slot);
+                q++;
+            }
         }
     }
     __syncwarp();
@@ -243,6 +279,201 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
     if (warp == 1) tmem_dealloc(tmem, TCOLS);
 }
 
+// ---- CTA pairs ----------------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ void umma_f8_pair(uint32_t tmem_d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t sfa, uint32_t sfb, uint32_t accumulate) {
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "setp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.block32 [%0], %1, %2, %3, [%5], [%6], p;\n\t}"
+                 :: "r"(tmem_d), "l"(da), "l"(db), "r"(idesc), "r"(accumulate), "r"(sfa), "r"(sfb) : "memory");
+}
+// The same 512 bytes of both CTAs' shared memory to the same columns of both tensor memories.
+__device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint32_t smem_addr) {
+    const uint64_t d = ((uint64_t)((128u >> 4) | (1u << 14)) << 32) | ((smem_addr & 0x3FFFFu) >> 4);
+    asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
+}
+
+static constexpr int PT = 384;                           // threads of a pair's CTA: copies, MMAs, scales, -, eight that finish
+static constexpr int PSTAGES = 6;                        // of 128 terms: 128 rows of a and 128 of b, 32 KB
+static constexpr int PSTAGE = 32768;
+static constexpr int PSF = 1536;                         // scale words of 512 terms: 128 rows of a, 256 of b
+static constexpr int PACC = 224;                         // second accumulator's first column: it shares 32 with the first
+static constexpr int PSFCOL = 480;
+static constexpr int PSMEM = PSTAGES * PSTAGE + SF_SLOTS * PSF + 1024;
+
+// A persistent pair of CTAs works 256 x 256 tiles: each CTA holds 128 rows of a and of b, and one MMA stream, issued by the even CTA,
+// multiplies for both; each CTA's tensor memory receives the sums of its own 128 rows of a and all 256 of b.  Two accumulators, so
+// that a tile's sums leave while the next tile's are made: 512 columns hold two of 256 and the scales only if the accumulators share
+// some, here 32, which the finishing warps read first and release; from there on the next tile's MMAs may run.
+// group: tiles are taken in bands of so many row blocks, column by column, so that what is in work at a time shares its operands in the L2.
+template <int TYPE>
+__global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, BlocksOperand A, BlocksOperand B,
+                                                               void* yv, long long ldy, int KB, int tiles_m, int tiles_n, int group, int vec, int* status) {
+    using T = typename ElemOf<TYPE>::type;
+    extern __shared__ uint8_t raw[];
+    __shared__ __align__(8) uint64_t bars[2 * PSTAGES + 2 * SF_SLOTS + 3];
+    __shared__ uint32_t tslot;
+    __shared__ int dead_flag;
+    volatile int* deadp = &dead_flag;
+    const uint32_t sRing = ((uint32_t)__cvta_generic_to_shared(raw) + 1023u) & ~1023u, sSF = sRing + PSTAGES * PSTAGE;
+    const uint32_t full = (uint32_t)__cvta_generic_to_shared(bars), empty = full + 8 * PSTAGES, sfFull = empty + 8 * PSTAGES, sfEmpty = sfFull + 8 * SF_SLOTS,
+                   accFull = sfEmpty + 8 * SF_SLOTS, accFree = accFull + 16;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = cluster_ctarank();
+    const int pair0 = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1), ntiles = tiles_m * tiles_n;
+
+    if (tid == 0) {
+        *deadp = 0;
+        for (int s = 0; s < PSTAGES; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
+        for (int s = 0; s < SF_SLOTS; s++) { mbar_init(sfFull + 8 * s, 2); mbar_init(sfEmpty + 8 * s, 1); }
+        mbar_init(accFull, 1); mbar_init(accFull + 8, 1); mbar_init(accFree, 16);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 1) tmem_alloc_pair((uint32_t)__cvta_generic_to_shared(&tslot), 512);
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();                                                    // both CTAs' barriers exist before either arrives on the other's
+    tc_fence_after();
+    const uint32_t tmem = *static_cast<volatile uint32_t*>(&tslot);
+    pdl_wait();
+    auto expire = [&](int code) { if (lane == 0) { if (status) atomicExch(status, code); *deadp = 1; } };
+    auto tile_at = [&](int t, int& m0, int& n0) {
+        const int band = t / (group * tiles_n), first = band * group, rows = min(group, tiles_m - first), i = t - first * tiles_n;
+        m0 = (first + i % rows) * 256;
+        n0 = i / rows * 256;
+    };
+
+    if (warp == 0) {
+        int g = 0;
+        bool dead = false;
+        for (int t = pair0; t < ntiles && !dead; t += pairs) {
+            int m0, n0;
+            tile_at(t, m0, n0);
+            m0 += (int)rank * 128; n0 += (int)rank * 128;
+            for (int kb = 0; kb < KB; kb++, g++) {
+                const int s = g % PSTAGES;
+                if (g >= PSTAGES && !mbar_wait_cluster_warp(empty + 8 * s, (g / PSTAGES - 1) & 1)) { expire(36); dead = true; break; }
+                if (elect_one()) {
+                    if (rank == 0) mbar_expect_tx(full + 8 * s, 2 * PSTAGE);   // both CTAs' copies are counted on the even one's barrier
+                    tma_load_2d_pair(sRing + s * PSTAGE, &tmA, kb * BLK, m0, full + 8 * s);
+                    tma_load_2d_pair(sRing + s * PSTAGE + 16384, &tmB, kb * BLK, n0, full + 8 * s);
+                }
+                __syncwarp();
+            }
+        }
+    } else if (warp == 1 && rank == 0) {
+        const uint32_t idesc = umma_idesc_f8(256, 256, A.format == TAB_E5M2, B.format == TAB_E5M2);
+        int g = 0, q = 0, a = 0;
+        bool dead = false;
+        for (int t = pair0; t < ntiles && !dead; t += pairs, a++) {
+            const uint32_t d = tmem + (a & 1) * PACC;
+            if (a >= 1 && !mbar_wait_cluster_warp(accFree, (a - 1) & 1)) { expire(37); break; }
+            tc_fence_after();
+            for (int kb = 0; kb < KB; kb++, g++) {
+                const int s = g % PSTAGES, j = kb & 3;
+                const uint32_t sfcol = tmem + PSFCOL + (q & 1) * 12;
+                if (j == 0) {
+                    const int slot = q % SF_SLOTS;
+                    if (!mbar_wait_cluster_warp(sfFull + 8 * slot, (q / SF_SLOTS) & 1)) { expire(38); dead = true; break; }
+                    tc_fence_after();
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < 3; i++) tmem_copy_scales_pair(sfcol + 4 * i, sSF + slot * PSF + 512 * i);
+                        umma_commit_pair(sfEmpty + 8 * slot);
+                    }
+                    __syncwarp();
+                }
+                if (!mbar_wait_cluster_warp(full + 8 * s, (g / PSTAGES) & 1)) { expire(39); dead = true; break; }
+                tc_fence_after();
+                if (elect_one()) {
+                    const uint64_t da = umma_desc(sRing + s * PSTAGE), db = umma_desc(sRing + s * PSTAGE + 16384);
+                    const uint32_t id = with_scale_byte(idesc, j);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) umma_f8_pair(d, da + 2 * i, db + 2 * i, id, sfcol, sfcol + 4, (kb | i) != 0);
+                    umma_commit_pair(empty + 8 * s);
+                    if (kb == KB - 1) umma_commit_pair(accFull + 8 * (a & 1));
+                }
+                __syncwarp();
+                if (j == 3 || kb == KB - 1) q++;
+            }
+        }
+    } else if (warp == 2) {
+        const int apack = scale_packing(A, 0), bpack = scale_packing(B, 0);
+        int t = pair0, kb = 0, m0 = 0, n0 = 0, q = 0;
+        uint4 w[3][4];
+        auto fetch = [&]() {
+            load_scales(A, apack, m0 + (int)rank * 128, kb, KB, lane, w[0]);
+            load_scales(B, bpack, n0, kb, KB, lane, w[1]);
+            load_scales(B, bpack, n0 + 128, kb, KB, lane, w[2]);
+        };
+        if (t < ntiles) { tile_at(t, m0, n0); fetch(); }
+        bool dead = false;
+        while (t < ntiles && !dead) {
+            uint4 now[3][4];
+#pragma unroll
+            for (int i = 0; i < 3; i++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) now[i][k] = w[i][k];
+            const int left = KB - kb;
+            kb += 16;
+            if (kb >= KB) { kb = 0; t += pairs; if (t < ntiles) tile_at(t, m0, n0); }
+            if (t < ntiles) fetch();
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (4 * j >= left || dead) continue;
+                const int slot = q % SF_SLOTS;
+                if (q >= SF_SLOTS && !mbar_wait_cluster_warp(sfEmpty + 8 * slot, (q / SF_SLOTS - 1) & 1)) { expire(40); dead = true; continue; }
+#pragma unroll
+                for (int i = 0; i < 3; i++) store_scales(sSF + slot * PSF + lane * 16 + 512 * i, now[i], j);
+                fence_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive_cluster(sfFull + 8 * slot, 0u);
+                q++;
+            }
+        }
+    } else if (warp >= 4) {
+        T* y = static_cast<T*>(yv);
+        const int quarter = (warp & 3) * 32, half = (warp - 4) >> 2;
+        int a = 0;
+        for (int t = pair0; t < ntiles; t += pairs, a++) {
+            int m0, n0;
+            tile_at(t, m0, n0);
+            const int row = m0 + (int)rank * 128 + quarter + lane;
+            if (!mbar_wait_cluster_warp(accFull + 8 * (a & 1), (a >> 1) & 1)) { expire(41); break; }
+            tc_fence_after();
+            // the shared columns: the last 32 of the first accumulator, the first 32 of the second
+            const bool shares = half == ((a & 1) ^ 1);
+            const uint32_t taddr = tmem + (a & 1) * PACC + half * 128 + ((uint32_t)quarter << 16);
+            if (!shares && lane == 0) mbar_arrive_cluster(accFree, 0u);
+#pragma unroll 1
+            for (int i = 0; i < 4; i++) {
+                const int cb = (half ? 3 - i : i) * 32;
+                uint32_t v[32];
+                tmem_ld32(taddr + cb, v);
+                if (shares && i == 0) {
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_cluster(accFree, 0u);
+                }
+                float o[32];
+#pragma unroll
+                for (int j = 0; j < 32; j++) o[j] = __uint_as_float(v[j]);
+                if (row < A.rows) store_row32(y + (long long)row * ldy, n0 + half * 128 + cb, B.rows, vec, o);
+            }
+            tc_fence_before();
+            __syncwarp();
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (*deadp != 0) {
+        for (int i = 0; i < 200; i++) __nanosleep(1000);                   // see the tile kernel
+        __syncthreads();
+    }
+    cluster_sync_all();                                                    // the other CTA neither reads this one's memory nor arrives on its barriers any more
+    pdl_launch_dependents();
+    if (warp == 1) tmem_dealloc_pair(tmem, 512);
+}
+
 // ---- host side ----------------------------------------------------------------------------------------------------------------
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -302,9 +533,50 @@ static int launch_tile(const MatmulBlocksParams& p, const BlocksPlan& pl, int* s
                          (int)tiles_c, pl.split, vec, status);
 }
 
+// How many pairs the device holds at once (0: none), asked of the occupancy calculator once per device.
+static int matmul_pairs() {
+    static std::mutex mu;
+    static int known[64] = {};                                             // 0 unknown, else pairs + 1
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    std::lock_guard<std::mutex> lock(mu);
+    if (!known[dev]) {
+        int clusters = 0;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(2); cfg.blockDim = dim3(PT); cfg.dynamicSmemBytes = PSMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = 2; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr; cfg.numAttrs = 1;
+        bool ok = true;
+        for (auto kernel : {matmul_blocks_pair_kernel<TAB_FP32>, matmul_blocks_pair_kernel<TAB_BF16>, matmul_blocks_pair_kernel<TAB_FP16>})
+            ok = ok && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PSMEM) == cudaSuccess &&
+                 cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters >= 1;
+        if (!ok) cudaGetLastError();
+        known[dev] = ok ? clusters + 1 : 1;
+    }
+    return known[dev] - 1;
+}
+
+static int launch_pair(const MatmulBlocksParams& p, int pairs, int* status, cudaStream_t stream) {
+    alignas(64) CUtensorMap tmA, tmB;
+    if (!blocks_map(&tmA, p.a, p.K, 128) || !blocks_map(&tmB, p.b, p.K, 128)) return TAB_E_TOO_LARGE;
+    const long long tiles_m = ((long long)p.a.rows + 255) / 256, tiles_n = ((long long)p.b.rows + 255) / 256, ntiles = tiles_m * tiles_n;
+    if (ntiles >= (1LL << 30)) return TAB_E_TOO_LARGE;
+    const int size = type_bytes(p.type);
+    const int vec = !(reinterpret_cast<uintptr_t>(p.y) & (8 * size - 1)) && p.ldy % 8 == 0;
+    const unsigned grid = 2u * (unsigned)std::min<long long>(ntiles, pairs);
+    snprintf(g_last_blocks_kernel, sizeof(g_last_blocks_kernel), "matmul_blocks_pair_kernel");
+    auto kernel = p.type == TAB_FP32 ? matmul_blocks_pair_kernel<TAB_FP32> : p.type == TAB_BF16 ? matmul_blocks_pair_kernel<TAB_BF16> : matmul_blocks_pair_kernel<TAB_FP16>;
+    return launch_pdl_as(false, 2u, kernel, dim3(grid), dim3(PT), (size_t)PSMEM, stream, tmA, tmB, p.a, p.b, p.y, p.ldy, blocks_of(p.K), (int)tiles_m, (int)tiles_n, 8, vec, status);
+}
+
 int matmul_blocks_dispatch(const MatmulBlocksParams& p, cudaStream_t stream) {
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
+    const long long tiles = ((long long)p.a.rows + 255) / 256 * (((long long)p.b.rows + 255) / 256);
+    const int pairs = matmul_pairs();
+    if (pairs > 0 && tiles * 2 > pairs) return launch_pair(p, pairs, status, stream);
     BlocksPlan pl = {128, false, 1, blocks_of(p.K), 6};
 #define TAB_MB(BN, SW) (p.type == TAB_FP32 ? launch_tile<BN, SW, TAB_FP32>(p, pl, status, stream) : p.type == TAB_BF16 ? launch_tile<BN, SW, TAB_BF16>(p, pl, status, stream) \
                                                                                                                      : launch_tile<BN, SW, TAB_FP16>(p, pl, status, stream))
