@@ -98,7 +98,7 @@ __device__ __forceinline__ void store_row32(T* y, int c0, int ncols, bool vec, c
 }
 
 static constexpr int TT = 256;                           // threads of a tile CTA
-static constexpr int SF_SLOTS = 4;                       // scale words of 512 terms each, in shared memory
+static constexpr int SF_SLOTS = 3;                       // of scale words of 16 blocks, in shared memory
 
 // One CTA: 128 rows of operand R times BN rows of operand C over this rank's share of the sum.  Warp 0 copies the operands, warp 1
 // issues the MMAs, warp 2 brings the scales, warps 4-7 finish.  A cluster shares out the sum: rank r of S takes blocks
@@ -111,11 +111,11 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
     extern __shared__ uint8_t raw[];
     constexpr int STAGE = (128 + BN) * 128;
     constexpr int CG = (BN + 127) / 128;                                   // groups of 128 rows of C
-    constexpr int SFB = 512 * (1 + CG);                                    // bytes of a slot of scales
+    constexpr int SFB = 512 * (1 + CG);                                    // bytes of four blocks' scales; a slot holds four of them
     constexpr int SFCOL = BN < 32 ? 32 : BN;                               // first tensor-memory column of the scales: two slots
     constexpr int TCOLS = SFCOL + 8 * (1 + CG) <= 64 ? 64 : SFCOL + 8 * (1 + CG) <= 128 ? 128 : SFCOL + 8 * (1 + CG) <= 256 ? 256 : 512;
     __shared__ __align__(8) uint64_t bars[16 + 2 * SF_SLOTS + 1];
-    __shared__ __align__(512) uint8_t sf[SF_SLOTS * SFB];
+    __shared__ __align__(512) uint8_t sf[SF_SLOTS * 4 * SFB];
     __shared__ uint32_t tslot;
     __shared__ int dead_flag;
     volatile int* deadp = &dead_flag;
@@ -156,22 +156,22 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
         }
     } else if (warp == 1) {
         const uint32_t idesc = umma_idesc_f8(128, BN, R.format == TAB_E5M2, C.format == TAB_E5M2);
-        bool dead = false;
         for (int kb = kb0, g = 0; kb < kb1; kb++, g++) {
-            const int s = g % nst, q = g >> 2, j = g & 3;
-            const uint32_t sfcol = tmem + SFCOL + (q & 1) * 4 * (1 + CG);
-            if (j == 0) {
-                const int slot = q % SF_SLOTS;
-                if (!mbar_wait_warp(sfFull + 8 * slot, (q / SF_SLOTS) & 1)) { expire(32); dead = true; break; }
+            const int s = g % nst, j = g & 3, q = g >> 4, slot = q % SF_SLOTS;
+            const uint32_t sfcol = tmem + SFCOL + ((g >> 2) & 1) * 4 * (1 + CG);
+            if ((g & 15) == 0) {
+                if (!mbar_wait_warp(sfFull + 8 * slot, (q / SF_SLOTS) & 1)) { expire(32); break; }
                 tc_fence_after();
+            }
+            if (j == 0) {
                 if (elect_one()) {
 #pragma unroll
-                    for (int i = 0; i < 1 + CG; i++) tmem_copy_scales(sfcol + 4 * i, sSF + slot * SFB + 512 * i);
-                    umma_commit(sfEmpty + 8 * slot);
+                    for (int i = 0; i < 1 + CG; i++) tmem_copy_scales(sfcol + 4 * i, sSF + (slot * 4 + ((g >> 2) & 3)) * SFB + 512 * i);
+                    if ((g & 12) == 12 || kb + 4 >= kb1) umma_commit(sfEmpty + 8 * slot);
                 }
                 __syncwarp();
             }
-            if (!mbar_wait_warp(full + 8 * s, (g / nst) & 1)) { expire(33); dead = true; break; }
+            if (!mbar_wait_warp(full + 8 * s, (g / nst) & 1)) { expire(33); break; }
             tc_fence_after();
             if (elect_one()) {
                 const uint64_t da = umma_desc(sRing + s * STAGE), db = umma_desc(sRing + s * STAGE + 128 * 128);
@@ -183,37 +183,22 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
             }
             __syncwarp();
         }
-        (void)dead;
     } else if (warp == 2) {
         const int rpack = scale_packing(R, kb0), cpack = scale_packing(C, kb0);
-        uint4 w[1 + CG][4];
-        auto fetch = [&](int kb) {
+        for (int kb = kb0, q = 0; kb < kb1; kb += 16, q++) {
+            uint4 w[1 + CG][4];
             load_scales(R, rpack, r0, kb, kb1, lane, w[0]);
 #pragma unroll
             for (int i = 0; i < CG; i++) load_scales(C, cpack, c0 + 128 * i, kb, kb1, lane, w[1 + i]);
-        };
-        if (kb0 < kb1) fetch(kb0);
-        bool dead = false;
-        int q = 0;
-        for (int kb = kb0; kb < kb1 && !dead; kb += 16) {
-            uint4 now[1 + CG][4];
+            const int slot = q % SF_SLOTS;
+            if (q >= SF_SLOTS && !mbar_wait_warp(sfEmpty + 8 * slot, (q / SF_SLOTS - 1) & 1)) { expire(34); break; }
 #pragma unroll
-            for (int i = 0; i < 1 + CG; i++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) now[i][k] = w[i][k];
-            if (kb + 16 < kb1) fetch(kb + 16);
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (kb + 4 * j >= kb1 || dead) continue;
-                const int slot = q % SF_SLOTS;
-                if (q >= SF_SLOTS && !mbar_wait_warp(sfEmpty + 8 * slot, (q / SF_SLOTS - 1) & 1)) { expire(34); dead = true; continue; }
-#pragma unroll
-                for (int i = 0; i < 1 + CG; i++) store_scales(sSF + slot * SFB + lane * 16 + 512 * i, now[i], j);
-                fence_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(sfFull + 8 * slot);
-                q++;
-            }
+                for (int i = 0; i < 1 + CG; i++) store_scales(sSF + (slot * 4 + j) * SFB + lane * 16 + 512 * i, w[i], j);
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(sfFull + 8 * slot);
         }
     }
     __syncwarp();
@@ -295,10 +280,10 @@ __device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint32_t s
 static constexpr int PT = 384;                           // threads of a pair's CTA: copies, MMAs, scales, -, eight that finish
 static constexpr int PSTAGES = 6;                        // of 128 terms: 128 rows of a and 128 of b, 32 KB
 static constexpr int PSTAGE = 32768;
-static constexpr int PSF = 1536;                         // scale words of 512 terms: 128 rows of a, 256 of b
+static constexpr int PSF = 1536;                         // scale words of 512 terms: 128 rows of a, 256 of b; a slot holds four of them
 static constexpr int PACC = 224;                         // second accumulator's first column: it shares 32 with the first
 static constexpr int PSFCOL = 480;
-static constexpr int PSMEM = PSTAGES * PSTAGE + SF_SLOTS * PSF + 1024;
+static constexpr int PSMEM = PSTAGES * PSTAGE + SF_SLOTS * 4 * PSF + 1024;
 
 // A persistent pair of CTAs works 256 x 256 tiles: each CTA holds 128 rows of a and of b, and one MMA stream, issued by the even CTA,
 // multiplies for both; each CTA's tensor memory receives the sums of its own 128 rows of a and all 256 of b.  Two accumulators, so
@@ -369,18 +354,20 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
             if (a >= 1 && !mbar_wait_cluster_warp(accFree, (a - 1) & 1)) { expire(37); break; }
             tc_fence_after();
             for (int kb = 0; kb < KB; kb++, g++) {
-                const int s = g % PSTAGES, j = kb & 3;
-                const uint32_t sfcol = tmem + PSFCOL + (q & 1) * 12;
-                if (j == 0) {
-                    const int slot = q % SF_SLOTS;
+                const int s = g % PSTAGES, j = kb & 3, slot = q % SF_SLOTS;
+                const uint32_t sfcol = tmem + PSFCOL + ((kb >> 2) & 1) * 12;
+                if ((kb & 15) == 0) {
                     if (!mbar_wait_cluster_warp(sfFull + 8 * slot, (q / SF_SLOTS) & 1)) { expire(38); dead = true; break; }
                     tc_fence_after();
+                }
+                if (j == 0) {
                     if (elect_one()) {
 #pragma unroll
-                        for (int i = 0; i < 3; i++) tmem_copy_scales_pair(sfcol + 4 * i, sSF + slot * PSF + 512 * i);
-                        umma_commit_pair(sfEmpty + 8 * slot);
+                        for (int i = 0; i < 3; i++) tmem_copy_scales_pair(sfcol + 4 * i, sSF + (slot * 4 + ((kb >> 2) & 3)) * PSF + 512 * i);
+                        if ((kb & 12) == 12 || kb + 4 >= KB) umma_commit_pair(sfEmpty + 8 * slot);
                     }
                     __syncwarp();
+                    if ((kb & 12) == 12 || kb + 4 >= KB) q++;
                 }
                 if (!mbar_wait_cluster_warp(full + 8 * s, (g / PSTAGES) & 1)) { expire(39); dead = true; break; }
                 tc_fence_after();
@@ -393,41 +380,31 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
                     if (kb == KB - 1) umma_commit_pair(accFull + 8 * (a & 1));
                 }
                 __syncwarp();
-                if (j == 3 || kb == KB - 1) q++;
             }
         }
     } else if (warp == 2) {
+        // A chunk of 16 blocks is fetched, stored and announced before the next one is asked for: the fence and the arrival on the other
+        // CTA's barrier would wait for loads under way.  Three slots keep the MMAs supplied meanwhile.
         const int apack = scale_packing(A, 0), bpack = scale_packing(B, 0);
-        int t = pair0, kb = 0, m0 = 0, n0 = 0, q = 0;
-        uint4 w[3][4];
-        auto fetch = [&]() {
-            load_scales(A, apack, m0 + (int)rank * 128, kb, KB, lane, w[0]);
-            load_scales(B, bpack, n0, kb, KB, lane, w[1]);
-            load_scales(B, bpack, n0 + 128, kb, KB, lane, w[2]);
-        };
-        if (t < ntiles) { tile_at(t, m0, n0); fetch(); }
         bool dead = false;
-        while (t < ntiles && !dead) {
-            uint4 now[3][4];
-#pragma unroll
-            for (int i = 0; i < 3; i++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) now[i][k] = w[i][k];
-            const int left = KB - kb;
-            kb += 16;
-            if (kb >= KB) { kb = 0; t += pairs; if (t < ntiles) tile_at(t, m0, n0); }
-            if (t < ntiles) fetch();
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (4 * j >= left || dead) continue;
+        int q = 0;
+        for (int t = pair0; t < ntiles && !dead; t += pairs) {
+            int m0, n0;
+            tile_at(t, m0, n0);
+            for (int kb = 0; kb < KB; kb += 16, q++) {
+                uint4 w[3][4];
+                load_scales(A, apack, m0 + (int)rank * 128, kb, KB, lane, w[0]);
+                load_scales(B, bpack, n0, kb, KB, lane, w[1]);
+                load_scales(B, bpack, n0 + 128, kb, KB, lane, w[2]);
                 const int slot = q % SF_SLOTS;
-                if (q >= SF_SLOTS && !mbar_wait_cluster_warp(sfEmpty + 8 * slot, (q / SF_SLOTS - 1) & 1)) { expire(40); dead = true; continue; }
+                if (q >= SF_SLOTS && !mbar_wait_cluster_warp(sfEmpty + 8 * slot, (q / SF_SLOTS - 1) & 1)) { expire(40); dead = true; break; }
 #pragma unroll
-                for (int i = 0; i < 3; i++) store_scales(sSF + slot * PSF + lane * 16 + 512 * i, now[i], j);
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int i = 0; i < 3; i++) store_scales(sSF + (slot * 4 + j) * PSF + lane * 16 + 512 * i, w[i], j);
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(sfFull + 8 * slot, 0u);
-                q++;
             }
         }
     } else if (warp >= 4) {
@@ -519,7 +496,7 @@ static int launch_tile(const MatmulBlocksParams& p, const BlocksPlan& pl, int* s
     {
         std::lock_guard<std::mutex> lock(mu);
         if (dev < 0 || dev >= 64 || !configured[dev]) {
-            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 * 1024);
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 208 * 1024);
             if (e != cudaSuccess) return record_cuda_error(e);
             if (dev >= 0 && dev < 64) configured[dev] = true;
         }
