@@ -10,6 +10,7 @@
 // blocks of 128, i.e. 512 terms.
 #include <algorithm>
 #include <cstdio>
+#include <cstdlib>
 #include <cuda.h>
 #include <mutex>
 #include "blocks_common.cuh"
@@ -85,15 +86,37 @@ __device__ __forceinline__ void store_scales(uint32_t at, const uint4 (&w)[4], i
     else sts_v4(at, w[0].w, w[1].w, w[2].w, w[3].w);
 }
 
-// 32 accumulators of a row (columns c0 .. c0+31 of ncols) to row-major memory.
+// A warp's 32 x 32 accumulators (lane: row, columns c0 .. c0+31 of ncols) to row-major memory.  vec: rows start on eight elements, and a
+// lane writes its own row in whole sectors.  Otherwise 16 columns at a time are turned round in 2 KB of shared memory (`stage`, this
+// warp's own; the rotation by row / 2 keeps both directions free of bank conflicts), so that 16 lanes write one row side by side.
 template <typename T>
-__device__ __forceinline__ void store_row32(T* y, int c0, int ncols, bool vec, const float (&v)[32]) {
+__device__ __forceinline__ void store_rows32(T* y, long long ldy, int row0, int nrows, int c0, int ncols, bool vec, const float (&v)[32], uint32_t stage, int lane) {
+    if (vec) {
+        if (row0 + lane >= nrows) return;
+        T* p = y + (long long)(row0 + lane) * ldy;
 #pragma unroll
-    for (int j = 0; j < 32; j += 8) {
-        float t[8];
+        for (int j = 0; j < 32; j += 8) {
+            float t[8];
 #pragma unroll
-        for (int i = 0; i < 8; i++) t[i] = v[j + i];
-        store8(y + c0 + j, ncols - (c0 + j), vec, t);
+            for (int i = 0; i < 8; i++) t[i] = v[j + i];
+            store8(p + c0 + j, ncols - (c0 + j), true, t);
+        }
+        return;
+    }
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+        __syncwarp();
+#pragma unroll
+        for (int j = 0; j < 16; j++) asm volatile("st.shared.f32 [%0], %1;" ::"r"(stage + (uint32_t)(lane * 16 + ((j + (lane >> 1)) & 15)) * 4u), "f"(v[h + j]) : "memory");
+        __syncwarp();
+        const int c = c0 + h + (lane & 15);
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int r = 2 * i + (lane >> 4);
+            float f;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(f) : "r"(stage + (uint32_t)(r * 16 + (((lane & 15) + (r >> 1)) & 15)) * 4u) : "memory");
+            if (row0 + r < nrows && c < ncols) y[(long long)(row0 + r) * ldy + c] = from_float<T>(f);
+        }
     }
 }
 
@@ -141,6 +164,7 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
     tc_fence_after();
     const uint32_t tmem = *static_cast<volatile uint32_t*>(&tslot);
     pdl_wait();
+    pdl_launch_dependents();
     auto expire = [&](int code) { if (lane == 0) { if (status) atomicExch(status, code); *deadp = 1; } };
 
     if (warp == 0) {
@@ -218,18 +242,19 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
                 float o[32];
 #pragma unroll
                 for (int j = 0; j < 32; j++) o[j] = __uint_as_float(v[j]);
-                if (row < R.rows) {
-                    if (SWAP) {
+                if (SWAP) {
+                    if (row < R.rows) {
 #pragma unroll
                         for (int j = 0; j < LC; j++) if (c0 + cb + j < C.rows) y[(long long)(c0 + cb + j) * ldy + row] = from_float<T>(o[j]);
-                    } else {
-                        store_row32(y + (long long)row * ldy, c0 + cb, min(C.rows, c0 + BN), vec, o);
                     }
+                } else {
+                    store_rows32(y, ldy, r0 + quarter, R.rows, c0 + cb, min(C.rows, c0 + BN), vec, o, sRing + (uint32_t)(warp - 4) * 2048u, lane);
                 }
             }
         }
     } else {
-        // partial results, [column][128 rows] floats, in the ring; a rank without blocks contributes zeros
+        // Partial results in the ring: [column][128 rows] floats, or [row][BN + 1] for a tile that is written as it is.  A rank without blocks
+        // contributes zeros.  Every rank finishes its share of the rows of y, in the order of the ranks, 32 neighbours of a row a warp.
         float* part = reinterpret_cast<float*>(raw + (sRing - (uint32_t)__cvta_generic_to_shared(raw)));
         if (warp >= 4) {
 #pragma unroll 1
@@ -237,19 +262,17 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
                 uint32_t v[32];
                 tmem_ld32(taddr + cb, v);
 #pragma unroll
-                for (int j = 0; j < LC; j++) part[(cb + j) * 128 + quarter + lane] = kb1 > kb0 ? __uint_as_float(v[j]) : 0.f;
+                for (int j = 0; j < LC; j++) part[SWAP ? (cb + j) * 128 + quarter + lane : (quarter + lane) * (BN + 1) + cb + j] = kb1 > kb0 ? __uint_as_float(v[j]) : 0.f;
             }
         }
         cluster_sync_all();
-        const int share = BN / split, cfirst = rank * share;               // columns this rank finishes
-        const int rl = tid & 127, rr = r0 + rl;
-        for (int c = cfirst + (tid >> 7); c < cfirst + share; c += 2) {
+        constexpr int YR = SWAP ? BN : 128, YC = SWAP ? 128 : BN, PITCH = SWAP ? 128 : BN + 1;   // rows and columns of y in the tile
+        const int y0 = SWAP ? c0 : r0, x0 = SWAP ? r0 : c0, ylim = SWAP ? C.rows : R.rows, xlim = SWAP ? R.rows : C.rows, share = YR / split;
+        for (int i = rank * share * (YC / 32) + warp, end = (rank + 1) * share * (YC / 32); i < end; i += TT / 32) {
+            const int yr = i / (YC / 32), xc = i % (YC / 32) * 32 + lane;
             float sum = 0.f;
-            for (int i = 0; i < split; i++) sum += ld_cluster_f32(sRing + (uint32_t)(c * 128 + rl) * 4u, (uint32_t)i);
-            if (rr < R.rows && c0 + c < C.rows) {
-                if (SWAP) y[(long long)(c0 + c) * ldy + rr] = from_float<T>(sum);
-                else y[(long long)rr * ldy + c0 + c] = from_float<T>(sum);
-            }
+            for (int k = 0; k < split; k++) sum += ld_cluster_f32(sRing + (uint32_t)(yr * PITCH + xc) * 4u, (uint32_t)k);
+            if (y0 + yr < ylim && x0 + xc < xlim) y[(long long)(y0 + yr) * ldy + x0 + xc] = from_float<T>(sum);
         }
         cluster_sync_all();                                                // nobody reads this CTA's memory any more
     }
@@ -260,7 +283,6 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
         for (int i = 0; i < 200; i++) __nanosleep(1000);
         __syncthreads();
     }
-    pdl_launch_dependents();
     if (warp == 1) tmem_dealloc(tmem, TCOLS);
 }
 
@@ -281,9 +303,11 @@ static constexpr int PT = 384;                           // threads of a pair's 
 static constexpr int PSTAGES = 6;                        // of 128 terms: 128 rows of a and 128 of b, 32 KB
 static constexpr int PSTAGE = 32768;
 static constexpr int PSF = 1536;                         // scale words of 512 terms: 128 rows of a, 256 of b; a slot holds four of them
+static constexpr int PSLOTS = 2;
+static_assert(PSTAGES * PSTAGE + PSLOTS * 4 * PSF + 8 * 2048 + 1024 + 512 <= UMMA_SMEM_MAX, "static and dynamic shared memory");
 static constexpr int PACC = 224;                         // second accumulator's first column: it shares 32 with the first
 static constexpr int PSFCOL = 480;
-static constexpr int PSMEM = PSTAGES * PSTAGE + SF_SLOTS * 4 * PSF + 1024;
+static constexpr int PSMEM = PSTAGES * PSTAGE + PSLOTS * 4 * PSF + 8 * 2048 + 1024;
 
 // A persistent pair of CTAs works 256 x 256 tiles: each CTA holds 128 rows of a and of b, and one MMA stream, issued by the even CTA,
 // multiplies for both; each CTA's tensor memory receives the sums of its own 128 rows of a and all 256 of b.  Two accumulators, so
@@ -295,13 +319,13 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
                                                                void* yv, long long ldy, int KB, int tiles_m, int tiles_n, int group, int vec, int* status) {
     using T = typename ElemOf<TYPE>::type;
     extern __shared__ uint8_t raw[];
-    __shared__ __align__(8) uint64_t bars[2 * PSTAGES + 2 * SF_SLOTS + 3];
+    __shared__ __align__(8) uint64_t bars[2 * PSTAGES + 2 * PSLOTS + 3];
     __shared__ uint32_t tslot;
     __shared__ int dead_flag;
     volatile int* deadp = &dead_flag;
-    const uint32_t sRing = ((uint32_t)__cvta_generic_to_shared(raw) + 1023u) & ~1023u, sSF = sRing + PSTAGES * PSTAGE;
-    const uint32_t full = (uint32_t)__cvta_generic_to_shared(bars), empty = full + 8 * PSTAGES, sfFull = empty + 8 * PSTAGES, sfEmpty = sfFull + 8 * SF_SLOTS,
-                   accFull = sfEmpty + 8 * SF_SLOTS, accFree = accFull + 16;
+    const uint32_t sRing = ((uint32_t)__cvta_generic_to_shared(raw) + 1023u) & ~1023u, sSF = sRing + PSTAGES * PSTAGE, sStage = sSF + PSLOTS * 4 * PSF;
+    const uint32_t full = (uint32_t)__cvta_generic_to_shared(bars), empty = full + 8 * PSTAGES, sfFull = empty + 8 * PSTAGES, sfEmpty = sfFull + 8 * PSLOTS,
+                   accFull = sfEmpty + 8 * PSLOTS, accFree = accFull + 16;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t rank = cluster_ctarank();
     const int pair0 = (int)(blockIdx.x >> 1), pairs = (int)(gridDim.x >> 1), ntiles = tiles_m * tiles_n;
@@ -309,7 +333,7 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
     if (tid == 0) {
         *deadp = 0;
         for (int s = 0; s < PSTAGES; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
-        for (int s = 0; s < SF_SLOTS; s++) { mbar_init(sfFull + 8 * s, 2); mbar_init(sfEmpty + 8 * s, 1); }
+        for (int s = 0; s < PSLOTS; s++) { mbar_init(sfFull + 8 * s, 2); mbar_init(sfEmpty + 8 * s, 1); }
         mbar_init(accFull, 1); mbar_init(accFull + 8, 1); mbar_init(accFree, 16);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -354,10 +378,10 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
             if (a >= 1 && !mbar_wait_cluster_warp(accFree, (a - 1) & 1)) { expire(37); break; }
             tc_fence_after();
             for (int kb = 0; kb < KB; kb++, g++) {
-                const int s = g % PSTAGES, j = kb & 3, slot = q % SF_SLOTS;
+                const int s = g % PSTAGES, j = kb & 3, slot = q % PSLOTS;
                 const uint32_t sfcol = tmem + PSFCOL + ((kb >> 2) & 1) * 12;
                 if ((kb & 15) == 0) {
-                    if (!mbar_wait_cluster_warp(sfFull + 8 * slot, (q / SF_SLOTS) & 1)) { expire(38); dead = true; break; }
+                    if (!mbar_wait_cluster_warp(sfFull + 8 * slot, (q / PSLOTS) & 1)) { expire(38); dead = true; break; }
                     tc_fence_after();
                 }
                 if (j == 0) {
@@ -384,7 +408,7 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
         }
     } else if (warp == 2) {
         // A chunk of 16 blocks is fetched, stored and announced before the next one is asked for: the fence and the arrival on the other
-        // CTA's barrier would wait for loads under way.  Three slots keep the MMAs supplied meanwhile.
+        // CTA's barrier would wait for loads under way.  Two slots, 32 blocks, keep the MMAs supplied meanwhile.
         const int apack = scale_packing(A, 0), bpack = scale_packing(B, 0);
         bool dead = false;
         int q = 0;
@@ -396,8 +420,8 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
                 load_scales(A, apack, m0 + (int)rank * 128, kb, KB, lane, w[0]);
                 load_scales(B, bpack, n0, kb, KB, lane, w[1]);
                 load_scales(B, bpack, n0 + 128, kb, KB, lane, w[2]);
-                const int slot = q % SF_SLOTS;
-                if (q >= SF_SLOTS && !mbar_wait_cluster_warp(sfEmpty + 8 * slot, (q / SF_SLOTS - 1) & 1)) { expire(40); dead = true; break; }
+                const int slot = q % PSLOTS;
+                if (q >= PSLOTS && !mbar_wait_cluster_warp(sfEmpty + 8 * slot, (q / PSLOTS - 1) & 1)) { expire(40); dead = true; break; }
 #pragma unroll
                 for (int j = 0; j < 4; j++)
 #pragma unroll
@@ -414,7 +438,6 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
         for (int t = pair0; t < ntiles; t += pairs, a++) {
             int m0, n0;
             tile_at(t, m0, n0);
-            const int row = m0 + (int)rank * 128 + quarter + lane;
             if (!mbar_wait_cluster_warp(accFull + 8 * (a & 1), (a >> 1) & 1)) { expire(41); break; }
             tc_fence_after();
             // the shared columns: the last 32 of the first accumulator, the first 32 of the second
@@ -434,7 +457,7 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
                 float o[32];
 #pragma unroll
                 for (int j = 0; j < 32; j++) o[j] = __uint_as_float(v[j]);
-                if (row < A.rows) store_row32(y + (long long)row * ldy, n0 + half * 128 + cb, B.rows, vec, o);
+                store_rows32(y, ldy, m0 + (int)rank * 128 + quarter, A.rows, n0 + half * 128 + cb, B.rows, vec, o, sStage + (uint32_t)(warp - 4) * 2048u, lane);
             }
             tc_fence_before();
             __syncwarp();
@@ -492,7 +515,7 @@ static int launch_tile(const MatmulBlocksParams& p, const BlocksPlan& pl, int* s
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return record_cuda_error(e);
-    const int smem = std::max(pl.nst * (128 + BN) * 128, pl.split > 1 ? BN * 512 : 0) + 1024;
+    const int smem = std::max(pl.nst * (128 + BN) * 128, pl.split > 1 ? 128 * (BN + 1) * 4 : 0) + 1024;
     {
         std::lock_guard<std::mutex> lock(mu);
         if (dev < 0 || dev >= 64 || !configured[dev]) {
@@ -548,17 +571,44 @@ static int launch_pair(const MatmulBlocksParams& p, int pairs, int* status, cuda
     return launch_pdl_as(false, 2u, kernel, dim3(grid), dim3(PT), (size_t)PSMEM, stream, tmA, tmB, p.a, p.b, p.y, p.ldy, blocks_of(p.K), (int)tiles_m, (int)tiles_n, 8, vec, status);
 }
 
+template <int BN, bool SWAP>
+static int launch_tile_type(const MatmulBlocksParams& p, const BlocksPlan& pl, int* status, cudaStream_t stream) {
+    return p.type == TAB_FP32 ? launch_tile<BN, SWAP, TAB_FP32>(p, pl, status, stream) : p.type == TAB_BF16 ? launch_tile<BN, SWAP, TAB_BF16>(p, pl, status, stream)
+                                                                                                            : launch_tile<BN, SWAP, TAB_FP16>(p, pl, status, stream);
+}
+
+static BlocksPlan blocks_plan(int M, int N, int KB, int sms) {
+    BlocksPlan pl = {128, false, 1, KB, 6};
+#ifdef TAB_TUNE
+    // Build-time diagnostic (-DTAB_TUNE, never in the shipped library): "columns,swap,split,stages" from the environment.
+    if (const char* env = getenv("TAB_MATMUL")) {
+        int swap = 0;
+        if (sscanf(env, "%d,%d,%d,%d", &pl.bn, &swap, &pl.split, &pl.nst) == 4) { pl.swap = swap != 0; pl.per = (KB + pl.split - 1) / pl.split; return pl; }
+    }
+#endif
+    return pl;
+}
+
 int matmul_blocks_dispatch(const MatmulBlocksParams& p, cudaStream_t stream) {
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     const long long tiles = ((long long)p.a.rows + 255) / 256 * (((long long)p.b.rows + 255) / 256);
     const int pairs = matmul_pairs();
-    if (pairs > 0 && tiles * 2 > pairs) return launch_pair(p, pairs, status, stream);
-    BlocksPlan pl = {128, false, 1, blocks_of(p.K), 6};
-#define TAB_MB(BN, SW) (p.type == TAB_FP32 ? launch_tile<BN, SW, TAB_FP32>(p, pl, status, stream) : p.type == TAB_BF16 ? launch_tile<BN, SW, TAB_BF16>(p, pl, status, stream) \
-                                                                                                                     : launch_tile<BN, SW, TAB_FP16>(p, pl, status, stream))
-    return TAB_MB(128, false);
-#undef TAB_MB
+    bool pair = pairs > 0 && tiles * 2 > pairs;
+#ifdef TAB_TUNE
+    if (const char* env = getenv("TAB_MATMUL")) pair = env[0] == 'p';
+#endif
+    if (pair) return launch_pair(p, pairs, status, stream);
+    const BlocksPlan pl = blocks_plan(p.a.rows, p.b.rows, blocks_of(p.K), sms);
+    if (pl.swap) {
+        if (pl.bn == 16) return launch_tile_type<16, true>(p, pl, status, stream);
+        if (pl.bn == 32) return launch_tile_type<32, true>(p, pl, status, stream);
+        return launch_tile_type<64, true>(p, pl, status, stream);
+    }
+    if (pl.bn == 64) return launch_tile_type<64, false>(p, pl, status, stream);
+    return launch_tile_type<128, false>(p, pl, status, stream);
 }
 
 }  // namespace tab
