@@ -13,6 +13,7 @@
 #include <cstdlib>
 #include <cuda.h>
 #include <mutex>
+#include <type_traits>
 #include "blocks_common.cuh"
 #include "umma_common.cuh"
 
@@ -474,6 +475,148 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
     if (warp == 1) tmem_dealloc_pair(tmem, 512);
 }
 
+// ---- few rows of a ----------------------------------------------------------------------------------------------------------------
+// Two 8-bit floats (low byte first) as fp16, exact for both formats.
+__device__ __forceinline__ uint32_t widen2(uint32_t two, bool e5m2) {
+    uint32_t h;
+    if (e5m2) asm("cvt.rn.f16x2.e5m2x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+    else asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"((uint16_t)two));
+    return h;
+}
+template <int FORMAT>
+__device__ __forceinline__ void widen16(const uint4& u, uint32_t (&h)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) { h[2 * i] = widen2(w[i] & 0xFFFFu, FORMAT == TAB_E5M2); h[2 * i + 1] = widen2(w[i] >> 16, FORMAT == TAB_E5M2); }
+}
+// 16 values of a row from k on; those behind its end are 0 and not read.
+__device__ __forceinline__ uint4 load_values16(const uint8_t* row, int k, int K) {
+    if (k + 16 <= K) return *reinterpret_cast<const uint4*>(row + k);
+    uint32_t w[4] = {0, 0, 0, 0};
+    for (int j = 0; j < 16; j++) if (k + j < K) w[j >> 2] |= (uint32_t)row[k + j] << (8 * (j & 3));
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// A load of weights that are read once.
+__device__ __forceinline__ uint4 ld_stream(const uint8_t* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.L1::no_allocate.L2::128B.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
+// sum + v * 2^(a - 127) * 2^(b - 127) for scale bytes (255: NaN).
+__device__ __forceinline__ float add_scaled(float sum, float v, int a, int b) {
+    const int e = a + b - 127;
+    if (e >= 1 && e <= 254 && a != 255 && b != 255) return fmaf(v, __uint_as_float((uint32_t)e << 23), sum);
+    if (a == 255 || b == 255) return __uint_as_float(0x7FC00000u);
+    const int h = (e - 127) >> 1;                                          // beyond fp32's exponents: in two steps
+    return sum + v * exp2_int(h) * exp2_int(e - 127 - h);
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+static constexpr int VMOST = 8;                          // rows of a
+static constexpr int VAHEAD = 4;                         // blocks of the sum a warp has under way
+
+// At most eight rows of a against all of b: every weight is read once and multiplied so few times that nothing but the reading counts,
+// so there is no pipeline through shared and tensor memory, whose start and end cost more than the reading of a few megabytes.  A warp
+// takes 16 rows of b and a share of the sum straight into registers, 16 bytes a lane, and multiplies in fp16, which holds every 8-bit
+// float, with fp32 sums (the sum's order is free as long as both operands agree, so a lane's 16 neighbours serve four MMAs).  A block's
+// sum is added under its scales; the warps' sums are added in their order.
+template <int FA, int FB>
+__global__ void __launch_bounds__(256, 2) matmul_blocks_rows_kernel(BlocksOperand A, BlocksOperand B, void* y, long long ldy, int type, int K, int per) {
+    __shared__ float part[8][16][9];
+    pdl_wait();
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, n0 = (int)blockIdx.x * 16, KB = (K + BLK - 1) / BLK;
+    const int kb1 = min(KB, (warp + 1) * per);
+    // rows that do not exist are read as the last one, and their results not written
+    const uint8_t* b[2];
+    const uint8_t* bs[2];
+    const uint8_t* as[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int row = min(n0 + g + 8 * i, B.rows - 1), m = min(2 * t + i, A.rows - 1);
+        b[i] = B.q + (long long)row * B.ld;
+        bs[i] = B.s + (long long)(row >> B.shift) * B.sr;
+        as[i] = A.s + (long long)(m >> A.shift) * A.sr;
+    }
+    const uint8_t* a = A.q + (long long)min(g, A.rows - 1) * A.ld;
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+    auto block = [&](const uint4 (&w)[2][2], const uint4 (&v)[2], const int (&sa)[2], const int (&sb)[2]) {
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            uint32_t w0[8], w1[8], x[8];
+            widen16<FB>(w[h][0], w0);
+            widen16<FB>(w[h][1], w1);
+            widen16<FA>(v[h], x);
+#pragma unroll
+            for (int j = 0; j < 4; j++) mma_f16(d, w0[2 * j], w1[2 * j], w0[2 * j + 1], w1[2 * j + 1], x[2 * j], x[2 * j + 1]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum[j] = add_scaled(sum[j], d[j], sa[j & 1], sb[j >> 1]);
+    };
+    const int whole = min(kb1, K / BLK);                                   // blocks that are not cut short by the row's end
+    int kb = warp * per;
+    auto several = [&](auto count) {
+        constexpr int N = decltype(count)::value;
+        uint4 w[N][2][2], v[N][2];
+        int sb[N][2], sa[N][2];
+#pragma unroll
+        for (int i = 0; i < N; i++) {
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const int k = (kb + i) * BLK + h * 64 + t * 16;
+#pragma unroll
+                for (int r = 0; r < 2; r++) w[i][h][r] = ld_stream(b[r] + k);
+                v[i][h] = *reinterpret_cast<const uint4*>(a + k);
+            }
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                sb[i][r] = bs[r][(long long)(kb + i) * B.sk];
+                sa[i][r] = as[r][(long long)(kb + i) * A.sk];
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < N; i++) block(w[i], v[i], sa[i], sb[i]);
+        kb += N;
+    };
+    while (kb + VAHEAD <= whole) several(std::integral_constant<int, VAHEAD>());
+    while (kb < whole) several(std::integral_constant<int, 1>());
+    if (kb < kb1) {                                                        // the row's last, short block
+        uint4 w[2][2], v[2];
+        int sb[2], sa[2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int k = kb * BLK + h * 64 + t * 16;
+#pragma unroll
+            for (int r = 0; r < 2; r++) w[h][r] = load_values16(b[r], k, K);
+            v[h] = load_values16(a, k, K);
+        }
+#pragma unroll
+        for (int r = 0; r < 2; r++) {
+            sb[r] = bs[r][(long long)kb * B.sk];
+            sa[r] = as[r][(long long)kb * A.sk];
+        }
+        block(w, v, sa, sb);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; j++) part[warp][g + 8 * (j >> 1)][2 * t + (j & 1)] = sum[j];
+    __syncthreads();
+    if (threadIdx.x < 128) {
+        const int n = threadIdx.x & 15, m = threadIdx.x >> 4;
+        if (n0 + n < B.rows && m < A.rows) {
+            float s = 0.f;
+            for (int i = 0; i < (int)blockDim.x / 32; i++) s += part[i][n][m];
+            const long long at = (long long)m * ldy + n0 + n;
+            if (type == TAB_FP32) static_cast<float*>(y)[at] = s;
+            else if (type == TAB_BF16) static_cast<__nv_bfloat16*>(y)[at] = __float2bfloat16_rn(s);
+            else static_cast<__half*>(y)[at] = __float2half_rn(s);
+        }
+    }
+}
+
 // ---- host side ----------------------------------------------------------------------------------------------------------------
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                   const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
@@ -571,6 +714,21 @@ static int launch_pair(const MatmulBlocksParams& p, int pairs, int* status, cuda
     return launch_pdl_as(false, 2u, kernel, dim3(grid), dim3(PT), (size_t)PSMEM, stream, tmA, tmB, p.a, p.b, p.y, p.ldy, blocks_of(p.K), (int)tiles_m, (int)tiles_n, 8, vec, status);
 }
 
+static int launch_rows(const MatmulBlocksParams& p, int sms, cudaStream_t stream) {
+    const int KB = blocks_of(p.K);
+    const unsigned grid = (unsigned)(((long long)p.b.rows + 15) / 16);
+    int warps = 8;
+#ifdef TAB_TUNE
+    if (const char* env = getenv("TAB_KW")) warps = atoi(env);
+#endif
+    const int per = (KB + warps - 1) / warps;
+    snprintf(g_last_blocks_kernel, sizeof(g_last_blocks_kernel), "matmul_blocks_rows_kernel %d warps", warps);
+#define TAB_MR(FA, FB) launch_pdl(matmul_blocks_rows_kernel<FA, FB>, dim3(grid), dim3(32 * warps), 0, stream, p.a, p.b, p.y, p.ldy, p.type, p.K, per)
+    if (p.a.format == TAB_E5M2) return p.b.format == TAB_E5M2 ? TAB_MR(TAB_E5M2, TAB_E5M2) : TAB_MR(TAB_E5M2, TAB_E4M3);
+    return p.b.format == TAB_E5M2 ? TAB_MR(TAB_E4M3, TAB_E5M2) : TAB_MR(TAB_E4M3, TAB_E4M3);
+#undef TAB_MR
+}
+
 template <int BN, bool SWAP>
 static int launch_tile_type(const MatmulBlocksParams& p, const BlocksPlan& pl, int* status, cudaStream_t stream) {
     return p.type == TAB_FP32 ? launch_tile<BN, SWAP, TAB_FP32>(p, pl, status, stream) : p.type == TAB_BF16 ? launch_tile<BN, SWAP, TAB_BF16>(p, pl, status, stream)
@@ -594,6 +752,11 @@ int matmul_blocks_dispatch(const MatmulBlocksParams& p, cudaStream_t stream) {
     if (stalled(status)) return TAB_E_STALLED;
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    bool few = p.a.rows <= VMOST;
+#ifdef TAB_TUNE
+    if (const char* env = getenv("TAB_MATMUL")) few = env[0] == 'v' && p.a.rows <= VMOST;
+#endif
+    if (few) return launch_rows(p, sms, stream);
     const long long tiles = ((long long)p.a.rows + 255) / 256 * (((long long)p.b.rows + 255) / 256);
     const int pairs = matmul_pairs();
     bool pair = pairs > 0 && tiles * 2 > pairs;
