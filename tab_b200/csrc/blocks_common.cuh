@@ -110,6 +110,7 @@ __device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
     const __half2 h = __floats2half2_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ uint32_t pack2(float a, float, float) { return __float_as_uint(a); }   // (fp32 has nothing to pack)
 __device__ __forceinline__ void store8(float* p, int n, bool vec, const float (&v)[8]) {
     if (vec && n >= 8) {
         asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"

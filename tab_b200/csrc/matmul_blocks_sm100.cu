@@ -87,20 +87,38 @@ __device__ __forceinline__ void store_scales(uint32_t at, const uint4 (&w)[4], i
     else sts_v4(at, w[0].w, w[1].w, w[2].w, w[3].w);
 }
 
-// A warp's 32 x 32 accumulators (lane: row, columns c0 .. c0+31 of ncols) to row-major memory.  vec: rows start on eight elements, and a
-// lane writes its own row in whole sectors.  Otherwise 16 columns at a time are turned round in 2 KB of shared memory (`stage`, this
-// warp's own; the rotation by row / 2 keeps both directions free of bank conflicts), so that 16 lanes write one row side by side.
+__device__ __forceinline__ void tma_store_2d(const void* tmap, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(src), "r"(x), "r"(y) : "memory");
+}
+// A warp's 32 x 32 accumulators (lane: row, columns c0 .. c0+31) to row-major memory, through 4 KB of shared memory (`stage`, this warp's
+// own).  A lane that writes its own row keeps the load and store unit busy for a cycle a row, and the loads of scales wait behind it.
+//   tma   (rows of y start and end on 16 bytes) boxes of 64 bytes x 32 rows, 64-byte swizzle, two buffers in turn; what lies outside y is not written
+//   else  16 columns at a time are turned round (the rotation by row / 2 keeps both directions free of bank conflicts) and written by
+//         16 lanes a row.
 template <typename T>
-__device__ __forceinline__ void store_rows32(T* y, long long ldy, int row0, int nrows, int c0, int ncols, bool vec, const float (&v)[32], uint32_t stage, int lane) {
-    if (vec) {
-        if (row0 + lane >= nrows) return;
-        T* p = y + (long long)(row0 + lane) * ldy;
+__device__ __forceinline__ void store_rows32(const void* tmY, T* y, long long ldy, int row0, int nrows, int c0, int ncols, bool tma, const float (&v)[32], uint32_t stage, uint32_t& turn, int lane) {
+    if (tma) {
+        constexpr int E = 64 / sizeof(T);
 #pragma unroll
-        for (int j = 0; j < 32; j += 8) {
-            float t[8];
+        for (int h = 0; h < 32; h += E) {
+            const uint32_t buf = stage + (turn & 1) * 2048u, row = buf + (uint32_t)lane * 64u, x = (uint32_t)(lane >> 1) & 3u;
+            turn++;
+            if (lane == 0) bulk_wait_read<1>();                            // the store before last has left this buffer
+            __syncwarp();
 #pragma unroll
-            for (int i = 0; i < 8; i++) t[i] = v[j + i];
-            store8(p + c0 + j, ncols - (c0 + j), true, t);
+            for (int c = 0; c < 4; c++) {
+                if (sizeof(T) == 4) {
+                    sts_v4(row + ((c ^ x) << 4), __float_as_uint(v[(h + 4 * c) & 31]), __float_as_uint(v[(h + 4 * c + 1) & 31]), __float_as_uint(v[(h + 4 * c + 2) & 31]), __float_as_uint(v[(h + 4 * c + 3) & 31]));
+                } else {
+                    sts_v4(row + ((c ^ x) << 4), pack2(v[8 * c], v[8 * c + 1], T()), pack2(v[8 * c + 2], v[8 * c + 3], T()), pack2(v[8 * c + 4], v[8 * c + 5], T()), pack2(v[8 * c + 6], v[8 * c + 7], T()));
+                }
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+                if (row0 < nrows && c0 + h < ncols) tma_store_2d(tmY, c0 + h, row0, buf);
+                bulk_commit();
+            }
         }
         return;
     }
@@ -128,12 +146,12 @@ static constexpr int SF_SLOTS = 3;                       // of scale words of 16
 // issues the MMAs, warp 2 brings the scales, warps 4-7 finish.  A cluster shares out the sum: rank r of S takes blocks
 // [r * per, (r+1) * per), the partial results meet in shared memory and every rank adds its share of the columns, in the order of
 // the ranks.  SWAP: R is b, the tile is transposed (few rows of a: the 128-row side of the MMA takes the weights).
-template <int BN, bool SWAP, int TYPE>
-__global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmC, BlocksOperand R, BlocksOperand C,
-                                                                void* yv, long long ldy, int KB, int per, int nst, int tiles_c, int split, int vec, int* status) {
+template <int BN, int KS, bool SWAP, int TYPE>
+__global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmY, BlocksOperand R, BlocksOperand C,
+                                                                void* yv, long long ldy, int KB, int per, int nst, int tiles_c, int split, int tma, int* status) {
     using T = typename ElemOf<TYPE>::type;
     extern __shared__ uint8_t raw[];
-    constexpr int STAGE = (128 + BN) * 128;
+    constexpr int STAGE = KS * (128 + BN) * 128;                           // KS blocks: their rows of R, then their rows of C
     constexpr int CG = (BN + 127) / 128;                                   // groups of 128 rows of C
     constexpr int SFB = 512 * (1 + CG);                                    // bytes of four blocks' scales; a slot holds four of them
     constexpr int SFCOL = BN < 32 ? 32 : BN;                               // first tensor-memory column of the scales: two slots
@@ -169,42 +187,45 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
     auto expire = [&](int code) { if (lane == 0) { if (status) atomicExch(status, code); *deadp = 1; } };
 
     if (warp == 0) {
-        for (int kb = kb0, g = 0; kb < kb1; kb++, g++) {
-            const int s = g % nst;
+        for (int kb = kb0, g = 0; kb < kb1; kb += KS, g++) {
+            const int s = g % nst, blocks = min(KS, kb1 - kb);
             if (g >= nst && !mbar_wait_warp(empty + 8 * s, (g / nst - 1) & 1)) { expire(31); break; }
             if (elect_one()) {
-                mbar_expect_tx(full + 8 * s, STAGE);
-                tma_load_2d(sRing + s * STAGE, &tmR, kb * BLK, r0, full + 8 * s);
-                tma_load_2d(sRing + s * STAGE + 128 * 128, &tmC, kb * BLK, c0, full + 8 * s);
+                mbar_expect_tx(full + 8 * s, (uint32_t)blocks * (128 + BN) * 128);
+                for (int i = 0; i < blocks; i++) {
+                    tma_load_2d(sRing + s * STAGE + i * 16384, &tmR, (kb + i) * BLK, r0, full + 8 * s);
+                    tma_load_2d(sRing + s * STAGE + KS * 16384 + i * BN * 128, &tmC, (kb + i) * BLK, c0, full + 8 * s);
+                }
             }
             __syncwarp();
         }
     } else if (warp == 1) {
         const uint32_t idesc = umma_idesc_f8(128, BN, R.format == TAB_E5M2, C.format == TAB_E5M2);
-        for (int kb = kb0, g = 0; kb < kb1; kb++, g++) {
-            const int s = g % nst, j = g & 3, q = g >> 4, slot = q % SF_SLOTS;
-            const uint32_t sfcol = tmem + SFCOL + ((g >> 2) & 1) * 4 * (1 + CG);
-            if ((g & 15) == 0) {
+        for (int kb = kb0, g = 0; kb < kb1; kb += KS, g++) {
+            const int s = g % nst, at = kb - kb0, q = at >> 4, slot = q % SF_SLOTS;
+            const uint32_t sfcol = tmem + SFCOL + ((at >> 2) & 1) * 4 * (1 + CG);
+            if ((at & 15) == 0) {
                 if (!mbar_wait_warp(sfFull + 8 * slot, (q / SF_SLOTS) & 1)) { expire(32); break; }
                 tc_fence_after();
-            }
-            if (j == 0) {
-                if (elect_one()) {
-#pragma unroll
-                    for (int i = 0; i < 1 + CG; i++) tmem_copy_scales(sfcol + 4 * i, sSF + (slot * 4 + ((g >> 2) & 3)) * SFB + 512 * i);
-                    if ((g & 12) == 12 || kb + 4 >= kb1) umma_commit(sfEmpty + 8 * slot);
-                }
-                __syncwarp();
             }
             if (!mbar_wait_warp(full + 8 * s, (g / nst) & 1)) { expire(33); break; }
             tc_fence_after();
             if (elect_one()) {
-                const uint64_t da = umma_desc(sRing + s * STAGE), db = umma_desc(sRing + s * STAGE + 128 * 128);
-                const uint32_t id = with_scale_byte(idesc, j);
+                if ((at & 3) == 0) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) umma_f8(tmem, da + 2 * i, db + 2 * i, id, sfcol, sfcol + 4, (g | i) != 0);
+                    for (int i = 0; i < 1 + CG; i++) tmem_copy_scales(sfcol + 4 * i, sSF + (slot * 4 + ((at >> 2) & 3)) * SFB + 512 * i);
+                    if ((at & 12) == 12 || kb + 4 >= kb1) umma_commit(sfEmpty + 8 * slot);
+                }
+#pragma unroll
+                for (int b = 0; b < KS; b++) {
+                    if (kb + b >= kb1) break;
+                    const uint64_t da = umma_desc(sRing + s * STAGE + b * 16384), db = umma_desc(sRing + s * STAGE + KS * 16384 + b * BN * 128);
+                    const uint32_t id = with_scale_byte(idesc, (uint32_t)((at + b) & 3));
+#pragma unroll
+                    for (int i = 0; i < 4; i++) umma_f8(tmem, da + 2 * i, db + 2 * i, id, sfcol, sfcol + 4, (at | b | i) != 0);
+                }
                 umma_commit(empty + 8 * s);
-                if (kb == kb1 - 1) umma_commit(accFull);
+                if (kb + KS >= kb1) umma_commit(accFull);
             }
             __syncwarp();
         }
@@ -236,6 +257,7 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
     constexpr int LC = BN < 32 ? 16 : 32;                                  // columns of a step
     if (split == 1) {
         if (warp >= 4) {
+            uint32_t turn = 0;
 #pragma unroll 1
             for (int cb = 0; cb < BN && c0 + cb < C.rows; cb += 32) {
                 uint32_t v[32];
@@ -249,9 +271,10 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
                         for (int j = 0; j < LC; j++) if (c0 + cb + j < C.rows) y[(long long)(c0 + cb + j) * ldy + row] = from_float<T>(o[j]);
                     }
                 } else {
-                    store_rows32(y, ldy, r0 + quarter, R.rows, c0 + cb, min(C.rows, c0 + BN), vec, o, sRing + (uint32_t)(warp - 4) * 2048u, lane);
+                    store_rows32(&tmY, y, ldy, r0 + quarter, R.rows, c0 + cb, C.rows, tma, o, sRing + (uint32_t)(warp - 4) * 4096u, turn, lane);
                 }
             }
+            if (!SWAP && tma && lane == 0) bulk_wait_all();
         }
     } else {
         // Partial results in the ring: [column][128 rows] floats, or [row][BN + 1] for a tile that is written as it is.  A rank without blocks
@@ -300,15 +323,15 @@ __device__ __forceinline__ void tmem_copy_scales_pair(uint32_t taddr, uint32_t s
     asm volatile("tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
 
-static constexpr int PT = 384;                           // threads of a pair's CTA: copies, MMAs, scales, -, eight that finish
+static constexpr int PT = 256;                           // threads of a pair's CTA: copies, MMAs, scales, -, four that finish
 static constexpr int PSTAGES = 6;                        // of 128 terms: 128 rows of a and 128 of b, 32 KB
 static constexpr int PSTAGE = 32768;
 static constexpr int PSF = 1536;                         // scale words of 512 terms: 128 rows of a, 256 of b; a slot holds four of them
 static constexpr int PSLOTS = 2;
-static_assert(PSTAGES * PSTAGE + PSLOTS * 4 * PSF + 8 * 2048 + 1024 + 512 <= UMMA_SMEM_MAX, "static and dynamic shared memory");
+static_assert(PSTAGES * PSTAGE + PSLOTS * 4 * PSF + 4 * 4096 + 1024 + 512 <= UMMA_SMEM_MAX, "static and dynamic shared memory");
 static constexpr int PACC = 224;                         // second accumulator's first column: it shares 32 with the first
 static constexpr int PSFCOL = 480;
-static constexpr int PSMEM = PSTAGES * PSTAGE + PSLOTS * 4 * PSF + 8 * 2048 + 1024;
+static constexpr int PSMEM = PSTAGES * PSTAGE + PSLOTS * 4 * PSF + 4 * 4096 + 1024;
 
 // A persistent pair of CTAs works 256 x 256 tiles: each CTA holds 128 rows of a and of b, and one MMA stream, issued by the even CTA,
 // multiplies for both; each CTA's tensor memory receives the sums of its own 128 rows of a and all 256 of b.  Two accumulators, so
@@ -316,8 +339,8 @@ static constexpr int PSMEM = PSTAGES * PSTAGE + PSLOTS * 4 * PSF + 8 * 2048 + 10
 // some, here 32, which the finishing warps read first and release; from there on the next tile's MMAs may run.
 // group: tiles are taken in bands of so many row blocks, column by column, so that what is in work at a time shares its operands in the L2.
 template <int TYPE>
-__global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, BlocksOperand A, BlocksOperand B,
-                                                               void* yv, long long ldy, int KB, int tiles_m, int tiles_n, int group, int vec, int* status) {
+__global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY, BlocksOperand A, BlocksOperand B,
+                                                               void* yv, long long ldy, int KB, int tiles_m, int tiles_n, int group, int tma, int* status) {
     using T = typename ElemOf<TYPE>::type;
     extern __shared__ uint8_t raw[];
     __shared__ __align__(8) uint64_t bars[2 * PSTAGES + 2 * PSLOTS + 3];
@@ -335,7 +358,7 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
         *deadp = 0;
         for (int s = 0; s < PSTAGES; s++) { mbar_init(full + 8 * s, 1); mbar_init(empty + 8 * s, 1); }
         for (int s = 0; s < PSLOTS; s++) { mbar_init(sfFull + 8 * s, 2); mbar_init(sfEmpty + 8 * s, 1); }
-        mbar_init(accFull, 1); mbar_init(accFull + 8, 1); mbar_init(accFree, 16);
+        mbar_init(accFull, 1); mbar_init(accFull + 8, 1); mbar_init(accFree, 8);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == 1) tmem_alloc_pair((uint32_t)__cvta_generic_to_shared(&tslot), 512);
@@ -379,32 +402,30 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
             if (a >= 1 && !mbar_wait_cluster_warp(accFree, (a - 1) & 1)) { expire(37); break; }
             tc_fence_after();
             for (int kb = 0; kb < KB; kb++, g++) {
-                const int s = g % PSTAGES, j = kb & 3, slot = q % PSLOTS;
+                const int s = g % PSTAGES, slot = q % PSLOTS;
                 const uint32_t sfcol = tmem + PSFCOL + ((kb >> 2) & 1) * 12;
                 if ((kb & 15) == 0) {
                     if (!mbar_wait_cluster_warp(sfFull + 8 * slot, (q / PSLOTS) & 1)) { expire(38); dead = true; break; }
                     tc_fence_after();
                 }
-                if (j == 0) {
-                    if (elect_one()) {
-#pragma unroll
-                        for (int i = 0; i < 3; i++) tmem_copy_scales_pair(sfcol + 4 * i, sSF + (slot * 4 + ((kb >> 2) & 3)) * PSF + 512 * i);
-                        if ((kb & 12) == 12 || kb + 4 >= KB) umma_commit_pair(sfEmpty + 8 * slot);
-                    }
-                    __syncwarp();
-                    if ((kb & 12) == 12 || kb + 4 >= KB) q++;
-                }
                 if (!mbar_wait_cluster_warp(full + 8 * s, (g / PSTAGES) & 1)) { expire(39); dead = true; break; }
                 tc_fence_after();
+                const bool last_scales = (kb & 3) == 0 && ((kb & 12) == 12 || kb + 4 >= KB);
                 if (elect_one()) {
+                    if ((kb & 3) == 0) {
+#pragma unroll
+                        for (int i = 0; i < 3; i++) tmem_copy_scales_pair(sfcol + 4 * i, sSF + (slot * 4 + ((kb >> 2) & 3)) * PSF + 512 * i);
+                        if (last_scales) umma_commit_pair(sfEmpty + 8 * slot);
+                    }
                     const uint64_t da = umma_desc(sRing + s * PSTAGE), db = umma_desc(sRing + s * PSTAGE + 16384);
-                    const uint32_t id = with_scale_byte(idesc, j);
+                    const uint32_t id = with_scale_byte(idesc, (uint32_t)(kb & 3));
 #pragma unroll
                     for (int i = 0; i < 4; i++) umma_f8_pair(d, da + 2 * i, db + 2 * i, id, sfcol, sfcol + 4, (kb | i) != 0);
                     umma_commit_pair(empty + 8 * s);
                     if (kb == KB - 1) umma_commit_pair(accFull + 8 * (a & 1));
                 }
                 __syncwarp();
+                if (last_scales) q++;
             }
         }
     } else if (warp == 2) {
@@ -434,35 +455,32 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
         }
     } else if (warp >= 4) {
         T* y = static_cast<T*>(yv);
-        const int quarter = (warp & 3) * 32, half = (warp - 4) >> 2;
+        const int quarter = (warp & 3) * 32;
+        uint32_t turn = 0;
         int a = 0;
         for (int t = pair0; t < ntiles; t += pairs, a++) {
             int m0, n0;
             tile_at(t, m0, n0);
             if (!mbar_wait_cluster_warp(accFull + 8 * (a & 1), (a >> 1) & 1)) { expire(41); break; }
             tc_fence_after();
-            // the shared columns: the last 32 of the first accumulator, the first 32 of the second
-            const bool shares = half == ((a & 1) ^ 1);
-            const uint32_t taddr = tmem + (a & 1) * PACC + half * 128 + ((uint32_t)quarter << 16);
-            if (!shares && lane == 0) mbar_arrive_cluster(accFree, 0u);
+            const uint32_t taddr = tmem + (a & 1) * PACC + ((uint32_t)quarter << 16);
 #pragma unroll 1
-            for (int i = 0; i < 4; i++) {
-                const int cb = (half ? 3 - i : i) * 32;
+            for (int i = 0; i < 8; i++) {
+                const int cb = ((a & 1) ? i : 7 - i) * 32;                 // the shared columns first: the first accumulator's last, the second's first
                 uint32_t v[32];
                 tmem_ld32(taddr + cb, v);
-                if (shares && i == 0) {
+                if (i == 0) {
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive_cluster(accFree, 0u);
+                    if (lane == 0) mbar_arrive_cluster(accFree, 0u);       // and this warp is done with the other accumulator
                 }
                 float o[32];
 #pragma unroll
                 for (int j = 0; j < 32; j++) o[j] = __uint_as_float(v[j]);
-                store_rows32(y, ldy, m0 + (int)rank * 128 + quarter, A.rows, n0 + half * 128 + cb, B.rows, vec, o, sStage + (uint32_t)(warp - 4) * 2048u, lane);
+                if (n0 + cb < B.rows) store_rows32(&tmY, y, ldy, m0 + (int)rank * 128 + quarter, A.rows, n0 + cb, B.rows, tma, o, sStage + (uint32_t)(warp - 4) * 4096u, turn, lane);
             }
-            tc_fence_before();
-            __syncwarp();
         }
+        if (tma && lane == 0) bulk_wait_all();
     }
     tc_fence_before();
     __syncthreads();
@@ -516,7 +534,7 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 }
 
 static constexpr int VMOST = 8;                          // rows of a
-static constexpr int VAHEAD = 4;                         // blocks of the sum a warp has under way
+static constexpr int VAHEAD = 2;                         // blocks of the sum a warp has under way
 
 // At most eight rows of a against all of b: every weight is read once and multiplied so few times that nothing but the reading counts,
 // so there is no pipeline through shared and tensor memory, whose start and end cost more than the reading of a few megabytes.  A warp
@@ -642,14 +660,27 @@ static bool blocks_map(CUtensorMap* m, const BlocksOperand& o, int K, unsigned b
               CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// y as store_rows32 writes it; false where its rows do not start, or do not end, on 16 bytes: a store is cut off at multiples of 16 bytes
+// only, and would write up to 12 bytes behind a row.
+static bool blocks_result_map(CUtensorMap* m, const MatmulBlocksParams& p) {
+    const cuuint64_t size = (cuuint64_t)type_bytes(p.type);
+    EncodeTiledFn fn = blocks_encode_fn();
+    if (!fn || (reinterpret_cast<uintptr_t>(p.y) & 15) || p.ldy * size % 16 || p.b.rows * size % 16 || p.ldy * size >= (1ULL << 40)) return false;
+    const cuuint64_t dims[2] = {(cuuint64_t)p.b.rows, (cuuint64_t)p.a.rows}, strides[1] = {p.ldy * size};
+    const cuuint32_t box[2] = {(cuuint32_t)(64 / size), 32}, estr[2] = {1, 1};
+    const CUtensorMapDataType type = p.type == TAB_FP32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : p.type == TAB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return fn(m, type, 2, p.y, dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 static thread_local char g_last_blocks_kernel[96] = "none";
 const char* matmul_blocks_last_kernel() { return g_last_blocks_kernel; }
 
-struct BlocksPlan { int bn; bool swap; int split, per, nst; };
+struct BlocksPlan { int bn; bool swap; int split, per, nst, ks; };
 
-template <int BN, bool SWAP, int TYPE>
+template <int BN, int KS, bool SWAP, int TYPE>
 static int launch_tile(const MatmulBlocksParams& p, const BlocksPlan& pl, int* status, cudaStream_t stream) {
-    auto kernel = matmul_blocks_tile_kernel<BN, SWAP, TYPE>;
+    auto kernel = matmul_blocks_tile_kernel<BN, KS, SWAP, TYPE>;
     const BlocksOperand &R = SWAP ? p.b : p.a, &C = SWAP ? p.a : p.b;
     alignas(64) CUtensorMap tmR, tmC;
     if (!blocks_map(&tmR, R, p.K, 128) || !blocks_map(&tmC, C, p.K, BN)) return TAB_E_TOO_LARGE;
@@ -658,7 +689,7 @@ static int launch_tile(const MatmulBlocksParams& p, const BlocksPlan& pl, int* s
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return record_cuda_error(e);
-    const int smem = std::max(pl.nst * (128 + BN) * 128, pl.split > 1 ? 128 * (BN + 1) * 4 : 0) + 1024;
+    const int smem = std::max(pl.nst * KS * (128 + BN) * 128, pl.split > 1 ? 128 * (BN + 1) * 4 : 0) + 1024;
     {
         std::lock_guard<std::mutex> lock(mu);
         if (dev < 0 || dev >= 64 || !configured[dev]) {
@@ -669,11 +700,11 @@ static int launch_tile(const MatmulBlocksParams& p, const BlocksPlan& pl, int* s
     }
     const long long tiles_r = (R.rows + 127) / 128, tiles_c = ((long long)C.rows + BN - 1) / BN, grid = tiles_r * tiles_c * pl.split;
     if (grid >= (1LL << 31)) return TAB_E_TOO_LARGE;
-    const int size = p.type == TAB_FP32 ? 4 : 2;
-    const int vec = !(reinterpret_cast<uintptr_t>(p.y) & (8 * size - 1)) && p.ldy % 8 == 0;
-    snprintf(g_last_blocks_kernel, sizeof(g_last_blocks_kernel), "matmul_blocks_tile_kernel<%d,%d> split %d stages %d", BN, (int)SWAP, pl.split, pl.nst);
-    return launch_pdl_as(false, (unsigned)pl.split, kernel, dim3((unsigned)grid), dim3(TT), (size_t)smem, stream, tmR, tmC, R, C, p.y, p.ldy, blocks_of(p.K), pl.per, pl.nst,
-                         (int)tiles_c, pl.split, vec, status);
+    alignas(64) CUtensorMap tmY = tmR;                                     // a stand-in where it is not used
+    const int tma = !SWAP && pl.split == 1 && blocks_result_map(&tmY, p);
+    snprintf(g_last_blocks_kernel, sizeof(g_last_blocks_kernel), "matmul_blocks_tile_kernel<%d,%d,%d> split %d stages %d", BN, KS, (int)SWAP, pl.split, pl.nst);
+    return launch_pdl_as(false, (unsigned)pl.split, kernel, dim3((unsigned)grid), dim3(TT), (size_t)smem, stream, tmR, tmC, tmY, R, C, p.y, p.ldy, blocks_of(p.K), pl.per, pl.nst,
+                         (int)tiles_c, pl.split, tma, status);
 }
 
 // How many pairs the device holds at once (0: none), asked of the occupancy calculator once per device.
@@ -706,12 +737,12 @@ static int launch_pair(const MatmulBlocksParams& p, int pairs, int* status, cuda
     if (!blocks_map(&tmA, p.a, p.K, 128) || !blocks_map(&tmB, p.b, p.K, 128)) return TAB_E_TOO_LARGE;
     const long long tiles_m = ((long long)p.a.rows + 255) / 256, tiles_n = ((long long)p.b.rows + 255) / 256, ntiles = tiles_m * tiles_n;
     if (ntiles >= (1LL << 30)) return TAB_E_TOO_LARGE;
-    const int size = type_bytes(p.type);
-    const int vec = !(reinterpret_cast<uintptr_t>(p.y) & (8 * size - 1)) && p.ldy % 8 == 0;
+    alignas(64) CUtensorMap tmY = tmA;
+    const int tma = blocks_result_map(&tmY, p);
     const unsigned grid = 2u * (unsigned)std::min<long long>(ntiles, pairs);
     snprintf(g_last_blocks_kernel, sizeof(g_last_blocks_kernel), "matmul_blocks_pair_kernel");
     auto kernel = p.type == TAB_FP32 ? matmul_blocks_pair_kernel<TAB_FP32> : p.type == TAB_BF16 ? matmul_blocks_pair_kernel<TAB_BF16> : matmul_blocks_pair_kernel<TAB_FP16>;
-    return launch_pdl_as(false, 2u, kernel, dim3(grid), dim3(PT), (size_t)PSMEM, stream, tmA, tmB, p.a, p.b, p.y, p.ldy, blocks_of(p.K), (int)tiles_m, (int)tiles_n, 8, vec, status);
+    return launch_pdl_as(false, 2u, kernel, dim3(grid), dim3(PT), (size_t)PSMEM, stream, tmA, tmB, tmY, p.a, p.b, p.y, p.ldy, blocks_of(p.K), (int)tiles_m, (int)tiles_n, 8, tma, status);
 }
 
 static int launch_rows(const MatmulBlocksParams& p, int sms, cudaStream_t stream) {
@@ -729,19 +760,19 @@ static int launch_rows(const MatmulBlocksParams& p, int sms, cudaStream_t stream
 #undef TAB_MR
 }
 
-template <int BN, bool SWAP>
+template <int BN, int KS, bool SWAP>
 static int launch_tile_type(const MatmulBlocksParams& p, const BlocksPlan& pl, int* status, cudaStream_t stream) {
-    return p.type == TAB_FP32 ? launch_tile<BN, SWAP, TAB_FP32>(p, pl, status, stream) : p.type == TAB_BF16 ? launch_tile<BN, SWAP, TAB_BF16>(p, pl, status, stream)
-                                                                                                            : launch_tile<BN, SWAP, TAB_FP16>(p, pl, status, stream);
+    return p.type == TAB_FP32 ? launch_tile<BN, KS, SWAP, TAB_FP32>(p, pl, status, stream) : p.type == TAB_BF16 ? launch_tile<BN, KS, SWAP, TAB_BF16>(p, pl, status, stream)
+                                                                                                                : launch_tile<BN, KS, SWAP, TAB_FP16>(p, pl, status, stream);
 }
 
 static BlocksPlan blocks_plan(int M, int N, int KB, int sms) {
-    BlocksPlan pl = {128, false, 1, KB, 6};
+    BlocksPlan pl = {128, false, 1, KB, 3, 2};
 #ifdef TAB_TUNE
-    // Build-time diagnostic (-DTAB_TUNE, never in the shipped library): "columns,swap,split,stages" from the environment.
+    // Build-time diagnostic (-DTAB_TUNE, never in the shipped library): "columns,swap,split,stages,blocks" from the environment.
     if (const char* env = getenv("TAB_MATMUL")) {
         int swap = 0;
-        if (sscanf(env, "%d,%d,%d,%d", &pl.bn, &swap, &pl.split, &pl.nst) == 4) { pl.swap = swap != 0; pl.per = (KB + pl.split - 1) / pl.split; return pl; }
+        if (sscanf(env, "%d,%d,%d,%d,%d", &pl.bn, &swap, &pl.split, &pl.nst, &pl.ks) == 5) { pl.swap = swap != 0; pl.per = (KB + pl.split - 1) / pl.split; return pl; }
     }
 #endif
     return pl;
@@ -765,13 +796,12 @@ int matmul_blocks_dispatch(const MatmulBlocksParams& p, cudaStream_t stream) {
 #endif
     if (pair) return launch_pair(p, pairs, status, stream);
     const BlocksPlan pl = blocks_plan(p.a.rows, p.b.rows, blocks_of(p.K), sms);
-    if (pl.swap) {
-        if (pl.bn == 16) return launch_tile_type<16, true>(p, pl, status, stream);
-        if (pl.bn == 32) return launch_tile_type<32, true>(p, pl, status, stream);
-        return launch_tile_type<64, true>(p, pl, status, stream);
-    }
-    if (pl.bn == 64) return launch_tile_type<64, false>(p, pl, status, stream);
-    return launch_tile_type<128, false>(p, pl, status, stream);
+#define TAB_BT(BN, KS, SW) if (pl.bn == BN && pl.ks == KS && pl.swap == SW) return launch_tile_type<BN, KS, SW>(p, pl, status, stream)
+    TAB_BT(16, 2, true); TAB_BT(32, 2, true); TAB_BT(64, 2, true); TAB_BT(64, 2, false); TAB_BT(128, 2, false);
+    TAB_BT(16, 1, true); TAB_BT(32, 1, true); TAB_BT(64, 1, true); TAB_BT(64, 1, false); TAB_BT(128, 1, false);
+    TAB_BT(16, 4, true); TAB_BT(32, 4, true); TAB_BT(64, 4, true); TAB_BT(64, 4, false);
+#undef TAB_BT
+    return TAB_E_TOO_LARGE;
 }
 
 }  // namespace tab
