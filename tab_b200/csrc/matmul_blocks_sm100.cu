@@ -745,13 +745,10 @@ static int launch_pair(const MatmulBlocksParams& p, int pairs, int* status, cuda
     return launch_pdl_as(false, 2u, kernel, dim3(grid), dim3(PT), (size_t)PSMEM, stream, tmA, tmB, tmY, p.a, p.b, p.y, p.ldy, blocks_of(p.K), (int)tiles_m, (int)tiles_n, 8, tma, status);
 }
 
-static int launch_rows(const MatmulBlocksParams& p, int sms, cudaStream_t stream) {
+static int launch_rows(const MatmulBlocksParams& p, cudaStream_t stream) {
     const int KB = blocks_of(p.K);
     const unsigned grid = (unsigned)(((long long)p.b.rows + 15) / 16);
-    int warps = 8;
-#ifdef TAB_TUNE
-    if (const char* env = getenv("TAB_KW")) warps = atoi(env);
-#endif
+    const int warps = 8;
     const int per = (KB + warps - 1) / warps;
     snprintf(g_last_blocks_kernel, sizeof(g_last_blocks_kernel), "matmul_blocks_rows_kernel %d warps", warps);
 #define TAB_MR(FA, FB) launch_pdl(matmul_blocks_rows_kernel<FA, FB>, dim3(grid), dim3(32 * warps), 0, stream, p.a, p.b, p.y, p.ldy, p.type, p.K, per)
@@ -766,8 +763,29 @@ static int launch_tile_type(const MatmulBlocksParams& p, const BlocksPlan& pl, i
                                                                                                                 : launch_tile<BN, KS, SWAP, TAB_FP16>(p, pl, status, stream);
 }
 
+// Tile, split and stages where there are too few tiles for the pairs.  Measured with cold operands (us, bf16 result, square scales of b):
+//   columns   Waits and issues cost the MMA warp about 300 cycles a stage whatever it holds, so a stage holds four blocks where a CTA has
+//             the SM to itself: 256x4096x4096, 128 x 64 tiles, stages of 1 / 2 / 4 blocks 17.4 / 12.5 / 10.6; of 128 x 128: 18.6 / 13.5.
+//             64 columns while that makes at most a tile an SM (1024x1024x8192 16.9, 128 columns 22.8), then 128 (1024x2048x2048 9.4,
+//             64 columns 10.0), and with two CTAs an SM small stages (2048x2048x2048 13.0, stages of two blocks 17.8; pairs 14.1).
+//   swap      At most 64 rows of a: the 128-row side takes the weights (16x8192x2048 6.9, else 9.7; 40x8192x2048 8.9 / 9.7).
+//   split     Meeting in shared memory costs about 1.2 us, a block of the sum 0.2: ranks keep eight blocks, and sums of fewer than 32 are
+//             not split (12x4096x4096: 1 / 4 / 8 ranks 11.7 / 8.0 / 8.3; 16x8192x2048 1 / 2 / 4 ranks 6.9 / 8.1 / 8.3; 128x128x8192: 8 ranks
+//             8.2, 4 9.9); wide tiles only while most SMs would idle (100x4096x4096, 64 tiles: 1 / 4 ranks 10.4 / 12.1).
 static BlocksPlan blocks_plan(int M, int N, int KB, int sms) {
-    BlocksPlan pl = {128, false, 1, KB, 3, 2};
+    const long long rows = ((long long)M + 127) / 128, tiles64 = rows * (((long long)N + 63) / 64), tiles128 = rows * (((long long)N + 127) / 128);
+    BlocksPlan pl = {64, M <= 64, 1, KB, 2, 4};
+    long long tiles = tiles64;
+    if (pl.swap) {
+        pl.bn = M <= 16 ? 16 : M <= 32 ? 32 : 64;
+        tiles = ((long long)N + 127) / 128;
+    } else if (tiles64 > sms) {
+        pl.bn = 128; pl.nst = 3; pl.ks = tiles128 <= sms ? 2 : 1;
+        tiles = tiles128;
+    }
+    while (pl.split < 8 && KB >= 32 && KB >= 16 * pl.split && tiles * 2 * pl.split <= (pl.swap ? 2 * sms : sms / 2)) pl.split *= 2;
+    if (pl.swap && tiles * pl.split > sms) { pl.ks = 2; pl.nst = pl.bn == 64 ? 2 : 3; }      // (room for a second CTA on an SM, or nearly)
+    pl.per = (KB + pl.split - 1) / pl.split;
 #ifdef TAB_TUNE
     // Build-time diagnostic (-DTAB_TUNE, never in the shipped library): "columns,swap,split,stages,blocks" from the environment.
     if (const char* env = getenv("TAB_MATMUL")) {
@@ -783,23 +801,20 @@ int matmul_blocks_dispatch(const MatmulBlocksParams& p, cudaStream_t stream) {
     if (stalled(status)) return TAB_E_STALLED;
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    bool few = p.a.rows <= VMOST;
-#ifdef TAB_TUNE
-    if (const char* env = getenv("TAB_MATMUL")) few = env[0] == 'v' && p.a.rows <= VMOST;
-#endif
-    if (few) return launch_rows(p, sms, stream);
-    const long long tiles = ((long long)p.a.rows + 255) / 256 * (((long long)p.b.rows + 255) / 256);
+    // pairs from two rounds of 128 x 128 tiles on: 1536x4096x1024 (384 of them) 15.8, single CTAs 17.1; 4096x1024x1024 (256) 12.4 / 9.9
+    const long long tiles128 = ((long long)p.a.rows + 127) / 128 * (((long long)p.b.rows + 127) / 128);
     const int pairs = matmul_pairs();
-    bool pair = pairs > 0 && tiles * 2 > pairs;
+    bool few = p.a.rows <= VMOST, pair = pairs > 0 && p.a.rows > 64 && tiles128 > 2LL * sms;
 #ifdef TAB_TUNE
-    if (const char* env = getenv("TAB_MATMUL")) pair = env[0] == 'p';
+    if (const char* env = getenv("TAB_MATMUL")) { few = env[0] == 'v' && p.a.rows <= VMOST; pair = env[0] == 'p'; }
 #endif
+    if (few) return launch_rows(p, stream);
     if (pair) return launch_pair(p, pairs, status, stream);
     const BlocksPlan pl = blocks_plan(p.a.rows, p.b.rows, blocks_of(p.K), sms);
 #define TAB_BT(BN, KS, SW) if (pl.bn == BN && pl.ks == KS && pl.swap == SW) return launch_tile_type<BN, KS, SW>(p, pl, status, stream)
-    TAB_BT(16, 2, true); TAB_BT(32, 2, true); TAB_BT(64, 2, true); TAB_BT(64, 2, false); TAB_BT(128, 2, false);
-    TAB_BT(16, 1, true); TAB_BT(32, 1, true); TAB_BT(64, 1, true); TAB_BT(64, 1, false); TAB_BT(128, 1, false);
-    TAB_BT(16, 4, true); TAB_BT(32, 4, true); TAB_BT(64, 4, true); TAB_BT(64, 4, false);
+    TAB_BT(16, 2, true); TAB_BT(32, 2, true); TAB_BT(64, 2, true);
+    TAB_BT(16, 4, true); TAB_BT(32, 4, true); TAB_BT(64, 4, true);
+    TAB_BT(64, 4, false); TAB_BT(128, 2, false); TAB_BT(128, 1, false);
 #undef TAB_BT
     return TAB_E_TOO_LARGE;
 }

@@ -181,7 +181,8 @@ def device_blocks(cuda, q, s, format):
 
 SIZES = [(1, 1, 1), (1, 128, 128), (1, 256, 1024), (2, 130, 96), (5, 512, 4096), (16, 100, 640), (17, 1000, 1040), (33, 64, 513), (64, 384, 256), (100, 129, 300),
          (128, 128, 127), (129, 257, 1000), (200, 2048, 512), (256, 256, 2048), (300, 300, 100), (513, 777, 1411), (1024, 512, 384), (40, 1024, 6000), (257, 1, 4100), (1, 5, 30000),
-         (2304, 1300, 700), (2600, 2900, 300), (1030, 10000, 513), (5000, 4100, 130)]
+         (2304, 1300, 700), (2600, 2900, 300), (1030, 10000, 513), (5000, 4100, 130),
+         (8, 72, 4500), (9, 1000, 4224), (16, 129, 16500), (24, 4000, 4096), (33, 9000, 8200), (64, 20000, 520), (65, 64, 9000), (140, 4100, 5000), (1000, 2100, 384), (1024, 16, 4096), (1500, 1500, 640)]
 
 
 @pytest.mark.gpu
