@@ -10,44 +10,117 @@
 
 namespace tab {
 
+// Eight values as they are loaded, so that 16-bit types take half of the registers; their magnitudes are compared as integers, two at a
+// time (the order of the bits is that of the values).
+template <int TYPE>
+struct Eight {
+    static constexpr int W = TYPE == TAB_FP32 ? 8 : 4;                     // words
+    static constexpr uint32_t SIGNS = TYPE == TAB_FP32 ? 0x7FFFFFFFu : 0x7FFF7FFFu;
+    static constexpr uint32_t INF = TYPE == TAB_FP32 ? 0x7F800000u : TYPE == TAB_BF16 ? 0x7F80u : 0x7C00u;
+    uint32_t w[W];
+    template <typename T>
+    __device__ __forceinline__ void load(const T* p, int n, bool vec) {
+        if (vec && n >= 8) {
+            if (TYPE == TAB_FP32) {
+                asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]), "=r"(w[4 % W]), "=r"(w[5 % W]), "=r"(w[6 % W]), "=r"(w[7 % W]) : "l"(p));
+            } else {
+                const uint4 u = *reinterpret_cast<const uint4*>(p);
+                w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < W; i++) w[i] = 0;
+        if (n <= 0) return;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (i >= n) continue;
+            if (TYPE == TAB_FP32) w[i % W] = reinterpret_cast<const uint32_t*>(p)[i];
+            else w[i / 2 % W] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[i] << (16 * (i & 1));
+        }
+    }
+    __device__ __forceinline__ float at(int i) const {
+        if (TYPE == TAB_FP32) return __uint_as_float(w[i % W]);
+        const uint32_t u = w[i / 2 % W];
+        if (TYPE == TAB_BF16) return __uint_as_float(i & 1 ? u & 0xFFFF0000u : u << 16);
+        return __half2float(__ushort_as_half((unsigned short)(i & 1 ? u >> 16 : u & 0xFFFFu)));
+    }
+    // Word i's magnitudes; with `odd` those of NaN and infinities are 0 (they keep to their own element).
+    __device__ __forceinline__ uint32_t size(int i, bool odd) const {
+        uint32_t u = w[i] & SIGNS;
+        if (odd) {
+            if (TYPE == TAB_FP32) u = u < INF ? u : 0u;
+            else u = ((u & 0xFFFFu) < INF ? u & 0xFFFFu : 0u) | ((u >> 16) < INF ? u & 0xFFFF0000u : 0u);
+        }
+        return u;
+    }
+    static __device__ __forceinline__ uint32_t most(uint32_t a, uint32_t b) { return TYPE == TAB_FP32 ? max(a, b) : __vmaxu2(a, b); }
+    // The larger of a word's magnitudes, in the type's bits; and those bits as the bits of a float.
+    static __device__ __forceinline__ uint32_t one(uint32_t a) { return TYPE == TAB_FP32 ? a : max(a & 0xFFFFu, a >> 16); }
+    static __device__ __forceinline__ uint32_t float_bits(uint32_t a) {
+        return TYPE == TAB_FP32 ? a : TYPE == TAB_BF16 ? a << 16 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)a)));
+    }
+    __device__ __forceinline__ uint32_t largest(bool odd) const {
+        uint32_t m = size(0, odd);
+#pragma unroll
+        for (int i = 1; i < W; i++) m = most(m, size(i, odd));
+        return one(m);
+    }
+};
+// narrow8 of eight floats where `odd` says that there may be infinities among them.
+template <int FORMAT>
+__device__ __forceinline__ uint2 narrow8_of(const float (&v)[8], float inv, bool odd) {
+    if (odd) return narrow8<FORMAT>(v, inv);
+    uint2 r;
+    r.x = narrow2<FORMAT>(v[0] * inv, v[1] * inv) | narrow2<FORMAT>(v[2] * inv, v[3] * inv) << 16;
+    r.y = narrow2<FORMAT>(v[4] * inv, v[5] * inv) | narrow2<FORMAT>(v[6] * inv, v[7] * inv) << 16;
+    return r;
+}
+
 static constexpr int QROWS = 4;              // blocks a half-warp of the rows kernel has in flight
 
 // hk half-warps of the sixteen lie along K, the others along M.
 template <int TYPE, int FORMAT>
 __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantBlocksParams p, int KB, int hk_log2, int chunks, int vec, int qvec) {
     using T = typename ElemOf<TYPE>::type;
+    using E = Eight<TYPE>;
     pdl_wait();
     const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
     const int hk = 1 << hk_log2, rstep = 16 >> hk_log2;
     const int kb = (int)(blockIdx.x % (unsigned)chunks) * hk + (half & (hk - 1));
     const long long row0 = (long long)(blockIdx.x / (unsigned)chunks) * (rstep * QROWS) + (half >> hk_log2);
     const int k0 = kb * BLK + l * 8, n = kb < KB ? p.K - k0 : 0;
-    float v[QROWS][8];
+    E v[QROWS];
 #pragma unroll
     for (int i = 0; i < QROWS; i++) {
         const long long m = row0 + i * rstep;
-        load8(static_cast<const T*>(p.x) + m * p.ldx + k0, m < p.M ? n : 0, vec, v[i]);
+        v[i].load(static_cast<const T*>(p.x) + m * p.ldx + k0, m < p.M ? n : 0, vec);
     }
     pdl_launch_dependents();
+    uint32_t high = 0;
+#pragma unroll
+    for (int i = 0; i < QROWS; i++) high = max(high, v[i].largest(false));
+    const bool odd = __any_sync(0xFFFFFFFFu, high >= E::INF);
 #pragma unroll
     for (int i = 0; i < QROWS; i++) {
         const long long m = row0 + i * rstep;
-        uint32_t a = 0;
+        const int e = scale_exponent(E::float_bits(half_warp_max(v[i].largest(odd))), FORMAT);
+        if (m >= p.M || kb >= KB) continue;                                // (shuffles of the next rows wait for these lanes)
+        float f[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) a = max(a, finite_bits(v[i][j]));
-        const int e = scale_exponent(half_warp_max(a), FORMAT);
-        if (m >= p.M || kb >= KB) continue;                                // (no shuffles below)
-        store_bytes8(p.q + m * p.ldq + k0, n, qvec, narrow8<FORMAT>(v[i], exp2_int(-e)));
+        for (int j = 0; j < 8; j++) f[j] = v[i].at(j);
+        store_bytes8(p.q + m * p.ldq + k0, n, qvec, narrow8_of<FORMAT>(f, exp2_int(-e), odd));
         if (l == 0) p.s[m * KB + kb] = (uint8_t)(e + 127);
     }
 }
 
 // 128 x 128 values: half-warp h holds rows 8h .. 8h+7, its lane l columns 8l .. 8l+7.
 template <int TYPE, int FORMAT, bool SQUARE>
-__global__ void __launch_bounds__(256, 2) quantize_tiles_kernel(QuantBlocksParams p, int KB, int MB, int vec, int qvec, int qtvec) {
+__global__ void __launch_bounds__(256, TYPE == TAB_FP32 ? 2 : 4) quantize_tiles_kernel(QuantBlocksParams p, int KB, int MB, int vec, int qvec, int qtvec) {
     using T = typename ElemOf<TYPE>::type;
-    __shared__ uint32_t colmax[16][BLK];
-    __shared__ uint32_t colexp[BLK];
+    using E = Eight<TYPE>;
+    __shared__ uint32_t colmax[16][16 * E::W + 1];                         // magnitudes as a lane's words hold them; a square's: word 0
+    __shared__ int colexp[BLK];
     __shared__ __align__(16) uint2 turned[BLK * 16];                       // [column][8 rows], chunks of a column permuted
     pdl_wait();
     const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
@@ -55,79 +128,79 @@ __global__ void __launch_bounds__(256, 2) quantize_tiles_kernel(QuantBlocksParam
     const long long mb = blockIdx.x / (unsigned)KB;
     const long long m0 = mb * BLK + half * 8;
     const int k0 = kb * BLK + l * 8, n = p.K - k0;
-    float v[8][8];
+    E v[8];
 #pragma unroll
-    for (int r = 0; r < 8; r++) load8(static_cast<const T*>(p.x) + (m0 + r) * p.ldx + k0, m0 + r < p.M ? n : 0, vec, v[r]);
+    for (int r = 0; r < 8; r++) v[r].load(static_cast<const T*>(p.x) + (m0 + r) * p.ldx + k0, m0 + r < p.M ? n : 0, vec);
     pdl_launch_dependents();
-    int ecol[8];
+    uint32_t a[E::W];
+    auto maxima = [&](bool odd) {
+#pragma unroll
+        for (int i = 0; i < E::W; i++) a[i] = v[0].size(i, odd);
+#pragma unroll
+        for (int r = 1; r < 8; r++)
+#pragma unroll
+            for (int i = 0; i < E::W; i++) a[i] = E::most(a[i], v[r].size(i, odd));
+        uint32_t m = a[0];
+#pragma unroll
+        for (int i = 1; i < E::W; i++) m = E::most(m, a[i]);
+        return E::one(m);
+    };
+    uint32_t high = maxima(false);
+    const bool odd = __any_sync(0xFFFFFFFFu, high >= E::INF);
+    if (odd) high = maxima(true);
+    int e = 0;                                                             // a square's scale
     if (SQUARE) {
-        uint32_t a = 0;
-#pragma unroll
-        for (int r = 0; r < 8; r++)
-#pragma unroll
-            for (int c = 0; c < 8; c++) a = max(a, finite_bits(v[r][c]));
-        a = half_warp_max(a);
-        if (l == 0) colmax[0][half] = a;
+        high = half_warp_max(high);
+        if (l == 0) colmax[half][0] = high;
         __syncthreads();
 #pragma unroll
-        for (int i = 0; i < 16; i++) a = max(a, colmax[0][i]);
-        const int e = scale_exponent(a, FORMAT);
+        for (int i = 0; i < 16; i++) high = max(high, colmax[i][0]);
+        e = scale_exponent(E::float_bits(high), FORMAT);
         if (threadIdx.x == 0) {
             if (p.s) p.s[mb * KB + kb] = (uint8_t)(e + 127);
             if (p.st) p.st[(long long)kb * MB + mb] = (uint8_t)(e + 127);
         }
-        const float inv = exp2_int(-e);
-        if (p.q) {
-#pragma unroll
-            for (int r = 0; r < 8; r++)
-                if (m0 + r < p.M) store_bytes8(p.q + (m0 + r) * p.ldq + k0, n, qvec, narrow8<FORMAT>(v[r], inv));
-        }
-#pragma unroll
-        for (int c = 0; c < 8; c++) ecol[c] = e;
     } else {
-        uint32_t a[8];
 #pragma unroll
-        for (int c = 0; c < 8; c++) a[c] = 0;
-#pragma unroll
-        for (int r = 0; r < 8; r++) {
-            uint32_t row = 0;
-#pragma unroll
-            for (int c = 0; c < 8; c++) {
-                const uint32_t b = finite_bits(v[r][c]);
-                row = max(row, b);
-                a[c] = max(a[c], b);
-            }
-            const int e = scale_exponent(half_warp_max(row), FORMAT);
-            if (m0 + r < p.M) {
-                store_bytes8(p.q + (m0 + r) * p.ldq + k0, n, qvec, narrow8<FORMAT>(v[r], exp2_int(-e)));
-                if (l == 0) p.s[(m0 + r) * KB + kb] = (uint8_t)(e + 127);
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < 8; c++) colmax[half][l * 8 + c] = a[c];
+        for (int i = 0; i < E::W; i++) colmax[half][l * E::W + i] = a[i];
         __syncthreads();
-        if (threadIdx.x < BLK) {
+        if (threadIdx.x < BLK / (8 / E::W)) {                              // a thread: one word's columns
             uint32_t b = 0;
 #pragma unroll
-            for (int i = 0; i < 16; i++) b = max(b, colmax[i][threadIdx.x]);
-            const int e = scale_exponent(b, FORMAT);
-            colexp[threadIdx.x] = (uint32_t)e;
-            const long long k = (long long)kb * BLK + threadIdx.x;
-            if (k < p.K) p.st[k * MB + mb] = (uint8_t)(e + 127);
-        }
-        __syncthreads();
+            for (int i = 0; i < 16; i++) b = E::most(b, colmax[i][threadIdx.x]);
 #pragma unroll
-        for (int c = 0; c < 8; c++) ecol[c] = (int)colexp[l * 8 + c];
+            for (int c = 0; c < 8 / E::W; c++) {
+                const int col = threadIdx.x * (8 / E::W) + c;
+                const int ec = scale_exponent(E::float_bits(TYPE == TAB_FP32 ? b : b >> (16 * c) & 0xFFFFu), FORMAT);
+                colexp[col] = ec;
+                const long long k = (long long)kb * BLK + col;
+                if (k < p.K) p.st[k * MB + mb] = (uint8_t)(ec + 127);
+            }
+        }
+    }
+    if (!SQUARE || p.q) {
+#pragma unroll
+        for (int r = 0; r < 8; r++) {
+            const int er = SQUARE ? e : scale_exponent(E::float_bits(half_warp_max(v[r].largest(odd))), FORMAT);
+            float f[8];
+#pragma unroll
+            for (int c = 0; c < 8; c++) f[c] = v[r].at(c);
+            if (m0 + r < p.M) {
+                store_bytes8(p.q + (m0 + r) * p.ldq + k0, n, qvec, narrow8_of<FORMAT>(f, exp2_int(-er), odd));
+                if (!SQUARE && l == 0) p.s[(m0 + r) * KB + kb] = (uint8_t)(er + 127);
+            }
+        }
     }
     if (SQUARE && !p.qt) return;
+    __syncthreads();
     // Chunk h of column c lies at place h ^ (c / 8): the sixteen lanes that write different columns, and the sixteen that read
     // different chunks, each meet all banks.
 #pragma unroll
     for (int c = 0; c < 8; c++) {
-        float t[8];
+        float f[8];
 #pragma unroll
-        for (int r = 0; r < 8; r++) t[r] = v[r][c];
-        turned[(l * 8 + c) * 16 + (half ^ l)] = narrow8<FORMAT>(t, exp2_int(-ecol[c]));
+        for (int r = 0; r < 8; r++) f[r] = v[r].at(c);
+        turned[(l * 8 + c) * 16 + (half ^ l)] = narrow8_of<FORMAT>(f, exp2_int(SQUARE ? -e : -colexp[l * 8 + c]), odd);
     }
     __syncthreads();
     const long long mt = mb * BLK + l * 8;
