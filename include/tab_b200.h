@@ -294,14 +294,16 @@ enum { TAB_E4M3 = 0, TAB_E5M2 = 1 };                   /* formats of 8-bit float
  * x [M][K] of `type`, row pitch ldx elements -> blocks.  s = 2^e with the least e >= -127 for which max|x| <= F * 2^e over the finite
  * values of the block, F the format's largest value (e = 0 where they are all zero); q = x / s rounded to nearest, ties to even.
  * NaN stays NaN; an infinity becomes NaN in e4m3, which has none, and stays one in e5m2; neither touches the other values of its block.
- *   square == 0   blocks of 128 consecutive values of a row: q [M][K], pitch ldq bytes, s [M][ceil(K/128)]; and, unless qt is NULL,
- *                 from the same reading of x, blocks of 128 consecutive values of a column: qt [K][M], pitch ldqt, st [K][ceil(M/128)].
- *   square == 1   blocks of 128 x 128: q [M][K], s [ceil(M/128)][ceil(K/128)] and / or their transposes qt [K][M],
- *                 st [ceil(K/128)][ceil(M/128)] (either pair may be NULL).
+ *   square == 0   blocks of 128 consecutive values of a row: q [M][K], pitch ldq bytes, and their scales block by block: that of row m,
+ *                 block j at s[j * lds + m].  Unless qt is NULL, from the same reading of x, blocks of 128 consecutive values of a column:
+ *                 qt [K][M], pitch ldqt, the scale of column k, block j at st[j * ldst + k].
+ *   square == 1   blocks of 128 x 128: q [M][K], s [ceil(M/128)][ceil(K/128)], pitch lds, and / or their transposes qt [K][M],
+ *                 st [ceil(K/128)][ceil(M/128)], pitch ldst (either pair may be NULL).
  * The last block of an axis may be short.  Bytes between rows are not written.
  */
 int tab_quantize_blocks_launch(const void* x, int type, long long ldx, long long M, int K, int format, int square,
-                               void* q, long long ldq, uint8_t* s, void* qt, long long ldqt, uint8_t* st, tab_stream_t stream);
+                               void* q, long long ldq, uint8_t* s, long long lds, void* qt, long long ldqt, uint8_t* st, long long ldst,
+                               tab_stream_t stream);
 
 /*
  * y[m][n] = sum over k of a[m][k] sa(m, k/128) b[n][k] sb(n, k/128), accumulated in fp32 and rounded once to `type`.
@@ -320,7 +322,7 @@ const char* tab_last_matmul_kernel(void);
  * ---- the residual stream between two blocks ------------------------------------------------------------------------------------
  *   u = norm(y) * w1 + b1      the norm behind a block; u = y without w1
  *   r = alpha * x + gate * u   the residual stream, kept in the type of y; without x the first term, without a gate its factor is left out
- *   h = norm(r) * w2 + b2      the norm before the next block, of r as it is kept; as values of that type or, with q, as blocks of 128
+ *   h = norm(r) * w2 + b2      the norm before the next block, of r as it is kept; as values of that type or, with q, as blocks of 128 of a row
  * norm(v) = v / sqrt(mean(v^2) + eps) (TAB_NORM_RMS) or (v - mean(v)) / sqrt(var(v) + eps) (TAB_NORM_LAYER), over the C elements of a row.
  * NULL where absent: x, w1, b1, gate, w2, b2, r, h, q (with s), stats; shifts b1, b2 belong to TAB_NORM_LAYER.  Pitches are in elements (bytes for q).  C <= 16384.
  * stats: float [M][4], kept for the backward pass.  Sums and statistics are fp32.
@@ -337,8 +339,8 @@ typedef struct {
     int C;
     long long M;
     void *r, *h, *q;
-    uint8_t* s;                  /* [M][ceil(C/128)] */
-    long long ldr, ldh, ldq;
+    uint8_t* s;                  /* the scale of row m, block j at s[j * lds + m] */
+    long long ldr, ldh, ldq, lds;
     int format;                  /* of q */
     float* stats;
 } tab_norm_t;

@@ -43,7 +43,7 @@ SYMBOLS = {
     "tab_conv2d_static_launch": (_c.c_int, [_c.c_void_p] * 5 + [_c.c_int] * 12 + [_c.c_void_p]),
     "tab_residual_threshold_launch": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_float, _c.c_int, _c.c_longlong, _c.c_void_p]),
     "tab_quantize_blocks_launch": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_longlong, _c.c_longlong, _c.c_int, _c.c_int, _c.c_int] +
-                                   [_c.c_void_p, _c.c_longlong, _c.c_void_p] * 2 + [_c.c_void_p]),
+                                   [_c.c_void_p, _c.c_longlong, _c.c_void_p, _c.c_longlong] * 2 + [_c.c_void_p]),
     "tab_matmul_blocks_launch": (_c.c_int, [_c.c_void_p, _c.c_int, _c.c_longlong, _c.c_void_p, _c.c_int, _c.c_longlong, _c.c_longlong] * 2 +
                                  [_c.c_void_p, _c.c_int, _c.c_longlong, _c.c_int, _c.c_int, _c.c_int, _c.c_void_p]),
     "tab_last_matmul_kernel": (_c.c_char_p, []),
@@ -60,7 +60,7 @@ class NormArgs(_c.Structure):
     """``tab_norm_t``."""
     _fields_ = ([(n, _c.c_void_p) for n in ("y", "x", "w1", "b1", "w2", "b2", "gate")] + [(n, _c.c_longlong) for n in ("ldy", "ldx", "ldg")] +
                 [(n, _c.c_int) for n in ("type", "ptype", "gtype", "gkind", "layer")] + [("alpha", _c.c_float), ("eps", _c.c_float), ("C", _c.c_int), ("M", _c.c_longlong)] +
-                [(n, _c.c_void_p) for n in ("r", "h", "q", "s")] + [(n, _c.c_longlong) for n in ("ldr", "ldh", "ldq")] + [("format", _c.c_int), ("stats", _c.c_void_p)])
+                [(n, _c.c_void_p) for n in ("r", "h", "q", "s")] + [(n, _c.c_longlong) for n in ("ldr", "ldh", "ldq", "lds")] + [("format", _c.c_int), ("stats", _c.c_void_p)])
 
 
 class NormBackwardArgs(_c.Structure):

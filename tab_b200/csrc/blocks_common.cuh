@@ -21,10 +21,12 @@ struct QuantBlocksParams {
     int format;                              // TAB_E4M3 or TAB_E5M2
     uint8_t* q;                              // [M][K], row pitch ldq
     long long ldq;
-    uint8_t* s;                              // rows: [M][ceil(K/128)]; squares: [ceil(M/128)][ceil(K/128)]
+    uint8_t* s;                              // rows: [ceil(K/128)][M], pitch lds; squares: [ceil(M/128)][ceil(K/128)]
+    long long lds;
     uint8_t* qt;                             // [K][M], row pitch ldqt
     long long ldqt;
-    uint8_t* st;                             // [K][ceil(M/128)]; squares: the transpose of s
+    uint8_t* st;                             // columns: [ceil(M/128)][K], pitch ldst; squares: the transpose of s
+    long long ldst;
 };
 int quantize_blocks_dispatch(const QuantBlocksParams& p, int type, bool square, cudaStream_t stream);
 

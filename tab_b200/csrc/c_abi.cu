@@ -402,16 +402,19 @@ static bool type_ok(int type) { return type == TAB_FP32 || type == TAB_BF16 || t
 static bool format_ok(int format) { return format == TAB_E4M3 || format == TAB_E5M2; }
 
 int tab_quantize_blocks_launch(const void* x, int type, long long ldx, long long M, int K, int format, int square,
-                               void* q, long long ldq, uint8_t* s, void* qt, long long ldqt, uint8_t* st, tab_stream_t stream) {
+                               void* q, long long ldq, uint8_t* s, long long lds, void* qt, long long ldqt, uint8_t* st, long long ldst,
+                               tab_stream_t stream) {
     if (!type_ok(type) || !format_ok(format) || (square != 0 && square != 1) || M < 0 || K < 0) return TAB_E_BAD_ARGUMENT;
     if (M == 0 || K == 0) return TAB_OK;
     if (!x || (!square && !q) || (!q && !qt) || (q && !s) || (qt && !st)) return TAB_E_NULL_POINTER;
+    const long long KB = blocks_of(K), MB = blocks_of(M);
     if ((M > 1 && (ldx < K || (q && ldq < K))) || (qt && K > 1 && ldqt < M)) return TAB_E_BAD_ARGUMENT;
+    if ((q && (square ? MB > 1 && lds < KB : KB > 1 && lds < M)) || (qt && (square ? KB > 1 && ldst < MB : MB > 1 && ldst < K))) return TAB_E_BAD_ARGUMENT;
     if (misaligned(x, (uintptr_t)type_bytes(type) - 1)) return TAB_E_ALIGNMENT;
     // pitches of single rows are of no account; beyond 2^31 rows or 2^40 elements between two of them the index arithmetic ends
-    if (M >= (1LL << 31) || (M > 1 && (ldx >= (1LL << 40) || ldq >= (1LL << 40))) || (K > 1 && ldqt >= (1LL << 40))) return TAB_E_TOO_LARGE;
-    QuantBlocksParams p = {x, M > 1 ? ldx : 0, M, K, format, static_cast<uint8_t*>(q), M > 1 ? ldq : 0, q ? s : nullptr,
-                           static_cast<uint8_t*>(qt), K > 1 ? ldqt : 0, qt ? st : nullptr};
+    if (M >= (1LL << 31) || (M > 1 && (ldx >= (1LL << 40) || ldq >= (1LL << 40))) || (K > 1 && ldqt >= (1LL << 40)) || (q && lds >= (1LL << 40)) || (qt && ldst >= (1LL << 40))) return TAB_E_TOO_LARGE;
+    QuantBlocksParams p = {x, M > 1 ? ldx : 0, M, K, format, static_cast<uint8_t*>(q), M > 1 ? ldq : 0, q ? s : nullptr, lds,
+                           static_cast<uint8_t*>(qt), K > 1 ? ldqt : 0, qt ? st : nullptr, ldst};
     return quantize_blocks_dispatch(p, type, square == 1, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -461,7 +464,7 @@ int tab_residual_norm_launch(const tab_norm_t* args, tab_stream_t stream) {
     if (p.gkind == TAB_GATE_NONE) p.gate = nullptr;
     if (!p.y || (p.gkind != TAB_GATE_NONE && !p.gate) || (p.q && !p.s) || ((p.h || p.q) && !p.w2)) return TAB_E_NULL_POINTER;
     if (p.q && !format_ok(p.format)) return TAB_E_BAD_ARGUMENT;
-    if (p.M > 1 && (p.ldy < p.C || (p.x && p.ldx < p.C) || (p.r && p.ldr < p.C) || (p.h && p.ldh < p.C) || (p.q && p.ldq < p.C) ||
+    if (p.M > 1 && (p.ldy < p.C || (p.x && p.ldx < p.C) || (p.r && p.ldr < p.C) || (p.h && p.ldh < p.C) || (p.q && p.ldq < p.C) || (p.q && p.C > BLK && p.lds < p.M) ||
                     (p.gkind == TAB_GATE_FULL && p.ldg < p.C) || (p.gkind == TAB_GATE_TOKEN && p.ldg < 0))) return TAB_E_BAD_ARGUMENT;
     if (odd_address(p.y, p.type) || odd_address(p.x, p.type) || odd_address(p.r, p.type) || odd_address(p.h, p.type) || odd_address(p.w1, p.ptype) ||
         odd_address(p.b1, p.ptype) || odd_address(p.w2, p.ptype) || odd_address(p.b2, p.ptype) || odd_address(p.gate, p.gtype) || misaligned(p.stats, 15))

@@ -250,6 +250,19 @@ std::vector<int64_t> with_last(const Tensor& t, int64_t n) {
     return s;
 }
 
+// Scales `shape` (rows x n) that lie block by block.
+Tensor new_scales(const Tensor& like, at::IntArrayRef shape, int64_t rows, int64_t n) {
+    const int64_t pitch = (rows + 15) / 16 * 16;
+    std::vector<int64_t> strides(shape.size());
+    int64_t step = 1;
+    for (int64_t i = (int64_t)shape.size() - 2; i >= 0; i--) {
+        strides[i] = step;
+        step *= shape[i];
+    }
+    strides.back() = pitch;
+    return make(like, {n * pitch}, at::kFloat8_e8m0fnu).as_strided(shape, strides);
+}
+
 struct Quantized { Tensor q, s, qt, st; };
 bool quantize_any(const Tensor& x, at::ScalarType dtype, bool both, bool square, Quantized& o) {
     Rows r;
@@ -257,14 +270,15 @@ bool quantize_any(const Tensor& x, at::ScalarType dtype, bool both, bool square,
     if (!on_cuda(x) || type_of(x) < 0 || format < 0 || (square && x.dim() != 2) || !r.of(x)) return false;
     const c10::cuda::CUDAGuard guard(x.device());
     o.q = new_blocks(x, x.sizes(), r.M, r.K, dtype);
-    o.s = square ? make(x, {blocks(r.M), blocks(r.K)}, at::kFloat8_e8m0fnu) : make(x, with_last(x, blocks(r.K)), at::kFloat8_e8m0fnu);
+    o.s = square ? make(x, {blocks(r.M), blocks(r.K)}, at::kFloat8_e8m0fnu) : new_scales(x, with_last(x, blocks(r.K)), r.M, blocks(r.K));
     if (both) {
         o.qt = new_blocks(x, {r.K, r.M}, r.K, r.M, dtype);
-        o.st = make(x, {square ? blocks(r.K) : r.K, blocks(r.M)}, at::kFloat8_e8m0fnu);
+        o.st = square ? make(x, {blocks(r.K), blocks(r.M)}, at::kFloat8_e8m0fnu) : new_scales(x, {r.K, blocks(r.M)}, r.K, blocks(r.M));
     }
-    return tab_quantize_blocks_launch(x.data_ptr(), type_of(x), r.pitch, r.M, (int)r.K, format, square, o.q.data_ptr(), (r.K + 15) / 16 * 16,
-                                      static_cast<uint8_t*>(o.s.data_ptr()), both ? o.qt.data_ptr() : nullptr, (r.M + 15) / 16 * 16,
-                                      both ? static_cast<uint8_t*>(o.st.data_ptr()) : nullptr, stream_of(x)) == TAB_OK;
+    const int64_t pk = (r.K + 15) / 16 * 16, pm = (r.M + 15) / 16 * 16;
+    return tab_quantize_blocks_launch(x.data_ptr(), type_of(x), r.pitch, r.M, (int)r.K, format, square, o.q.data_ptr(), pk, static_cast<uint8_t*>(o.s.data_ptr()),
+                                      square ? blocks(r.K) : pm, both ? o.qt.data_ptr() : nullptr, pm, both ? static_cast<uint8_t*>(o.st.data_ptr()) : nullptr,
+                                      square ? blocks(r.M) : pk, stream_of(x)) == TAB_OK;
 }
 py::object quantized(const Tensor& x, at::ScalarType dtype, bool both, bool square) {
     Quantized o;
@@ -286,14 +300,15 @@ struct Operand {
     bool of(const Tensor& q, const Tensor& s) {
         if (!on_cuda(q) || !on_cuda(s) || s.device() != q.device() || format_of(q.scalar_type()) < 0 || s.scalar_type() != at::kFloat8_e8m0fnu || !r.of(q)) return false;
         if (s.dim() == 0 || s.size(-1) != blocks(r.K)) return false;
-        if (s.dim() == 2) {
-            sr = s.stride(0); sk = s.stride(1);
-        } else if (s.is_contiguous()) {
-            sr = blocks(r.K); sk = 1;
-        } else {
-            return false;
+        sk = s.stride(-1);
+        int64_t rows = 1, step = 0;                                        // leading dimensions that are one axis of even strides
+        for (int64_t i = s.dim() - 2; i >= 0; i--) {
+            if (s.size(i) == 1) continue;
+            if (step == 0) sr = s.stride(i);
+            else if (s.stride(i) != step) return false;
+            step = s.stride(i) * s.size(i);
+            rows *= s.size(i);
         }
-        const int64_t rows = s.numel() / blocks(r.K);
         if (rows != r.M && rows != blocks(r.M)) return false;
         share = rows == r.M ? 1 : 128;
         return true;
@@ -426,8 +441,8 @@ bool norm_any(Norm& n, const Tensor& y, c10::optional<at::ScalarType> quantize, 
         n.a.format = format_of(*quantize);
         if (n.a.format < 0 || !n.a.w2) return false;
         h = new_blocks(y, y.sizes(), n.r.M, n.r.K, *quantize);
-        s = make(y, with_last(y, blocks(n.r.K)), at::kFloat8_e8m0fnu);
-        n.a.q = h.data_ptr(); n.a.ldq = (n.r.K + 15) / 16 * 16; n.a.s = static_cast<uint8_t*>(s.data_ptr());
+        s = new_scales(y, with_last(y, blocks(n.r.K)), n.r.M, blocks(n.r.K));
+        n.a.q = h.data_ptr(); n.a.ldq = (n.r.K + 15) / 16 * 16; n.a.lds = (n.r.M + 15) / 16 * 16; n.a.s = static_cast<uint8_t*>(s.data_ptr());
     } else if (n.a.w2) {
         h = make(y, y.sizes(), y.scalar_type());
         n.a.h = h.data_ptr(); n.a.ldh = n.r.K;

@@ -37,55 +37,86 @@ __device__ __forceinline__ void tmem_copy_scales(uint32_t taddr, uint32_t smem_a
     const uint64_t d = ((uint64_t)((128u >> 4) | (1u << 14)) << 32) | ((smem_addr & 0x3FFFFu) >> 4);
     asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(d) : "memory");
 }
+__device__ __forceinline__ void sts_b32(uint32_t at, uint32_t v) { asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory"); }
 __device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
     float v;
     asm volatile("{\n\t.reg .b32 ra;\n\tmapa.shared::cluster.u32 ra, %1, %2;\n\tld.shared::cluster.f32 %0, [ra];\n\t}" : "=f"(v) : "r"(addr), "r"(rank) : "memory");
     return v;
 }
 
-// The scales of 16 blocks from kb on (127 = 2^0 where there is no block or row) of row lane, lane + 32, lane + 64 or lane + 96 of the 128
-// from row0 on, four blocks to a word.  Only blocks below kb1 are read.  A load from memory takes longer than the MMAs of four blocks
-// when the operands' copies fill the memory system, so 16 blocks are asked for at a time, as one vector where the layout allows.
-// packed: 16 or 4 scales of a row, from a multiple of so many on, are one aligned vector or word; 1: bytes of any stride.
-__device__ __forceinline__ int scale_packing(const BlocksOperand& o, int kb0) {
-    if (o.sk != 1) return 1;
-    const uintptr_t at = reinterpret_cast<uintptr_t>(o.s) | (uintptr_t)o.sr | (uintptr_t)kb0;
-    return (at & 15) == 0 ? 16 : (at & 3) == 0 ? 4 : 1;
-}
-__device__ __forceinline__ void load_scales(const BlocksOperand& o, int packed, int row0, int kb, int kb1, int lane, uint4 (&w)[4]) {
+// The scales of 16 blocks from kb on of the 128 rows from row0 on, brought from memory by a warp (load), and written to shared memory as
+// the tensor memory wants them, four blocks a time (store).  127 = 2^0 stands where there is no block or row; only blocks below kb1
+// are read.  A load takes longer than the MMAs of four blocks when the operands' copies fill the memory system, hence 16 at a time.
+//   layout 1     block by block, as the quantiser writes them (sr == 1): lane l holds rows 4l .. 4l+3, a word for each block
+//   layout 16, 4 row by row (sk == 1), 16 or 4 scales of a row one aligned vector or word; 0: bytes of any strides; a square's scale serves
+//                all rows.  Lane l holds rows l, l + 32, l + 64, l + 96, a word for four blocks.
+struct ScaleLoader {
+    int layout;
+    uint32_t w[16];
+    __device__ __forceinline__ ScaleLoader(const BlocksOperand& o, int kb0) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(o.s);
+        if (o.shift == 0 && o.sr == 1 && (at & 3) == 0 && o.sk % 4 == 0) layout = 1;
+        else if (o.sk != 1) layout = 0;
+        else layout = ((at | (uintptr_t)o.sr | (uintptr_t)kb0) & 15) == 0 ? 16 : ((at | (uintptr_t)o.sr | (uintptr_t)kb0) & 3) == 0 ? 4 : 0;
+    }
+    __device__ __forceinline__ void load(const BlocksOperand& o, int row0, int kb, int kb1, int lane) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        if (i > 0 && o.shift) { w[i] = w[0]; continue; }                   // one scale for all 128 rows
-        const int row = row0 + i * 32 + lane;
-        w[i] = make_uint4(0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu, 0x7F7F7F7Fu);
-        if ((o.shift ? row0 : row) >= o.rows) continue;
-        const uint8_t* s = o.s + (long long)(o.shift ? row0 >> o.shift : row) * o.sr + (long long)kb * o.sk;
-        if (packed == 16 && kb + 16 <= kb1) {
-            w[i] = *reinterpret_cast<const uint4*>(s);
-            continue;
+        for (int i = 0; i < 16; i++) w[i] = 0x7F7F7F7Fu;
+        if (layout == 1) {
+            const int row = row0 + 4 * lane, n = o.rows - row;
+            const uint8_t* s = o.s + row + (long long)kb * o.sk;
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                if (kb + i >= kb1 || n <= 0) continue;
+                if (n >= 4) {
+                    w[i] = *reinterpret_cast<const uint32_t*>(s + i * o.sk);
+                } else {
+                    for (int j = 0; j < n; j++) w[i] = (w[i] & ~(0xFFu << (8 * j))) | (uint32_t)s[i * o.sk + j] << (8 * j);
+                }
+            }
+            return;
         }
-        uint32_t v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-            v[j] = 0x7F7F7F7Fu;
-            if (packed >= 4 && kb + 4 * j + 4 <= kb1) {
-                v[j] = reinterpret_cast<const uint32_t*>(s)[j];
-            } else if (kb + 4 * j < kb1) {
-                v[j] = 0;
+        for (int i = 0; i < 4; i++) {
+            const int row = o.shift ? row0 : row0 + i * 32 + lane;
+            if (i > 0 && o.shift) {
 #pragma unroll
-                for (int b = 0; b < 4; b++) v[j] |= (kb + 4 * j + b < kb1 ? (uint32_t)s[(4 * j + b) * o.sk] : 127u) << (8 * b);
+                for (int j = 0; j < 4; j++) w[4 * i + j] = w[j];
+                continue;
+            }
+            if (row >= o.rows) continue;
+            const uint8_t* s = o.s + (long long)(row >> o.shift) * o.sr + (long long)kb * o.sk;
+            if (layout == 16 && kb + 16 <= kb1) {
+                const uint4 u = *reinterpret_cast<const uint4*>(s);
+                w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
+                continue;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                if (layout >= 4 && kb + 4 * j + 4 <= kb1) {
+                    w[4 * i + j] = reinterpret_cast<const uint32_t*>(s)[j];
+                } else if (kb + 4 * j < kb1) {
+                    uint32_t v = 0;
+#pragma unroll
+                    for (int b = 0; b < 4; b++) v |= (kb + 4 * j + b < kb1 ? (uint32_t)s[(4 * j + b) * o.sk] : 127u) << (8 * b);
+                    w[4 * i + j] = v;
+                }
             }
         }
-        w[i] = make_uint4(v[0], v[1], v[2], v[3]);
     }
-}
-// Word j of the four vectors, as the tensor memory wants it.
-__device__ __forceinline__ void store_scales(uint32_t at, const uint4 (&w)[4], int j) {
-    if (j == 0) sts_v4(at, w[0].x, w[1].x, w[2].x, w[3].x);
-    else if (j == 1) sts_v4(at, w[0].y, w[1].y, w[2].y, w[3].y);
-    else if (j == 2) sts_v4(at, w[0].z, w[1].z, w[2].z, w[3].z);
-    else sts_v4(at, w[0].w, w[1].w, w[2].w, w[3].w);
-}
+    // The words of blocks 4j .. 4j+3: row r at at + (r % 32) * 16 + (r / 32) * 4.
+    __device__ __forceinline__ void store(uint32_t at, int j, int lane) const {
+        if (layout != 1) {
+            sts_v4(at + lane * 16, w[j], w[4 + j], w[8 + j], w[12 + j]);
+            return;
+        }
+        const uint32_t a = __byte_perm(w[4 * j], w[4 * j + 1], 0x5140), b = __byte_perm(w[4 * j + 2], w[4 * j + 3], 0x5140);   // rows 0, 1 of two blocks
+        const uint32_t c = __byte_perm(w[4 * j], w[4 * j + 1], 0x7362), d = __byte_perm(w[4 * j + 2], w[4 * j + 3], 0x7362);   // rows 2, 3
+        const uint32_t to = at + (uint32_t)((4 * lane) & 31) * 16u + (uint32_t)(lane >> 3) * 4u;
+        sts_b32(to, __byte_perm(a, b, 0x5410)); sts_b32(to + 16, __byte_perm(a, b, 0x7632));
+        sts_b32(to + 32, __byte_perm(c, d, 0x5410)); sts_b32(to + 48, __byte_perm(c, d, 0x7632));
+    }
+};
 
 __device__ __forceinline__ void tma_store_2d(const void* tmap, int x, int y, uint32_t src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(tmap), "r"(src), "r"(x), "r"(y) : "memory");
@@ -230,18 +261,18 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
             __syncwarp();
         }
     } else if (warp == 2) {
-        const int rpack = scale_packing(R, kb0), cpack = scale_packing(C, kb0);
+        ScaleLoader r(R, kb0), c(C, kb0);
         for (int kb = kb0, q = 0; kb < kb1; kb += 16, q++) {
-            uint4 w[1 + CG][4];
-            load_scales(R, rpack, r0, kb, kb1, lane, w[0]);
-#pragma unroll
-            for (int i = 0; i < CG; i++) load_scales(C, cpack, c0 + 128 * i, kb, kb1, lane, w[1 + i]);
+            static_assert(CG == 1, "one group of 128 rows on either side");
+            r.load(R, r0, kb, kb1, lane);
+            c.load(C, c0, kb, kb1, lane);
             const int slot = q % SF_SLOTS;
             if (q >= SF_SLOTS && !mbar_wait_warp(sfEmpty + 8 * slot, (q / SF_SLOTS - 1) & 1)) { expire(34); break; }
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int i = 0; i < 1 + CG; i++) store_scales(sSF + (slot * 4 + j) * SFB + lane * 16 + 512 * i, w[i], j);
+            for (int j = 0; j < 4; j++) {
+                r.store(sSF + (slot * 4 + j) * SFB, j, lane);
+                c.store(sSF + (slot * 4 + j) * SFB + 512, j, lane);
+            }
             fence_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(sfFull + 8 * slot);
@@ -431,23 +462,25 @@ __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_con
     } else if (warp == 2) {
         // A chunk of 16 blocks is fetched, stored and announced before the next one is asked for: the fence and the arrival on the other
         // CTA's barrier would wait for loads under way.  Two slots, 32 blocks, keep the MMAs supplied meanwhile.
-        const int apack = scale_packing(A, 0), bpack = scale_packing(B, 0);
+        ScaleLoader wa(A, 0), w0(B, 0), w1(B, 0);
         bool dead = false;
         int q = 0;
         for (int t = pair0; t < ntiles && !dead; t += pairs) {
             int m0, n0;
             tile_at(t, m0, n0);
             for (int kb = 0; kb < KB; kb += 16, q++) {
-                uint4 w[3][4];
-                load_scales(A, apack, m0 + (int)rank * 128, kb, KB, lane, w[0]);
-                load_scales(B, bpack, n0, kb, KB, lane, w[1]);
-                load_scales(B, bpack, n0 + 128, kb, KB, lane, w[2]);
+                wa.load(A, m0 + (int)rank * 128, kb, KB, lane);
+                w0.load(B, n0, kb, KB, lane);
+                w1.load(B, n0 + 128, kb, KB, lane);
                 const int slot = q % PSLOTS;
                 if (q >= PSLOTS && !mbar_wait_cluster_warp(sfEmpty + 8 * slot, (q / PSLOTS - 1) & 1)) { expire(40); dead = true; break; }
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-#pragma unroll
-                    for (int i = 0; i < 3; i++) store_scales(sSF + (slot * 4 + j) * PSF + lane * 16 + 512 * i, w[i], j);
+                for (int j = 0; j < 4; j++) {
+                    const uint32_t at = sSF + (slot * 4 + j) * PSF;
+                    wa.store(at, j, lane);
+                    w0.store(at + 512, j, lane);
+                    w1.store(at + 1024, j, lane);
+                }
                 fence_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(sfFull + 8 * slot, 0u);

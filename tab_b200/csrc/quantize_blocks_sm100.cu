@@ -77,7 +77,7 @@ __device__ __forceinline__ uint2 narrow8_of(const float (&v)[8], float inv, bool
     return r;
 }
 
-static constexpr int QROWS = 4;              // blocks a half-warp of the rows kernel has in flight
+static constexpr int QROWS = 2;              // blocks a half-warp of the rows kernel has in flight
 
 // hk half-warps of the sixteen lie along K, the others along M.
 template <int TYPE, int FORMAT>
@@ -110,13 +110,13 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantBlocksParams p,
 #pragma unroll
         for (int j = 0; j < 8; j++) f[j] = v[i].at(j);
         store_bytes8(p.q + m * p.ldq + k0, n, qvec, narrow8_of<FORMAT>(f, exp2_int(-e), odd));
-        if (l == 0) p.s[m * KB + kb] = (uint8_t)(e + 127);
+        if (l == 0) p.s[kb * p.lds + m] = (uint8_t)(e + 127);
     }
 }
 
 // 128 x 128 values: half-warp h holds rows 8h .. 8h+7, its lane l columns 8l .. 8l+7.
 template <int TYPE, int FORMAT, bool SQUARE>
-__global__ void __launch_bounds__(256, TYPE == TAB_FP32 ? 2 : 4) quantize_tiles_kernel(QuantBlocksParams p, int KB, int MB, int vec, int qvec, int qtvec) {
+__global__ void __launch_bounds__(256, TYPE == TAB_FP32 ? 2 : SQUARE ? 4 : 3) quantize_tiles_kernel(QuantBlocksParams p, int KB, int vec, int qvec, int qtvec) {
     using T = typename ElemOf<TYPE>::type;
     using E = Eight<TYPE>;
     __shared__ uint32_t colmax[16][16 * E::W + 1];                         // magnitudes as a lane's words hold them; a square's: word 0
@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(256, TYPE == TAB_FP32 ? 2 : 4) quantize_tiles_
         for (int i = 0; i < 16; i++) high = max(high, colmax[i][0]);
         e = scale_exponent(E::float_bits(high), FORMAT);
         if (threadIdx.x == 0) {
-            if (p.s) p.s[mb * KB + kb] = (uint8_t)(e + 127);
-            if (p.st) p.st[(long long)kb * MB + mb] = (uint8_t)(e + 127);
+            if (p.s) p.s[mb * p.lds + kb] = (uint8_t)(e + 127);
+            if (p.st) p.st[kb * p.ldst + mb] = (uint8_t)(e + 127);
         }
     } else {
 #pragma unroll
@@ -174,21 +174,38 @@ __global__ void __launch_bounds__(256, TYPE == TAB_FP32 ? 2 : 4) quantize_tiles_
                 const int ec = scale_exponent(E::float_bits(TYPE == TAB_FP32 ? b : b >> (16 * c) & 0xFFFFu), FORMAT);
                 colexp[col] = ec;
                 const long long k = (long long)kb * BLK + col;
-                if (k < p.K) p.st[k * MB + mb] = (uint8_t)(ec + 127);
+                if (k < p.K) p.st[mb * p.ldst + k] = (uint8_t)(ec + 127);
             }
         }
+    }
+    int mine = e;                                                          // the scale of row 8h + l / 2 of this half-warp, in lane l
+    if (!SQUARE) {
+        // Eight rows' maxima over sixteen lanes: in every step a lane hands half of its rows to its neighbour and keeps the others, eight
+        // shuffles instead of 32, and each lane then finds one row's scale instead of eight.
+        uint32_t m[8];
+#pragma unroll
+        for (int r = 0; r < 8; r++) m[r] = v[r].largest(odd);
+#pragma unroll
+        for (int o = 8; o > 1; o >>= 1) {
+            const bool upper = l & o;
+#pragma unroll
+            for (int r = 0; r < o / 2; r++) {
+                const uint32_t give = upper ? m[r] : m[r + o / 2], keep = upper ? m[r + o / 2] : m[r];
+                m[r] = max(keep, __shfl_xor_sync(0xFFFFFFFFu, give, o));
+            }
+        }
+        m[0] = max(m[0], __shfl_xor_sync(0xFFFFFFFFu, m[0], 1));
+        mine = scale_exponent(E::float_bits(m[0]), FORMAT);
+        if (!(l & 1) && m0 + l / 2 < p.M) p.s[kb * p.lds + m0 + l / 2] = (uint8_t)(mine + 127);
     }
     if (!SQUARE || p.q) {
 #pragma unroll
         for (int r = 0; r < 8; r++) {
-            const int er = SQUARE ? e : scale_exponent(E::float_bits(half_warp_max(v[r].largest(odd))), FORMAT);
+            const int er = SQUARE ? e : __shfl_sync(0xFFFFFFFFu, mine, (threadIdx.x & 16) + 2 * r);
             float f[8];
 #pragma unroll
             for (int c = 0; c < 8; c++) f[c] = v[r].at(c);
-            if (m0 + r < p.M) {
-                store_bytes8(p.q + (m0 + r) * p.ldq + k0, n, qvec, narrow8_of<FORMAT>(f, exp2_int(-er), odd));
-                if (!SQUARE && l == 0) p.s[(m0 + r) * KB + kb] = (uint8_t)(er + 127);
-            }
+            if (m0 + r < p.M) store_bytes8(p.q + (m0 + r) * p.ldq + k0, n, qvec, narrow8_of<FORMAT>(f, exp2_int(-er), odd));
         }
     }
     if (SQUARE && !p.qt) return;
@@ -229,8 +246,8 @@ static int launch_quantize_blocks(const QuantBlocksParams& p, bool square, cudaS
     }
     const long long MB = (p.M + BLK - 1) / BLK, grid = MB * KB;
     if (grid >= (1LL << 31)) return TAB_E_TOO_LARGE;
-    if (square) return launch_pdl(quantize_tiles_kernel<TYPE, FORMAT, true>, dim3((unsigned)grid), dim3(256), 0, stream, p, KB, (int)MB, vec, qvec, qtvec);
-    return launch_pdl(quantize_tiles_kernel<TYPE, FORMAT, false>, dim3((unsigned)grid), dim3(256), 0, stream, p, KB, (int)MB, vec, qvec, qtvec);
+    if (square) return launch_pdl(quantize_tiles_kernel<TYPE, FORMAT, true>, dim3((unsigned)grid), dim3(256), 0, stream, p, KB, vec, qvec, qtvec);
+    return launch_pdl(quantize_tiles_kernel<TYPE, FORMAT, false>, dim3((unsigned)grid), dim3(256), 0, stream, p, KB, vec, qvec, qtvec);
 }
 
 int quantize_blocks_dispatch(const QuantBlocksParams& p, int type, bool square, cudaStream_t stream) {

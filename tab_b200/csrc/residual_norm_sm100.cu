@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_kernel(Norm
                 const int e = scale_exponent(half_warp_max(a), p.format);
                 const float inv = exp2_int(-e);
                 store_bytes8(static_cast<uint8_t*>(p.q) + m * p.ldq + c, n, flags & V_Q, p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(v[i], inv) : narrow8<TAB_E4M3>(v[i], inv));
-                if ((g & 15) == 0 && n > 0) p.s[m * ((p.C + BLK - 1) / BLK) + c / BLK] = (uint8_t)(e + 127);
+                if ((g & 15) == 0 && n > 0) p.s[(long long)(c / BLK) * p.lds + m] = (uint8_t)(e + 127);
             }
         }
     }

@@ -460,6 +460,12 @@ def _new_blocks(shape, rows, n, dtype, device):
     return held[:, :n].view(shape)
 
 
+def _new_scales(shape, rows, n, device):
+    """Scales ``shape`` (``rows`` x ``n``) that lie block by block: a quantiser's CTA, which has one block of many rows, writes them side by
+    side, and so the product reads them."""
+    return torch.empty((n, -(-rows // 16) * 16), dtype=torch.float8_e8m0fnu, device=device)[:, :rows].t().view(shape)
+
+
 def _format(dtype):
     if dtype not in _FORMATS:
         raise RuntimeError("dtype must be torch.float8_e4m3fn or torch.float8_e5m2")
@@ -476,7 +482,8 @@ def quantize_blocks(x, dtype=torch.float8_e4m3fn, columns=False):
     ``columns``: also ``(qt, st)``, from the same reading of ``x``: its transpose ``[K, rows]`` with blocks along the rows of ``x``,
     ``st`` ``[K, ceil(rows/128)]`` - what a product that sums over the rows takes (the gradient of a dense layer's weights).
 
-    Rows of ``q`` and ``qt`` start on 16 bytes, as ``matmul_blocks`` wants them."""
+    Rows of ``q`` and ``qt`` start on 16 bytes, as ``matmul_blocks`` wants them; the scales lie block by block in memory, the form it reads
+    fastest."""
     done = _try("quantize_blocks", x, dtype, columns)
     if done is not None:
         return done
@@ -485,11 +492,11 @@ def quantize_blocks(x, dtype=torch.float8_e4m3fn, columns=False):
     M, K, ldx = _rows(x, "x")
     with torch.cuda.device(x.device):
         q = _new_blocks(tuple(x.shape), M, K, dtype, x.device)
-        s = torch.empty((*x.shape[:-1], _blocks(K)), dtype=torch.float8_e8m0fnu, device=x.device)
+        s = _new_scales((*x.shape[:-1], _blocks(K)), M, _blocks(K), x.device)
         qt = _new_blocks((K, M), K, M, dtype, x.device) if columns else None
-        st = torch.empty((K, _blocks(M)), dtype=torch.float8_e8m0fnu, device=x.device) if columns else None
-        rc = _cabi.lib().tab_quantize_blocks_launch(x.data_ptr(), _TYPES[x.dtype], ldx, M, K, fmt, 0, q.data_ptr(), -(-K // 16) * 16, s.data_ptr(),
-                                                    qt.data_ptr() if columns else None, -(-M // 16) * 16, st.data_ptr() if columns else None,
+        st = _new_scales((K, _blocks(M)), K, _blocks(M), x.device) if columns else None
+        rc = _cabi.lib().tab_quantize_blocks_launch(x.data_ptr(), _TYPES[x.dtype], ldx, M, K, fmt, 0, q.data_ptr(), -(-K // 16) * 16, s.data_ptr(), -(-M // 16) * 16,
+                                                    qt.data_ptr() if columns else None, -(-M // 16) * 16, st.data_ptr() if columns else None, -(-K // 16) * 16,
                                                     _stream_ptr(x.device))
     _cabi.check(rc, "tab_quantize_blocks_launch")
     return (q, s, qt, st) if columns else (q, s)
@@ -512,8 +519,8 @@ def quantize_blocks2d(w, dtype=torch.float8_e4m3fn, transposed=False):
         s = torch.empty((_blocks(M), _blocks(K)), dtype=torch.float8_e8m0fnu, device=w.device)
         qt = _new_blocks((K, M), K, M, dtype, w.device) if transposed else None
         st = torch.empty((_blocks(K), _blocks(M)), dtype=torch.float8_e8m0fnu, device=w.device) if transposed else None
-        rc = _cabi.lib().tab_quantize_blocks_launch(w.data_ptr(), _TYPES[w.dtype], ldx, M, K, fmt, 1, q.data_ptr(), -(-K // 16) * 16, s.data_ptr(),
-                                                    qt.data_ptr() if transposed else None, -(-M // 16) * 16, st.data_ptr() if transposed else None,
+        rc = _cabi.lib().tab_quantize_blocks_launch(w.data_ptr(), _TYPES[w.dtype], ldx, M, K, fmt, 1, q.data_ptr(), -(-K // 16) * 16, s.data_ptr(), _blocks(K),
+                                                    qt.data_ptr() if transposed else None, -(-M // 16) * 16, st.data_ptr() if transposed else None, _blocks(M),
                                                     _stream_ptr(w.device))
     _cabi.check(rc, "tab_quantize_blocks_launch")
     return (q, s, qt, st) if transposed else (q, s)
@@ -641,8 +648,8 @@ def _residual_norm(y, residual, pre_weight, pre_bias, post_weight, post_bias, ga
             a.r, a.ldr = r.data_ptr(), C
         if quantize is not None:
             h = _new_blocks(tuple(y.shape), M, C, quantize, y.device)
-            s = torch.empty((*y.shape[:-1], _blocks(C)), dtype=torch.float8_e8m0fnu, device=y.device)
-            a.q, a.ldq, a.s = h.data_ptr(), -(-C // 16) * 16, s.data_ptr()
+            s = _new_scales((*y.shape[:-1], _blocks(C)), M, _blocks(C), y.device)
+            a.q, a.ldq, a.s, a.lds = h.data_ptr(), -(-C // 16) * 16, s.data_ptr(), -(-M // 16) * 16
         elif pre_weight is not None:
             h = torch.empty(y.shape, dtype=y.dtype, device=y.device)
             a.h, a.ldh = h.data_ptr(), C

@@ -19,16 +19,17 @@ def np_bytes(t):
 # ---- refusals, on the CPU ---------------------------------------------------------------------------------------------
 
 def quantize_args(**over):
-    a = dict(x=BASE, type=1, ldx=256, M=4, K=256, format=0, square=0, q=BASE, ldq=256, s=BASE, qt=None, ldqt=0, st=None)
+    a = dict(x=BASE, type=1, ldx=256, M=4, K=256, format=0, square=0, q=BASE, ldq=256, s=BASE, lds=16, qt=None, ldqt=0, st=None, ldst=0)
     a.update(over)
     return [*a.values(), None]
 
 
 @pytest.mark.parametrize("over, code", [
     (dict(type=3), -1), (dict(type=-1), -1), (dict(format=2), -1), (dict(square=2), -1), (dict(M=-1), -1), (dict(K=-1), -1),
-    (dict(M=0), 0), (dict(K=0), 0), (dict(x=None), -2), (dict(q=None), -2), (dict(s=None), -2), (dict(qt=BASE, ldqt=16), -2),
-    (dict(square=1, q=None, s=None), -2), (dict(ldx=255), -1), (dict(ldq=255), -1), (dict(qt=BASE, st=BASE, ldqt=3), -1),
-    (dict(x=BASE + 1), -6), (dict(type=0, x=BASE + 2), -6), (dict(M=1 << 31), -5), (dict(ldx=1 << 40), -5),
+    (dict(M=0), 0), (dict(K=0), 0), (dict(x=None), -2), (dict(q=None), -2), (dict(s=None), -2), (dict(qt=BASE, ldqt=16, ldst=256), -2),
+    (dict(square=1, q=None, s=None), -2), (dict(ldx=255), -1), (dict(ldq=255), -1), (dict(qt=BASE, st=BASE, ldqt=3, ldst=256), -1), (dict(lds=3), -1), (dict(qt=BASE, st=BASE, ldqt=16, M=129, ldst=255, lds=256), -1), (dict(square=1, M=129, lds=1), -1),
+    (dict(square=1, qt=BASE, st=BASE, ldqt=16, lds=2, ldst=0), -1), (dict(lds=1 << 40), -5),
+    (dict(x=BASE + 1), -6), (dict(type=0, x=BASE + 2), -6), (dict(M=1 << 31, lds=1 << 31), -5), (dict(ldx=1 << 40), -5),
 ])
 def test_quantize_blocks_refuses(over, code):
     assert _cabi.lib().tab_quantize_blocks_launch(*quantize_args(**over)) == code
@@ -147,14 +148,14 @@ def test_quantize_blocks_strided_and_bounded(cuda):
         assert np.array_equal(np_bytes(s), ws) and ref.same_bytes(np_bytes(q), wq, "e4m3")
     l, x = _cabi.lib(), big[:9, :200].contiguous()
     for qt in (None, torch.full((202, 16), 0xAA, dtype=torch.uint8, device=cuda)):
-        q, s, st = (torch.full(z, 0xAA, dtype=torch.uint8, device=cuda) for z in ((11, 208), (11, 2), (202, 1)))
-        assert l.tab_quantize_blocks_launch(x.data_ptr(), 1, 200, 9, 200, 0, 0, q.data_ptr(), 208, s.data_ptr(), qt.data_ptr() if qt is not None else None, 16,
-                                            st.data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+        q, s, st = (torch.full(z, 0xAA, dtype=torch.uint8, device=cuda) for z in ((11, 208), (3, 13), (2, 207)))
+        assert l.tab_quantize_blocks_launch(x.data_ptr(), 1, 200, 9, 200, 0, 0, q.data_ptr(), 208, s.data_ptr(), 13, qt.data_ptr() if qt is not None else None, 16,
+                                            st.data_ptr(), 207, torch.cuda.current_stream().cuda_stream) == 0
         wq, ws = ref.quantize(x.double().cpu().numpy(), "e4m3")
-        assert np.array_equal(q[:9, :200].cpu().numpy(), wq) and np.array_equal(s[:9].cpu().numpy(), ws)
-        assert bool((q[:, 200:] == 0xAA).all()) and bool((q[9:] == 0xAA).all()) and bool((s[9:] == 0xAA).all())
+        assert np.array_equal(q[:9, :200].cpu().numpy(), wq) and np.array_equal(s[:2, :9].cpu().numpy(), ws.T)
+        assert bool((q[:, 200:] == 0xAA).all()) and bool((q[9:] == 0xAA).all()) and bool((s[:, 9:] == 0xAA).all()) and bool((s[2:] == 0xAA).all())
         if qt is not None:
-            assert bool((qt[:, 9:] == 0xAA).all()) and bool((qt[200:] == 0xAA).all()) and bool((st[200:] == 0xAA).all())
+            assert bool((qt[:, 9:] == 0xAA).all()) and bool((qt[200:] == 0xAA).all()) and bool((st[:, 200:] == 0xAA).all()) and bool((st[1:] == 0xAA).all())
 
 
 # ---- product ----------------------------------------------------------------------------------------------------------
@@ -186,15 +187,18 @@ SIZES = [(1, 1, 1), (1, 128, 128), (1, 256, 1024), (2, 130, 96), (5, 512, 4096),
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("squares", [(False, True), (False, False), (True, True)])
+@pytest.mark.parametrize("squares, turned", [((False, True), False), ((False, False), False), ((True, True), False), ((False, False), True)])
 @pytest.mark.parametrize("M, N, K", SIZES)
-def test_matmul_blocks_exact(cuda, M, N, K, squares):
+def test_matmul_blocks_exact(cuda, M, N, K, squares, turned):
     """Whole numbers: |product| <= 4 * 4 * 4 * 4, sums of 30000 of them stay below 2^24, so every order of additions gives the same."""
     rng = np.random.default_rng(M + 3 * N + 7 * K)
     fa, fb = ("e4m3", "e5m2") if K % 2 else ("e4m3", "e4m3")
     a, b = random_blocks(rng, M, K, fa, squares[0], True), random_blocks(rng, N, K, fb, squares[1], True)
     want = ref.values(*a, fa) @ ref.values(*b, fb).T
-    y = TAB.matmul_blocks(*device_blocks(cuda, *a, fa), *device_blocks(cuda, *b, fb), out_dtype=torch.float32)
+    (qa, sa), (qb, sb) = device_blocks(cuda, *a, fa), device_blocks(cuda, *b, fb)
+    if turned:                                                      # as quantize_blocks lays them out: block by block
+        sa, sb = (TAB.ops._new_scales(tuple(s.shape), *s.shape, cuda).copy_(s) for s in (sa, sb))
+    y = TAB.matmul_blocks(qa, sa, qb, sb, out_dtype=torch.float32)
     assert y.shape == (M, N) and np.array_equal(y.cpu().numpy(), want)
     assert _cabi.lib().tab_device_status() == 0
 

@@ -24,7 +24,7 @@ def forward_args(**over):
 @pytest.mark.parametrize("over, code", [
     (dict(type=3), -1), (dict(ptype=-1), -1), (dict(gtype=7), -1), (dict(gkind=4), -1), (dict(layer=2), -1), (dict(M=-1), -1), (dict(C=-1), -1), (dict(b1=BASE), -1),
     (dict(b2=BASE), -1), (dict(M=0), 0), (dict(C=0), 0), (dict(y=None), -2), (dict(gate=None), -2), (dict(w2=None), -2), (dict(q=BASE, ldq=64), -2),
-    (dict(q=BASE, s=BASE, ldq=64, format=5), -1), (dict(ldy=63), -1), (dict(ldx=1), -1), (dict(ldr=0), -1), (dict(ldh=63), -1), (dict(gkind=3, ldg=63), -1),
+    (dict(q=BASE, s=BASE, ldq=64, lds=16, format=5), -1), (dict(q=BASE, s=BASE, ldq=256, lds=3, C=256, ldy=256, ldx=256, ldr=256, ldh=256), -1), (dict(ldy=63), -1), (dict(ldx=1), -1), (dict(ldr=0), -1), (dict(ldh=63), -1), (dict(gkind=3, ldg=63), -1),
     (dict(gkind=1, ldg=-1), -1), (dict(q=BASE, s=BASE, ldq=63), -1), (dict(y=BASE + 1), -6), (dict(w1=BASE + 2), -6), (dict(gate=BASE + 1), -6), (dict(stats=BASE + 8), -6),
     (dict(C=16385), -5), (dict(M=1 << 31), -5),
 ])
