@@ -79,21 +79,23 @@ __device__ __forceinline__ uint2 narrow8_of(const float (&v)[8], float inv, bool
 
 static constexpr int QROWS = 2;              // blocks a half-warp of the rows kernel has in flight
 
-// hk half-warps of the sixteen lie along K, the others along M.
+// Half-warps take blocks of two neighbouring columns of blocks (of one, where there is no more), the others rows; scales are gathered so
+// that those of a column of blocks leave side by side.
 template <int TYPE, int FORMAT>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(QuantBlocksParams p, int KB, int hk_log2, int chunks, int vec, int qvec) {
+__global__ void __launch_bounds__(256) quantize_rows_kernel(QuantBlocksParams p, int KB, int two, int chunks, int vec, int qvec) {
     using T = typename ElemOf<TYPE>::type;
     using E = Eight<TYPE>;
+    __shared__ uint8_t scales[16 * QROWS];
     pdl_wait();
     const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
-    const int hk = 1 << hk_log2, rstep = 16 >> hk_log2;
-    const int kb = (int)(blockIdx.x % (unsigned)chunks) * hk + (half & (hk - 1));
-    const long long row0 = (long long)(blockIdx.x / (unsigned)chunks) * (rstep * QROWS) + (half >> hk_log2);
+    const int hr = half >> two, rstep = 16 >> two, rows = rstep * QROWS;
+    const int kb = (int)(blockIdx.x % (unsigned)chunks << two) + (half & two);
+    const long long row0 = (long long)(blockIdx.x / (unsigned)chunks) * rows;
     const int k0 = kb * BLK + l * 8, n = kb < KB ? p.K - k0 : 0;
     E v[QROWS];
 #pragma unroll
     for (int i = 0; i < QROWS; i++) {
-        const long long m = row0 + i * rstep;
+        const long long m = row0 + i * rstep + hr;
         v[i].load(static_cast<const T*>(p.x) + m * p.ldx + k0, m < p.M ? n : 0, vec);
     }
     pdl_launch_dependents();
@@ -103,14 +105,18 @@ __global__ void __launch_bounds__(256) quantize_rows_kernel(QuantBlocksParams p,
     const bool odd = __any_sync(0xFFFFFFFFu, high >= E::INF);
 #pragma unroll
     for (int i = 0; i < QROWS; i++) {
-        const long long m = row0 + i * rstep;
+        const long long m = row0 + i * rstep + hr;
         const int e = scale_exponent(E::float_bits(half_warp_max(v[i].largest(odd))), FORMAT);
-        if (m >= p.M || kb >= KB) continue;                                // (shuffles of the next rows wait for these lanes)
+        if (l == 0) scales[(half & two) * rows + i * rstep + hr] = (uint8_t)(e + 127);
         float f[8];
 #pragma unroll
         for (int j = 0; j < 8; j++) f[j] = v[i].at(j);
-        store_bytes8(p.q + m * p.ldq + k0, n, qvec, narrow8_of<FORMAT>(f, exp2_int(-e), odd));
-        if (l == 0) p.s[kb * p.lds + m] = (uint8_t)(e + 127);
+        if (m < p.M && kb < KB) store_bytes8(p.q + m * p.ldq + k0, n, qvec, narrow8_of<FORMAT>(f, exp2_int(-e), odd));
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < rows << two) {
+        const int r = threadIdx.x % rows, c = (int)(blockIdx.x % (unsigned)chunks << two) + threadIdx.x / rows;
+        if (row0 + r < p.M && c < KB) p.s[c * p.lds + row0 + r] = scales[threadIdx.x];
     }
 }
 
@@ -119,8 +125,8 @@ template <int TYPE, int FORMAT, bool SQUARE>
 __global__ void __launch_bounds__(256, TYPE == TAB_FP32 ? 2 : SQUARE ? 4 : 3) quantize_tiles_kernel(QuantBlocksParams p, int KB, int vec, int qvec, int qtvec) {
     using T = typename ElemOf<TYPE>::type;
     using E = Eight<TYPE>;
-    __shared__ uint32_t colmax[16][16 * E::W + 1];                         // magnitudes as a lane's words hold them; a square's: word 0
-    __shared__ int colexp[BLK];
+    __shared__ uint32_t colmax[16][16 * E::W];                             // word i of lane l at [i * 16 + l]; a square's maxima: word 0
+    __shared__ int colexp[BLK];                                            // of column 8l + c at [c * 16 + l]
     __shared__ __align__(16) uint2 turned[BLK * 16];                       // [column][8 rows], chunks of a column permuted
     pdl_wait();
     const int half = threadIdx.x >> 4, l = threadIdx.x & 15;
@@ -162,19 +168,17 @@ __global__ void __launch_bounds__(256, TYPE == TAB_FP32 ? 2 : SQUARE ? 4 : 3) qu
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < E::W; i++) colmax[half][l * E::W + i] = a[i];
+        for (int i = 0; i < E::W; i++) colmax[half][i * 16 + l] = a[i];
         __syncthreads();
-        if (threadIdx.x < BLK / (8 / E::W)) {                              // a thread: one word's columns
+        if (threadIdx.x < 16 * E::W) {                                     // a thread: the columns of one word
             uint32_t b = 0;
 #pragma unroll
             for (int i = 0; i < 16; i++) b = E::most(b, colmax[i][threadIdx.x]);
 #pragma unroll
             for (int c = 0; c < 8 / E::W; c++) {
-                const int col = threadIdx.x * (8 / E::W) + c;
+                const int in8 = half * (8 / E::W) + c;                     // of the lane's eight columns
                 const int ec = scale_exponent(E::float_bits(TYPE == TAB_FP32 ? b : b >> (16 * c) & 0xFFFFu), FORMAT);
-                colexp[col] = ec;
-                const long long k = (long long)kb * BLK + col;
-                if (k < p.K) p.st[mb * p.ldst + k] = (uint8_t)(ec + 127);
+                colexp[in8 * 16 + l] = ec;
             }
         }
     }
@@ -210,6 +214,8 @@ __global__ void __launch_bounds__(256, TYPE == TAB_FP32 ? 2 : SQUARE ? 4 : 3) qu
     }
     if (SQUARE && !p.qt) return;
     __syncthreads();
+    if (!SQUARE && threadIdx.x < BLK && kb * BLK + (int)threadIdx.x < p.K)
+        p.st[mb * p.ldst + kb * BLK + threadIdx.x] = (uint8_t)(colexp[(threadIdx.x & 7) * 16 + (threadIdx.x >> 3)] + 127);
     // Chunk h of column c lies at place h ^ (c / 8): the sixteen lanes that write different columns, and the sixteen that read
     // different chunks, each meet all banks.
 #pragma unroll
@@ -217,7 +223,7 @@ __global__ void __launch_bounds__(256, TYPE == TAB_FP32 ? 2 : SQUARE ? 4 : 3) qu
         float f[8];
 #pragma unroll
         for (int r = 0; r < 8; r++) f[r] = v[r].at(c);
-        turned[(l * 8 + c) * 16 + (half ^ l)] = narrow8_of<FORMAT>(f, exp2_int(SQUARE ? -e : -colexp[l * 8 + c]), odd);
+        turned[(l * 8 + c) * 16 + (half ^ l)] = narrow8_of<FORMAT>(f, exp2_int(SQUARE ? -e : -colexp[c * 16 + l]), odd);
     }
     __syncthreads();
     const long long mt = mb * BLK + l * 8;
@@ -238,11 +244,10 @@ static int launch_quantize_blocks(const QuantBlocksParams& p, bool square, cudaS
     const int vec = !(reinterpret_cast<uintptr_t>(p.x) & xmask) && p.ldx % 8 == 0;
     const int qvec = !(reinterpret_cast<uintptr_t>(p.q) & 7) && p.ldq % 8 == 0, qtvec = !(reinterpret_cast<uintptr_t>(p.qt) & 7) && p.ldqt % 8 == 0;
     if (!square && !p.qt) {
-        int hl = 0;
-        while (hl < 4 && (1 << hl) < KB) hl++;
-        const long long chunks = (KB + (1 << hl) - 1) >> hl, rows = (16 >> hl) * QROWS, grid = chunks * ((p.M + rows - 1) / rows);
+        const int two = KB > 1;
+        const long long chunks = (KB + two) >> two, rows = (16 >> two) * QROWS, grid = chunks * ((p.M + rows - 1) / rows);
         if (grid >= (1LL << 31)) return TAB_E_TOO_LARGE;
-        return launch_pdl(quantize_rows_kernel<TYPE, FORMAT>, dim3((unsigned)grid), dim3(256), 0, stream, p, KB, hl, (int)chunks, vec, qvec);
+        return launch_pdl(quantize_rows_kernel<TYPE, FORMAT>, dim3((unsigned)grid), dim3(256), 0, stream, p, KB, two, (int)chunks, vec, qvec);
     }
     const long long MB = (p.M + BLK - 1) / BLK, grid = MB * KB;
     if (grid >= (1LL << 31)) return TAB_E_TOO_LARGE;
