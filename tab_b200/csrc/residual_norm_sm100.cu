@@ -10,7 +10,9 @@
 // mean.  Sums over rows (weights', shifts' and channel gate's gradients) stay in the registers of the threads that own the columns
 // while a CTA walks through its rows; the CTAs' sums are added in a fixed order by a second launch: no atomics, the same bits every time.
 #include <algorithm>
+#include <mutex>
 #include "blocks_common.cuh"
+#include "umma_common.cuh"
 
 namespace tab {
 
@@ -317,6 +319,353 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
         }
 }
 
+// ---- many rows ------------------------------------------------------------------------------------------------------------------
+// The same with CTAs that stay: rows come by bulk copies into a ring in shared memory, a few rows ahead, so that the memory is asked for the
+// next rows while the threads meet over this one; a thread keeps its eight columns' weights (forward) or their sums (backward) in
+// registers from row to row, so that weights are read once a CTA and not once a row.  Rows and their pitches are multiples of 16 bytes
+// and eight elements here; the kernels above take everything else.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(mbar) : "memory");
+}
+// Eight values in shared memory at `at` + column * size.
+template <int TYPE>
+__device__ __forceinline__ void lds8(uint32_t row, int c, float (&v)[8]) {
+    using T = typename ElemOf<TYPE>::type;
+    if (TYPE == TAB_FP32) {
+        const int4 a = lds_v4(row + c * 4), b = lds_v4(row + c * 4 + 16);
+        v[0] = __int_as_float(a.x); v[1] = __int_as_float(a.y); v[2] = __int_as_float(a.z); v[3] = __int_as_float(a.w);
+        v[4] = __int_as_float(b.x); v[5] = __int_as_float(b.y); v[6] = __int_as_float(b.z); v[7] = __int_as_float(b.w);
+    } else {
+        const int4 a = lds_v4(row + c * 2);
+        if constexpr (TYPE != TAB_FP32) widen8(make_uint4((uint32_t)a.x, (uint32_t)a.y, (uint32_t)a.z, (uint32_t)a.w), v, T());
+    }
+}
+// Sums over the CTA, the same in all threads; `bank` alternates as in row_sums.
+template <int WARPS, int N>
+__device__ __forceinline__ void cta_sums(float (&v)[N], float (*exchange)[N][32], int& bank) {
+#pragma unroll
+    for (int i = 0; i < N; i++)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v[i] += __shfl_xor_sync(0xFFFFFFFFu, v[i], o);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < N; i++) exchange[bank][i][warp] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        float s = 0.f;
+        if (WARPS >= 4) {
+#pragma unroll
+            for (int w = 0; w < WARPS; w += 4) {
+                const float4 e = *reinterpret_cast<const float4*>(&exchange[bank][i][w]);
+                s += (e.x + e.y) + (e.z + e.w);
+            }
+        }
+        v[i] = s;
+    }
+    bank ^= 1;
+}
+
+template <int TYPE, int THREADS, bool LAYER>
+__global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREADS : 1) : 1024 / THREADS) residual_norm_stream_kernel(NormParams p, int flags, int stages, int* status) {
+    using T = typename ElemOf<TYPE>::type;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ __align__(8) uint64_t bars[8];
+    __shared__ __align__(16) float exchange[2][1][32];
+    const int g = threadIdx.x, c = g * 8;
+    const bool mine = c < p.C;
+    const uint32_t row_bytes = (uint32_t)p.C * sizeof(T), sRing = (uint32_t)__cvta_generic_to_shared(ring), full = (uint32_t)__cvta_generic_to_shared(bars);
+    const float inv_c = 1.f / (float)p.C;
+    int bank = 0;
+    bool dead = false;
+    if (g == 0) {
+        for (int s = 0; s < stages; s++) mbar_init(full + 8 * s, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_wait();
+    auto request = [&](long long m, int s) {
+        const uint32_t at = sRing + (uint32_t)s * 2 * row_bytes;
+        mbar_expect_tx(full + 8 * s, p.x ? 2 * row_bytes : row_bytes);
+        bulk_load(at, static_cast<const T*>(p.y) + m * p.ldy, row_bytes, full + 8 * s);
+        if (p.x) bulk_load(at + row_bytes, static_cast<const T*>(p.x) + m * p.ldx, row_bytes, full + 8 * s);
+    };
+    const long long step = gridDim.x;
+    if (g == 0)
+        for (int s = 0; s < stages; s++)
+            if (blockIdx.x + s * step < p.M) request(blockIdx.x + s * step, s);
+    float w1[8], w2[8], gate[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) w1[j] = w2[j] = gate[j] = 0.f;
+    if (mine) {
+        if (p.w1) load8_any(p.w1, p.ptype, c, 8, flags & V_W1, w1);
+        if (p.w2) load8_any(p.w2, p.ptype, c, 8, flags & V_W2, w2);
+        if (p.gkind == TAB_GATE_CHANNEL) load8_any(p.gate, p.gtype, c, 8, flags & V_G, gate);
+    }
+    int slot = 0, turn = 0;
+    for (long long m = blockIdx.x; m < p.M; m += step) {
+        if (!dead && !mbar_wait(full + 8 * slot, turn & 1)) { dead = true; if (status) atomicExch(status, 42); }
+        const uint32_t at = sRing + (uint32_t)slot * 2 * row_bytes;
+        float v[8], x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = x[j] = 0.f;
+        if (mine) {
+            lds8<TYPE>(at, c, v);
+            if (p.x) lds8<TYPE>(at + row_bytes, c, x);
+        }
+        // Both sums of a norm; the first barrier of a row also says that everybody has read it, and its place is filled again.
+        bool open = true;
+        auto refill = [&]() {
+            if (open && g == 0 && m + stages * step < p.M) request(m + stages * step, slot);
+            open = false;
+        };
+        auto normalise = [&](float& mean, float& inverse) {
+            float s[1];
+            mean = 0.f;
+            if (LAYER) {
+                s[0] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+                cta_sums<THREADS / 32, 1>(s, exchange, bank);
+                refill();
+                mean = s[0] * inv_c;
+            }
+            s[0] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                if (LAYER && mine) v[j] -= mean;
+                s[0] += v[j] * v[j];
+            }
+            cta_sums<THREADS / 32, 1>(s, exchange, bank);
+            refill();
+            inverse = 1.f / sqrtf(s[0] * inv_c + p.eps);
+        };
+        float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
+        if (p.w1) {
+            normalise(st.x, st.y);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = v[j] * st.y * w1[j];
+            if (LAYER && p.b1 && mine) {
+                float b[8];
+                load8_any(p.b1, p.ptype, c, 8, flags & V_B1, b);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] += b[j];
+            }
+        }
+        if (p.gkind == TAB_GATE_CHANNEL) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] *= gate[j];
+        } else if (p.gkind != TAB_GATE_NONE && mine) {
+            float f[8];
+            if (p.gkind == TAB_GATE_FULL) {
+                load8_any(p.gate, p.gtype, m * p.ldg + c, 8, flags & V_G, f);
+            } else {
+                const float one = load_any(p.gate, p.gtype, m * p.ldg);
+#pragma unroll
+                for (int j = 0; j < 8; j++) f[j] = one;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] *= f[j];
+        }
+        if (p.x) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = fmaf(p.alpha, x[j], v[j]);
+        }
+        if (mine && p.r) store8(static_cast<T*>(p.r) + m * p.ldr + c, 8, flags & V_R, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = to_float(from_float<T>(v[j]));          // r as it is kept
+        if (p.w2) {
+            normalise(st.z, st.w);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = v[j] * st.w * w2[j];
+            if (LAYER && p.b2 && mine) {
+                float b[8];
+                load8_any(p.b2, p.ptype, c, 8, flags & V_B2, b);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] += b[j];
+            }
+            if (p.h && mine) store8(static_cast<T*>(p.h) + m * p.ldh + c, 8, flags & V_H, v);
+            if (p.q) {
+                uint32_t a = 0;
+#pragma unroll
+                for (int j = 0; j < 8; j++) a = max(a, mine ? finite_bits(v[j]) : 0u);
+                const int e = scale_exponent(half_warp_max(a), p.format);
+                const float inv = exp2_int(-e);
+                if (mine) {
+                    store_bytes8(static_cast<uint8_t*>(p.q) + m * p.ldq + c, 8, flags & V_Q, p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(v, inv) : narrow8<TAB_E4M3>(v, inv));
+                    if ((g & 15) == 0) p.s[(long long)(c / BLK) * p.lds + m] = (uint8_t)(e + 127);
+                }
+            }
+        }
+        if (open) { __syncthreads(); refill(); }
+        if (p.stats && g == 0) *reinterpret_cast<float4*>(p.stats + 4 * m) = st;
+        if (++slot == stages) { slot = 0; turn++; }
+    }
+    pdl_launch_dependents();
+    if (dead) for (int i = 0; i < 200; i++) __nanosleep(1000);             // copies that may still be under way land before this memory is another's
+}
+
+template <int TYPE, int THREADS, bool LAYER>
+__global__ void __launch_bounds__(THREADS, THREADS < 512 ? 512 / THREADS : 1) residual_norm_backward_stream_kernel(NormBackwardParams b, int flags, int stages, int* status) {
+    using T = typename ElemOf<TYPE>::type;
+    const NormParams& p = b.f;
+    constexpr int NS = NORM_SUMS<LAYER>;
+    extern __shared__ __align__(128) uint8_t ring[];
+    __shared__ __align__(8) uint64_t bars[8];
+    __shared__ __align__(16) float exchange[2][3][32];
+    const int g = threadIdx.x, c = g * 8;
+    const bool mine = c < p.C;
+    const uint32_t row_bytes = (uint32_t)p.C * sizeof(T), sRing = (uint32_t)__cvta_generic_to_shared(ring), full = (uint32_t)__cvta_generic_to_shared(bars);
+    const uint32_t sPar = sRing + (uint32_t)stages * 4 * row_bytes;        // fp32: w2, w1, gate
+    const float inv_c = 1.f / (float)p.C;
+    const bool pre = p.w2 && b.gh, post = p.w1 != nullptr, want_u = post || p.gkind != TAB_GATE_NONE;
+    int bank = 0;
+    bool dead = false;
+    if (g == 0) {
+        for (int s = 0; s < stages; s++) mbar_init(full + 8 * s, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    __syncthreads();
+    pdl_wait();
+    auto request = [&](long long m, int s) {
+        const uint32_t at = sRing + (uint32_t)s * 4 * row_bytes;
+        mbar_expect_tx(full + 8 * s, row_bytes * ((pre ? 2u : 0u) + (b.gr ? 1u : 0u) + (want_u ? 1u : 0u)));
+        if (pre) {
+            bulk_load(at, static_cast<const T*>(b.gh) + m * b.ldgh, row_bytes, full + 8 * s);
+            bulk_load(at + row_bytes, static_cast<const T*>(p.r) + m * p.ldr, row_bytes, full + 8 * s);
+        }
+        if (b.gr) bulk_load(at + 2 * row_bytes, static_cast<const T*>(b.gr) + m * b.ldgr, row_bytes, full + 8 * s);
+        if (want_u) bulk_load(at + 3 * row_bytes, static_cast<const T*>(p.y) + m * p.ldy, row_bytes, full + 8 * s);
+    };
+    const long long step = gridDim.x;
+    if (g == 0)
+        for (int s = 0; s < stages; s++)
+            if (blockIdx.x + s * step < p.M) request(blockIdx.x + s * step, s);
+    if (mine) {                                                            // a thread reads back what it wrote itself
+        float w[8];
+        auto keep = [&](int k) {
+            sts_v4(sPar + (uint32_t)(k * p.C + c) * 4u, __float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]));
+            sts_v4(sPar + (uint32_t)(k * p.C + c) * 4u + 16u, __float_as_uint(w[4]), __float_as_uint(w[5]), __float_as_uint(w[6]), __float_as_uint(w[7]));
+        };
+        if (pre) { load8_any(p.w2, p.ptype, c, 8, flags & V_W2, w); keep(0); }
+        if (post) { load8_any(p.w1, p.ptype, c, 8, flags & V_W1, w); keep(1); }
+        if (p.gkind == TAB_GATE_CHANNEL) { load8_any(p.gate, p.gtype, c, 8, flags & V_G, w); keep(2); }
+    }
+    float sum[NS][8];
+#pragma unroll
+    for (int k = 0; k < NS; k++)
+#pragma unroll
+        for (int j = 0; j < 8; j++) sum[k][j] = 0.f;
+    float4 next = make_float4(0.f, 1.f, 0.f, 1.f);
+    if (p.stats && blockIdx.x < p.M) next = *reinterpret_cast<const float4*>(p.stats + 4 * (long long)blockIdx.x);
+    int slot = 0, turn = 0;
+    for (long long m = blockIdx.x; m < p.M; m += step) {
+        const float4 st = next;
+        if (p.stats && m + step < p.M) next = *reinterpret_cast<const float4*>(p.stats + 4 * (m + step));
+        if (!dead && !mbar_wait(full + 8 * slot, turn & 1)) { dead = true; if (status) atomicExch(status, 43); }
+        const uint32_t at = sRing + (uint32_t)slot * 4 * row_bytes;
+        float dr[8], red[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < 8; j++) dr[j] = 0.f;
+        if (b.gr && mine) lds8<TYPE>(at + 2 * row_bytes, c, dr);
+        if (pre) {
+            float t[8], rh[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) t[j] = rh[j] = 0.f;
+            if (mine) {
+                float w[8];
+                lds8<TYPE>(at, c, t);
+                lds8<TYPE>(at + row_bytes, c, rh);
+                lds8<TAB_FP32>(sPar, c, w);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    rh[j] = (rh[j] - st.z) * st.w;
+                    sum[0][j] += t[j] * rh[j];
+                    if (LAYER) sum[NS - 2][j] += t[j];
+                    t[j] *= w[j];
+                    red[0] += t[j] * rh[j];
+                    if (LAYER) red[1] += t[j];
+                }
+            }
+            cta_sums<THREADS / 32, 3>(red, exchange, bank);
+            const float c1 = red[0] * inv_c, c2 = LAYER ? red[1] * inv_c : 0.f;
+            if (mine)
+#pragma unroll
+                for (int j = 0; j < 8; j++) dr[j] += st.w * (t[j] - rh[j] * c1 - c2);
+        }
+        if (b.dx && mine) {
+            float d[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) d[j] = p.alpha * dr[j];
+            store8(static_cast<T*>(b.dx) + m * b.lddx + c, 8, flags & V_DX, d);
+        }
+        float yv[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) yv[j] = 0.f;
+        red[0] = red[1] = red[2] = 0.f;
+        if (want_u && mine) {
+            float w[8], gv[8], u[8];
+            lds8<TYPE>(at + 3 * row_bytes, c, yv);
+#pragma unroll
+            for (int j = 0; j < 8; j++) { w[j] = 1.f; gv[j] = 1.f; }
+            if (post) lds8<TAB_FP32>(sPar + (uint32_t)p.C * 4u, c, w);
+            if (p.gkind == TAB_GATE_CHANNEL) {
+                lds8<TAB_FP32>(sPar + (uint32_t)p.C * 8u, c, gv);
+            } else if (p.gkind == TAB_GATE_FULL) {
+                load8_any(p.gate, p.gtype, m * p.ldg + c, 8, flags & V_G, gv);
+            } else if (p.gkind == TAB_GATE_TOKEN) {
+                const float one = load_any(p.gate, p.gtype, m * p.ldg);
+#pragma unroll
+                for (int j = 0; j < 8; j++) gv[j] = one;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                yv[j] = (yv[j] - st.x) * st.y;                             // y itself without a norm: mean 0, deviation 1
+                u[j] = yv[j] * w[j];
+            }
+            if (LAYER && p.b1 && p.gkind != TAB_GATE_NONE) {
+                float s[8];
+                load8_any(p.b1, p.ptype, c, 8, flags & V_B1, s);
+#pragma unroll
+                for (int j = 0; j < 8; j++) u[j] += s[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                u[j] *= dr[j];                                             // the gate's gradient
+                red[2] += u[j];
+                if (p.gkind == TAB_GATE_CHANNEL) sum[2][j] += u[j];
+                const float du = dr[j] * gv[j];
+                dr[j] = du * w[j];
+                if (post) {
+                    sum[1][j] += du * yv[j];
+                    if (LAYER) sum[NS - 1][j] += du;
+                    red[0] += dr[j] * yv[j];
+                    if (LAYER) red[1] += dr[j];
+                }
+            }
+            if (p.gkind == TAB_GATE_FULL && b.dgate) store8_any(b.dgate, p.gtype, m * p.C + c, 8, flags & V_DG, u);
+        }
+        // everybody has read the row behind the next barrier
+        if (post || p.gkind == TAB_GATE_TOKEN) cta_sums<THREADS / 32, 3>(red, exchange, bank);
+        else __syncthreads();
+        if (g == 0 && m + stages * step < p.M) request(m + stages * step, slot);
+        if (p.gkind == TAB_GATE_TOKEN && b.dgate && g == 0) store_any(b.dgate, p.gtype, m, red[2]);
+        if (b.dy && mine) {
+            if (post) {
+                const float c1 = red[0] * inv_c, c2 = LAYER ? red[1] * inv_c : 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; j++) dr[j] = st.y * (dr[j] - yv[j] * c1 - c2);
+            }
+            store8(static_cast<T*>(b.dy) + m * b.lddy + c, 8, flags & V_DY, dr);
+        }
+        if (++slot == stages) { slot = 0; turn++; }
+    }
+    pdl_launch_dependents();
+    if (b.partial && mine)
+#pragma unroll
+        for (int k = 0; k < NS; k++) store8(b.partial + ((long long)blockIdx.x * NS + k) * p.C + c, 8, true, sum[k]);
+    if (dead) for (int i = 0; i < 200; i++) __nanosleep(1000);
+}
+
 // The CTAs' sums of a column, in their order: eight threads take every eighth of them, then one adds the eight.
 __global__ void __launch_bounds__(256) norm_sums_kernel(const float* partial, int parts, int NS, int C, int type, void* o0, void* o1, void* o2, int gtype, void* o3, void* o4) {
     __shared__ float acc[8][33];
@@ -343,6 +692,7 @@ static int norm_flags(const NormParams& p, int type) {
            (on8(p.q, p.ldq, 1) ? V_Q : 0) | (on8(p.w1, 0, w) ? V_W1 : 0) | (on8(p.b1, 0, w) ? V_B1 : 0) | (on8(p.w2, 0, w) ? V_W2 : 0) |
            (on8(p.b2, 0, w) ? V_B2 : 0) | (on8(p.gate, p.gkind == TAB_GATE_FULL ? p.ldg : 0, g) ? V_G : 0);
 }
+static constexpr int NORM_CTAS = 4 * 148;                                  // most CTAs of a stream kernel
 // How many parts of the rows are summed on their own (one for each group of threads of the backward kernel).
 static int norm_groups(int C) { return C <= 1024 ? 4 : 1; }
 static long long norm_parts(long long M, int C) {
@@ -350,7 +700,7 @@ static long long norm_parts(long long M, int C) {
     const long long wanted = std::min<long long>((long long)ctas * G, M);
     return (wanted + G - 1) / G * G;
 }
-size_t residual_norm_partial_bytes(long long M, int C) { return (size_t)norm_parts(M, C) * 5 * (size_t)C * sizeof(float); }
+size_t residual_norm_partial_bytes(long long M, int C) { return (size_t)std::max(norm_parts(M, C), std::min<long long>(M, NORM_CTAS)) * 5 * (size_t)C * sizeof(float); }
 
 template <int TYPE, int GT, int NV>
 static int launch_norm(const NormParams& p, cudaStream_t stream) {
@@ -361,24 +711,90 @@ static int launch_norm(const NormParams& p, cudaStream_t stream) {
     if (p.layer) return launch_pdl(residual_norm_kernel<TYPE, GT, NV, true>, dim3((unsigned)grid), dim3(GT < 128 ? 128 : GT), 0, stream, p, flags);
     return launch_pdl(residual_norm_kernel<TYPE, GT, NV, false>, dim3((unsigned)grid), dim3(GT < 128 ? 128 : GT), 0, stream, p, flags);
 }
+// What a stream kernel is launched with: CTAs that are all resident, and rows in flight.
+struct StreamPlan { int ctas, stages; size_t smem; };
+// row_bytes: of one row's tensors; fixed: bytes besides the ring.  0 stages: it does not fit, or does not pay.
+template <auto KERNEL>
+static StreamPlan stream_plan(int threads, long long M, size_t row_bytes, size_t fixed) {
+    StreamPlan pl = {0, 0, 0};
+    int dev = 0, sms = 148;
+    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return pl;
+    const int each = std::max(1, 1024 / threads);                      // CTAs an SM could hold by its threads
+    const size_t room = 226 * 1024;
+    for (int n = each; n >= 1 && !pl.stages; n = n > 1 ? n / 2 : 0) {
+        const size_t share = room / n - 2048;
+        const long long stages = share > fixed ? (long long)((share - fixed) / row_bytes) : 0;
+        if (stages >= 2 && M >= 2LL * n * sms) { pl.stages = (int)std::min<long long>(stages, 4); pl.ctas = std::min(n * sms, NORM_CTAS); }
+    }
+    if (!pl.stages) return pl;
+    pl.smem = pl.stages * row_bytes + fixed;
+    static std::mutex mu;
+    static bool configured[64] = {};
+    std::lock_guard<std::mutex> lock(mu);
+    if (dev < 0 || dev >= 64 || !configured[dev]) {
+        if (cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)room) != cudaSuccess) { cudaGetLastError(); pl.stages = 0; return pl; }
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+    }
+    return pl;
+}
+static bool rows16(const void* p, long long ld, int size) { return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld * size % 16 == 0); }
+// TAB_E_TOO_LARGE: the stream kernel does not take the problem.
+template <int TYPE, int THREADS>
+static int launch_norm_stream(const NormParams& p, cudaStream_t stream) {
+    const int s = type_bytes(TYPE), flags = norm_flags(p, TYPE);
+    if (p.C % 8 || !rows16(p.y, p.ldy, s) || !rows16(p.x, p.ldx, s)) return TAB_E_TOO_LARGE;
+    auto kernel = p.layer ? residual_norm_stream_kernel<TYPE, THREADS, true> : residual_norm_stream_kernel<TYPE, THREADS, false>;
+    const StreamPlan pl = p.layer ? stream_plan<residual_norm_stream_kernel<TYPE, THREADS, true>>(THREADS < 512 ? 2 * THREADS : 1024, p.M, 2 * (size_t)p.C * s, 0)
+                                  : stream_plan<residual_norm_stream_kernel<TYPE, THREADS, false>>(THREADS, p.M, 2 * (size_t)p.C * s, 0);
+    if (!pl.stages) return TAB_E_TOO_LARGE;
+    int* status = device_status_word();
+    if (stalled(status)) return TAB_E_STALLED;
+    return launch_pdl(kernel, dim3((unsigned)std::min<long long>(p.M, pl.ctas)), dim3(THREADS), pl.smem, stream, p, flags, pl.stages, status);
+}
+static int launch_norm_sums(const NormBackwardParams& b, int parts, cudaStream_t stream) {
+    const NormParams& p = b.f;
+    const int NS = p.layer ? NORM_SUMS<true> : NORM_SUMS<false>;
+    return launch_pdl(norm_sums_kernel, dim3((unsigned)((p.C + 31) / 32), (unsigned)NS), dim3(256), 0, stream, (const float*)b.partial, parts, NS, p.C, p.ptype, b.dw2, b.dw1,
+                      p.gkind == TAB_GATE_CHANNEL ? b.dgate : nullptr, p.gtype, p.layer ? b.db2 : nullptr, p.layer ? b.db1 : nullptr);
+}
+static bool wants_sums(const NormBackwardParams& b) { return b.dw1 || b.db1 || b.dw2 || b.db2 || (b.f.gkind == TAB_GATE_CHANNEL && b.dgate); }
+static int backward_flags(const NormBackwardParams& b, int type) {
+    const int s = type_bytes(type);
+    return norm_flags(b.f, type) | (on8(b.gr, b.ldgr, s) ? V_GR : 0) | (on8(b.gh, b.ldgh, s) ? V_GH : 0) | (on8(b.dy, b.lddy, s) ? V_DY : 0) |
+           (on8(b.dx, b.lddx, s) ? V_DX : 0) | (on8(b.dgate, b.f.C, type_bytes(b.f.gtype)) ? V_DG : 0);
+}
+template <int TYPE, int THREADS>
+static int launch_norm_backward_stream(NormBackwardParams b, cudaStream_t stream) {
+    const NormParams& p = b.f;
+    const int s = type_bytes(TYPE);
+    const bool pre = p.w2 && b.gh, want_u = p.w1 || p.gkind != TAB_GATE_NONE;
+    if (p.C % 8 || (pre && (!rows16(b.gh, b.ldgh, s) || !rows16(p.r, p.ldr, s))) || !rows16(b.gr, b.ldgr, s) || (want_u && !rows16(p.y, p.ldy, s)) || (!pre && !b.gr && !want_u)) return TAB_E_TOO_LARGE;
+    auto kernel = p.layer ? residual_norm_backward_stream_kernel<TYPE, THREADS, true> : residual_norm_backward_stream_kernel<TYPE, THREADS, false>;
+    const size_t fixed = 12 * (size_t)p.C, row = 4 * (size_t)p.C * s;
+    const StreamPlan pl = p.layer ? stream_plan<residual_norm_backward_stream_kernel<TYPE, THREADS, true>>(std::min(1024, 2 * THREADS), p.M, row, fixed)
+                                  : stream_plan<residual_norm_backward_stream_kernel<TYPE, THREADS, false>>(std::min(1024, 2 * THREADS), p.M, row, fixed);
+    if (!pl.stages) return TAB_E_TOO_LARGE;
+    int* status = device_status_word();
+    if (stalled(status)) return TAB_E_STALLED;
+    const bool sums = wants_sums(b);
+    if (!sums) b.partial = nullptr;
+    const int ctas = (int)std::min<long long>(p.M, pl.ctas);
+    const int rc = launch_pdl(kernel, dim3((unsigned)ctas), dim3(THREADS), pl.smem, stream, b, backward_flags(b, TYPE), pl.stages, status);
+    return rc != TAB_OK || !sums ? rc : launch_norm_sums(b, ctas, stream);
+}
+
 template <int TYPE, int GT, int NV>
 static int launch_norm_backward(NormBackwardParams b, cudaStream_t stream) {
     constexpr int G = GT < 128 ? 128 / GT : 1;
     const NormParams& p = b.f;
-    const int s = type_bytes(TYPE);
-    const int flags = norm_flags(p, TYPE) | (on8(b.gr, b.ldgr, s) ? V_GR : 0) | (on8(b.gh, b.ldgh, s) ? V_GH : 0) | (on8(b.dy, b.lddy, s) ? V_DY : 0) |
-                      (on8(b.dx, b.lddx, s) ? V_DX : 0) | (on8(b.dgate, p.C, type_bytes(p.gtype)) ? V_DG : 0);
     const long long parts = norm_parts(p.M, p.C), rows_each = (p.M + parts - 1) / parts;
-    void* dgate = p.gkind == TAB_GATE_CHANNEL ? b.dgate : nullptr;
-    const bool sums = b.dw1 || b.db1 || b.dw2 || b.db2 || dgate;
+    const bool sums = wants_sums(b);
     if (!sums) b.partial = nullptr;
     const dim3 grid((unsigned)(parts / G)), block(GT < 128 ? 128 : GT);
+    const int flags = backward_flags(b, TYPE);
     const int rc = p.layer ? launch_pdl(residual_norm_backward_kernel<TYPE, GT, NV, true>, grid, block, 0, stream, b, flags, rows_each)
                            : launch_pdl(residual_norm_backward_kernel<TYPE, GT, NV, false>, grid, block, 0, stream, b, flags, rows_each);
-    if (rc != TAB_OK || !sums) return rc;
-    const int NS = p.layer ? NORM_SUMS<true> : NORM_SUMS<false>;
-    return launch_pdl(norm_sums_kernel, dim3((unsigned)((p.C + 31) / 32), (unsigned)NS), dim3(256), 0, stream, (const float*)b.partial, (int)parts, NS, p.C, p.ptype, b.dw2, b.dw1, dgate, p.gtype,
-                      p.layer ? b.db2 : nullptr, p.layer ? b.db1 : nullptr);
+    return rc != TAB_OK || !sums ? rc : launch_norm_sums(b, (int)parts, stream);
 }
 
 #define TAB_NORM_SIZES(F, C, ARG) \
@@ -391,12 +807,23 @@ static int launch_norm_backward(NormBackwardParams b, cudaStream_t stream) {
 
 template <int TYPE>
 static int norm_sizes(const NormParams& p, cudaStream_t stream) {
+    int rc = TAB_E_TOO_LARGE;
+    if (p.C > 1024 && p.C <= 2048) rc = launch_norm_stream<TYPE, 256>(p, stream);
+    else if (p.C > 2048 && p.C <= 4096) rc = launch_norm_stream<TYPE, 512>(p, stream);
+    else if (p.C > 4096 && p.C <= 8192) rc = launch_norm_stream<TYPE, 1024>(p, stream);
+    if (rc != TAB_E_TOO_LARGE) return rc;
 #define TAB_NORM_F(GT, NV) launch_norm<TYPE, GT, NV>
     TAB_NORM_SIZES(TAB_NORM_F, p.C, p);
 #undef TAB_NORM_F
 }
 template <int TYPE>
 static int norm_backward_sizes(const NormBackwardParams& b, cudaStream_t stream) {
+    int rc = TAB_E_TOO_LARGE;
+    if (b.f.C > 256 && b.f.C <= 1024) rc = launch_norm_backward_stream<TYPE, 128>(b, stream);
+    else if (b.f.C > 1024 && b.f.C <= 2048) rc = launch_norm_backward_stream<TYPE, 256>(b, stream);
+    else if (b.f.C > 2048 && b.f.C <= 4096) rc = launch_norm_backward_stream<TYPE, 512>(b, stream);
+    else if (b.f.C > 4096 && b.f.C <= 8192) rc = launch_norm_backward_stream<TYPE, 1024>(b, stream);
+    if (rc != TAB_E_TOO_LARGE) return rc;
 #define TAB_NORM_B(GT, NV) launch_norm_backward<TYPE, GT, NV>
     TAB_NORM_SIZES(TAB_NORM_B, b.f.C, b);
 #undef TAB_NORM_B

@@ -95,6 +95,17 @@ CASES = [
     ((4, 16384), "bf16", "fp32", "rms", "channel", True, True, True, 1.0),
     ((3, 12345), "fp32", "fp32", "layer", "full", True, True, True, 1.0),
     ((2000, 64), "bf16", "fp32", "rms", "token", True, True, True, 1.0),
+    # many rows
+    ((1300, 264), "fp32", "fp32", "layer", "token", True, True, True, 1.0),
+    ((2500, 512), "bf16", "bf16", "rms", "channel", True, True, True, 1.5),
+    ((1300, 1032), "bf16", "fp32", "rms", "token", True, True, True, 1.0),
+    ((700, 2048), "fp16", "fp32", "layer", "channel", True, True, True, 1.0),
+    ((700, 4096), "bf16", "fp32", "rms", "channel", True, True, True, 1.25),
+    ((333, 4000), "fp32", "fp32", "layer", "full", True, True, True, 1.0),
+    ((640, 3064), "bf16", "bf16", "rms", None, False, True, True, 1.0),
+    ((600, 2056), "bf16", "fp32", "rms", "full", True, False, False, 1.0),
+    ((400, 8192), "bf16", "fp32", "layer", "channel", True, True, True, 1.0),
+    ((310, 5008), "fp16", "fp32", "rms", "token", False, True, True, 1.0),
 ]
 
 
@@ -134,7 +145,8 @@ def test_residual_norm(cuda, case):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("format", ["e4m3", "e5m2"])
-@pytest.mark.parametrize("shape, type, kind", [((1, 4096), "bf16", "rms"), ((33, 100), "fp32", "layer"), ((2, 9, 1411), "bf16", "rms"), ((3, 9000), "fp16", "layer"), ((260, 128), "bf16", "rms")])
+@pytest.mark.parametrize("shape, type, kind", [((1, 4096), "bf16", "rms"), ((33, 100), "fp32", "layer"), ((2, 9, 1411), "bf16", "rms"), ((3, 9000), "fp16", "layer"), ((260, 128), "bf16", "rms"),
+                                               ((700, 4096), "bf16", "rms"), ((310, 8192), "bf16", "layer"), ((600, 1416), "fp32", "rms")])
 def test_residual_norm_quantized(cuda, shape, type, kind, format):
     """h as blocks: what the stored r gives in 64 bits, up to the roundings of fp32 (64 units of 2^-24 of the largest of the block) and then
     half a step of the format under the block's scale."""
