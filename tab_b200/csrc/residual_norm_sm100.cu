@@ -327,17 +327,73 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(mbar) : "memory");
 }
-// Eight values in shared memory at `at` + column * size.
+// Two floats an instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 z, x, y;\n\tmov.b64 {%0, %1}, z;}" : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{.reg .b64 x, y, w, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 w, {%6, %7};\n\tfma.rn.f32x2 z, x, y, w;\n\tmov.b64 {%0, %1}, z;}"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 both(float a) { return make_float2(a, a); }
+using Pairs = float2[4];                                                   // a thread's eight columns
+__device__ __forceinline__ void to_pairs(const float (&v)[8], Pairs& p) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) p[i] = make_float2(v[2 * i], v[2 * i + 1]);
+}
+__device__ __forceinline__ float sum_of(const Pairs& p) {
+    const float2 s = add2(add2(p[0], p[1]), add2(p[2], p[3]));
+    return s.x + s.y;
+}
+// Sum of a[i] * b[i].
+__device__ __forceinline__ float dot_of(const Pairs& a, const Pairs& b) {
+    const float2 s = fma2(a[0], b[0], mul2(a[1], b[1])), t = fma2(a[2], b[2], mul2(a[3], b[3])), u = add2(s, t);
+    return u.x + u.y;
+}
+__device__ __forceinline__ void pairs_any(const void* p, int type, long long at, Pairs& v) {
+    float f[8];
+    load8_any(p, type, at, 8, true, f);
+    to_pairs(f, v);
+}
+// Eight values of a row in shared memory.
 template <int TYPE>
-__device__ __forceinline__ void lds8(uint32_t row, int c, float (&v)[8]) {
+__device__ __forceinline__ void lds_pairs(uint32_t row, int c, Pairs& v) {
     using T = typename ElemOf<TYPE>::type;
-    if (TYPE == TAB_FP32) {
+    if constexpr (TYPE == TAB_FP32) {
         const int4 a = lds_v4(row + c * 4), b = lds_v4(row + c * 4 + 16);
-        v[0] = __int_as_float(a.x); v[1] = __int_as_float(a.y); v[2] = __int_as_float(a.z); v[3] = __int_as_float(a.w);
-        v[4] = __int_as_float(b.x); v[5] = __int_as_float(b.y); v[6] = __int_as_float(b.z); v[7] = __int_as_float(b.w);
+        v[0] = make_float2(__int_as_float(a.x), __int_as_float(a.y)); v[1] = make_float2(__int_as_float(a.z), __int_as_float(a.w));
+        v[2] = make_float2(__int_as_float(b.x), __int_as_float(b.y)); v[3] = make_float2(__int_as_float(b.z), __int_as_float(b.w));
     } else {
         const int4 a = lds_v4(row + c * 2);
-        if constexpr (TYPE != TAB_FP32) widen8(make_uint4((uint32_t)a.x, (uint32_t)a.y, (uint32_t)a.z, (uint32_t)a.w), v, T());
+        float f[8];
+        widen8(make_uint4((uint32_t)a.x, (uint32_t)a.y, (uint32_t)a.z, (uint32_t)a.w), f, T());
+        to_pairs(f, v);
+    }
+}
+// Eight results to memory; `kept`: they become what was stored.
+template <int TYPE>
+__device__ __forceinline__ void store_pairs(void* p, long long at, Pairs& v, bool kept) {
+    using T = typename ElemOf<TYPE>::type;
+    if constexpr (TYPE == TAB_FP32) {
+        const float f[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+        if (p) store8(static_cast<float*>(p) + at, 8, true, f);
+    } else {
+        const uint4 u = make_uint4(pack2(v[0].x, v[0].y, T()), pack2(v[1].x, v[1].y, T()), pack2(v[2].x, v[2].y, T()), pack2(v[3].x, v[3].y, T()));
+        if (p) *reinterpret_cast<uint4*>(static_cast<T*>(p) + at) = u;
+        if (kept) {
+            float f[8];
+            widen8(u, f, T());
+            to_pairs(f, v);
+        }
     }
 }
 // Sums over the CTA, the same in all threads; `bank` alternates as in row_sums.
@@ -354,21 +410,26 @@ __device__ __forceinline__ void cta_sums(float (&v)[N], float (*exchange)[N][32]
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        float s = 0.f;
-        if (WARPS >= 4) {
+        if (WARPS <= 8) {
+            float s = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS; w += 4) {
                 const float4 e = *reinterpret_cast<const float4*>(&exchange[bank][i][w]);
                 s += (e.x + e.y) + (e.z + e.w);
             }
+            v[i] = s;
+        } else {
+            float s = exchange[bank][i][lane & (WARPS - 1)];
+#pragma unroll
+            for (int o = WARPS / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xFFFFFFFFu, s, o);
+            v[i] = s;
         }
-        v[i] = s;
     }
     bank ^= 1;
 }
 
-template <int TYPE, int THREADS, bool LAYER>
-__global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREADS : 1) : 1024 / THREADS) residual_norm_stream_kernel(NormParams p, int flags, int stages, int* status) {
+template <int TYPE, int THREADS, bool LAYER, bool QUANT>
+__global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREADS : 1) : 1024 / THREADS) residual_norm_stream_kernel(NormParams p, int stages, int* status) {
     using T = typename ElemOf<TYPE>::type;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[8];
@@ -395,26 +456,30 @@ __global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREAD
     if (g == 0)
         for (int s = 0; s < stages; s++)
             if (blockIdx.x + s * step < p.M) request(blockIdx.x + s * step, s);
-    float w1[8], w2[8], gate[8];
+    Pairs w1, w2, gate;
 #pragma unroll
-    for (int j = 0; j < 8; j++) w1[j] = w2[j] = gate[j] = 0.f;
+    for (int j = 0; j < 4; j++) w1[j] = w2[j] = gate[j] = both(0.f);
     if (mine) {
-        if (p.w1) load8_any(p.w1, p.ptype, c, 8, flags & V_W1, w1);
-        if (p.w2) load8_any(p.w2, p.ptype, c, 8, flags & V_W2, w2);
-        if (p.gkind == TAB_GATE_CHANNEL) load8_any(p.gate, p.gtype, c, 8, flags & V_G, gate);
+        if (p.w1) pairs_any(p.w1, p.ptype, c, w1);
+        if (p.w2) pairs_any(p.w2, p.ptype, c, w2);
+        if (p.gkind == TAB_GATE_CHANNEL) pairs_any(p.gate, p.gtype, c, gate);
     }
+    const bool gate_now = p.gkind == TAB_GATE_CHANNEL && (LAYER || !p.w1);
+    if (!LAYER && p.gkind == TAB_GATE_CHANNEL && p.w1)                     // no shift between the two: one factor
+#pragma unroll
+        for (int j = 0; j < 4; j++) w1[j] = mul2(w1[j], gate[j]);
     int slot = 0, turn = 0;
     for (long long m = blockIdx.x; m < p.M; m += step) {
         if (!dead && !mbar_wait(full + 8 * slot, turn & 1)) { dead = true; if (status) atomicExch(status, 42); }
         const uint32_t at = sRing + (uint32_t)slot * 2 * row_bytes;
-        float v[8], x[8];
+        Pairs v, x;
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = x[j] = 0.f;
+        for (int j = 0; j < 4; j++) v[j] = x[j] = both(0.f);
         if (mine) {
-            lds8<TYPE>(at, c, v);
-            if (p.x) lds8<TYPE>(at + row_bytes, c, x);
+            lds_pairs<TYPE>(at, c, v);
+            if (p.x) lds_pairs<TYPE>(at + row_bytes, c, x);
         }
-        // Both sums of a norm; the first barrier of a row also says that everybody has read it, and its place is filled again.
+        // The first barrier of a row also says that everybody has read it, and its place is filled again.
         bool open = true;
         auto refill = [&]() {
             if (open && g == 0 && m + stages * step < p.M) request(m + stages * step, slot);
@@ -424,74 +489,93 @@ __global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREAD
             float s[1];
             mean = 0.f;
             if (LAYER) {
-                s[0] = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+                s[0] = sum_of(v);
                 cta_sums<THREADS / 32, 1>(s, exchange, bank);
                 refill();
                 mean = s[0] * inv_c;
-            }
-            s[0] = 0.f;
+                if (mine)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                if (LAYER && mine) v[j] -= mean;
-                s[0] += v[j] * v[j];
+                    for (int j = 0; j < 4; j++) v[j] = add2(v[j], both(-mean));
             }
+            s[0] = dot_of(v, v);
             cta_sums<THREADS / 32, 1>(s, exchange, bank);
             refill();
             inverse = 1.f / sqrtf(s[0] * inv_c + p.eps);
+        };
+        auto shift = [&](const void* b) {
+            Pairs f;
+            if (!mine) return;
+            pairs_any(b, p.ptype, c, f);
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = add2(v[j], f[j]);
         };
         float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
         if (p.w1) {
             normalise(st.x, st.y);
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = v[j] * st.y * w1[j];
-            if (LAYER && p.b1 && mine) {
-                float b[8];
-                load8_any(p.b1, p.ptype, c, 8, flags & V_B1, b);
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] += b[j];
-            }
+            for (int j = 0; j < 4; j++) v[j] = mul2(mul2(v[j], both(st.y)), w1[j]);
+            if (LAYER && p.b1) shift(p.b1);
         }
-        if (p.gkind == TAB_GATE_CHANNEL) {
+        if (gate_now) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] *= gate[j];
-        } else if (p.gkind != TAB_GATE_NONE && mine) {
-            float f[8];
+            for (int j = 0; j < 4; j++) v[j] = mul2(v[j], gate[j]);
+        } else if ((p.gkind == TAB_GATE_FULL || p.gkind == TAB_GATE_TOKEN) && mine) {
+            Pairs f;
             if (p.gkind == TAB_GATE_FULL) {
-                load8_any(p.gate, p.gtype, m * p.ldg + c, 8, flags & V_G, f);
+                pairs_any(p.gate, p.gtype, m * p.ldg + c, f);
             } else {
                 const float one = load_any(p.gate, p.gtype, m * p.ldg);
 #pragma unroll
-                for (int j = 0; j < 8; j++) f[j] = one;
+                for (int j = 0; j < 4; j++) f[j] = both(one);
             }
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] *= f[j];
+            for (int j = 0; j < 4; j++) v[j] = mul2(v[j], f[j]);
         }
         if (p.x) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = fmaf(p.alpha, x[j], v[j]);
+            for (int j = 0; j < 4; j++) v[j] = fma2(both(p.alpha), x[j], v[j]);
         }
-        if (mine && p.r) store8(static_cast<T*>(p.r) + m * p.ldr + c, 8, flags & V_R, v);
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = to_float(from_float<T>(v[j]));          // r as it is kept
+        store_pairs<TYPE>(mine ? p.r : nullptr, m * p.ldr + c, v, true);           // v: r as it is kept
         if (p.w2) {
             normalise(st.z, st.w);
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = v[j] * st.w * w2[j];
-            if (LAYER && p.b2 && mine) {
-                float b[8];
-                load8_any(p.b2, p.ptype, c, 8, flags & V_B2, b);
+            for (int j = 0; j < 4; j++) v[j] = mul2(mul2(v[j], both(st.w)), w2[j]);
+            if (LAYER && p.b2) shift(p.b2);
+            if (p.h && mine) store_pairs<TYPE>(p.h, m * p.ldh + c, v, false);
+            if (QUANT) {
+                // The larger magnitude, which fmaxf takes past NaN; a block with an infinity is looked at again.
+                float a = 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[j] += b[j];
-            }
-            if (p.h && mine) store8(static_cast<T*>(p.h) + m * p.ldh + c, 8, flags & V_H, v);
-            if (p.q) {
-                uint32_t a = 0;
+                for (int j = 0; j < 4; j++) a = fmaxf(a, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
 #pragma unroll
-                for (int j = 0; j < 8; j++) a = max(a, mine ? finite_bits(v[j]) : 0u);
-                const int e = scale_exponent(half_warp_max(a), p.format);
+                for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+                const float f[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+                const bool odd = __any_sync(0xFFFFFFFFu, isinf(a));
+                uint32_t bits = __float_as_uint(a);
+                if (odd) {
+                    bits = 0;
+#pragma unroll
+                    for (int j = 0; j < 8; j++) bits = max(bits, finite_bits(f[j]));
+                    bits = half_warp_max(bits);
+                }
+                const int e = scale_exponent(bits, p.format);
                 const float inv = exp2_int(-e);
+                uint2 o;
+                if (odd) o = p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(f, inv) : narrow8<TAB_E4M3>(f, inv);
+                else {
+                    Pairs y;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) y[j] = mul2(v[j], both(inv));
+                    if (p.format == TAB_E5M2) {
+                        o.x = __byte_perm(narrow2<TAB_E5M2>(y[0].x, y[0].y), narrow2<TAB_E5M2>(y[1].x, y[1].y), 0x5410);
+                        o.y = __byte_perm(narrow2<TAB_E5M2>(y[2].x, y[2].y), narrow2<TAB_E5M2>(y[3].x, y[3].y), 0x5410);
+                    } else {
+                        o.x = __byte_perm(narrow2<TAB_E4M3>(y[0].x, y[0].y), narrow2<TAB_E4M3>(y[1].x, y[1].y), 0x5410);
+                        o.y = __byte_perm(narrow2<TAB_E4M3>(y[2].x, y[2].y), narrow2<TAB_E4M3>(y[3].x, y[3].y), 0x5410);
+                    }
+                }
                 if (mine) {
-                    store_bytes8(static_cast<uint8_t*>(p.q) + m * p.ldq + c, 8, flags & V_Q, p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(v, inv) : narrow8<TAB_E4M3>(v, inv));
+                    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.q) + m * p.ldq + c) = o;
                     if ((g & 15) == 0) p.s[(long long)(c / BLK) * p.lds + m] = (uint8_t)(e + 127);
                 }
             }
@@ -504,21 +588,22 @@ __global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREAD
     if (dead) for (int i = 0; i < 200; i++) __nanosleep(1000);             // copies that may still be under way land before this memory is another's
 }
 
-template <int TYPE, int THREADS, bool LAYER>
-__global__ void __launch_bounds__(THREADS, THREADS < 512 ? 512 / THREADS : 1) residual_norm_backward_stream_kernel(NormBackwardParams b, int flags, int stages, int* status) {
+template <int TYPE, int THREADS, bool LAYER, bool TOKEN>
+__global__ void __launch_bounds__(THREADS, THREADS < 512 ? 512 / THREADS : 1) residual_norm_backward_stream_kernel(NormBackwardParams b, int stages, int* status) {
     using T = typename ElemOf<TYPE>::type;
     const NormParams& p = b.f;
-    constexpr int NS = NORM_SUMS<LAYER>;
+    constexpr int NS = NORM_SUMS<LAYER>, N1 = LAYER ? 2 : 1, N2 = N1 + (TOKEN ? 1 : 0);
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[8];
-    __shared__ __align__(16) float exchange[2][3][32];
+    __shared__ __align__(16) float exchange1[2][N1][32];
+    __shared__ __align__(16) float exchange2[2][N2][32];
     const int g = threadIdx.x, c = g * 8;
     const bool mine = c < p.C;
     const uint32_t row_bytes = (uint32_t)p.C * sizeof(T), sRing = (uint32_t)__cvta_generic_to_shared(ring), full = (uint32_t)__cvta_generic_to_shared(bars);
     const uint32_t sPar = sRing + (uint32_t)stages * 4 * row_bytes;        // fp32: w2, w1, gate
     const float inv_c = 1.f / (float)p.C;
     const bool pre = p.w2 && b.gh, post = p.w1 != nullptr, want_u = post || p.gkind != TAB_GATE_NONE;
-    int bank = 0;
+    int bank1 = 0, bank2 = 0;
     bool dead = false;
     if (g == 0) {
         for (int s = 0; s < stages; s++) mbar_init(full + 8 * s, 1);
@@ -541,20 +626,21 @@ __global__ void __launch_bounds__(THREADS, THREADS < 512 ? 512 / THREADS : 1) re
         for (int s = 0; s < stages; s++)
             if (blockIdx.x + s * step < p.M) request(blockIdx.x + s * step, s);
     if (mine) {                                                            // a thread reads back what it wrote itself
-        float w[8];
+        Pairs w;
         auto keep = [&](int k) {
-            sts_v4(sPar + (uint32_t)(k * p.C + c) * 4u, __float_as_uint(w[0]), __float_as_uint(w[1]), __float_as_uint(w[2]), __float_as_uint(w[3]));
-            sts_v4(sPar + (uint32_t)(k * p.C + c) * 4u + 16u, __float_as_uint(w[4]), __float_as_uint(w[5]), __float_as_uint(w[6]), __float_as_uint(w[7]));
+            const uint32_t to = sPar + (uint32_t)(k * p.C + c) * 4u;
+            sts_v4(to, __float_as_uint(w[0].x), __float_as_uint(w[0].y), __float_as_uint(w[1].x), __float_as_uint(w[1].y));
+            sts_v4(to + 16u, __float_as_uint(w[2].x), __float_as_uint(w[2].y), __float_as_uint(w[3].x), __float_as_uint(w[3].y));
         };
-        if (pre) { load8_any(p.w2, p.ptype, c, 8, flags & V_W2, w); keep(0); }
-        if (post) { load8_any(p.w1, p.ptype, c, 8, flags & V_W1, w); keep(1); }
-        if (p.gkind == TAB_GATE_CHANNEL) { load8_any(p.gate, p.gtype, c, 8, flags & V_G, w); keep(2); }
+        if (pre) { pairs_any(p.w2, p.ptype, c, w); keep(0); }
+        if (post) { pairs_any(p.w1, p.ptype, c, w); keep(1); }
+        if (p.gkind == TAB_GATE_CHANNEL) { pairs_any(p.gate, p.gtype, c, w); keep(2); }
     }
-    float sum[NS][8];
+    float2 sum[NS][4];
 #pragma unroll
     for (int k = 0; k < NS; k++)
 #pragma unroll
-        for (int j = 0; j < 8; j++) sum[k][j] = 0.f;
+        for (int j = 0; j < 4; j++) sum[k][j] = both(0.f);
     float4 next = make_float4(0.f, 1.f, 0.f, 1.f);
     if (p.stats && blockIdx.x < p.M) next = *reinterpret_cast<const float4*>(p.stats + 4 * (long long)blockIdx.x);
     int slot = 0, turn = 0;
@@ -563,106 +649,135 @@ __global__ void __launch_bounds__(THREADS, THREADS < 512 ? 512 / THREADS : 1) re
         if (p.stats && m + step < p.M) next = *reinterpret_cast<const float4*>(p.stats + 4 * (m + step));
         if (!dead && !mbar_wait(full + 8 * slot, turn & 1)) { dead = true; if (status) atomicExch(status, 43); }
         const uint32_t at = sRing + (uint32_t)slot * 4 * row_bytes;
-        float dr[8], red[3] = {0.f, 0.f, 0.f};
+        Pairs dr;
 #pragma unroll
-        for (int j = 0; j < 8; j++) dr[j] = 0.f;
-        if (b.gr && mine) lds8<TYPE>(at + 2 * row_bytes, c, dr);
+        for (int j = 0; j < 4; j++) dr[j] = both(0.f);
+        if (b.gr && mine) lds_pairs<TYPE>(at + 2 * row_bytes, c, dr);
         if (pre) {
-            float t[8], rh[8];
+            Pairs t, rh;
+            float red[N1];
 #pragma unroll
-            for (int j = 0; j < 8; j++) t[j] = rh[j] = 0.f;
+            for (int j = 0; j < 4; j++) t[j] = rh[j] = both(0.f);
             if (mine) {
-                float w[8];
-                lds8<TYPE>(at, c, t);
-                lds8<TYPE>(at + row_bytes, c, rh);
-                lds8<TAB_FP32>(sPar, c, w);
+                Pairs w;
+                lds_pairs<TYPE>(at, c, t);
+                lds_pairs<TYPE>(at + row_bytes, c, rh);
+                lds_pairs<TAB_FP32>(sPar, c, w);
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    rh[j] = (rh[j] - st.z) * st.w;
-                    sum[0][j] += t[j] * rh[j];
-                    if (LAYER) sum[NS - 2][j] += t[j];
-                    t[j] *= w[j];
-                    red[0] += t[j] * rh[j];
-                    if (LAYER) red[1] += t[j];
+                for (int j = 0; j < 4; j++) {
+                    if (LAYER) rh[j] = add2(rh[j], both(-st.z));
+                    rh[j] = mul2(rh[j], both(st.w));
+                    sum[0][j] = fma2(t[j], rh[j], sum[0][j]);
+                    if (LAYER) sum[NS - 2][j] = add2(sum[NS - 2][j], t[j]);
+                    t[j] = mul2(t[j], w[j]);
                 }
             }
-            cta_sums<THREADS / 32, 3>(red, exchange, bank);
-            const float c1 = red[0] * inv_c, c2 = LAYER ? red[1] * inv_c : 0.f;
+            red[0] = dot_of(t, rh);
+            if (LAYER) red[N1 - 1] = sum_of(t);
+            cta_sums<THREADS / 32, N1>(red, exchange1, bank1);
+            const float c1 = -red[0] * inv_c, c2 = LAYER ? -red[N1 - 1] * inv_c : 0.f;
             if (mine)
 #pragma unroll
-                for (int j = 0; j < 8; j++) dr[j] += st.w * (t[j] - rh[j] * c1 - c2);
+                for (int j = 0; j < 4; j++) {
+                    t[j] = fma2(rh[j], both(c1), t[j]);
+                    if (LAYER) t[j] = add2(t[j], both(c2));
+                    dr[j] = fma2(t[j], both(st.w), dr[j]);
+                }
         }
         if (b.dx && mine) {
-            float d[8];
+            Pairs d;
 #pragma unroll
-            for (int j = 0; j < 8; j++) d[j] = p.alpha * dr[j];
-            store8(static_cast<T*>(b.dx) + m * b.lddx + c, 8, flags & V_DX, d);
+            for (int j = 0; j < 4; j++) d[j] = mul2(dr[j], both(p.alpha));
+            store_pairs<TYPE>(b.dx, m * b.lddx + c, d, false);
         }
-        float yv[8];
+        Pairs yv;
+        float red[N2];
 #pragma unroll
-        for (int j = 0; j < 8; j++) yv[j] = 0.f;
-        red[0] = red[1] = red[2] = 0.f;
+        for (int i = 0; i < N2; i++) red[i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; j++) yv[j] = both(0.f);
         if (want_u && mine) {
-            float w[8], gv[8], u[8];
-            lds8<TYPE>(at + 3 * row_bytes, c, yv);
+            Pairs w, gv, u;
+            lds_pairs<TYPE>(at + 3 * row_bytes, c, yv);
 #pragma unroll
-            for (int j = 0; j < 8; j++) { w[j] = 1.f; gv[j] = 1.f; }
-            if (post) lds8<TAB_FP32>(sPar + (uint32_t)p.C * 4u, c, w);
+            for (int j = 0; j < 4; j++) w[j] = gv[j] = both(1.f);
+            if (post) lds_pairs<TAB_FP32>(sPar + (uint32_t)p.C * 4u, c, w);
             if (p.gkind == TAB_GATE_CHANNEL) {
-                lds8<TAB_FP32>(sPar + (uint32_t)p.C * 8u, c, gv);
+                lds_pairs<TAB_FP32>(sPar + (uint32_t)p.C * 8u, c, gv);
             } else if (p.gkind == TAB_GATE_FULL) {
-                load8_any(p.gate, p.gtype, m * p.ldg + c, 8, flags & V_G, gv);
-            } else if (p.gkind == TAB_GATE_TOKEN) {
+                pairs_any(p.gate, p.gtype, m * p.ldg + c, gv);
+            } else if (TOKEN) {
                 const float one = load_any(p.gate, p.gtype, m * p.ldg);
 #pragma unroll
-                for (int j = 0; j < 8; j++) gv[j] = one;
+                for (int j = 0; j < 4; j++) gv[j] = both(one);
             }
+            if (post)
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                yv[j] = (yv[j] - st.x) * st.y;                             // y itself without a norm: mean 0, deviation 1
-                u[j] = yv[j] * w[j];
-            }
-            if (LAYER && p.b1 && p.gkind != TAB_GATE_NONE) {
-                float s[8];
-                load8_any(p.b1, p.ptype, c, 8, flags & V_B1, s);
+                for (int j = 0; j < 4; j++) {
+                    if (LAYER) yv[j] = add2(yv[j], both(-st.x));
+                    yv[j] = mul2(yv[j], both(st.y));
+                }
+            if (p.gkind != TAB_GATE_NONE) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) u[j] += s[j];
-            }
+                for (int j = 0; j < 4; j++) u[j] = mul2(yv[j], w[j]);
+                if (LAYER && p.b1) {
+                    Pairs s;
+                    pairs_any(p.b1, p.ptype, c, s);
 #pragma unroll
-            for (int j = 0; j < 8; j++) {
-                u[j] *= dr[j];                                             // the gate's gradient
-                red[2] += u[j];
-                if (p.gkind == TAB_GATE_CHANNEL) sum[2][j] += u[j];
-                const float du = dr[j] * gv[j];
-                dr[j] = du * w[j];
-                if (post) {
-                    sum[1][j] += du * yv[j];
-                    if (LAYER) sum[NS - 1][j] += du;
-                    red[0] += dr[j] * yv[j];
-                    if (LAYER) red[1] += dr[j];
+                    for (int j = 0; j < 4; j++) u[j] = add2(u[j], s[j]);
+                }
+                if (p.gkind == TAB_GATE_CHANNEL) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sum[2][j] = fma2(u[j], dr[j], sum[2][j]);
+                } else if (TOKEN) {
+                    red[N2 - 1] = dot_of(u, dr);
+                } else if (b.dgate) {
+                    float d[8];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) { d[2 * j] = u[j].x * dr[j].x; d[2 * j + 1] = u[j].y * dr[j].y; }
+                    store8_any(b.dgate, p.gtype, m * p.C + c, 8, true, d);
                 }
             }
-            if (p.gkind == TAB_GATE_FULL && b.dgate) store8_any(b.dgate, p.gtype, m * p.C + c, 8, flags & V_DG, u);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 du = mul2(dr[j], gv[j]);
+                if (post) {
+                    sum[1][j] = fma2(du, yv[j], sum[1][j]);
+                    if (LAYER) sum[NS - 1][j] = add2(sum[NS - 1][j], du);
+                }
+                dr[j] = mul2(du, w[j]);
+            }
+            if (post) {
+                red[0] = dot_of(dr, yv);
+                if (LAYER) red[1 % N2] = sum_of(dr);
+            }
         }
         // everybody has read the row behind the next barrier
-        if (post || p.gkind == TAB_GATE_TOKEN) cta_sums<THREADS / 32, 3>(red, exchange, bank);
+        if (post || TOKEN) cta_sums<THREADS / 32, N2>(red, exchange2, bank2);
         else __syncthreads();
         if (g == 0 && m + stages * step < p.M) request(m + stages * step, slot);
-        if (p.gkind == TAB_GATE_TOKEN && b.dgate && g == 0) store_any(b.dgate, p.gtype, m, red[2]);
+        if (TOKEN && b.dgate && g == 0) store_any(b.dgate, p.gtype, m, red[N2 - 1]);
         if (b.dy && mine) {
             if (post) {
-                const float c1 = red[0] * inv_c, c2 = LAYER ? red[1] * inv_c : 0.f;
+                const float c1 = -red[0] * inv_c, c2 = LAYER ? -red[1 % N2] * inv_c : 0.f;
 #pragma unroll
-                for (int j = 0; j < 8; j++) dr[j] = st.y * (dr[j] - yv[j] * c1 - c2);
+                for (int j = 0; j < 4; j++) {
+                    dr[j] = fma2(yv[j], both(c1), dr[j]);
+                    if (LAYER) dr[j] = add2(dr[j], both(c2));
+                    dr[j] = mul2(dr[j], both(st.y));
+                }
             }
-            store8(static_cast<T*>(b.dy) + m * b.lddy + c, 8, flags & V_DY, dr);
+            store_pairs<TYPE>(b.dy, m * b.lddy + c, dr, false);
         }
         if (++slot == stages) { slot = 0; turn++; }
     }
     pdl_launch_dependents();
     if (b.partial && mine)
 #pragma unroll
-        for (int k = 0; k < NS; k++) store8(b.partial + ((long long)blockIdx.x * NS + k) * p.C + c, 8, true, sum[k]);
+        for (int k = 0; k < NS; k++) {
+            const float f[8] = {sum[k][0].x, sum[k][0].y, sum[k][1].x, sum[k][1].y, sum[k][2].x, sum[k][2].y, sum[k][3].x, sum[k][3].y};
+            store8(b.partial + ((long long)blockIdx.x * NS + k) * p.C + c, 8, true, f);
+        }
     if (dead) for (int i = 0; i < 200; i++) __nanosleep(1000);
 }
 
@@ -692,7 +807,7 @@ static int norm_flags(const NormParams& p, int type) {
            (on8(p.q, p.ldq, 1) ? V_Q : 0) | (on8(p.w1, 0, w) ? V_W1 : 0) | (on8(p.b1, 0, w) ? V_B1 : 0) | (on8(p.w2, 0, w) ? V_W2 : 0) |
            (on8(p.b2, 0, w) ? V_B2 : 0) | (on8(p.gate, p.gkind == TAB_GATE_FULL ? p.ldg : 0, g) ? V_G : 0);
 }
-static constexpr int NORM_CTAS = 4 * 148;                                  // most CTAs of a stream kernel
+static constexpr int NORM_CTAS = 8 * 148;                                  // most CTAs of a stream kernel
 // How many parts of the rows are summed on their own (one for each group of threads of the backward kernel).
 static int norm_groups(int C) { return C <= 1024 ? 4 : 1; }
 static long long norm_parts(long long M, int C) {
@@ -738,18 +853,26 @@ static StreamPlan stream_plan(int threads, long long M, size_t row_bytes, size_t
     return pl;
 }
 static bool rows16(const void* p, long long ld, int size) { return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld * size % 16 == 0); }
+// Whether all tensors that are there have rows a stream kernel can move eight elements at a time.
+static bool norm_streams(const NormParams& p, int type, int flags) {
+    const int s = type_bytes(type);
+    return p.C % 8 == 0 && rows16(p.y, p.ldy, s) && rows16(p.x, p.ldx, s) && (!p.r || (flags & V_R)) && (!p.h || (flags & V_H)) && (!p.q || (flags & V_Q)) && (!p.w1 || (flags & V_W1)) &&
+           (!p.b1 || (flags & V_B1)) && (!p.w2 || (flags & V_W2)) && (!p.b2 || (flags & V_B2)) && (p.gkind < TAB_GATE_CHANNEL || (flags & V_G));
+}
 // TAB_E_TOO_LARGE: the stream kernel does not take the problem.
-template <int TYPE, int THREADS>
-static int launch_norm_stream(const NormParams& p, cudaStream_t stream) {
-    const int s = type_bytes(TYPE), flags = norm_flags(p, TYPE);
-    if (p.C % 8 || !rows16(p.y, p.ldy, s) || !rows16(p.x, p.ldx, s)) return TAB_E_TOO_LARGE;
-    auto kernel = p.layer ? residual_norm_stream_kernel<TYPE, THREADS, true> : residual_norm_stream_kernel<TYPE, THREADS, false>;
-    const StreamPlan pl = p.layer ? stream_plan<residual_norm_stream_kernel<TYPE, THREADS, true>>(THREADS < 512 ? 2 * THREADS : 1024, p.M, 2 * (size_t)p.C * s, 0)
-                                  : stream_plan<residual_norm_stream_kernel<TYPE, THREADS, false>>(THREADS, p.M, 2 * (size_t)p.C * s, 0);
+template <int TYPE, int THREADS, bool LAYER, bool QUANT>
+static int launch_norm_stream_as(const NormParams& p, cudaStream_t stream) {
+    const StreamPlan pl = stream_plan<residual_norm_stream_kernel<TYPE, THREADS, LAYER, QUANT>>(!LAYER ? THREADS : THREADS < 512 ? 2 * THREADS : 1024, p.M, 2 * (size_t)p.C * type_bytes(TYPE), 0);
     if (!pl.stages) return TAB_E_TOO_LARGE;
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
-    return launch_pdl(kernel, dim3((unsigned)std::min<long long>(p.M, pl.ctas)), dim3(THREADS), pl.smem, stream, p, flags, pl.stages, status);
+    return launch_pdl(residual_norm_stream_kernel<TYPE, THREADS, LAYER, QUANT>, dim3((unsigned)std::min<long long>(p.M, pl.ctas)), dim3(THREADS), pl.smem, stream, p, pl.stages, status);
+}
+template <int TYPE, int THREADS>
+static int launch_norm_stream(const NormParams& p, cudaStream_t stream) {
+    if (!norm_streams(p, TYPE, norm_flags(p, TYPE))) return TAB_E_TOO_LARGE;
+    if (p.layer) return p.q ? launch_norm_stream_as<TYPE, THREADS, true, true>(p, stream) : launch_norm_stream_as<TYPE, THREADS, true, false>(p, stream);
+    return p.q ? launch_norm_stream_as<TYPE, THREADS, false, true>(p, stream) : launch_norm_stream_as<TYPE, THREADS, false, false>(p, stream);
 }
 static int launch_norm_sums(const NormBackwardParams& b, int parts, cudaStream_t stream) {
     const NormParams& p = b.f;
@@ -763,26 +886,32 @@ static int backward_flags(const NormBackwardParams& b, int type) {
     return norm_flags(b.f, type) | (on8(b.gr, b.ldgr, s) ? V_GR : 0) | (on8(b.gh, b.ldgh, s) ? V_GH : 0) | (on8(b.dy, b.lddy, s) ? V_DY : 0) |
            (on8(b.dx, b.lddx, s) ? V_DX : 0) | (on8(b.dgate, b.f.C, type_bytes(b.f.gtype)) ? V_DG : 0);
 }
-template <int TYPE, int THREADS>
-static int launch_norm_backward_stream(NormBackwardParams b, cudaStream_t stream) {
+template <int TYPE, int THREADS, bool LAYER, bool TOKEN>
+static int launch_norm_backward_stream_as(NormBackwardParams b, cudaStream_t stream) {
     const NormParams& p = b.f;
-    const int s = type_bytes(TYPE);
-    const bool pre = p.w2 && b.gh, want_u = p.w1 || p.gkind != TAB_GATE_NONE;
-    if (p.C % 8 || (pre && (!rows16(b.gh, b.ldgh, s) || !rows16(p.r, p.ldr, s))) || !rows16(b.gr, b.ldgr, s) || (want_u && !rows16(p.y, p.ldy, s)) || (!pre && !b.gr && !want_u)) return TAB_E_TOO_LARGE;
-    auto kernel = p.layer ? residual_norm_backward_stream_kernel<TYPE, THREADS, true> : residual_norm_backward_stream_kernel<TYPE, THREADS, false>;
-    const size_t fixed = 12 * (size_t)p.C, row = 4 * (size_t)p.C * s;
-    const StreamPlan pl = p.layer ? stream_plan<residual_norm_backward_stream_kernel<TYPE, THREADS, true>>(std::min(1024, 2 * THREADS), p.M, row, fixed)
-                                  : stream_plan<residual_norm_backward_stream_kernel<TYPE, THREADS, false>>(std::min(1024, 2 * THREADS), p.M, row, fixed);
+    const StreamPlan pl = stream_plan<residual_norm_backward_stream_kernel<TYPE, THREADS, LAYER, TOKEN>>(std::min(1024, 2 * THREADS), p.M, 4 * (size_t)p.C * type_bytes(TYPE), 12 * (size_t)p.C);
     if (!pl.stages) return TAB_E_TOO_LARGE;
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
     const bool sums = wants_sums(b);
     if (!sums) b.partial = nullptr;
     const int ctas = (int)std::min<long long>(p.M, pl.ctas);
-    const int rc = launch_pdl(kernel, dim3((unsigned)ctas), dim3(THREADS), pl.smem, stream, b, backward_flags(b, TYPE), pl.stages, status);
+    const int rc = launch_pdl(residual_norm_backward_stream_kernel<TYPE, THREADS, LAYER, TOKEN>, dim3((unsigned)ctas), dim3(THREADS), pl.smem, stream, b, pl.stages, status);
     return rc != TAB_OK || !sums ? rc : launch_norm_sums(b, ctas, stream);
 }
-
+template <int TYPE, int THREADS>
+static int launch_norm_backward_stream(const NormBackwardParams& b, cudaStream_t stream) {
+    NormParams f = b.f;
+    const int flags = backward_flags(b, TYPE);
+    const bool pre = f.w2 && b.gh, want_u = f.w1 || f.gkind != TAB_GATE_NONE, token = f.gkind == TAB_GATE_TOKEN;
+    if (!pre) f.w2 = f.b2 = f.r = nullptr;                                 // not looked at
+    if (!want_u) f.y = nullptr;
+    f.x = f.h = f.q = nullptr;
+    if (!norm_streams(f, TYPE, flags) || (pre && !(flags & V_GH)) || (b.gr && !(flags & V_GR)) || (b.dy && !(flags & V_DY)) || (b.dx && !(flags & V_DX)) ||
+        (f.gkind == TAB_GATE_FULL && b.dgate && !(flags & V_DG)) || (!pre && !b.gr && !want_u)) return TAB_E_TOO_LARGE;
+    if (f.layer) return token ? launch_norm_backward_stream_as<TYPE, THREADS, true, true>(b, stream) : launch_norm_backward_stream_as<TYPE, THREADS, true, false>(b, stream);
+    return token ? launch_norm_backward_stream_as<TYPE, THREADS, false, true>(b, stream) : launch_norm_backward_stream_as<TYPE, THREADS, false, false>(b, stream);
+}
 template <int TYPE, int GT, int NV>
 static int launch_norm_backward(NormBackwardParams b, cudaStream_t stream) {
     constexpr int G = GT < 128 ? 128 / GT : 1;
@@ -808,7 +937,8 @@ static int launch_norm_backward(NormBackwardParams b, cudaStream_t stream) {
 template <int TYPE>
 static int norm_sizes(const NormParams& p, cudaStream_t stream) {
     int rc = TAB_E_TOO_LARGE;
-    if (p.C > 1024 && p.C <= 2048) rc = launch_norm_stream<TYPE, 256>(p, stream);
+    if (p.C > 256 && p.C <= 1024) rc = launch_norm_stream<TYPE, 128>(p, stream);
+    else if (p.C > 1024 && p.C <= 2048) rc = launch_norm_stream<TYPE, 256>(p, stream);
     else if (p.C > 2048 && p.C <= 4096) rc = launch_norm_stream<TYPE, 512>(p, stream);
     else if (p.C > 4096 && p.C <= 8192) rc = launch_norm_stream<TYPE, 1024>(p, stream);
     if (rc != TAB_E_TOO_LARGE) return rc;
