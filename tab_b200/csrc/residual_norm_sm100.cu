@@ -410,7 +410,9 @@ __device__ __forceinline__ void cta_sums(float (&v)[N], float (*exchange)[N][32]
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        if (WARPS <= 8) {
+        if (WARPS < 4) {
+            v[i] = exchange[bank][i][0] + exchange[bank][i][WARPS - 1];
+        } else if (WARPS <= 8) {
             float s = 0.f;
 #pragma unroll
             for (int w = 0; w < WARPS; w += 4) {
@@ -428,16 +430,20 @@ __device__ __forceinline__ void cta_sums(float (&v)[N], float (*exchange)[N][32]
     bank ^= 1;
 }
 
-template <int TYPE, int THREADS, bool LAYER, bool QUANT>
-__global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREADS : 1) : 1024 / THREADS) residual_norm_stream_kernel(NormParams p, int stages, int* status) {
+// A thread has NV times eight columns, THREADS * 8 apart; what a row costs whatever its length (waits, meetings, addresses) is most of a
+// row's instructions at one.  FAST: both norms, a residual and no gate or one of channels, known when the kernel is compiled.
+template <int TYPE, int THREADS, int NV, bool LAYER, bool QUANT, bool FAST>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_stream_kernel(NormParams p, int stages, int* status) {
     using T = typename ElemOf<TYPE>::type;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[8];
     __shared__ __align__(16) float exchange[2][1][32];
-    const int g = threadIdx.x, c = g * 8;
-    const bool mine = c < p.C;
+    constexpr int WARPS = THREADS / 32;
+    const int g = threadIdx.x;
     const uint32_t row_bytes = (uint32_t)p.C * sizeof(T), sRing = (uint32_t)__cvta_generic_to_shared(ring), full = (uint32_t)__cvta_generic_to_shared(bars);
     const float inv_c = 1.f / (float)p.C;
+    const bool post = FAST || p.w1, has_x = FAST || p.x, pre = FAST || p.w2;
+    const int gkind = FAST ? (int)TAB_GATE_CHANNEL : p.gkind;
     int bank = 0;
     bool dead = false;
     if (g == 0) {
@@ -448,36 +454,43 @@ __global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREAD
     pdl_wait();
     auto request = [&](long long m, int s) {
         const uint32_t at = sRing + (uint32_t)s * 2 * row_bytes;
-        mbar_expect_tx(full + 8 * s, p.x ? 2 * row_bytes : row_bytes);
+        mbar_expect_tx(full + 8 * s, has_x ? 2 * row_bytes : row_bytes);
         bulk_load(at, static_cast<const T*>(p.y) + m * p.ldy, row_bytes, full + 8 * s);
-        if (p.x) bulk_load(at + row_bytes, static_cast<const T*>(p.x) + m * p.ldx, row_bytes, full + 8 * s);
+        if (has_x) bulk_load(at + row_bytes, static_cast<const T*>(p.x) + m * p.ldx, row_bytes, full + 8 * s);
     };
     const long long step = gridDim.x;
     if (g == 0)
         for (int s = 0; s < stages; s++)
             if (blockIdx.x + s * step < p.M) request(blockIdx.x + s * step, s);
-    Pairs w1, w2, gate;
+    bool mine[NV];
+    Pairs w1[NV], w2[NV], gate[NV];
 #pragma unroll
-    for (int j = 0; j < 4; j++) w1[j] = w2[j] = gate[j] = both(0.f);
-    if (mine) {
-        if (p.w1) pairs_any(p.w1, p.ptype, c, w1);
-        if (p.w2) pairs_any(p.w2, p.ptype, c, w2);
-        if (p.gkind == TAB_GATE_CHANNEL) pairs_any(p.gate, p.gtype, c, gate);
+    for (int i = 0; i < NV; i++) {
+        const int c = (i * THREADS + g) * 8;
+        mine[i] = c < p.C;
+#pragma unroll
+        for (int j = 0; j < 4; j++) { w1[i][j] = w2[i][j] = both(0.f); gate[i][j] = both(1.f); }
+        if (!mine[i]) continue;
+        if (p.w1) pairs_any(p.w1, p.ptype, c, w1[i]);
+        if (p.w2) pairs_any(p.w2, p.ptype, c, w2[i]);
+        if (p.gkind == TAB_GATE_CHANNEL) pairs_any(p.gate, p.gtype, c, gate[i]);
+        if (!LAYER && post && gkind == TAB_GATE_CHANNEL)                   // no shift between the two: one factor
+#pragma unroll
+            for (int j = 0; j < 4; j++) w1[i][j] = mul2(w1[i][j], gate[i][j]);
     }
-    const bool gate_now = p.gkind == TAB_GATE_CHANNEL && (LAYER || !p.w1);
-    if (!LAYER && p.gkind == TAB_GATE_CHANNEL && p.w1)                     // no shift between the two: one factor
-#pragma unroll
-        for (int j = 0; j < 4; j++) w1[j] = mul2(w1[j], gate[j]);
+    const bool gate_now = gkind == TAB_GATE_CHANNEL && (LAYER || !post);
     int slot = 0, turn = 0;
     for (long long m = blockIdx.x; m < p.M; m += step) {
         if (!dead && !mbar_wait(full + 8 * slot, turn & 1)) { dead = true; if (status) atomicExch(status, 42); }
         const uint32_t at = sRing + (uint32_t)slot * 2 * row_bytes;
-        Pairs v, x;
+        Pairs v[NV], x[NV];
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = x[j] = both(0.f);
-        if (mine) {
-            lds_pairs<TYPE>(at, c, v);
-            if (p.x) lds_pairs<TYPE>(at + row_bytes, c, x);
+        for (int i = 0; i < NV; i++) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[i][j] = x[i][j] = both(0.f);
+            if (!mine[i]) continue;
+            lds_pairs<TYPE>(at, (i * THREADS + g) * 8, v[i]);
+            if (has_x) lds_pairs<TYPE>(at + row_bytes, (i * THREADS + g) * 8, x[i]);
         }
         // The first barrier of a row also says that everybody has read it, and its place is filled again.
         bool open = true;
@@ -489,67 +502,94 @@ __global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREAD
             float s[1];
             mean = 0.f;
             if (LAYER) {
-                s[0] = sum_of(v);
-                cta_sums<THREADS / 32, 1>(s, exchange, bank);
+                s[0] = sum_of(v[0]);
+#pragma unroll
+                for (int i = 1; i < NV; i++) s[0] += sum_of(v[i]);
+                cta_sums<WARPS, 1>(s, exchange, bank);
                 refill();
                 mean = s[0] * inv_c;
-                if (mine)
 #pragma unroll
-                    for (int j = 0; j < 4; j++) v[j] = add2(v[j], both(-mean));
+                for (int i = 0; i < NV; i++)
+                    if (mine[i])
+#pragma unroll
+                        for (int j = 0; j < 4; j++) v[i][j] = add2(v[i][j], both(-mean));
             }
-            s[0] = dot_of(v, v);
-            cta_sums<THREADS / 32, 1>(s, exchange, bank);
+            s[0] = dot_of(v[0], v[0]);
+#pragma unroll
+            for (int i = 1; i < NV; i++) s[0] += dot_of(v[i], v[i]);
+            cta_sums<WARPS, 1>(s, exchange, bank);
             refill();
             inverse = 1.f / sqrtf(s[0] * inv_c + p.eps);
         };
         auto shift = [&](const void* b) {
-            Pairs f;
-            if (!mine) return;
-            pairs_any(b, p.ptype, c, f);
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = add2(v[j], f[j]);
+            for (int i = 0; i < NV; i++) {
+                Pairs f;
+                if (!mine[i]) continue;
+                pairs_any(b, p.ptype, (i * THREADS + g) * 8, f);
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[i][j] = add2(v[i][j], f[j]);
+            }
         };
         float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
-        if (p.w1) {
+        if (post) {
             normalise(st.x, st.y);
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = mul2(mul2(v[j], both(st.y)), w1[j]);
+            for (int i = 0; i < NV; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[i][j] = mul2(mul2(v[i][j], both(st.y)), w1[i][j]);
             if (LAYER && p.b1) shift(p.b1);
         }
         if (gate_now) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = mul2(v[j], gate[j]);
-        } else if ((p.gkind == TAB_GATE_FULL || p.gkind == TAB_GATE_TOKEN) && mine) {
-            Pairs f;
-            if (p.gkind == TAB_GATE_FULL) {
-                pairs_any(p.gate, p.gtype, m * p.ldg + c, f);
-            } else {
-                const float one = load_any(p.gate, p.gtype, m * p.ldg);
+            for (int i = 0; i < NV; i++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) f[j] = both(one);
+                for (int j = 0; j < 4; j++) v[i][j] = mul2(v[i][j], gate[i][j]);
+        } else if (gkind == TAB_GATE_FULL) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                Pairs f;
+                if (!mine[i]) continue;
+                pairs_any(p.gate, p.gtype, m * p.ldg + (i * THREADS + g) * 8, f);
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[i][j] = mul2(v[i][j], f[j]);
             }
+        } else if (gkind == TAB_GATE_TOKEN) {
+            const float one = load_any(p.gate, p.gtype, m * p.ldg);
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = mul2(v[j], f[j]);
-        }
-        if (p.x) {
+            for (int i = 0; i < NV; i++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = fma2(both(p.alpha), x[j], v[j]);
+                for (int j = 0; j < 4; j++) v[i][j] = mul2(v[i][j], both(one));
         }
-        store_pairs<TYPE>(mine ? p.r : nullptr, m * p.ldr + c, v, true);           // v: r as it is kept
-        if (p.w2) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if (has_x) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[i][j] = fma2(both(p.alpha), x[i][j], v[i][j]);
+            }
+            store_pairs<TYPE>(mine[i] ? p.r : nullptr, m * p.ldr + (i * THREADS + g) * 8, v[i], true);     // v: r as it is kept
+        }
+        if (pre) {
             normalise(st.z, st.w);
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[j] = mul2(mul2(v[j], both(st.w)), w2[j]);
+            for (int i = 0; i < NV; i++)
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[i][j] = mul2(mul2(v[i][j], both(st.w)), w2[i][j]);
             if (LAYER && p.b2) shift(p.b2);
-            if (p.h && mine) store_pairs<TYPE>(p.h, m * p.ldh + c, v, false);
-            if (QUANT) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const int c = (i * THREADS + g) * 8;
+                if (!QUANT) {
+                    if (mine[i]) store_pairs<TYPE>(p.h, m * p.ldh + c, v[i], false);
+                    continue;
+                }
                 // The larger magnitude, which fmaxf takes past NaN; a block with an infinity is looked at again.
                 float a = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; j++) a = fmaxf(a, fmaxf(fabsf(v[j].x), fabsf(v[j].y)));
+                for (int j = 0; j < 4; j++) a = fmaxf(a, fmaxf(fabsf(v[i][j].x), fabsf(v[i][j].y)));
 #pragma unroll
                 for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
-                const float f[8] = {v[0].x, v[0].y, v[1].x, v[1].y, v[2].x, v[2].y, v[3].x, v[3].y};
+                const float f[8] = {v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y, v[i][2].x, v[i][2].y, v[i][3].x, v[i][3].y};
                 const bool odd = __any_sync(0xFFFFFFFFu, isinf(a));
                 uint32_t bits = __float_as_uint(a);
                 if (odd) {
@@ -561,11 +601,12 @@ __global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREAD
                 const int e = scale_exponent(bits, p.format);
                 const float inv = exp2_int(-e);
                 uint2 o;
-                if (odd) o = p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(f, inv) : narrow8<TAB_E4M3>(f, inv);
-                else {
+                if (odd) {
+                    o = p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(f, inv) : narrow8<TAB_E4M3>(f, inv);
+                } else {
                     Pairs y;
 #pragma unroll
-                    for (int j = 0; j < 4; j++) y[j] = mul2(v[j], both(inv));
+                    for (int j = 0; j < 4; j++) y[j] = mul2(v[i][j], both(inv));
                     if (p.format == TAB_E5M2) {
                         o.x = __byte_perm(narrow2<TAB_E5M2>(y[0].x, y[0].y), narrow2<TAB_E5M2>(y[1].x, y[1].y), 0x5410);
                         o.y = __byte_perm(narrow2<TAB_E5M2>(y[2].x, y[2].y), narrow2<TAB_E5M2>(y[3].x, y[3].y), 0x5410);
@@ -574,7 +615,7 @@ __global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREAD
                         o.y = __byte_perm(narrow2<TAB_E4M3>(y[2].x, y[2].y), narrow2<TAB_E4M3>(y[3].x, y[3].y), 0x5410);
                     }
                 }
-                if (mine) {
+                if (mine[i]) {
                     *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.q) + m * p.ldq + c) = o;
                     if ((g & 15) == 0) p.s[(long long)(c / BLK) * p.lds + m] = (uint8_t)(e + 127);
                 }
@@ -588,21 +629,23 @@ __global__ void __launch_bounds__(THREADS, LAYER ? (THREADS < 512 ? 512 / THREAD
     if (dead) for (int i = 0; i < 200; i++) __nanosleep(1000);             // copies that may still be under way land before this memory is another's
 }
 
-template <int TYPE, int THREADS, bool LAYER, bool TOKEN>
-__global__ void __launch_bounds__(THREADS, THREADS < 512 ? 512 / THREADS : 1) residual_norm_backward_stream_kernel(NormBackwardParams b, int stages, int* status) {
+// What a row's sums are needed for is read from the ring again behind the meeting instead of being kept: registers are what the sums
+// over rows leave.  FAST: both norms and all gradients, and no gate or one of channels.
+template <int TYPE, int THREADS, int NV, bool LAYER, bool TOKEN, bool FAST>
+__global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_backward_stream_kernel(NormBackwardParams b, int stages, int* status) {
     using T = typename ElemOf<TYPE>::type;
     const NormParams& p = b.f;
-    constexpr int NS = NORM_SUMS<LAYER>, N1 = LAYER ? 2 : 1, N2 = N1 + (TOKEN ? 1 : 0);
+    constexpr int NS = NORM_SUMS<LAYER>, N1 = LAYER ? 2 : 1, N2 = N1 + (TOKEN ? 1 : 0), WARPS = THREADS / 32;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[8];
     __shared__ __align__(16) float exchange1[2][N1][32];
     __shared__ __align__(16) float exchange2[2][N2][32];
-    const int g = threadIdx.x, c = g * 8;
-    const bool mine = c < p.C;
+    const int g = threadIdx.x;
     const uint32_t row_bytes = (uint32_t)p.C * sizeof(T), sRing = (uint32_t)__cvta_generic_to_shared(ring), full = (uint32_t)__cvta_generic_to_shared(bars);
-    const uint32_t sPar = sRing + (uint32_t)stages * 4 * row_bytes;        // fp32: w2, w1, gate
+    const uint32_t plane = (uint32_t)p.C * 2u, sPar = sRing + (uint32_t)stages * 4 * row_bytes;   // fp32: w2, w1, gate, each a plane of the first four of eight and one of the others
     const float inv_c = 1.f / (float)p.C;
-    const bool pre = p.w2 && b.gh, post = p.w1 != nullptr, want_u = post || p.gkind != TAB_GATE_NONE;
+    const bool pre = FAST || (p.w2 && b.gh), post = FAST || p.w1, has_gr = FAST || b.gr, channel = p.gkind == TAB_GATE_CHANNEL;
+    const bool want_u = post || p.gkind != TAB_GATE_NONE;
     int bank1 = 0, bank2 = 0;
     bool dead = false;
     if (g == 0) {
@@ -613,34 +656,46 @@ __global__ void __launch_bounds__(THREADS, THREADS < 512 ? 512 / THREADS : 1) re
     pdl_wait();
     auto request = [&](long long m, int s) {
         const uint32_t at = sRing + (uint32_t)s * 4 * row_bytes;
-        mbar_expect_tx(full + 8 * s, row_bytes * ((pre ? 2u : 0u) + (b.gr ? 1u : 0u) + (want_u ? 1u : 0u)));
+        mbar_expect_tx(full + 8 * s, row_bytes * ((pre ? 2u : 0u) + (has_gr ? 1u : 0u) + (want_u ? 1u : 0u)));
         if (pre) {
             bulk_load(at, static_cast<const T*>(b.gh) + m * b.ldgh, row_bytes, full + 8 * s);
             bulk_load(at + row_bytes, static_cast<const T*>(p.r) + m * p.ldr, row_bytes, full + 8 * s);
         }
-        if (b.gr) bulk_load(at + 2 * row_bytes, static_cast<const T*>(b.gr) + m * b.ldgr, row_bytes, full + 8 * s);
+        if (has_gr) bulk_load(at + 2 * row_bytes, static_cast<const T*>(b.gr) + m * b.ldgr, row_bytes, full + 8 * s);
         if (want_u) bulk_load(at + 3 * row_bytes, static_cast<const T*>(p.y) + m * p.ldy, row_bytes, full + 8 * s);
     };
     const long long step = gridDim.x;
     if (g == 0)
         for (int s = 0; s < stages; s++)
             if (blockIdx.x + s * step < p.M) request(blockIdx.x + s * step, s);
-    if (mine) {                                                            // a thread reads back what it wrote itself
+    bool mine[NV];
+#pragma unroll
+    for (int i = 0; i < NV; i++) {                                         // a thread reads back what it wrote itself
+        const int c = (i * THREADS + g) * 8;
+        mine[i] = c < p.C;
+        if (!mine[i]) continue;
         Pairs w;
         auto keep = [&](int k) {
-            const uint32_t to = sPar + (uint32_t)(k * p.C + c) * 4u;
+            const uint32_t to = sPar + (uint32_t)k * 2 * plane + (uint32_t)c * 2u;
             sts_v4(to, __float_as_uint(w[0].x), __float_as_uint(w[0].y), __float_as_uint(w[1].x), __float_as_uint(w[1].y));
-            sts_v4(to + 16u, __float_as_uint(w[2].x), __float_as_uint(w[2].y), __float_as_uint(w[3].x), __float_as_uint(w[3].y));
+            sts_v4(to + plane, __float_as_uint(w[2].x), __float_as_uint(w[2].y), __float_as_uint(w[3].x), __float_as_uint(w[3].y));
         };
         if (pre) { pairs_any(p.w2, p.ptype, c, w); keep(0); }
         if (post) { pairs_any(p.w1, p.ptype, c, w); keep(1); }
-        if (p.gkind == TAB_GATE_CHANNEL) { pairs_any(p.gate, p.gtype, c, w); keep(2); }
+        if (channel) { pairs_any(p.gate, p.gtype, c, w); keep(2); }
     }
-    float2 sum[NS][4];
+    auto param = [&](int k, int c, Pairs& w) {
+        const int4 u = lds_v4(sPar + (uint32_t)k * 2 * plane + (uint32_t)c * 2u), v = lds_v4(sPar + (uint32_t)k * 2 * plane + plane + (uint32_t)c * 2u);
+        w[0] = make_float2(__int_as_float(u.x), __int_as_float(u.y)); w[1] = make_float2(__int_as_float(u.z), __int_as_float(u.w));
+        w[2] = make_float2(__int_as_float(v.x), __int_as_float(v.y)); w[3] = make_float2(__int_as_float(v.z), __int_as_float(v.w));
+    };
+    float2 sum[NS][NV][4];
 #pragma unroll
     for (int k = 0; k < NS; k++)
 #pragma unroll
-        for (int j = 0; j < 4; j++) sum[k][j] = both(0.f);
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) sum[k][i][j] = both(0.f);
     float4 next = make_float4(0.f, 1.f, 0.f, 1.f);
     if (p.stats && blockIdx.x < p.M) next = *reinterpret_cast<const float4*>(p.stats + 4 * (long long)blockIdx.x);
     int slot = 0, turn = 0;
@@ -649,75 +704,92 @@ __global__ void __launch_bounds__(THREADS, THREADS < 512 ? 512 / THREADS : 1) re
         if (p.stats && m + step < p.M) next = *reinterpret_cast<const float4*>(p.stats + 4 * (m + step));
         if (!dead && !mbar_wait(full + 8 * slot, turn & 1)) { dead = true; if (status) atomicExch(status, 43); }
         const uint32_t at = sRing + (uint32_t)slot * 4 * row_bytes;
-        Pairs dr;
+        // r^ and gh w2 of eight columns
+        auto upper = [&](int c, Pairs& rh, Pairs& t, Pairs& gh) {
+            Pairs w;
+            lds_pairs<TYPE>(at, c, gh);
+            lds_pairs<TYPE>(at + row_bytes, c, rh);
+            param(0, c, w);
 #pragma unroll
-        for (int j = 0; j < 4; j++) dr[j] = both(0.f);
-        if (b.gr && mine) lds_pairs<TYPE>(at + 2 * row_bytes, c, dr);
+            for (int j = 0; j < 4; j++) {
+                rh[j] = LAYER ? mul2(add2(rh[j], both(-st.z)), both(st.w)) : mul2(rh[j], both(st.w));
+                t[j] = mul2(gh[j], w[j]);
+            }
+        };
+        Pairs dr[NV];
+        float c1 = 0.f, c2 = 0.f;
         if (pre) {
-            Pairs t, rh;
             float red[N1];
 #pragma unroll
-            for (int j = 0; j < 4; j++) t[j] = rh[j] = both(0.f);
-            if (mine) {
-                Pairs w;
-                lds_pairs<TYPE>(at, c, t);
-                lds_pairs<TYPE>(at + row_bytes, c, rh);
-                lds_pairs<TAB_FP32>(sPar, c, w);
+            for (int n = 0; n < N1; n++) red[n] = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                if (!mine[i]) continue;
+                Pairs rh, t, gh;
+                upper((i * THREADS + g) * 8, rh, t, gh);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    if (LAYER) rh[j] = add2(rh[j], both(-st.z));
-                    rh[j] = mul2(rh[j], both(st.w));
-                    sum[0][j] = fma2(t[j], rh[j], sum[0][j]);
-                    if (LAYER) sum[NS - 2][j] = add2(sum[NS - 2][j], t[j]);
-                    t[j] = mul2(t[j], w[j]);
+                    sum[0][i][j] = fma2(gh[j], rh[j], sum[0][i][j]);
+                    if (LAYER) sum[NS - 2][i][j] = add2(sum[NS - 2][i][j], gh[j]);
                 }
+                red[0] += dot_of(t, rh);
+                if (LAYER) red[N1 - 1] += sum_of(t);
             }
-            red[0] = dot_of(t, rh);
-            if (LAYER) red[N1 - 1] = sum_of(t);
-            cta_sums<THREADS / 32, N1>(red, exchange1, bank1);
-            const float c1 = -red[0] * inv_c, c2 = LAYER ? -red[N1 - 1] * inv_c : 0.f;
-            if (mine)
+            cta_sums<WARPS, N1>(red, exchange1, bank1);
+            c1 = -red[0] * inv_c;
+            c2 = LAYER ? -red[N1 - 1] * inv_c : 0.f;
+        }
+        // y^ of eight columns
+        auto lower = [&](int c, Pairs& yv) {
+            lds_pairs<TYPE>(at + 3 * row_bytes, c, yv);
+            if (post)
+#pragma unroll
+                for (int j = 0; j < 4; j++) yv[j] = LAYER ? mul2(add2(yv[j], both(-st.x)), both(st.y)) : mul2(yv[j], both(st.y));
+        };
+        const float one = TOKEN ? load_any(p.gate, p.gtype, m * p.ldg) : 1.f;
+        float red[N2];
+#pragma unroll
+        for (int n = 0; n < N2; n++) red[n] = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int c = (i * THREADS + g) * 8;
+#pragma unroll
+            for (int j = 0; j < 4; j++) dr[i][j] = both(0.f);
+            if (!mine[i]) continue;
+            if (has_gr) lds_pairs<TYPE>(at + 2 * row_bytes, c, dr[i]);
+            if (pre) {
+                Pairs rh, t, gh;
+                upper(c, rh, t, gh);
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     t[j] = fma2(rh[j], both(c1), t[j]);
                     if (LAYER) t[j] = add2(t[j], both(c2));
-                    dr[j] = fma2(t[j], both(st.w), dr[j]);
+                    dr[i][j] = fma2(t[j], both(st.w), dr[i][j]);
                 }
-        }
-        if (b.dx && mine) {
-            Pairs d;
+            }
+            if (FAST || b.dx) {
+                Pairs d;
 #pragma unroll
-            for (int j = 0; j < 4; j++) d[j] = mul2(dr[j], both(p.alpha));
-            store_pairs<TYPE>(b.dx, m * b.lddx + c, d, false);
-        }
-        Pairs yv;
-        float red[N2];
+                for (int j = 0; j < 4; j++) d[j] = mul2(dr[i][j], both(p.alpha));
+                store_pairs<TYPE>(b.dx, m * b.lddx + c, d, false);
+            }
+            if (!want_u) continue;
+            Pairs yv, w, gv;
+            lower(c, yv);
+            if (post) param(1, c, w);
+            else
 #pragma unroll
-        for (int i = 0; i < N2; i++) red[i] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 4; j++) yv[j] = both(0.f);
-        if (want_u && mine) {
-            Pairs w, gv, u;
-            lds_pairs<TYPE>(at + 3 * row_bytes, c, yv);
-#pragma unroll
-            for (int j = 0; j < 4; j++) w[j] = gv[j] = both(1.f);
-            if (post) lds_pairs<TAB_FP32>(sPar + (uint32_t)p.C * 4u, c, w);
-            if (p.gkind == TAB_GATE_CHANNEL) {
-                lds_pairs<TAB_FP32>(sPar + (uint32_t)p.C * 8u, c, gv);
-            } else if (p.gkind == TAB_GATE_FULL) {
+                for (int j = 0; j < 4; j++) w[j] = both(1.f);
+            if (channel) {
+                param(2, c, gv);
+            } else if (!FAST && p.gkind == TAB_GATE_FULL) {
                 pairs_any(p.gate, p.gtype, m * p.ldg + c, gv);
-            } else if (TOKEN) {
-                const float one = load_any(p.gate, p.gtype, m * p.ldg);
+            } else {
 #pragma unroll
                 for (int j = 0; j < 4; j++) gv[j] = both(one);
             }
-            if (post)
-#pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    if (LAYER) yv[j] = add2(yv[j], both(-st.x));
-                    yv[j] = mul2(yv[j], both(st.y));
-                }
-            if (p.gkind != TAB_GATE_NONE) {
+            if (channel || (!FAST && p.gkind != TAB_GATE_NONE)) {
+                Pairs u;
 #pragma unroll
                 for (int j = 0; j < 4; j++) u[j] = mul2(yv[j], w[j]);
                 if (LAYER && p.b1) {
@@ -726,77 +798,97 @@ __global__ void __launch_bounds__(THREADS, THREADS < 512 ? 512 / THREADS : 1) re
 #pragma unroll
                     for (int j = 0; j < 4; j++) u[j] = add2(u[j], s[j]);
                 }
-                if (p.gkind == TAB_GATE_CHANNEL) {
+                if (channel) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) sum[2][j] = fma2(u[j], dr[j], sum[2][j]);
+                    for (int j = 0; j < 4; j++) sum[2][i][j] = fma2(u[j], dr[i][j], sum[2][i][j]);
                 } else if (TOKEN) {
-                    red[N2 - 1] = dot_of(u, dr);
+                    red[N2 - 1] += dot_of(u, dr[i]);
                 } else if (b.dgate) {
                     float d[8];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) { d[2 * j] = u[j].x * dr[j].x; d[2 * j + 1] = u[j].y * dr[j].y; }
+                    for (int j = 0; j < 4; j++) { d[2 * j] = u[j].x * dr[i][j].x; d[2 * j + 1] = u[j].y * dr[i][j].y; }
                     store8_any(b.dgate, p.gtype, m * p.C + c, 8, true, d);
                 }
             }
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float2 du = mul2(dr[j], gv[j]);
+                const float2 du = mul2(dr[i][j], gv[j]);
                 if (post) {
-                    sum[1][j] = fma2(du, yv[j], sum[1][j]);
-                    if (LAYER) sum[NS - 1][j] = add2(sum[NS - 1][j], du);
+                    sum[1][i][j] = fma2(du, yv[j], sum[1][i][j]);
+                    if (LAYER) sum[NS - 1][i][j] = add2(sum[NS - 1][i][j], du);
                 }
-                dr[j] = mul2(du, w[j]);
+                dr[i][j] = mul2(du, w[j]);                                 // from here on the gradient at y^
             }
             if (post) {
-                red[0] = dot_of(dr, yv);
-                if (LAYER) red[1 % N2] = sum_of(dr);
+                red[0] += dot_of(dr[i], yv);
+                if (LAYER) red[1 % N2] += sum_of(dr[i]);
             }
         }
-        // everybody has read the row behind the next barrier
-        if (post || TOKEN) cta_sums<THREADS / 32, N2>(red, exchange2, bank2);
-        else __syncthreads();
-        if (g == 0 && m + stages * step < p.M) request(m + stages * step, slot);
+        if (post || TOKEN) cta_sums<WARPS, N2>(red, exchange2, bank2);
         if (TOKEN && b.dgate && g == 0) store_any(b.dgate, p.gtype, m, red[N2 - 1]);
-        if (b.dy && mine) {
-            if (post) {
-                const float c1 = -red[0] * inv_c, c2 = LAYER ? -red[1 % N2] * inv_c : 0.f;
+        if (FAST || b.dy) {
+            c1 = -red[0] * inv_c;
+            c2 = LAYER ? -red[1 % N2] * inv_c : 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    dr[j] = fma2(yv[j], both(c1), dr[j]);
-                    if (LAYER) dr[j] = add2(dr[j], both(c2));
-                    dr[j] = mul2(dr[j], both(st.y));
+            for (int i = 0; i < NV; i++) {
+                const int c = (i * THREADS + g) * 8;
+                if (!mine[i]) continue;
+                if (post) {
+                    Pairs yv;
+                    lower(c, yv);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        dr[i][j] = fma2(yv[j], both(c1), dr[i][j]);
+                        if (LAYER) dr[i][j] = add2(dr[i][j], both(c2));
+                        dr[i][j] = mul2(dr[i][j], both(st.y));
+                    }
                 }
+                store_pairs<TYPE>(b.dy, m * b.lddy + c, dr[i], false);
             }
-            store_pairs<TYPE>(b.dy, m * b.lddy + c, dr, false);
         }
+        __syncthreads();                                                   // everybody has read the row
+        if (g == 0 && m + stages * step < p.M) request(m + stages * step, slot);
         if (++slot == stages) { slot = 0; turn++; }
     }
     pdl_launch_dependents();
-    if (b.partial && mine)
+    if (b.partial)
 #pragma unroll
-        for (int k = 0; k < NS; k++) {
-            const float f[8] = {sum[k][0].x, sum[k][0].y, sum[k][1].x, sum[k][1].y, sum[k][2].x, sum[k][2].y, sum[k][3].x, sum[k][3].y};
-            store8(b.partial + ((long long)blockIdx.x * NS + k) * p.C + c, 8, true, f);
-        }
+        for (int i = 0; i < NV; i++)
+            if (mine[i])
+#pragma unroll
+                for (int k = 0; k < NS; k++) {
+                    const float2(&s)[4] = sum[k][i];
+                    const float f[8] = {s[0].x, s[0].y, s[1].x, s[1].y, s[2].x, s[2].y, s[3].x, s[3].y};
+                    store8(b.partial + ((long long)blockIdx.x * NS + k) * p.C + (i * THREADS + g) * 8, 8, true, f);
+                }
     if (dead) for (int i = 0; i < 200; i++) __nanosleep(1000);
 }
 
-// The CTAs' sums of a column, in their order: eight threads take every eighth of them, then one adds the eight.
-__global__ void __launch_bounds__(256) norm_sums_kernel(const float* partial, int parts, int NS, int C, int type, void* o0, void* o1, void* o2, int gtype, void* o3, void* o4) {
-    __shared__ float acc[8][33];
+// The CTAs' sums of a column, in a fixed order: 32 threads take every 32nd of them, four at a time, and one adds theirs.
+__global__ void __launch_bounds__(1024) norm_sums_kernel(const float* partial, int parts, int NS, int C, int type, void* o0, void* o1, void* o2, int gtype, void* o3, void* o4) {
+    __shared__ float acc[32][33];
     pdl_wait();
+    pdl_launch_dependents();
     const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, k = blockIdx.y;
     void* out = k == 0 ? o0 : k == 1 ? o1 : k == 2 ? o2 : k == 3 ? o3 : o4;
-    float s = 0.f;
-    if (out && c < C)
-        for (int i = slice; i < parts; i += 8) s += partial[((long long)i * NS + k) * C + c];
-    acc[slice][lane] = s;
-    __syncthreads();
-    if (slice == 0 && out && c < C) {
-        for (int i = 1; i < 8; i++) s += acc[i][lane];
-        store_any(out, k == 2 ? gtype : type, c, s);
+    if (!out) return;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < C) {
+        const float* from = partial + (long long)k * C + c;
+        const long long pitch = (long long)NS * C;
+        int i = slice;
+        for (; i + 96 < parts; i += 128)
+#pragma unroll
+            for (int j = 0; j < 4; j++) s[j] += from[(i + 32 * j) * pitch];
+        for (; i < parts; i += 32) s[0] += from[i * pitch];
     }
-    pdl_launch_dependents();
+    acc[slice][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (slice) return;
+    float v = 0.f;
+#pragma unroll
+    for (int i = 0; i < 32; i++) v += acc[i][lane];
+    if (c < C) store_any(out, k == 2 ? gtype : type, c, v);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
@@ -828,15 +920,14 @@ static int launch_norm(const NormParams& p, cudaStream_t stream) {
 }
 // What a stream kernel is launched with: CTAs that are all resident, and rows in flight.
 struct StreamPlan { int ctas, stages; size_t smem; };
-// row_bytes: of one row's tensors; fixed: bytes besides the ring.  0 stages: it does not fit, or does not pay.
+// row_bytes: of one row's tensors; fixed: bytes besides the ring.  0 stages: it does not fit, or there are too few rows to stay for.
 template <auto KERNEL>
 static StreamPlan stream_plan(int threads, long long M, size_t row_bytes, size_t fixed) {
     StreamPlan pl = {0, 0, 0};
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return pl;
-    const int each = std::max(1, 1024 / threads);                      // CTAs an SM could hold by its threads
-    const size_t room = 226 * 1024;
-    for (int n = each; n >= 1 && !pl.stages; n = n > 1 ? n / 2 : 0) {
+    const size_t room = 225 * 1024;
+    for (int n = 512 / threads; n >= 1 && !pl.stages; n /= 2) {            // CTAs an SM holds by its registers
         const size_t share = room / n - 2048;
         const long long stages = share > fixed ? (long long)((share - fixed) / row_bytes) : 0;
         if (stages >= 2 && M >= 2LL * n * sms) { pl.stages = (int)std::min<long long>(stages, 4); pl.ctas = std::min(n * sms, NORM_CTAS); }
@@ -860,24 +951,28 @@ static bool norm_streams(const NormParams& p, int type, int flags) {
            (!p.b1 || (flags & V_B1)) && (!p.w2 || (flags & V_W2)) && (!p.b2 || (flags & V_B2)) && (p.gkind < TAB_GATE_CHANNEL || (flags & V_G));
 }
 // TAB_E_TOO_LARGE: the stream kernel does not take the problem.
-template <int TYPE, int THREADS, bool LAYER, bool QUANT>
+template <int TYPE, int THREADS, int NV, bool LAYER, bool QUANT, bool FAST>
 static int launch_norm_stream_as(const NormParams& p, cudaStream_t stream) {
-    const StreamPlan pl = stream_plan<residual_norm_stream_kernel<TYPE, THREADS, LAYER, QUANT>>(!LAYER ? THREADS : THREADS < 512 ? 2 * THREADS : 1024, p.M, 2 * (size_t)p.C * type_bytes(TYPE), 0);
+    constexpr auto kernel = residual_norm_stream_kernel<TYPE, THREADS, NV, LAYER, QUANT, FAST>;
+    const StreamPlan pl = stream_plan<kernel>(THREADS, p.M, 2 * (size_t)p.C * type_bytes(TYPE), 0);
     if (!pl.stages) return TAB_E_TOO_LARGE;
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
-    return launch_pdl(residual_norm_stream_kernel<TYPE, THREADS, LAYER, QUANT>, dim3((unsigned)std::min<long long>(p.M, pl.ctas)), dim3(THREADS), pl.smem, stream, p, pl.stages, status);
+    return launch_pdl(kernel, dim3((unsigned)std::min<long long>(p.M, pl.ctas)), dim3(THREADS), pl.smem, stream, p, pl.stages, status);
 }
-template <int TYPE, int THREADS>
+template <int TYPE, int THREADS, int NV>
 static int launch_norm_stream(const NormParams& p, cudaStream_t stream) {
-    if (!norm_streams(p, TYPE, norm_flags(p, TYPE))) return TAB_E_TOO_LARGE;
-    if (p.layer) return p.q ? launch_norm_stream_as<TYPE, THREADS, true, true>(p, stream) : launch_norm_stream_as<TYPE, THREADS, true, false>(p, stream);
-    return p.q ? launch_norm_stream_as<TYPE, THREADS, false, true>(p, stream) : launch_norm_stream_as<TYPE, THREADS, false, false>(p, stream);
+    if (!norm_streams(p, TYPE, norm_flags(p, TYPE)) || (!p.h && !p.q && p.w2)) return TAB_E_TOO_LARGE;
+    const bool fast = p.w1 && p.x && p.w2 && p.r && (p.gkind == TAB_GATE_NONE || p.gkind == TAB_GATE_CHANNEL);
+    if (p.h && p.q) return TAB_E_TOO_LARGE;
+#define TAB_NS(L, Q) (fast ? launch_norm_stream_as<TYPE, THREADS, NV, L, Q, true>(p, stream) : launch_norm_stream_as<TYPE, THREADS, NV, L, Q, false>(p, stream))
+    return p.layer ? (p.q ? TAB_NS(true, true) : TAB_NS(true, false)) : (p.q ? TAB_NS(false, true) : TAB_NS(false, false));
+#undef TAB_NS
 }
 static int launch_norm_sums(const NormBackwardParams& b, int parts, cudaStream_t stream) {
     const NormParams& p = b.f;
     const int NS = p.layer ? NORM_SUMS<true> : NORM_SUMS<false>;
-    return launch_pdl(norm_sums_kernel, dim3((unsigned)((p.C + 31) / 32), (unsigned)NS), dim3(256), 0, stream, (const float*)b.partial, parts, NS, p.C, p.ptype, b.dw2, b.dw1,
+    return launch_pdl(norm_sums_kernel, dim3((unsigned)((p.C + 31) / 32), (unsigned)NS), dim3(1024), 0, stream, (const float*)b.partial, parts, NS, p.C, p.ptype, b.dw2, b.dw1,
                       p.gkind == TAB_GATE_CHANNEL ? b.dgate : nullptr, p.gtype, p.layer ? b.db2 : nullptr, p.layer ? b.db1 : nullptr);
 }
 static bool wants_sums(const NormBackwardParams& b) { return b.dw1 || b.db1 || b.dw2 || b.db2 || (b.f.gkind == TAB_GATE_CHANNEL && b.dgate); }
@@ -886,20 +981,21 @@ static int backward_flags(const NormBackwardParams& b, int type) {
     return norm_flags(b.f, type) | (on8(b.gr, b.ldgr, s) ? V_GR : 0) | (on8(b.gh, b.ldgh, s) ? V_GH : 0) | (on8(b.dy, b.lddy, s) ? V_DY : 0) |
            (on8(b.dx, b.lddx, s) ? V_DX : 0) | (on8(b.dgate, b.f.C, type_bytes(b.f.gtype)) ? V_DG : 0);
 }
-template <int TYPE, int THREADS, bool LAYER, bool TOKEN>
+template <int TYPE, int THREADS, int NV, bool LAYER, bool TOKEN, bool FAST>
 static int launch_norm_backward_stream_as(NormBackwardParams b, cudaStream_t stream) {
     const NormParams& p = b.f;
-    const StreamPlan pl = stream_plan<residual_norm_backward_stream_kernel<TYPE, THREADS, LAYER, TOKEN>>(std::min(1024, 2 * THREADS), p.M, 4 * (size_t)p.C * type_bytes(TYPE), 12 * (size_t)p.C);
+    constexpr auto kernel = residual_norm_backward_stream_kernel<TYPE, THREADS, NV, LAYER, TOKEN, FAST>;
+    const StreamPlan pl = stream_plan<kernel>(THREADS, p.M, 4 * (size_t)p.C * type_bytes(TYPE), 12 * (size_t)p.C);
     if (!pl.stages) return TAB_E_TOO_LARGE;
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
     const bool sums = wants_sums(b);
     if (!sums) b.partial = nullptr;
     const int ctas = (int)std::min<long long>(p.M, pl.ctas);
-    const int rc = launch_pdl(residual_norm_backward_stream_kernel<TYPE, THREADS, LAYER, TOKEN>, dim3((unsigned)ctas), dim3(THREADS), pl.smem, stream, b, pl.stages, status);
+    const int rc = launch_pdl(kernel, dim3((unsigned)ctas), dim3(THREADS), pl.smem, stream, b, pl.stages, status);
     return rc != TAB_OK || !sums ? rc : launch_norm_sums(b, ctas, stream);
 }
-template <int TYPE, int THREADS>
+template <int TYPE, int THREADS, int NV>
 static int launch_norm_backward_stream(const NormBackwardParams& b, cudaStream_t stream) {
     NormParams f = b.f;
     const int flags = backward_flags(b, TYPE);
@@ -909,8 +1005,11 @@ static int launch_norm_backward_stream(const NormBackwardParams& b, cudaStream_t
     f.x = f.h = f.q = nullptr;
     if (!norm_streams(f, TYPE, flags) || (pre && !(flags & V_GH)) || (b.gr && !(flags & V_GR)) || (b.dy && !(flags & V_DY)) || (b.dx && !(flags & V_DX)) ||
         (f.gkind == TAB_GATE_FULL && b.dgate && !(flags & V_DG)) || (!pre && !b.gr && !want_u)) return TAB_E_TOO_LARGE;
-    if (f.layer) return token ? launch_norm_backward_stream_as<TYPE, THREADS, true, true>(b, stream) : launch_norm_backward_stream_as<TYPE, THREADS, true, false>(b, stream);
-    return token ? launch_norm_backward_stream_as<TYPE, THREADS, false, true>(b, stream) : launch_norm_backward_stream_as<TYPE, THREADS, false, false>(b, stream);
+    const bool fast = pre && f.w1 && b.gr && b.dx && b.dy && (f.gkind == TAB_GATE_NONE || f.gkind == TAB_GATE_CHANNEL);
+#define TAB_NB(L) (token ? launch_norm_backward_stream_as<TYPE, THREADS, NV, L, true, false>(b, stream) : fast ? launch_norm_backward_stream_as<TYPE, THREADS, NV, L, false, true>(b, stream) \
+                                                                                             : launch_norm_backward_stream_as<TYPE, THREADS, NV, L, false, false>(b, stream))
+    return f.layer ? TAB_NB(true) : TAB_NB(false);
+#undef TAB_NB
 }
 template <int TYPE, int GT, int NV>
 static int launch_norm_backward(NormBackwardParams b, cudaStream_t stream) {
@@ -937,10 +1036,11 @@ static int launch_norm_backward(NormBackwardParams b, cudaStream_t stream) {
 template <int TYPE>
 static int norm_sizes(const NormParams& p, cudaStream_t stream) {
     int rc = TAB_E_TOO_LARGE;
-    if (p.C > 256 && p.C <= 1024) rc = launch_norm_stream<TYPE, 128>(p, stream);
-    else if (p.C > 1024 && p.C <= 2048) rc = launch_norm_stream<TYPE, 256>(p, stream);
-    else if (p.C > 2048 && p.C <= 4096) rc = launch_norm_stream<TYPE, 512>(p, stream);
-    else if (p.C > 4096 && p.C <= 8192) rc = launch_norm_stream<TYPE, 1024>(p, stream);
+    if (p.C > 256 && p.C <= 512) rc = launch_norm_stream<TYPE, 64, 1>(p, stream);
+    else if (p.C > 512 && p.C <= 1024) rc = launch_norm_stream<TYPE, 64, 2>(p, stream);
+    else if (p.C > 1024 && p.C <= 2048) rc = launch_norm_stream<TYPE, 128, 2>(p, stream);
+    else if (p.C > 2048 && p.C <= 4096) rc = launch_norm_stream<TYPE, 256, 2>(p, stream);
+    else if (p.C > 4096 && p.C <= 8192) rc = launch_norm_stream<TYPE, 512, 2>(p, stream);
     if (rc != TAB_E_TOO_LARGE) return rc;
 #define TAB_NORM_F(GT, NV) launch_norm<TYPE, GT, NV>
     TAB_NORM_SIZES(TAB_NORM_F, p.C, p);
@@ -949,10 +1049,11 @@ static int norm_sizes(const NormParams& p, cudaStream_t stream) {
 template <int TYPE>
 static int norm_backward_sizes(const NormBackwardParams& b, cudaStream_t stream) {
     int rc = TAB_E_TOO_LARGE;
-    if (b.f.C > 256 && b.f.C <= 1024) rc = launch_norm_backward_stream<TYPE, 128>(b, stream);
-    else if (b.f.C > 1024 && b.f.C <= 2048) rc = launch_norm_backward_stream<TYPE, 256>(b, stream);
-    else if (b.f.C > 2048 && b.f.C <= 4096) rc = launch_norm_backward_stream<TYPE, 512>(b, stream);
-    else if (b.f.C > 4096 && b.f.C <= 8192) rc = launch_norm_backward_stream<TYPE, 1024>(b, stream);
+    if (b.f.C > 256 && b.f.C <= 512) rc = launch_norm_backward_stream<TYPE, 64, 1>(b, stream);
+    else if (b.f.C > 512 && b.f.C <= 1024) rc = launch_norm_backward_stream<TYPE, 64, 2>(b, stream);
+    else if (b.f.C > 1024 && b.f.C <= 2048) rc = launch_norm_backward_stream<TYPE, 128, 2>(b, stream);
+    else if (b.f.C > 2048 && b.f.C <= 4096) rc = launch_norm_backward_stream<TYPE, 256, 2>(b, stream);
+    else if (b.f.C > 4096 && b.f.C <= 8192) rc = launch_norm_backward_stream<TYPE, 512, 2>(b, stream);
     if (rc != TAB_E_TOO_LARGE) return rc;
 #define TAB_NORM_B(GT, NV) launch_norm_backward<TYPE, GT, NV>
     TAB_NORM_SIZES(TAB_NORM_B, b.f.C, b);
