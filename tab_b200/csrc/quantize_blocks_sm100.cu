@@ -86,15 +86,6 @@ struct Eight {
     }
 };
 
-// e + 127 of the block's scale 2^e from the bits of its largest magnitude m * 2^k: k - 8 (e5m2: k - 15), one more where m > 1.75, which
-// the addition carries into the exponent; at least 0; 127 for a block of zeros.
-template <int FORMAT>
-__device__ __forceinline__ uint32_t scale_byte(uint32_t bits) {
-    const int b = (int)((bits + 0x1FFFFFu) >> 23) - (FORMAT == TAB_E5M2 ? 15 : 8);
-    return bits == 0 ? 127u : (uint32_t)max(b, 0);
-}
-// 2^-e as the bits of a float: e + 127 is at most 247, so this is a normal number.
-__device__ __forceinline__ uint32_t inverse_bits(uint32_t scale) { return (254u - scale) << 23; }
 // Eight scaled values as bytes; `odd`: infinities may be among them.
 template <int FORMAT>
 __device__ __forceinline__ uint2 bytes8(const float (&v)[8], bool odd) {

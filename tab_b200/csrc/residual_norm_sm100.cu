@@ -11,6 +11,7 @@
 // while a CTA walks through its rows; the CTAs' sums are added in a fixed order by a second launch: no atomics, the same bits every time.
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 #include "blocks_common.cuh"
 #include "umma_common.cuh"
 
@@ -38,6 +39,31 @@ __device__ __forceinline__ void store_any(void* p, int type, long long at, float
 // Which tensors' rows start on the boundary of eight elements (host side fills it in).
 enum { V_Y = 1, V_X = 2, V_R = 4, V_H = 8, V_Q = 16, V_W1 = 32, V_B1 = 64, V_W2 = 128, V_B2 = 256, V_G = 512, V_GR = 1024, V_GH = 2048, V_DY = 4096, V_DX = 8192, V_DG = 16384 };
 
+// The columns of a thread, NV times eight of them.  VEC: eight neighbours, which move as one vector (all rows start on eight elements and
+// have a multiple of them); else every 32nd of a warp's 256, so that a warp's single elements lie side by side.
+template <int GT, int NV, bool VEC>
+struct Columns {
+    int g, C;
+    __device__ __forceinline__ int at(int i, int j) const { return VEC ? (i * GT + g) * 8 + j : (i * GT + (g & ~31)) * 8 + j * 32 + (g & 31); }
+    __device__ __forceinline__ bool in(int i, int j) const { return at(i, VEC ? 0 : j) < C; }
+    __device__ __forceinline__ void load(const void* p, int type, long long row, int i, float (&v)[8]) const {
+        if (VEC) {
+            load8_any(p, type, row + at(i, 0), in(i, 0) ? 8 : 0, true, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = in(i, j) ? load_any(p, type, row + at(i, j)) : 0.f;
+        }
+    }
+    __device__ __forceinline__ void store(void* p, int type, long long row, int i, const float (&v)[8]) const {
+        if (VEC) {
+            store8_any(p, type, row + at(i, 0), in(i, 0) ? 8 : 0, true, v);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) if (in(i, j)) store_any(p, type, row + at(i, j), v[j]);
+        }
+    }
+};
+
 // Sums of N values over the GT threads of a row, the same in all of them.  `bank` alternates between two exchange buffers, so that one
 // barrier a sum is enough: a buffer is written again only behind the barrier of the sum in between.
 template <int GT, int N>
@@ -63,8 +89,8 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*exchange)[32][N]
 }
 
 // Mean (0 where not centred) and 1 / deviation of the row in v.
-template <int GT, int NV, bool LAYER>
-__device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], int C, int g, float eps, float (*exchange)[32][1], int& bank) {
+template <int GT, int NV, bool VEC, bool LAYER>
+__device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], const Columns<GT, NV, VEC>& col, float eps, float (*exchange)[32][1], int& bank) {
     float s[1] = {0.f}, mean = 0.f;
     if (LAYER) {
 #pragma unroll
@@ -72,104 +98,121 @@ __device__ __forceinline__ float2 row_stats(const float (&v)[NV][8], int C, int 
 #pragma unroll
             for (int j = 0; j < 8; j++) s[0] += v[i][j];                   // elements behind the row's end are 0
         row_sums<GT, 1>(s, exchange, bank);
-        mean = s[0] / (float)C;
+        mean = s[0] / (float)col.C;
         s[0] = 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-        const int n = C - (i * GT + g) * 8;
+    for (int i = 0; i < NV; i++)
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            const float d = LAYER ? (j < n ? v[i][j] - mean : 0.f) : v[i][j];
+            const float d = LAYER ? (col.in(i, j) ? v[i][j] - mean : 0.f) : v[i][j];
             s[0] += d * d;
         }
-    }
     row_sums<GT, 1>(s, exchange, bank);
-    return make_float2(mean, 1.f / sqrtf(s[0] / (float)C + eps));
+    return make_float2(mean, 1.f / sqrtf(s[0] / (float)col.C + eps));
 }
 
-template <int TYPE, int GT, int NV, bool LAYER>
-__global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_kernel(NormParams p, int flags) {
+// A row by GT threads, at once.
+template <int TYPE, int GT, int NV, bool VEC, bool LAYER>
+__global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_kernel(NormParams p) {
     using T = typename ElemOf<TYPE>::type;
     __shared__ float exchange[2][32][1];
     constexpr int G = GT < 128 ? 128 / GT : 1;
-    const int g = threadIdx.x % GT;
+    const Columns<GT, NV, VEC> col = {(int)threadIdx.x % GT, p.C};
+    const int g = col.g;
     const long long m = (long long)blockIdx.x * G + threadIdx.x / GT;
     int bank = 0;
     pdl_wait();
     if (G > 1 && m >= p.M) return;                                         // a row is one warp's here: no barrier below
-    const T *y = static_cast<const T*>(p.y) + m * p.ldy, *x = static_cast<const T*>(p.x) + m * p.ldx;
     float v[NV][8], xv[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const int c = (i * GT + g) * 8;
-        load8(y + c, p.C - c, flags & V_Y, v[i]);
-        if (p.x) load8(x + c, p.C - c, flags & V_X, xv[i]);
+        col.load(p.y, TYPE, m * p.ldy, i, v[i]);
+        if (p.x) col.load(p.x, TYPE, m * p.ldx, i, xv[i]);
     }
     pdl_launch_dependents();
     float4 st = make_float4(0.f, 1.f, 0.f, 1.f);
     if (p.w1) {
-        const float2 s = row_stats<GT, NV, LAYER>(v, p.C, g, p.eps, exchange, bank);
+        const float2 s = row_stats<GT, NV, VEC, LAYER>(v, col, p.eps, exchange, bank);
         st.x = s.x; st.y = s.y;
     }
     const float gtoken = p.gkind == TAB_GATE_TOKEN ? load_any(p.gate, p.gtype, m * p.ldg) : 1.f;
 #pragma unroll
     for (int i = 0; i < NV; i++) {
-        const int c = (i * GT + g) * 8, n = p.C - c;
         float t[8];
         if (p.w1) {
-            load8_any(p.w1, p.ptype, c, n, flags & V_W1, t);
+            col.load(p.w1, p.ptype, 0, i, t);
 #pragma unroll
             for (int j = 0; j < 8; j++) v[i][j] = (v[i][j] - st.x) * st.y * t[j];
             if (p.b1) {
-                load8_any(p.b1, p.ptype, c, n, flags & V_B1, t);
+                col.load(p.b1, p.ptype, 0, i, t);
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[i][j] += t[j];
             }
         }
-        if (p.gkind != TAB_GATE_NONE) {
-            if (p.gkind == TAB_GATE_TOKEN) {
+        if (p.gkind == TAB_GATE_CHANNEL || p.gkind == TAB_GATE_FULL) {
+            col.load(p.gate, p.gtype, p.gkind == TAB_GATE_FULL ? m * p.ldg : 0, i, t);
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[i][j] *= gtoken;
-            } else {
-                load8_any(p.gate, p.gtype, (p.gkind == TAB_GATE_FULL ? m * p.ldg : 0) + c, n, flags & V_G, t);
+            for (int j = 0; j < 8; j++) v[i][j] *= t[j];
+        } else if (p.gkind == TAB_GATE_TOKEN) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) v[i][j] *= t[j];
-            }
+            for (int j = 0; j < 8; j++) v[i][j] *= gtoken;
         }
         if (p.x) {
 #pragma unroll
             for (int j = 0; j < 8; j++) v[i][j] = fmaf(p.alpha, xv[i][j], v[i][j]);
         }
-        if (p.r) store8(static_cast<T*>(p.r) + m * p.ldr + c, n, flags & V_R, v[i]);
+        if (p.r) col.store(p.r, TYPE, m * p.ldr, i, v[i]);
         // r is what is kept: the norm below is that of the rounded values (elements behind the row's end stay 0 for its sums)
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[i][j] = j < n ? to_float(from_float<T>(v[i][j])) : 0.f;
+        for (int j = 0; j < 8; j++) v[i][j] = col.in(i, j) ? to_float(from_float<T>(v[i][j])) : 0.f;
     }
     if (p.w2) {
-        const float2 s = row_stats<GT, NV, LAYER>(v, p.C, g, p.eps, exchange, bank);
+        const float2 s = row_stats<GT, NV, VEC, LAYER>(v, col, p.eps, exchange, bank);
         st.z = s.x; st.w = s.y;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int c = (i * GT + g) * 8, n = p.C - c;
             float t[8];
-            load8_any(p.w2, p.ptype, c, n, flags & V_W2, t);
+            col.load(p.w2, p.ptype, 0, i, t);
 #pragma unroll
             for (int j = 0; j < 8; j++) v[i][j] = (v[i][j] - st.z) * st.w * t[j];
             if (p.b2) {
-                load8_any(p.b2, p.ptype, c, n, flags & V_B2, t);
+                col.load(p.b2, p.ptype, 0, i, t);
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[i][j] += t[j];
             }
-            if (p.h) store8(static_cast<T*>(p.h) + m * p.ldh + c, n, flags & V_H, v[i]);
-            if (p.q) {                                                     // sixteen threads hold a block
-                uint32_t a = 0;
+            if (p.h) col.store(p.h, TYPE, m * p.ldh, i, v[i]);
+            if (!p.q) continue;
+            uint8_t* q = static_cast<uint8_t*>(p.q) + m * p.ldq;
+            uint32_t a[2] = {0, 0};                                        // VEC: sixteen threads hold a block; else a warp holds two, four columns a lane of each
 #pragma unroll
-                for (int j = 0; j < 8; j++) a = max(a, j < n ? finite_bits(v[i][j]) : 0u);
-                const int e = scale_exponent(half_warp_max(a), p.format);
+            for (int j = 0; j < 8; j++) {
+                const uint32_t b = col.in(i, j) ? finite_bits(v[i][j]) : 0u;
+                a[VEC ? 0 : j >> 2] = max(a[VEC ? 0 : j >> 2], b);
+            }
+            if (VEC) {
+                const int e = scale_exponent(half_warp_max(a[0]), p.format), c = col.at(i, 0);
                 const float inv = exp2_int(-e);
-                store_bytes8(static_cast<uint8_t*>(p.q) + m * p.ldq + c, n, flags & V_Q, p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(v[i], inv) : narrow8<TAB_E4M3>(v[i], inv));
-                if ((g & 15) == 0 && n > 0) p.s[(long long)(c / BLK) * p.lds + m] = (uint8_t)(e + 127);
+                if (c < p.C) {
+                    *reinterpret_cast<uint2*>(q + c) = p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(v[i], inv) : narrow8<TAB_E4M3>(v[i], inv);
+                    if ((g & 15) == 0) p.s[(long long)(c / BLK) * p.lds + m] = (uint8_t)(e + 127);
+                }
+            } else {
+                float sc[8];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const uint32_t top = half_warp_max(max(a[h], __shfl_xor_sync(0xFFFFFFFFu, a[h], 16)));
+                    const int e = scale_exponent(top, p.format), c = col.at(i, 4 * h);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sc[4 * h + j] = exp2_int(-e);
+                    if ((g & 31) == 0 && c < p.C) p.s[(long long)(c / BLK) * p.lds + m] = (uint8_t)(e + 127);
+                }
+                float y[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) y[j] = v[i][j] * sc[j];
+                const uint2 o = p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(y, 1.f) : narrow8<TAB_E4M3>(y, 1.f);
+#pragma unroll
+                for (int j = 0; j < 8; j++) if (col.in(i, j)) q[col.at(i, j)] = (uint8_t)((j < 4 ? o.x : o.y) >> (8 * (j & 3)));
             }
         }
     }
@@ -179,13 +222,14 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_kernel(Norm
 // Sums over rows that a thread keeps: of w2, w1, the channel gate, and with shifts of b2, b1.
 template <bool LAYER> constexpr int NORM_SUMS = LAYER ? 5 : 3;
 
-template <int TYPE, int GT, int NV, bool LAYER>
-__global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_kernel(NormBackwardParams b, int flags, long long rows_each) {
-    using T = typename ElemOf<TYPE>::type;
+// rows_each rows by GT threads, one after the other.
+template <int TYPE, int GT, int NV, bool VEC, bool LAYER>
+__global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_kernel(NormBackwardParams b, long long rows_each) {
     const NormParams& p = b.f;
     constexpr int G = GT < 128 ? 128 / GT : 1, NS = NORM_SUMS<LAYER>;
     __shared__ float exchange[2][32][3];
-    const int g = threadIdx.x % GT;
+    const Columns<GT, NV, VEC> col = {(int)threadIdx.x % GT, p.C};
+    const int g = col.g;
     const long long part = (long long)blockIdx.x * G + threadIdx.x / GT, m0 = part * rows_each, m1 = min(p.M, m0 + rows_each);
     int bank = 0;
     float sum[NS][NV][8];
@@ -204,22 +248,20 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
         float red[3] = {0.f, 0.f, 0.f};
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int c = (i * GT + g) * 8, n = p.C - c;
-            if (b.gr) load8(static_cast<const T*>(b.gr) + m * b.ldgr + c, n, flags & V_GR, dr[i]);
+            if (b.gr) col.load(b.gr, TYPE, m * b.ldgr, i, dr[i]);
             else
 #pragma unroll
                 for (int j = 0; j < 8; j++) dr[i][j] = 0.f;
-            if (want_u) load8(static_cast<const T*>(p.y) + m * p.ldy + c, n, flags & V_Y, yv[i]);
+            if (want_u) col.load(p.y, TYPE, m * p.ldy, i, yv[i]);
         }
         if (pre) {
             float t[NV][8], rh[NV][8];
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                const int c = (i * GT + g) * 8, n = p.C - c;
-                load8(static_cast<const T*>(b.gh) + m * b.ldgh + c, n, flags & V_GH, t[i]);
-                load8(static_cast<const T*>(p.r) + m * p.ldr + c, n, flags & V_R, rh[i]);
+                col.load(b.gh, TYPE, m * b.ldgh, i, t[i]);
+                col.load(p.r, TYPE, m * p.ldr, i, rh[i]);
                 float w[8];
-                load8_any(p.w2, p.ptype, c, n, flags & V_W2, w);
+                col.load(p.w2, p.ptype, 0, i, w);
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     rh[i][j] = (rh[i][j] - st.z) * st.w;
@@ -242,12 +284,11 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
         float t[NV][8];
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            const int c = (i * GT + g) * 8, n = p.C - c;
             if (b.dx) {
                 float d[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) d[j] = p.alpha * dr[i][j];
-                store8(static_cast<T*>(b.dx) + m * b.lddx + c, n, flags & V_DX, d);
+                col.store(b.dx, TYPE, m * b.lddx, i, d);
             }
             if (!want_u) {
 #pragma unroll
@@ -256,9 +297,9 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
             }
             float w[8], gv[8], u[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++) { w[j] = 1.f; gv[j] = gtoken; if (j >= n) dr[i][j] = 0.f; }
-            if (post) load8_any(p.w1, p.ptype, c, n, flags & V_W1, w);
-            if (p.gkind == TAB_GATE_CHANNEL || p.gkind == TAB_GATE_FULL) load8_any(p.gate, p.gtype, (p.gkind == TAB_GATE_FULL ? m * p.ldg : 0) + c, n, flags & V_G, gv);
+            for (int j = 0; j < 8; j++) { w[j] = 1.f; gv[j] = gtoken; if (!col.in(i, j)) dr[i][j] = 0.f; }
+            if (post) col.load(p.w1, p.ptype, 0, i, w);
+            if (p.gkind == TAB_GATE_CHANNEL || p.gkind == TAB_GATE_FULL) col.load(p.gate, p.gtype, p.gkind == TAB_GATE_FULL ? m * p.ldg : 0, i, gv);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 yv[i][j] = (yv[i][j] - st.x) * st.y;                       // y itself without a norm: mean 0, deviation 1
@@ -266,7 +307,7 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
             }
             if (p.gkind != TAB_GATE_NONE && p.b1) {
                 float s[8];
-                load8_any(p.b1, p.ptype, c, n, flags & V_B1, s);
+                col.load(p.b1, p.ptype, 0, i, s);
 #pragma unroll
                 for (int j = 0; j < 8; j++) u[j] += s[j];
             }
@@ -274,7 +315,7 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
                 float d[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) d[j] = dr[i][j] * u[j];
-                store8_any(b.dgate, p.gtype, m * p.C + c, n, flags & V_DG, d);
+                col.store(b.dgate, p.gtype, m * p.C, i, d);
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -299,12 +340,11 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
         if (b.dy) {
 #pragma unroll
             for (int i = 0; i < NV; i++) {
-                const int c = (i * GT + g) * 8, n = p.C - c;
                 if (post) {
 #pragma unroll
                     for (int j = 0; j < 8; j++) t[i][j] = st.y * (t[i][j] - yv[i][j] * c1 - c2);
                 }
-                store8(static_cast<T*>(b.dy) + m * b.lddy + c, n, flags & V_DY, t[i]);
+                col.store(b.dy, TYPE, m * b.lddy, i, t[i]);
             }
         }
     }
@@ -313,10 +353,7 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
 #pragma unroll
     for (int k = 0; k < NS; k++)
 #pragma unroll
-        for (int i = 0; i < NV; i++) {
-            const int c = (i * GT + g) * 8;
-            store8(b.partial + (part * NS + k) * p.C + c, p.C - c, p.C % 8 == 0, sum[k][i]);
-        }
+        for (int i = 0; i < NV; i++) col.store(b.partial, TAB_FP32, (part * NS + k) * p.C, i, sum[k][i]);
 }
 
 // ---- many rows ------------------------------------------------------------------------------------------------------------------
@@ -398,7 +435,7 @@ __device__ __forceinline__ void store_pairs(void* p, long long at, Pairs& v, boo
 }
 // Sums over the CTA, the same in all threads; `bank` alternates as in row_sums.
 template <int WARPS, int N>
-__device__ __forceinline__ void cta_sums(float (&v)[N], float (*exchange)[N][32], int& bank) {
+__device__ __forceinline__ void cta_sums(float (&v)[N], float (*exchange)[N][WARPS < 4 ? 4 : WARPS], int& bank) {
 #pragma unroll
     for (int i = 0; i < N; i++)
 #pragma unroll
@@ -410,7 +447,8 @@ __device__ __forceinline__ void cta_sums(float (&v)[N], float (*exchange)[N][32]
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        if (WARPS < 4) {
+        if (WARPS == 1) {
+        } else if (WARPS < 4) {
             v[i] = exchange[bank][i][0] + exchange[bank][i][WARPS - 1];
         } else if (WARPS <= 8) {
             float s = 0.f;
@@ -437,8 +475,8 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_stream_k
     using T = typename ElemOf<TYPE>::type;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[8];
-    __shared__ __align__(16) float exchange[2][1][32];
     constexpr int WARPS = THREADS / 32;
+    __shared__ __align__(16) float exchange[2][1][WARPS < 4 ? 4 : WARPS];
     const int g = threadIdx.x;
     const uint32_t row_bytes = (uint32_t)p.C * sizeof(T), sRing = (uint32_t)__cvta_generic_to_shared(ring), full = (uint32_t)__cvta_generic_to_shared(bars);
     const float inv_c = 1.f / (float)p.C;
@@ -576,48 +614,53 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_stream_k
 #pragma unroll
                 for (int j = 0; j < 4; j++) v[i][j] = mul2(mul2(v[i][j], both(st.w)), w2[i][j]);
             if (LAYER && p.b2) shift(p.b2);
+            if (!QUANT) {
 #pragma unroll
-            for (int i = 0; i < NV; i++) {
-                const int c = (i * THREADS + g) * 8;
-                if (!QUANT) {
-                    if (mine[i]) store_pairs<TYPE>(p.h, m * p.ldh + c, v[i], false);
-                    continue;
+                for (int i = 0; i < NV; i++)
+                    if (mine[i]) store_pairs<TYPE>(p.h, m * p.ldh + (i * THREADS + g) * 8, v[i], false);
+            } else {
+                // The larger magnitudes, which fmaxf takes past NaN; rows with an infinity are looked at again.
+                float a[NV], most = 0.f;
+#pragma unroll
+                for (int i = 0; i < NV; i++) {
+                    a[i] = fmaxf(fmaxf(fmaxf(fabsf(v[i][0].x), fabsf(v[i][0].y)), fmaxf(fabsf(v[i][1].x), fabsf(v[i][1].y))),
+                                 fmaxf(fmaxf(fabsf(v[i][2].x), fabsf(v[i][2].y)), fmaxf(fabsf(v[i][3].x), fabsf(v[i][3].y))));
+                    most = fmaxf(most, a[i]);
                 }
-                // The larger magnitude, which fmaxf takes past NaN; a block with an infinity is looked at again.
-                float a = 0.f;
+                const bool odd = __any_sync(0xFFFFFFFFu, isinf(most));
 #pragma unroll
-                for (int j = 0; j < 4; j++) a = fmaxf(a, fmaxf(fabsf(v[i][j].x), fabsf(v[i][j].y)));
+                for (int i = 0; i < NV; i++) {
+                    const int c = (i * THREADS + g) * 8;
+                    const float f[8] = {v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y, v[i][2].x, v[i][2].y, v[i][3].x, v[i][3].y};
+                    uint32_t bits = __float_as_uint(a[i]);
+                    if (odd) {
+                        bits = 0;
 #pragma unroll
-                for (int o = 8; o > 0; o >>= 1) a = fmaxf(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
-                const float f[8] = {v[i][0].x, v[i][0].y, v[i][1].x, v[i][1].y, v[i][2].x, v[i][2].y, v[i][3].x, v[i][3].y};
-                const bool odd = __any_sync(0xFFFFFFFFu, isinf(a));
-                uint32_t bits = __float_as_uint(a);
-                if (odd) {
-                    bits = 0;
-#pragma unroll
-                    for (int j = 0; j < 8; j++) bits = max(bits, finite_bits(f[j]));
-                    bits = half_warp_max(bits);
-                }
-                const int e = scale_exponent(bits, p.format);
-                const float inv = exp2_int(-e);
-                uint2 o;
-                if (odd) {
-                    o = p.format == TAB_E5M2 ? narrow8<TAB_E5M2>(f, inv) : narrow8<TAB_E4M3>(f, inv);
-                } else {
-                    Pairs y;
-#pragma unroll
-                    for (int j = 0; j < 4; j++) y[j] = mul2(v[i][j], both(inv));
-                    if (p.format == TAB_E5M2) {
-                        o.x = __byte_perm(narrow2<TAB_E5M2>(y[0].x, y[0].y), narrow2<TAB_E5M2>(y[1].x, y[1].y), 0x5410);
-                        o.y = __byte_perm(narrow2<TAB_E5M2>(y[2].x, y[2].y), narrow2<TAB_E5M2>(y[3].x, y[3].y), 0x5410);
-                    } else {
-                        o.x = __byte_perm(narrow2<TAB_E4M3>(y[0].x, y[0].y), narrow2<TAB_E4M3>(y[1].x, y[1].y), 0x5410);
-                        o.y = __byte_perm(narrow2<TAB_E4M3>(y[2].x, y[2].y), narrow2<TAB_E4M3>(y[3].x, y[3].y), 0x5410);
+                        for (int j = 0; j < 8; j++) bits = max(bits, finite_bits(f[j]));
                     }
-                }
-                if (mine[i]) {
-                    *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.q) + m * p.ldq + c) = o;
-                    if ((g & 15) == 0) p.s[(long long)(c / BLK) * p.lds + m] = (uint8_t)(e + 127);
+                    bits = half_warp_max(bits);
+                    uint2 o;
+                    uint32_t s;
+                    auto round = [&](auto format) {
+                        constexpr int F = decltype(format)::value;
+                        s = scale_byte<F>(bits);
+                        const float inv = __uint_as_float(inverse_bits(s));
+                        if (odd) {
+                            o = narrow8<F>(f, inv);
+                            return;
+                        }
+                        Pairs y;
+#pragma unroll
+                        for (int j = 0; j < 4; j++) y[j] = mul2(v[i][j], both(inv));
+                        o.x = __byte_perm(narrow2<F>(y[0].x, y[0].y), narrow2<F>(y[1].x, y[1].y), 0x5410);
+                        o.y = __byte_perm(narrow2<F>(y[2].x, y[2].y), narrow2<F>(y[3].x, y[3].y), 0x5410);
+                    };
+                    if (p.format == TAB_E5M2) round(std::integral_constant<int, TAB_E5M2>());
+                    else round(std::integral_constant<int, TAB_E4M3>());
+                    if (mine[i]) {
+                        *reinterpret_cast<uint2*>(static_cast<uint8_t*>(p.q) + m * p.ldq + c) = o;
+                        if ((g & 15) == 0) p.s[(long long)(c / BLK) * p.lds + m] = (uint8_t)s;
+                    }
                 }
             }
         }
@@ -631,15 +674,16 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_stream_k
 
 // What a row's sums are needed for is read from the ring again behind the meeting instead of being kept: registers are what the sums
 // over rows leave.  FAST: both norms and all gradients, and no gate or one of channels.
+constexpr int backward_threads(int nv, bool layer) { return nv == 1 && !layer ? 1024 : 512; }    // an SM holds, by registers
 template <int TYPE, int THREADS, int NV, bool LAYER, bool TOKEN, bool FAST>
-__global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_backward_stream_kernel(NormBackwardParams b, int stages, int* status) {
+__global__ void __launch_bounds__(THREADS, backward_threads(NV, LAYER) / THREADS) residual_norm_backward_stream_kernel(NormBackwardParams b, int stages, int* status) {
     using T = typename ElemOf<TYPE>::type;
     const NormParams& p = b.f;
     constexpr int NS = NORM_SUMS<LAYER>, N1 = LAYER ? 2 : 1, N2 = N1 + (TOKEN ? 1 : 0), WARPS = THREADS / 32;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[8];
-    __shared__ __align__(16) float exchange1[2][N1][32];
-    __shared__ __align__(16) float exchange2[2][N2][32];
+    __shared__ __align__(16) float exchange1[2][N1][WARPS < 4 ? 4 : WARPS];
+    __shared__ __align__(16) float exchange2[2][N2][WARPS < 4 ? 4 : WARPS];
     const int g = threadIdx.x;
     const uint32_t row_bytes = (uint32_t)p.C * sizeof(T), sRing = (uint32_t)__cvta_generic_to_shared(ring), full = (uint32_t)__cvta_generic_to_shared(bars);
     const uint32_t plane = (uint32_t)p.C * 2u, sPar = sRing + (uint32_t)stages * 4 * row_bytes;   // fp32: w2, w1, gate, each a plane of the first four of eight and one of the others
@@ -864,31 +908,40 @@ __global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_backward
     if (dead) for (int i = 0; i < 200; i++) __nanosleep(1000);
 }
 
-// The CTAs' sums of a column, in a fixed order: 32 threads take every 32nd of them, four at a time, and one adds theirs.
+// The CTAs' sums of a column, in a fixed order: 32 warps take every 32nd of them, four columns a lane (one where rows of sums do not start
+// on 16 bytes), and one warp adds theirs.
+template <int V>
 __global__ void __launch_bounds__(1024) norm_sums_kernel(const float* partial, int parts, int NS, int C, int type, void* o0, void* o1, void* o2, int gtype, void* o3, void* o4) {
-    __shared__ float acc[32][33];
+    __shared__ float acc[32][32 * V + 1];
     pdl_wait();
     pdl_launch_dependents();
-    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c = blockIdx.x * 32 + lane, k = blockIdx.y;
+    const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5, c0 = blockIdx.x * 32 * V, k = blockIdx.y;
     void* out = k == 0 ? o0 : k == 1 ? o1 : k == 2 ? o2 : k == 3 ? o3 : o4;
     if (!out) return;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
-    if (c < C) {
-        const float* from = partial + (long long)k * C + c;
-        const long long pitch = (long long)NS * C;
-        int i = slice;
-        for (; i + 96 < parts; i += 128)
+    float s[V];
 #pragma unroll
-            for (int j = 0; j < 4; j++) s[j] += from[(i + 32 * j) * pitch];
-        for (; i < parts; i += 32) s[0] += from[i * pitch];
+    for (int j = 0; j < V; j++) s[j] = 0.f;
+    if (c0 + lane * V < C) {                                               // (C is a multiple of V)
+        const float* from = partial + (long long)k * C + c0 + lane * V;
+        const long long pitch = (long long)NS * C;
+#pragma unroll 8
+        for (int i = slice; i < parts; i += 32) {
+            if (V == 4) {
+                const float4 f = *reinterpret_cast<const float4*>(from + i * pitch);
+                s[0] += f.x; s[1 % V] += f.y; s[2 % V] += f.z; s[3 % V] += f.w;
+            } else {
+                s[0] += from[i * pitch];
+            }
+        }
     }
-    acc[slice][lane] = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+    for (int j = 0; j < V; j++) acc[slice][lane * V + j] = s[j];
     __syncthreads();
-    if (slice) return;
+    if ((int)threadIdx.x >= 32 * V) return;
     float v = 0.f;
 #pragma unroll
-    for (int i = 0; i < 32; i++) v += acc[i][lane];
-    if (c < C) store_any(out, k == 2 ? gtype : type, c, v);
+    for (int i = 0; i < 32; i++) v += acc[i][threadIdx.x];
+    if (c0 + (int)threadIdx.x < C) store_any(out, k == 2 ? gtype : type, c0 + threadIdx.x, v);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
@@ -899,36 +952,59 @@ static int norm_flags(const NormParams& p, int type) {
            (on8(p.q, p.ldq, 1) ? V_Q : 0) | (on8(p.w1, 0, w) ? V_W1 : 0) | (on8(p.b1, 0, w) ? V_B1 : 0) | (on8(p.w2, 0, w) ? V_W2 : 0) |
            (on8(p.b2, 0, w) ? V_B2 : 0) | (on8(p.gate, p.gkind == TAB_GATE_FULL ? p.ldg : 0, g) ? V_G : 0);
 }
-static constexpr int NORM_CTAS = 8 * 148;                                  // most CTAs of a stream kernel
-// How many parts of the rows are summed on their own (one for each group of threads of the backward kernel).
-static int norm_groups(int C) { return C <= 1024 ? 4 : 1; }
+static constexpr int NORM_CTAS = 16 * 148;                                 // most CTAs of a stream kernel
+// How many parts of the rows the general kernel sums on their own (one for each group of threads): some rows for each, since the sums of
+// a part are as many bytes as the rows of one.
+static int norm_groups(int C) { return C <= 256 ? 4 : 1; }
 static long long norm_parts(long long M, int C) {
-    const int G = norm_groups(C), ctas = 148 * (C <= 2048 ? 4 : C <= 4096 ? 2 : 1);
-    const long long wanted = std::min<long long>((long long)ctas * G, M);
+    const int G = norm_groups(C);
+    const long long most = 148LL * G * (C <= 2048 ? 4 : C <= 4096 ? 2 : 1), wanted = std::min(most, std::min(M, std::max(148LL * G, M / 4)));
     return (wanted + G - 1) / G * G;
 }
 size_t residual_norm_partial_bytes(long long M, int C) { return (size_t)std::max(norm_parts(M, C), std::min<long long>(M, NORM_CTAS)) * 5 * (size_t)C * sizeof(float); }
+static bool rows16(const void* p, long long ld, int size) { return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld * size % 16 == 0); }
+// Whether all tensors that are there have rows that move eight elements at a time.
+static bool norm_vectors(const NormParams& p, int type, int flags) {
+    return p.C % 8 == 0 && (!p.y || (flags & V_Y)) && (!p.x || (flags & V_X)) && (!p.r || (flags & V_R)) && (!p.h || (flags & V_H)) && (!p.q || (flags & V_Q)) && (!p.w1 || (flags & V_W1)) &&
+           (!p.b1 || (flags & V_B1)) && (!p.w2 || (flags & V_W2)) && (!p.b2 || (flags & V_B2)) && (p.gkind < TAB_GATE_CHANNEL || (flags & V_G));
+}
+static bool wants_sums(const NormBackwardParams& b) { return b.dw1 || b.db1 || b.dw2 || b.db2 || (b.f.gkind == TAB_GATE_CHANNEL && b.dgate); }
+static int backward_flags(const NormBackwardParams& b, int type) {
+    const int s = type_bytes(type);
+    return norm_flags(b.f, type) | (on8(b.gr, b.ldgr, s) ? V_GR : 0) | (on8(b.gh, b.ldgh, s) ? V_GH : 0) | (on8(b.dy, b.lddy, s) ? V_DY : 0) |
+           (on8(b.dx, b.lddx, s) ? V_DX : 0) | (on8(b.dgate, b.f.C, type_bytes(b.f.gtype)) ? V_DG : 0);
+}
+static bool backward_vectors(const NormBackwardParams& b, int type) {
+    NormParams f = b.f;
+    const int flags = backward_flags(b, type);
+    if (!(f.w2 && b.gh)) f.w2 = f.b2 = f.r = nullptr;                      // not looked at
+    if (!f.w1 && f.gkind == TAB_GATE_NONE) f.y = nullptr;
+    f.x = f.h = f.q = nullptr;
+    return norm_vectors(f, type, flags) && (!(f.w2 && b.gh) || (flags & V_GH)) && (!b.gr || (flags & V_GR)) && (!b.dy || (flags & V_DY)) && (!b.dx || (flags & V_DX)) &&
+           (!(f.gkind == TAB_GATE_FULL && b.dgate) || (flags & V_DG));
+}
 
 template <int TYPE, int GT, int NV>
 static int launch_norm(const NormParams& p, cudaStream_t stream) {
     constexpr int G = GT < 128 ? 128 / GT : 1;
     const long long grid = (p.M + G - 1) / G;
     if (grid >= (1LL << 31)) return TAB_E_TOO_LARGE;
-    const int flags = norm_flags(p, TYPE);
-    if (p.layer) return launch_pdl(residual_norm_kernel<TYPE, GT, NV, true>, dim3((unsigned)grid), dim3(GT < 128 ? 128 : GT), 0, stream, p, flags);
-    return launch_pdl(residual_norm_kernel<TYPE, GT, NV, false>, dim3((unsigned)grid), dim3(GT < 128 ? 128 : GT), 0, stream, p, flags);
+#define TAB_NK(V, L) launch_pdl(residual_norm_kernel<TYPE, GT, NV, V, L>, dim3((unsigned)grid), dim3(GT < 128 ? 128 : GT), 0, stream, p)
+    if (norm_vectors(p, TYPE, norm_flags(p, TYPE))) return p.layer ? TAB_NK(true, true) : TAB_NK(true, false);
+    return p.layer ? TAB_NK(false, true) : TAB_NK(false, false);
+#undef TAB_NK
 }
 // What a stream kernel is launched with: CTAs that are all resident, and rows in flight.
 struct StreamPlan { int ctas, stages; size_t smem; };
 // row_bytes: of one row's tensors; fixed: bytes besides the ring.  0 stages: it does not fit, or there are too few rows to stay for.
 template <auto KERNEL>
-static StreamPlan stream_plan(int threads, long long M, size_t row_bytes, size_t fixed) {
+static StreamPlan stream_plan(int each, long long M, size_t row_bytes, size_t fixed) {
     StreamPlan pl = {0, 0, 0};
     int dev = 0, sms = 148;
     if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return pl;
-    const size_t room = 225 * 1024;
-    for (int n = 512 / threads; n >= 1 && !pl.stages; n /= 2) {            // CTAs an SM holds by its registers
-        const size_t share = room / n - 2048;
+    const size_t room = 226 * 1024;
+    for (int n = each; n >= 1 && !pl.stages; n--) {                        // each: CTAs an SM holds by its registers
+        const size_t share = std::min<size_t>(room, 228 * 1024 / n - 1536);    // less a kilobyte that every CTA is charged and what is static
         const long long stages = share > fixed ? (long long)((share - fixed) / row_bytes) : 0;
         if (stages >= 2 && M >= 2LL * n * sms) { pl.stages = (int)std::min<long long>(stages, 4); pl.ctas = std::min(n * sms, NORM_CTAS); }
     }
@@ -943,18 +1019,11 @@ static StreamPlan stream_plan(int threads, long long M, size_t row_bytes, size_t
     }
     return pl;
 }
-static bool rows16(const void* p, long long ld, int size) { return !p || (!(reinterpret_cast<uintptr_t>(p) & 15) && ld * size % 16 == 0); }
-// Whether all tensors that are there have rows a stream kernel can move eight elements at a time.
-static bool norm_streams(const NormParams& p, int type, int flags) {
-    const int s = type_bytes(type);
-    return p.C % 8 == 0 && rows16(p.y, p.ldy, s) && rows16(p.x, p.ldx, s) && (!p.r || (flags & V_R)) && (!p.h || (flags & V_H)) && (!p.q || (flags & V_Q)) && (!p.w1 || (flags & V_W1)) &&
-           (!p.b1 || (flags & V_B1)) && (!p.w2 || (flags & V_W2)) && (!p.b2 || (flags & V_B2)) && (p.gkind < TAB_GATE_CHANNEL || (flags & V_G));
-}
 // TAB_E_TOO_LARGE: the stream kernel does not take the problem.
 template <int TYPE, int THREADS, int NV, bool LAYER, bool QUANT, bool FAST>
 static int launch_norm_stream_as(const NormParams& p, cudaStream_t stream) {
     constexpr auto kernel = residual_norm_stream_kernel<TYPE, THREADS, NV, LAYER, QUANT, FAST>;
-    const StreamPlan pl = stream_plan<kernel>(THREADS, p.M, 2 * (size_t)p.C * type_bytes(TYPE), 0);
+    const StreamPlan pl = stream_plan<kernel>(512 / THREADS, p.M, 2 * (size_t)p.C * type_bytes(TYPE), 0);
     if (!pl.stages) return TAB_E_TOO_LARGE;
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
@@ -962,7 +1031,8 @@ static int launch_norm_stream_as(const NormParams& p, cudaStream_t stream) {
 }
 template <int TYPE, int THREADS, int NV>
 static int launch_norm_stream(const NormParams& p, cudaStream_t stream) {
-    if (!norm_streams(p, TYPE, norm_flags(p, TYPE)) || (!p.h && !p.q && p.w2)) return TAB_E_TOO_LARGE;
+    const int s = type_bytes(TYPE);
+    if (!norm_vectors(p, TYPE, norm_flags(p, TYPE)) || !rows16(p.y, p.ldy, s) || !rows16(p.x, p.ldx, s) || (!p.h && !p.q && p.w2)) return TAB_E_TOO_LARGE;
     const bool fast = p.w1 && p.x && p.w2 && p.r && (p.gkind == TAB_GATE_NONE || p.gkind == TAB_GATE_CHANNEL);
     if (p.h && p.q) return TAB_E_TOO_LARGE;
 #define TAB_NS(L, Q) (fast ? launch_norm_stream_as<TYPE, THREADS, NV, L, Q, true>(p, stream) : launch_norm_stream_as<TYPE, THREADS, NV, L, Q, false>(p, stream))
@@ -972,20 +1042,18 @@ static int launch_norm_stream(const NormParams& p, cudaStream_t stream) {
 static int launch_norm_sums(const NormBackwardParams& b, int parts, cudaStream_t stream) {
     const NormParams& p = b.f;
     const int NS = p.layer ? NORM_SUMS<true> : NORM_SUMS<false>;
-    return launch_pdl(norm_sums_kernel, dim3((unsigned)((p.C + 31) / 32), (unsigned)NS), dim3(1024), 0, stream, (const float*)b.partial, parts, NS, p.C, p.ptype, b.dw2, b.dw1,
-                      p.gkind == TAB_GATE_CHANNEL ? b.dgate : nullptr, p.gtype, p.layer ? b.db2 : nullptr, p.layer ? b.db1 : nullptr);
-}
-static bool wants_sums(const NormBackwardParams& b) { return b.dw1 || b.db1 || b.dw2 || b.db2 || (b.f.gkind == TAB_GATE_CHANNEL && b.dgate); }
-static int backward_flags(const NormBackwardParams& b, int type) {
-    const int s = type_bytes(type);
-    return norm_flags(b.f, type) | (on8(b.gr, b.ldgr, s) ? V_GR : 0) | (on8(b.gh, b.ldgh, s) ? V_GH : 0) | (on8(b.dy, b.lddy, s) ? V_DY : 0) |
-           (on8(b.dx, b.lddx, s) ? V_DX : 0) | (on8(b.dgate, b.f.C, type_bytes(b.f.gtype)) ? V_DG : 0);
+    void *dgate = p.gkind == TAB_GATE_CHANNEL ? b.dgate : nullptr, *db2 = p.layer ? b.db2 : nullptr, *db1 = p.layer ? b.db1 : nullptr;
+    if (p.C % 4 == 0)
+        return launch_pdl(norm_sums_kernel<4>, dim3((unsigned)((p.C + 127) / 128), (unsigned)NS), dim3(1024), 0, stream, (const float*)b.partial, parts, NS, p.C, p.ptype, b.dw2, b.dw1, dgate,
+                          p.gtype, db2, db1);
+    return launch_pdl(norm_sums_kernel<1>, dim3((unsigned)((p.C + 31) / 32), (unsigned)NS), dim3(1024), 0, stream, (const float*)b.partial, parts, NS, p.C, p.ptype, b.dw2, b.dw1, dgate, p.gtype,
+                      db2, db1);
 }
 template <int TYPE, int THREADS, int NV, bool LAYER, bool TOKEN, bool FAST>
 static int launch_norm_backward_stream_as(NormBackwardParams b, cudaStream_t stream) {
     const NormParams& p = b.f;
     constexpr auto kernel = residual_norm_backward_stream_kernel<TYPE, THREADS, NV, LAYER, TOKEN, FAST>;
-    const StreamPlan pl = stream_plan<kernel>(THREADS, p.M, 4 * (size_t)p.C * type_bytes(TYPE), 12 * (size_t)p.C);
+    const StreamPlan pl = stream_plan<kernel>(backward_threads(NV, LAYER) / THREADS, p.M, 4 * (size_t)p.C * type_bytes(TYPE), (p.gkind == TAB_GATE_CHANNEL ? 12 : 8) * (size_t)p.C);
     if (!pl.stages) return TAB_E_TOO_LARGE;
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
@@ -995,21 +1063,14 @@ static int launch_norm_backward_stream_as(NormBackwardParams b, cudaStream_t str
     const int rc = launch_pdl(kernel, dim3((unsigned)ctas), dim3(THREADS), pl.smem, stream, b, pl.stages, status);
     return rc != TAB_OK || !sums ? rc : launch_norm_sums(b, ctas, stream);
 }
-template <int TYPE, int THREADS, int NV>
+template <int TYPE, int THREADS, int NV, bool LAYER>
 static int launch_norm_backward_stream(const NormBackwardParams& b, cudaStream_t stream) {
-    NormParams f = b.f;
-    const int flags = backward_flags(b, TYPE);
+    const NormParams& f = b.f;
     const bool pre = f.w2 && b.gh, want_u = f.w1 || f.gkind != TAB_GATE_NONE, token = f.gkind == TAB_GATE_TOKEN;
-    if (!pre) f.w2 = f.b2 = f.r = nullptr;                                 // not looked at
-    if (!want_u) f.y = nullptr;
-    f.x = f.h = f.q = nullptr;
-    if (!norm_streams(f, TYPE, flags) || (pre && !(flags & V_GH)) || (b.gr && !(flags & V_GR)) || (b.dy && !(flags & V_DY)) || (b.dx && !(flags & V_DX)) ||
-        (f.gkind == TAB_GATE_FULL && b.dgate && !(flags & V_DG)) || (!pre && !b.gr && !want_u)) return TAB_E_TOO_LARGE;
-    const bool fast = pre && f.w1 && b.gr && b.dx && b.dy && (f.gkind == TAB_GATE_NONE || f.gkind == TAB_GATE_CHANNEL);
-#define TAB_NB(L) (token ? launch_norm_backward_stream_as<TYPE, THREADS, NV, L, true, false>(b, stream) : fast ? launch_norm_backward_stream_as<TYPE, THREADS, NV, L, false, true>(b, stream) \
-                                                                                             : launch_norm_backward_stream_as<TYPE, THREADS, NV, L, false, false>(b, stream))
-    return f.layer ? TAB_NB(true) : TAB_NB(false);
-#undef TAB_NB
+    if (!backward_vectors(b, TYPE) || (!pre && !b.gr && !want_u)) return TAB_E_TOO_LARGE;
+    if (token) return launch_norm_backward_stream_as<TYPE, THREADS, NV, LAYER, true, false>(b, stream);
+    if (pre && f.w1 && b.gr && b.dx && b.dy && f.gkind != TAB_GATE_FULL) return launch_norm_backward_stream_as<TYPE, THREADS, NV, LAYER, false, true>(b, stream);
+    return launch_norm_backward_stream_as<TYPE, THREADS, NV, LAYER, false, false>(b, stream);
 }
 template <int TYPE, int GT, int NV>
 static int launch_norm_backward(NormBackwardParams b, cudaStream_t stream) {
@@ -1019,15 +1080,15 @@ static int launch_norm_backward(NormBackwardParams b, cudaStream_t stream) {
     const bool sums = wants_sums(b);
     if (!sums) b.partial = nullptr;
     const dim3 grid((unsigned)(parts / G)), block(GT < 128 ? 128 : GT);
-    const int flags = backward_flags(b, TYPE);
-    const int rc = p.layer ? launch_pdl(residual_norm_backward_kernel<TYPE, GT, NV, true>, grid, block, 0, stream, b, flags, rows_each)
-                           : launch_pdl(residual_norm_backward_kernel<TYPE, GT, NV, false>, grid, block, 0, stream, b, flags, rows_each);
+#define TAB_NK(V, L) launch_pdl(residual_norm_backward_kernel<TYPE, GT, NV, V, L>, grid, block, 0, stream, b, rows_each)
+    const int rc = backward_vectors(b, TYPE) ? (p.layer ? TAB_NK(true, true) : TAB_NK(true, false)) : (p.layer ? TAB_NK(false, true) : TAB_NK(false, false));
+#undef TAB_NK
     return rc != TAB_OK || !sums ? rc : launch_norm_sums(b, (int)parts, stream);
 }
 
 #define TAB_NORM_SIZES(F, C, ARG) \
     if (C <= 256) return F(32, 1)(ARG, stream); \
-    if (C <= 1024) return F(32, 4)(ARG, stream); \
+    if (C <= 1024) return F(128, 1)(ARG, stream); \
     if (C <= 2048) return F(128, 2)(ARG, stream); \
     if (C <= 4096) return F(256, 2)(ARG, stream); \
     if (C <= 8192) return F(512, 2)(ARG, stream); \
@@ -1048,12 +1109,22 @@ static int norm_sizes(const NormParams& p, cudaStream_t stream) {
 }
 template <int TYPE>
 static int norm_backward_sizes(const NormBackwardParams& b, cudaStream_t stream) {
+    // Centred norms have five sums over rows instead of three to hold: twice the registers, half the threads.
     int rc = TAB_E_TOO_LARGE;
-    if (b.f.C > 256 && b.f.C <= 512) rc = launch_norm_backward_stream<TYPE, 64, 1>(b, stream);
-    else if (b.f.C > 512 && b.f.C <= 1024) rc = launch_norm_backward_stream<TYPE, 64, 2>(b, stream);
-    else if (b.f.C > 1024 && b.f.C <= 2048) rc = launch_norm_backward_stream<TYPE, 128, 2>(b, stream);
-    else if (b.f.C > 2048 && b.f.C <= 4096) rc = launch_norm_backward_stream<TYPE, 256, 2>(b, stream);
-    else if (b.f.C > 4096 && b.f.C <= 8192) rc = launch_norm_backward_stream<TYPE, 512, 2>(b, stream);
+    const int C = b.f.C;
+    if (b.f.layer) {
+        if (C > 256 && C <= 512) rc = launch_norm_backward_stream<TYPE, 64, 1, true>(b, stream);
+        else if (C > 512 && C <= 1024) rc = launch_norm_backward_stream<TYPE, 128, 1, true>(b, stream);
+        else if (C > 1024 && C <= 2048) rc = launch_norm_backward_stream<TYPE, 256, 1, true>(b, stream);
+        else if (C > 2048 && C <= 4096) rc = launch_norm_backward_stream<TYPE, 512, 1, true>(b, stream);
+        else if (C > 4096 && C <= 8192) rc = launch_norm_backward_stream<TYPE, 512, 2, true>(b, stream);
+    } else {
+        if (C > 256 && C <= 512) rc = launch_norm_backward_stream<TYPE, 32, 2, false>(b, stream);
+        else if (C > 512 && C <= 1024) rc = launch_norm_backward_stream<TYPE, 64, 2, false>(b, stream);
+        else if (C > 1024 && C <= 2048) rc = launch_norm_backward_stream<TYPE, 128, 2, false>(b, stream);
+        else if (C > 2048 && C <= 4096) rc = launch_norm_backward_stream<TYPE, 256, 2, false>(b, stream);
+        else if (C > 4096 && C <= 8192) rc = launch_norm_backward_stream<TYPE, 512, 2, false>(b, stream);
+    }
     if (rc != TAB_E_TOO_LARGE) return rc;
 #define TAB_NORM_B(GT, NV) launch_norm_backward<TYPE, GT, NV>
     TAB_NORM_SIZES(TAB_NORM_B, b.f.C, b);
