@@ -470,8 +470,9 @@ __device__ __forceinline__ void cta_sums(float (&v)[N], float (*exchange)[N][WAR
 
 // A thread has NV times eight columns, THREADS * 8 apart; what a row costs whatever its length (waits, meetings, addresses) is most of a
 // row's instructions at one.  FAST: both norms, a residual and no gate or one of channels, known when the kernel is compiled.
+constexpr int forward_threads(bool layer, bool fast) { return fast && !layer ? 640 : 512; }              // an SM holds, by registers
 template <int TYPE, int THREADS, int NV, bool LAYER, bool QUANT, bool FAST>
-__global__ void __launch_bounds__(THREADS, 512 / THREADS) residual_norm_stream_kernel(NormParams p, int stages, int* status) {
+__global__ void __launch_bounds__(THREADS, forward_threads(LAYER, FAST) / THREADS) residual_norm_stream_kernel(NormParams p, int stages, int* status) {
     using T = typename ElemOf<TYPE>::type;
     extern __shared__ __align__(128) uint8_t ring[];
     __shared__ __align__(8) uint64_t bars[8];
@@ -1023,7 +1024,7 @@ static StreamPlan stream_plan(int each, long long M, size_t row_bytes, size_t fi
 template <int TYPE, int THREADS, int NV, bool LAYER, bool QUANT, bool FAST>
 static int launch_norm_stream_as(const NormParams& p, cudaStream_t stream) {
     constexpr auto kernel = residual_norm_stream_kernel<TYPE, THREADS, NV, LAYER, QUANT, FAST>;
-    const StreamPlan pl = stream_plan<kernel>(512 / THREADS, p.M, 2 * (size_t)p.C * type_bytes(TYPE), 0);
+    const StreamPlan pl = stream_plan<kernel>(forward_threads(LAYER, FAST) / THREADS, p.M, 2 * (size_t)p.C * type_bytes(TYPE), 0);
     if (!pl.stages) return TAB_E_TOO_LARGE;
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;

@@ -239,6 +239,57 @@ def test_matmul_blocks_non_finite(cuda):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M, N", [(3, 200), (40, 200), (200, 300), (2304, 1300)])
+def test_matmul_blocks_nan_scales(cuda, M, N):
+    """A scale of NaN (the byte 255) voids the results of its row, or of its square's rows, and no others; whole kernels apart."""
+    rng = np.random.default_rng(M)
+    a, b = random_blocks(rng, M, 520, "e4m3", False, True), random_blocks(rng, N, 520, "e4m3", True, True)
+    want = ref.values(*a, "e4m3") @ ref.values(*b, "e4m3").T
+    a[1][M - 1, 2], b[1][1, 4] = 255, 255
+    y = TAB.matmul_blocks(*device_blocks(cuda, *a, "e4m3"), *device_blocks(cuda, *b, "e4m3"), out_dtype=torch.float32).cpu().numpy()
+    hit = np.zeros_like(want, bool)
+    hit[M - 1], hit[:, 128:256] = True, True
+    assert np.isnan(y[hit]).all() and np.array_equal(y[~hit], want[~hit])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M, N", [(2, 100), (40, 200), (200, 300), (2304, 1300)])
+def test_matmul_blocks_far_scales(cuda, M, N):
+    """Scales at the ends of their range whose products are not: 2^-120 against 2^100."""
+    rng = np.random.default_rng(N)
+    a, b = random_blocks(rng, M, 300, "e4m3", False, True), random_blocks(rng, N, 300, "e4m3", False, True)
+    want = ref.values(*a, "e4m3") @ ref.values(*b, "e4m3").T
+    far = lambda o, e: (o[0], (o[1].astype(int) + e).astype(np.uint8))
+    y = TAB.matmul_blocks(*device_blocks(cuda, *far(a, -120), "e4m3"), *device_blocks(cuda, *far(b, 100), "e4m3"), out_dtype=torch.float32).cpu().numpy()
+    assert np.array_equal(y.astype(np.float64) * 2.0 ** 20, want)
+
+
+@pytest.mark.gpu
+def test_blocks_beyond_32_bits(cuda):
+    """More than 2^31 values: quantised along both axes and multiplied; rows near the ends against the reference."""
+    M, K, N = 66000, 32768 + 128, 16
+    rows = [0, 1, 31337, 65279, M - 2, M - 1]
+    x = torch.empty(M, K, dtype=torch.bfloat16, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    for i in range(0, M, 6000):
+        x[i:i + 6000].normal_(generator=gen)
+    q, s, qt, st = TAB.quantize_blocks(x, columns=True)
+    v = x[rows].double().cpu().numpy()
+    wq, ws = ref.quantize(v, "e4m3")
+    assert ref.same_bytes(np_bytes(q[rows]), wq, "e4m3") and np.array_equal(np_bytes(s[rows]), ws)
+    cols = [0, 127, 20000, K - 1]
+    wq, ws = ref.quantize(x[:, cols].t().contiguous().double().cpu().numpy(), "e4m3")
+    assert ref.same_bytes(np_bytes(qt[cols]), wq, "e4m3") and np.array_equal(np_bytes(st[cols]), ws)
+    del qt, st, x
+    b = random_blocks(np.random.default_rng(2), N, K, "e4m3", True, True)
+    y = TAB.matmul_blocks(q, s, *device_blocks(cuda, *b, "e4m3"), out_dtype=torch.float32)
+    qa, sa = np_bytes(q[rows]), np_bytes(s[rows])
+    va, vb = ref.values(qa, sa, "e4m3"), ref.values(*b, "e4m3")
+    assert np.all(np.abs(y[rows].double().cpu().numpy() - va @ vb.T) <= np.abs(va) @ np.abs(vb).T * K * 2.0 ** -23)
+    assert _cabi.lib().tab_device_status() == 0
+
+
+@pytest.mark.gpu
 def test_matmul_blocks_layouts(cuda):
     """Leading dimensions, scales of any strides, slices of operands, an empty sum, empty results, bytes behind the result."""
     rng = np.random.default_rng(4)
@@ -379,3 +430,97 @@ def test_second_derivatives_are_refused(cuda, monkeypatch, native):
         g, = torch.autograd.grad(y.sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="differentiable"):
             g.sum().backward()
+
+
+# ---- together, as they are used ---------------------------------------------------------------------------------------
+
+def block_step(x, params, training):
+    """A residual block's dense half: norm, up, rectifier squared, down, norm, gate, residual, next norm."""
+    w1, w2, up, down, gate = params
+    if training:
+        h = tab_nn.residual_norm(x, pre_weight=w1)[1]
+        y = tab_nn.block_linear(torch.relu(tab_nn.block_linear(h, up)).square(), down)
+        return tab_nn.residual_norm(y, x, pre_weight=w1, post_weight=w2, gate=gate, residual_scale=0.9)
+    _, q, s = TAB.residual_norm(x, pre_weight=w1, quantize=torch.float8_e4m3fn)
+    y = torch.relu(up(q, s)).square()
+    return TAB.residual_norm(down(y), x, pre_weight=w1, post_weight=w2, gate=gate, residual_scale=0.9)
+
+
+def block_params(cuda, C, F):
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    n = lambda *s: torch.randn(*s, device=cuda, generator=gen)
+    return 1 + 0.1 * n(C), 1 + 0.1 * n(C), n(F, C) / C ** 0.5, n(C, F) / F ** 0.5, 0.5 + 0.1 * n(C)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens", [1, 7, 200, 600])
+def test_block_for_serving_and_training_agree(cuda, tokens):
+    """The same block from prepared layers, its first norm handing over blocks, and in its differentiable form: equal but for values
+    whose fp32 and bf16 forms round to different 8-bit floats (a step is 2^-3 of a value, its half 2^-4; few values, and a sum of many)."""
+    C, F = 384, 1000
+    params = block_params(cuda, C, F)
+    x = torch.randn(tokens, C, device=cuda).bfloat16()
+    served = block_step(x, (*params[:2], tab_nn.BlockLinear.from_float(params[2]), tab_nn.BlockLinear.from_float(params[3]), params[4]), False)
+    trained = block_step(x, params, True)
+    for a, b in zip(served, trained):
+        assert float((a.float() - b.float()).norm() / b.float().norm()) <= 2.0 ** -4
+
+
+@pytest.mark.gpu
+def test_block_in_a_graph(cuda):
+    """Forward and backward captured once and replayed on other inputs, beside a second graph and eager calls: the eager results, bit for bit."""
+    C, F, T = 256, 520, 160
+    params = [p.requires_grad_() for p in block_params(cuda, C, F)]
+    inputs = [torch.randn(T, C, device=cuda).bfloat16() for _ in range(3)]
+
+    def step(x):
+        x = x.detach().requires_grad_()
+        r, h = block_step(x, params, True)
+        return [r.detach(), h.detach(), *torch.autograd.grad((r, h), (x, *params), (torch.ones_like(r), torch.ones_like(h)))]
+
+    eager = [step(x) for x in inputs]
+    graphs = []
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(inputs[0])
+    torch.cuda.synchronize()
+    for _ in range(2):
+        place, g = inputs[0].clone(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(place)
+        graphs.append((place, g, out))
+    for i, (x, want) in enumerate(zip(inputs, eager)):
+        place, g, out = graphs[i % 2]
+        place.copy_(x)
+        g.replay()
+        other = step(inputs[(i + 1) % 3])
+        assert all(torch.equal(a, b) for a, b in zip(out, want)) and all(torch.equal(a, b) for a, b in zip(other, eager[(i + 1) % 3]))
+
+
+@pytest.mark.gpu
+def test_streams_side_by_side(cuda):
+    """The same calls on two streams at once: each one's own results."""
+    C, F = 512, 700
+    params = block_params(cuda, C, F)
+    xs = [torch.randn(t, C, device=cuda).bfloat16() for t in (3, 300, 900, 40)]
+    want = [block_step(x, params, True) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for i in range(20):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(block_step(xs[i % 4], params, True))
+    torch.cuda.synchronize()
+    for i, pair in enumerate(got):
+        assert all(torch.equal(a, b) for a, b in zip(pair, want[i % 4]))
+    assert _cabi.lib().tab_device_status() == 0
+
+
+@pytest.mark.gpu
+def test_empty_rows_and_sums(cuda):
+    x = torch.randn(3, 0, device=cuda)
+    q, s, qt, st = TAB.quantize_blocks(x, columns=True)
+    assert q.shape == (3, 0) and s.shape == (3, 0) and qt.shape == (0, 3) and st.shape == (0, 1)
+    assert not TAB.matmul_blocks(q, s, q, s).any()
+    q, s = TAB.quantize_blocks(torch.randn(0, 128, device=cuda))
+    assert q.shape == (0, 128) and s.shape == (0, 1)

@@ -246,3 +246,19 @@ def test_residual_norm_forms(cuda):
             TAB.residual_norm(z, **kw)
     with pytest.raises(_cabi.TabError, match="exceeds"):
         TAB.residual_norm(torch.zeros(1, 16385, device=cuda), pre_weight=torch.ones(16385, device=cuda))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(9, 100), (700, 1032)])
+@pytest.mark.parametrize("only", NAMES)
+def test_one_gradient_alone(cuda, shape, only):
+    """A single gradient asked for is that of all of them: other kernels may form it, so up to fp32 roundings (as counted above)."""
+    t, gr, gh = make(8, shape, "fp32", "fp32", "layer", "channel", True, True, True)
+    dev = {k: v.to(cuda) for k, v in t.items()}
+    grads = []
+    for names in (NAMES, (only,)):
+        leaves = {k: v.clone().requires_grad_(k in names) for k, v in dev.items()}
+        out = tab_nn.residual_norm(**leaves, kind="layer")
+        grads.append(torch.autograd.grad(out, leaves[only], (gr.to(cuda), gh.to(cuda)))[0])
+    size = float(grads[0].abs().max()) + 30 * (1 if only in ("y", "residual") else shape[0] ** 0.5)
+    assert float((grads[0] - grads[1]).abs().max()) <= size * (96 + 4 * shape[0] ** 0.5) * 2.0 ** -24
