@@ -1,6 +1,7 @@
 // 8-bit floats in blocks of 128 with one power-of-two scale each, and the operators around them: types, scales and element access
 // shared by the kernels behind tab_quantize_blocks_launch, tab_matmul_blocks_launch and tab_residual_norm_launch.
 #pragma once
+#include <atomic>
 #include <cstdint>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -11,6 +12,18 @@ namespace tab {
 constexpr int BLK = 128;                     // values that share a scale
 
 inline int blocks_of(long long n) { return (int)((n + BLK - 1) / BLK); }
+// SMs of the current device.
+inline int blocks_sms() {
+    static std::atomic<int> known[64];
+    int dev = 0, n = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    n = known[dev].load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) { cudaGetLastError(); n = 148; }
+        known[dev].store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
 inline int type_bytes(int type) { return type == TAB_FP32 ? 4 : 2; }
 
 // What the quantiser is given.  Pitches are in elements; a null output is not written.

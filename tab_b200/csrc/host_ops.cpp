@@ -6,6 +6,7 @@
 // then runs its own body, which names what is wrong or does the rare case, so that there is one set of messages.
 #include <torch/extension.h>
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include "../../include/tab_b200.h"
@@ -230,37 +231,41 @@ struct Rows {
     }
 };
 
-// 8-bit values of `shape` (rows x n), every row starting on 16 bytes; the pitch.
-Tensor new_blocks(const Tensor& like, at::IntArrayRef shape, int64_t rows, int64_t n, at::ScalarType dtype) {
+// An uninitialised tensor, past the dispatcher (two or three of them are most of what a small call costs the host).
+Tensor fresh(const Tensor& like, at::IntArrayRef size, at::IntArrayRef strides, at::ScalarType dtype) {
+    return Tensor(at::detail::empty_strided_cuda(size, strides, like.options().dtype(dtype)));
+}
+Tensor fresh(const Tensor& like, at::IntArrayRef size, at::ScalarType dtype) { return Tensor(at::detail::empty_cuda(size, like.options().dtype(dtype))); }
+using Strides = c10::SmallVector<int64_t, 6>;
+
+// 8-bit values of `shape` (rows x n), every row starting on 16 bytes.
+Tensor new_blocks(const Tensor& like, at::IntArrayRef shape, int64_t n, at::ScalarType dtype) {
     const int64_t pitch = (n + 15) / 16 * 16;
-    if (pitch == n) return make(like, shape, dtype);
-    Tensor held = make(like, {rows, pitch}, dtype);
-    std::vector<int64_t> strides(shape.size());
+    if (pitch == n) return fresh(like, shape, dtype);
+    Strides strides(shape.size(), 1);
     int64_t step = pitch;
-    for (int64_t i = (int64_t)shape.size() - 1; i >= 0; i--) {
-        if (i == (int64_t)shape.size() - 1) { strides[i] = 1; continue; }
+    for (int64_t i = (int64_t)shape.size() - 2; i >= 0; i--) {
         strides[i] = step;
         step *= shape[i];
     }
-    return held.as_strided(shape, strides);
+    return fresh(like, shape, strides, dtype);
 }
-std::vector<int64_t> with_last(const Tensor& t, int64_t n) {
-    std::vector<int64_t> s(t.sizes().begin(), t.sizes().end());
+Strides with_last(const Tensor& t, int64_t n) {
+    Strides s(t.sizes().begin(), t.sizes().end());
     s.back() = n;
     return s;
 }
 
-// Scales `shape` (rows x n) that lie block by block.
-Tensor new_scales(const Tensor& like, at::IntArrayRef shape, int64_t rows, int64_t n) {
-    const int64_t pitch = (rows + 15) / 16 * 16;
-    std::vector<int64_t> strides(shape.size());
+// Scales `shape` that lie block by block.
+Tensor new_scales(const Tensor& like, at::IntArrayRef shape, int64_t rows) {
+    Strides strides(shape.size());
     int64_t step = 1;
     for (int64_t i = (int64_t)shape.size() - 2; i >= 0; i--) {
         strides[i] = step;
         step *= shape[i];
     }
-    strides.back() = pitch;
-    return make(like, {n * pitch}, at::kFloat8_e8m0fnu).as_strided(shape, strides);
+    strides.back() = (rows + 15) / 16 * 16;
+    return fresh(like, shape, strides, at::kFloat8_e8m0fnu);
 }
 
 struct Quantized { Tensor q, s, qt, st; };
@@ -269,11 +274,11 @@ bool quantize_any(const Tensor& x, at::ScalarType dtype, bool both, bool square,
     const int format = format_of(dtype);
     if (!on_cuda(x) || type_of(x) < 0 || format < 0 || (square && x.dim() != 2) || !r.of(x)) return false;
     const c10::cuda::CUDAGuard guard(x.device());
-    o.q = new_blocks(x, x.sizes(), r.M, r.K, dtype);
-    o.s = square ? make(x, {blocks(r.M), blocks(r.K)}, at::kFloat8_e8m0fnu) : new_scales(x, with_last(x, blocks(r.K)), r.M, blocks(r.K));
+    o.q = new_blocks(x, x.sizes(), r.K, dtype);
+    o.s = square ? fresh(x, {blocks(r.M), blocks(r.K)}, at::kFloat8_e8m0fnu) : new_scales(x, with_last(x, blocks(r.K)), r.M);
     if (both) {
-        o.qt = new_blocks(x, {r.K, r.M}, r.K, r.M, dtype);
-        o.st = square ? make(x, {blocks(r.K), blocks(r.M)}, at::kFloat8_e8m0fnu) : new_scales(x, {r.K, blocks(r.M)}, r.K, blocks(r.M));
+        o.qt = new_blocks(x, {r.K, r.M}, r.M, dtype);
+        o.st = square ? fresh(x, {blocks(r.K), blocks(r.M)}, at::kFloat8_e8m0fnu) : new_scales(x, {r.K, blocks(r.M)}, r.K);
     }
     const int64_t pk = (r.K + 15) / 16 * 16, pm = (r.M + 15) / 16 * 16;
     return tab_quantize_blocks_launch(x.data_ptr(), type_of(x), r.pitch, r.M, (int)r.K, format, square, o.q.data_ptr(), pk, static_cast<uint8_t*>(o.s.data_ptr()),
@@ -319,7 +324,7 @@ bool matmul_any(const Tensor& a, const Tensor& as, const Tensor& b, const Tensor
     const int type = type_of(dtype);
     if (type < 0 || !A.of(a, as) || !B.of(b, bs) || b.dim() != 2 || A.r.K != B.r.K || a.device() != b.device()) return false;
     const c10::cuda::CUDAGuard guard(a.device());
-    y = make(a, with_last(a, B.r.M), dtype);
+    y = fresh(a, with_last(a, B.r.M), dtype);
     return tab_matmul_blocks_launch(a.data_ptr(), format_of(a.scalar_type()), A.r.pitch, static_cast<const uint8_t*>(as.data_ptr()), A.share, A.sr, A.sk,
                                     b.data_ptr(), format_of(b.scalar_type()), B.r.pitch, static_cast<const uint8_t*>(bs.data_ptr()), B.share, B.sr, B.sk,
                                     y.data_ptr(), type, B.r.M, (int)A.r.M, (int)B.r.M, (int)A.r.K, stream_of(a)) == TAB_OK;
@@ -436,18 +441,18 @@ struct Norm {
 // r (undefined where it is y), h or its blocks, statistics where asked for.
 bool norm_any(Norm& n, const Tensor& y, c10::optional<at::ScalarType> quantize, bool stats, Tensor& r, Tensor& h, Tensor& s, Tensor& st) {
     const c10::cuda::CUDAGuard guard(y.device());
-    if (!n.plain()) { r = make(y, y.sizes(), y.scalar_type()); n.a.r = r.data_ptr(); n.a.ldr = n.r.K; }
+    if (!n.plain()) { r = fresh(y, y.sizes(), y.scalar_type()); n.a.r = r.data_ptr(); n.a.ldr = n.r.K; }
     if (quantize.has_value()) {
         n.a.format = format_of(*quantize);
         if (n.a.format < 0 || !n.a.w2) return false;
-        h = new_blocks(y, y.sizes(), n.r.M, n.r.K, *quantize);
-        s = new_scales(y, with_last(y, blocks(n.r.K)), n.r.M, blocks(n.r.K));
+        h = new_blocks(y, y.sizes(), n.r.K, *quantize);
+        s = new_scales(y, with_last(y, blocks(n.r.K)), n.r.M);
         n.a.q = h.data_ptr(); n.a.ldq = (n.r.K + 15) / 16 * 16; n.a.lds = (n.r.M + 15) / 16 * 16; n.a.s = static_cast<uint8_t*>(s.data_ptr());
     } else if (n.a.w2) {
-        h = make(y, y.sizes(), y.scalar_type());
+        h = fresh(y, y.sizes(), y.scalar_type());
         n.a.h = h.data_ptr(); n.a.ldh = n.r.K;
     }
-    if (stats) { st = make(y, {n.r.M, 4}, at::kFloat); n.a.stats = st.data_ptr<float>(); }
+    if (stats) { st = fresh(y, {n.r.M, 4}, at::kFloat); n.a.stats = st.data_ptr<float>(); }
     return tab_residual_norm_launch(&n.a, stream_of(y)) == TAB_OK;
 }
 const Tensor& given(const OptTensor& t) {
@@ -513,13 +518,13 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
             size_t input = 0;                                              // autograd numbers the tensors that there are
             for (size_t i = 0; i < 7; i++) {
                 if (!grads_of[i].like.defined() || (i == 1 && !residual) || !ctx->needs_input_grad(input++)) continue;
-                out[i] = make(grads_of[i].like, grads_of[i].like.sizes(), grads_of[i].like.scalar_type());
+                out[i] = fresh(grads_of[i].like, grads_of[i].like.sizes(), grads_of[i].like.scalar_type());
                 *grads_of[i].p = out[i].data_ptr();
                 sums = sums || i > 1;
             }
             b.lddy = b.lddx = n.r.K;
             Tensor partial;
-            if (sums) { partial = make(y, {(int64_t)(tab_residual_norm_workspace_bytes(n.r.M, (int)n.r.K) / 4)}, at::kFloat); b.partial = partial.data_ptr<float>(); }
+            if (sums) { partial = fresh(y, {(int64_t)(tab_residual_norm_workspace_bytes(n.r.M, (int)n.r.K) / 4)}, at::kFloat); b.partial = partial.data_ptr<float>(); }
             ok = ok && tab_residual_norm_backward_launch(&b, stream_of(y)) == TAB_OK;
         }
         TORCH_CHECK(ok, "residual_norm: a launch of the backward pass failed [cudaError ", tab_last_cuda_error(), "]");

@@ -706,10 +706,19 @@ static bool blocks_result_map(CUtensorMap* m, const MatmulBlocksParams& p) {
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-static thread_local char g_last_blocks_kernel[96] = "none";
-const char* matmul_blocks_last_kernel() { return g_last_blocks_kernel; }
-
 struct BlocksPlan { int bn; bool swap; int split, per, nst, ks; };
+
+// What the thread launched last, put into words when somebody asks.
+static thread_local struct { int kind; BlocksPlan plan; } g_last = {0, {}};
+const char* matmul_blocks_last_kernel() {
+    static thread_local char text[96];
+    const BlocksPlan& p = g_last.plan;
+    if (g_last.kind == 0) return "none";
+    if (g_last.kind == 1) return "matmul_blocks_rows_kernel";
+    if (g_last.kind == 3) return "matmul_blocks_pair_kernel";
+    snprintf(text, sizeof(text), "matmul_blocks_tile_kernel<%d,%d,%d> split %d stages %d", p.bn, p.ks, (int)p.swap, p.split, p.nst);
+    return text;
+}
 
 template <int BN, int KS, bool SWAP, int TYPE>
 static int launch_tile(const MatmulBlocksParams& p, const BlocksPlan& pl, int* status, cudaStream_t stream) {
@@ -735,7 +744,7 @@ static int launch_tile(const MatmulBlocksParams& p, const BlocksPlan& pl, int* s
     if (grid >= (1LL << 31)) return TAB_E_TOO_LARGE;
     alignas(64) CUtensorMap tmY = tmR;                                     // a stand-in where it is not used
     const int tma = !SWAP && pl.split == 1 && blocks_result_map(&tmY, p);
-    snprintf(g_last_blocks_kernel, sizeof(g_last_blocks_kernel), "matmul_blocks_tile_kernel<%d,%d,%d> split %d stages %d", BN, KS, (int)SWAP, pl.split, pl.nst);
+    g_last.kind = 2; g_last.plan = pl;
     return launch_pdl_as(false, (unsigned)pl.split, kernel, dim3((unsigned)grid), dim3(TT), (size_t)smem, stream, tmR, tmC, tmY, R, C, p.y, p.ldy, blocks_of(p.K), pl.per, pl.nst,
                          (int)tiles_c, pl.split, tma, status);
 }
@@ -773,7 +782,7 @@ static int launch_pair(const MatmulBlocksParams& p, int pairs, int* status, cuda
     alignas(64) CUtensorMap tmY = tmA;
     const int tma = blocks_result_map(&tmY, p);
     const unsigned grid = 2u * (unsigned)std::min<long long>(ntiles, pairs);
-    snprintf(g_last_blocks_kernel, sizeof(g_last_blocks_kernel), "matmul_blocks_pair_kernel");
+    g_last.kind = 3;
     auto kernel = p.type == TAB_FP32 ? matmul_blocks_pair_kernel<TAB_FP32> : p.type == TAB_BF16 ? matmul_blocks_pair_kernel<TAB_BF16> : matmul_blocks_pair_kernel<TAB_FP16>;
     return launch_pdl_as(false, 2u, kernel, dim3(grid), dim3(PT), (size_t)PSMEM, stream, tmA, tmB, tmY, p.a, p.b, p.y, p.ldy, blocks_of(p.K), (int)tiles_m, (int)tiles_n, 8, tma, status);
 }
@@ -783,7 +792,7 @@ static int launch_rows(const MatmulBlocksParams& p, cudaStream_t stream) {
     const unsigned grid = (unsigned)(((long long)p.b.rows + 15) / 16);
     const int warps = 8;
     const int per = (KB + warps - 1) / warps;
-    snprintf(g_last_blocks_kernel, sizeof(g_last_blocks_kernel), "matmul_blocks_rows_kernel %d warps", warps);
+    g_last.kind = 1;
 #define TAB_MR(FA, FB) launch_pdl(matmul_blocks_rows_kernel<FA, FB>, dim3(grid), dim3(32 * warps), 0, stream, p.a, p.b, p.y, p.ldy, p.type, p.K, per)
     if (p.a.format == TAB_E5M2) return p.b.format == TAB_E5M2 ? TAB_MR(TAB_E5M2, TAB_E5M2) : TAB_MR(TAB_E5M2, TAB_E4M3);
     return p.b.format == TAB_E5M2 ? TAB_MR(TAB_E4M3, TAB_E5M2) : TAB_MR(TAB_E4M3, TAB_E4M3);
@@ -832,8 +841,7 @@ static BlocksPlan blocks_plan(int M, int N, int KB, int sms) {
 int matmul_blocks_dispatch(const MatmulBlocksParams& p, cudaStream_t stream) {
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) == cudaSuccess) cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int sms = blocks_sms();
     // pairs from two rounds of 128 x 128 tiles on: 1536x4096x1024 (384 of them) 15.8, single CTAs 17.1; 4096x1024x1024 (256) 12.4 / 9.9
     const long long tiles128 = ((long long)p.a.rows + 127) / 128 * (((long long)p.b.rows + 127) / 128);
     const int pairs = matmul_pairs();

@@ -1001,8 +1001,9 @@ struct StreamPlan { int ctas, stages; size_t smem; };
 template <auto KERNEL>
 static StreamPlan stream_plan(int each, long long M, size_t row_bytes, size_t fixed) {
     StreamPlan pl = {0, 0, 0};
-    int dev = 0, sms = 148;
-    if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return pl;
+    int dev = 0;
+    const int sms = blocks_sms();
+    if (M < 2LL * sms || cudaGetDevice(&dev) != cudaSuccess) return pl;
     const size_t room = 226 * 1024;
     for (int n = each; n >= 1 && !pl.stages; n--) {                        // each: CTAs an SM holds by its registers
         const size_t share = std::min<size_t>(room, 228 * 1024 / n - 1536);    // less a kilobyte that every CTA is charged and what is static
