@@ -46,21 +46,29 @@ struct Columns {
     int g, C;
     __device__ __forceinline__ int at(int i, int j) const { return VEC ? (i * GT + g) * 8 + j : (i * GT + (g & ~31)) * 8 + j * 32 + (g & 31); }
     __device__ __forceinline__ bool in(int i, int j) const { return at(i, VEC ? 0 : j) < C; }
-    __device__ __forceinline__ void load(const void* p, int type, long long row, int i, float (&v)[8]) const {
-        if (VEC) {
-            load8_any(p, type, row + at(i, 0), in(i, 0) ? 8 : 0, true, v);
-        } else {
+    template <typename T>
+    __device__ __forceinline__ void singles(const T* p, int n, float (&v)[8]) const {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = in(i, j) ? load_any(p, type, row + at(i, j)) : 0.f;
-        }
+        for (int j = 0; j < 8; j++) v[j] = 32 * j < n ? to_float(p[32 * j]) : 0.f;
+    }
+    template <typename T>
+    __device__ __forceinline__ void put(T* p, int n, const float (&v)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; j++) if (32 * j < n) p[32 * j] = from_float<T>(v[j]);
+    }
+    __device__ __forceinline__ void load(const void* p, int type, long long row, int i, float (&v)[8]) const {
+        const int c = at(i, 0);
+        if (VEC) load8_any(p, type, row + c, c < C ? 8 : 0, true, v);
+        else if (type == TAB_FP32) singles(static_cast<const float*>(p) + row + c, C - c, v);
+        else if (type == TAB_BF16) singles(static_cast<const __nv_bfloat16*>(p) + row + c, C - c, v);
+        else singles(static_cast<const __half*>(p) + row + c, C - c, v);
     }
     __device__ __forceinline__ void store(void* p, int type, long long row, int i, const float (&v)[8]) const {
-        if (VEC) {
-            store8_any(p, type, row + at(i, 0), in(i, 0) ? 8 : 0, true, v);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; j++) if (in(i, j)) store_any(p, type, row + at(i, j), v[j]);
-        }
+        const int c = at(i, 0);
+        if (VEC) store8_any(p, type, row + c, c < C ? 8 : 0, true, v);
+        else if (type == TAB_FP32) put(static_cast<float*>(p) + row + c, C - c, v);
+        else if (type == TAB_BF16) put(static_cast<__nv_bfloat16*>(p) + row + c, C - c, v);
+        else put(static_cast<__half*>(p) + row + c, C - c, v);
     }
 };
 
