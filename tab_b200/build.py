@@ -18,7 +18,7 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtab_b200.so")
 SOURCES = ["c_abi.cu", "quantize_sm100.cu", "conv_sm100.cu", "conv_umma_sm100.cu", "umma_probe.cu", "conv_static_sm100.cu", "chain_sm100.cu", "pipe_probe.cu",
-           "quantize_blocks_sm100.cu", "matmul_blocks_sm100.cu", "residual_norm_sm100.cu"]
+           "quantize_blocks_sm100.cu", "matmul_blocks_sm100.cu", "residual_norm_sm100.cu", "residual_norm_backward_sm100.cu"]
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC", "-Xptxas", "-v"]
 
@@ -41,7 +41,7 @@ def build_library(force=False, verbose=False):
     ptxas resource report, which is also kept as ``build/libtab_b200.ptxas.txt``."""
     from concurrent.futures import ThreadPoolExecutor
     srcs = [os.path.join(CSRC, s) for s in SOURCES]
-    hdrs = [os.path.join(CSRC, "tab_kernels.cuh"), os.path.join(CSRC, "umma_common.cuh"), os.path.join(CSRC, "blocks_common.cuh"),
+    hdrs = [os.path.join(CSRC, "tab_kernels.cuh"), os.path.join(CSRC, "umma_common.cuh"), os.path.join(CSRC, "blocks_common.cuh"), os.path.join(CSRC, "residual_norm_common.cuh"),
             os.path.join(ROOT, "include", "tab_b200.h"), __file__]
     objdir = os.path.join(ROOT, "build", "libtab_b200")
     os.makedirs(objdir, exist_ok=True)

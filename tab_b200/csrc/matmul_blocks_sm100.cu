@@ -768,8 +768,8 @@ static int matmul_pairs() {
         for (auto kernel : {matmul_blocks_pair_kernel<TAB_FP32>, matmul_blocks_pair_kernel<TAB_BF16>, matmul_blocks_pair_kernel<TAB_FP16>})
             ok = ok && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PSMEM) == cudaSuccess &&
                  cudaOccupancyMaxActiveClusters(&clusters, kernel, &cfg) == cudaSuccess && clusters >= 1;
-        if (!ok) cudaGetLastError();
-        known[dev] = ok ? clusters + 1 : 1;
+        if (!ok) { cudaGetLastError(); return 0; }                         // (asked again by the next call)
+        known[dev] = clusters + 1;
     }
     return known[dev] - 1;
 }
