@@ -85,13 +85,13 @@ int tab_conv2d_set_path(int path);
    tiles, " +next" when the launch also quantises its result for the next layer.  Static storage per thread. */
 const char* tab_last_conv_kernel(void);
 /*
- * Every wait inside the tensor-core kernel and inside tab_quantize_auto_launch's kernel is bounded; a wait that ran out makes
+ * Every wait inside the tensor-core kernels, tab_quantize_auto_launch's and the residual norms' is bounded; a wait that ran out makes
  * the kernel record a code and return early, leaving its outputs incomplete (a state block is zero again all the same).  From
  * then on the entry points that launch these kernels return TAB_E_STALLED, until this call: it synchronises the current device,
  * returns the code and clears it (0 = none; 11-19: a role of the tensor-core kernel gave up on an mbarrier; 21: the grid-wide
  * meeting point of tab_conv2d_bits_next_launch, whose CTAs - one per SM at most - wait for one another: other work that occupies
  * SMs for a second can cause it; 22: that of tab_quantize_auto_launch, a cooperative launch, whose CTAs run at the same time
- * whatever other streams do).  A non-zero code invalidates the outputs of every launch on the device since the previous call.
+ * whatever other streams do; 31-41: tab_matmul_blocks_launch; 42, 43: tab_residual_norm_launch and its backward form).  A non-zero code invalidates the outputs of every launch on the device since the previous call.
  */
 int tab_device_status(void);
 

@@ -176,7 +176,8 @@ static constexpr int SF_SLOTS = 3;                       // of scale words of 16
 // One CTA: 128 rows of operand R times BN rows of operand C over this rank's share of the sum.  Warp 0 copies the operands, warp 1
 // issues the MMAs, warp 2 brings the scales, warps 4-7 finish.  A cluster shares out the sum: rank r of S takes blocks
 // [r * per, (r+1) * per), the partial results meet in shared memory and every rank adds its share of the columns, in the order of
-// the ranks.  SWAP: R is b, the tile is transposed (few rows of a: the 128-row side of the MMA takes the weights).
+// the ranks.  SWAP: R is b, the tile is transposed (few rows of a: the 128-row side of the MMA takes the weights).  What bounds it is start
+// and end (4 us of a call on next to nothing) and what an SM takes in, 43 to 64 bytes a cycle; us at sizes: see blocks_plan.
 template <int BN, int KS, bool SWAP, int TYPE>
 __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_constant__ CUtensorMap tmR, const __grid_constant__ CUtensorMap tmC, const __grid_constant__ CUtensorMap tmY, BlocksOperand R, BlocksOperand C,
                                                                 void* yv, long long ldy, int KB, int per, int nst, int tiles_c, int split, int tma, int* status) {
@@ -368,6 +369,8 @@ static constexpr int PSMEM = PSTAGES * PSTAGE + PSLOTS * 4 * PSF + 4 * 4096 + 10
 // multiplies for both; each CTA's tensor memory receives the sums of its own 128 rows of a and all 256 of b.  Two accumulators, so
 // that a tile's sums leave while the next tile's are made: 512 columns hold two of 256 and the scales only if the accumulators share
 // some, here 32, which the finishing warps read first and release; from there on the next tile's MMAs may run.
+// 4096x8192x4096 with bf16 results: 104 us in bursts (2.65 PFLOP/s; tensor pipe 68 % busy under the profiler), 127 in loops of a second, where the
+// 1000 W cap sets the clock; 128 x 128 tiles of single CTAs 149.  A CTA takes in 32 KB in the 512 cycles of a stage's MMAs, about all an SM can.
 // group: tiles are taken in bands of so many row blocks, column by column, so that what is in work at a time shares its operands in the L2.
 template <int TYPE>
 __global__ void __launch_bounds__(PT) matmul_blocks_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const __grid_constant__ CUtensorMap tmY, BlocksOperand A, BlocksOperand B,
@@ -573,7 +576,8 @@ static constexpr int VAHEAD = 2;                         // blocks of the sum a 
 // so there is no pipeline through shared and tensor memory, whose start and end cost more than the reading of a few megabytes.  A warp
 // takes 16 rows of b and a share of the sum straight into registers, 16 bytes a lane, and multiplies in fp16, which holds every 8-bit
 // float, with fp32 sums (the sum's order is free as long as both operands agree, so a lane's 16 neighbours serve four MMAs).  A block's
-// sum is added under its scales; the warps' sums are added in their order.
+// sum is added under its scales; the warps' sums are added in their order.  Cold weights: 1x4096x4096 6.1 us (the tile kernel 8.4), 1x8192x8192
+// 16.4 (15.1), 1x1024x4096 4.4 (6.4), 1x512x512 2.1 (4.3); up to 64 rows this way were slower from 16 on (24x4096x4096 10.8, 8.3).
 template <int FA, int FB>
 __global__ void __launch_bounds__(256, 2) matmul_blocks_rows_kernel(BlocksOperand A, BlocksOperand B, void* y, long long ldy, int type, int K, int per) {
     __shared__ float part[8][16][9];

@@ -142,6 +142,8 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------
+// us with weights, gate, residual, bf16: 8192x4096 71 with the sums' launch (403 MB: 5.7 TB/s), 4096x8192 75; centred 130 (five sums over rows leave one
+// CTA of 512 threads on an SM).  One vector a thread and twice the warps: 90.
 // What a row's sums are needed for is read from the ring again behind the meeting instead of being kept: registers are what the sums
 // over rows leave.  FAST: both norms and all gradients, and no gate or one of channels.
 constexpr int backward_threads(int nv, bool layer) { return nv == 1 && !layer ? 1024 : 512; }    // an SM holds, by registers
@@ -455,7 +457,10 @@ template <int TYPE, int THREADS, int NV, bool LAYER, bool TOKEN, bool FAST>
 static int launch_norm_backward_stream_as(NormBackwardParams b, cudaStream_t stream) {
     const NormParams& p = b.f;
     constexpr auto kernel = residual_norm_backward_stream_kernel<TYPE, THREADS, NV, LAYER, TOKEN, FAST>;
-    const StreamPlan pl = stream_plan<kernel>(backward_threads(NV, LAYER) / THREADS, p.M, 4 * (size_t)p.C * type_bytes(TYPE), (p.gkind == TAB_GATE_CHANNEL ? 12 : 8) * (size_t)p.C);
+    // Below two rows an SM the general kernel is as fast (148x4096 8.9 us, this one 10.3; 296: 11.6 / 12.2; 444: 14.2 / 13.9; 2048: 72 / 26); a
+    // CTA has some rows to itself, since its sums are as many bytes as some of them (us at 592x4096 / 2048x1024: 1 row 14.5 / 18.1, 4 rows 16.4 / 15.6).
+    if (p.M < 2LL * blocks_sms()) return TAB_E_TOO_LARGE;
+    const StreamPlan pl = stream_plan<kernel>(backward_threads(NV, LAYER) / THREADS, p.M, p.C <= 2048 ? 4 : 2, 4 * (size_t)p.C * type_bytes(TYPE), (p.gkind == TAB_GATE_CHANNEL ? 12 : 8) * (size_t)p.C);
     if (!pl.stages) return TAB_E_TOO_LARGE;
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;

@@ -227,18 +227,22 @@ static bool norm_vectors(const NormParams& p, int type, int flags) {
 
 // What a stream kernel is launched with: CTAs that are all resident, and rows in flight.
 struct StreamPlan { int ctas, stages; size_t smem; };
-// row_bytes: of one row's tensors; fixed: bytes besides the ring.  0 stages: it does not fit, or there are too few rows to stay for.
+// each: CTAs an SM holds by its registers; rows: least rows of a CTA (fewer CTAs than fit, but one an SM); row_bytes: of one row's tensors;
+// fixed: bytes besides the ring.  0 stages: it does not fit.
 template <auto KERNEL>
-static StreamPlan stream_plan(int each, long long M, size_t row_bytes, size_t fixed) {
+static StreamPlan stream_plan(int each, long long M, int rows, size_t row_bytes, size_t fixed) {
     StreamPlan pl = {0, 0, 0};
     int dev = 0;
     const int sms = blocks_sms();
-    if (M < 2LL * sms || cudaGetDevice(&dev) != cudaSuccess) return pl;
+    if (cudaGetDevice(&dev) != cudaSuccess) return pl;
     const size_t room = 226 * 1024;
-    for (int n = each; n >= 1 && !pl.stages; n--) {                        // each: CTAs an SM holds by its registers
+    for (int n = each; n >= 1 && !pl.stages; n--) {
         const size_t share = std::min<size_t>(room, 228 * 1024 / n - 1536);    // less a kilobyte that every CTA is charged and what is static
         const long long stages = share > fixed ? (long long)((share - fixed) / row_bytes) : 0;
-        if (stages >= 2 && M >= 2LL * n * sms) { pl.stages = (int)std::min<long long>(stages, 4); pl.ctas = std::min(n * sms, NORM_CTAS); }
+        if (stages >= 2) {
+            pl.stages = (int)std::min<long long>(stages, 4);
+            pl.ctas = (int)std::min<long long>(std::min(n * sms, NORM_CTAS), std::max<long long>(sms, M / rows));
+        }
     }
     if (!pl.stages) return pl;
     pl.smem = pl.stages * row_bytes + fixed;
