@@ -524,3 +524,41 @@ def test_empty_rows_and_sums(cuda):
     assert not TAB.matmul_blocks(q, s, q, s).any()
     q, s = TAB.quantize_blocks(torch.randn(0, 128, device=cuda))
     assert q.shape == (0, 128) and s.shape == (0, 1)
+
+
+@pytest.mark.gpu
+def test_single_vectors(cuda):
+    """Tensors of one dimension are one row, through every operator and both directions."""
+    x, w, g = torch.randn(300, device=cuda), torch.randn(130, 300, device=cuda), torch.randn(130, device=cuda)
+    q, s = TAB.quantize_blocks(x)
+    q2, s2 = TAB.quantize_blocks(x[None])
+    wq = TAB.quantize_blocks2d(w)
+    assert q.shape == (300,) and s.shape == (3,) and torch.equal(q.view(torch.uint8), q2[0].view(torch.uint8)) and torch.equal(s.view(torch.uint8), s2[0].view(torch.uint8))
+    assert torch.equal(TAB.matmul_blocks(q, s, *wq), TAB.matmul_blocks(q2, s2, *wq)[0])
+    results = []
+    for v, grad in ((x, g), (x[None], g[None])):
+        leaves = [v.clone().requires_grad_(), w.clone().requires_grad_()]
+        y = tab_nn.block_linear(*leaves)
+        results.append([y.detach().reshape(-1), *(d.reshape(-1) for d in torch.autograd.grad(y, leaves, grad))])
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    p = torch.rand(300, device=cuda)
+    one, many = TAB.residual_norm(x, x, pre_weight=p, gate=p), TAB.residual_norm(x[None], x[None], pre_weight=p, gate=p)
+    assert all(torch.equal(a, b[0]) for a, b in zip(one, many))
+
+
+@pytest.mark.gpu
+def test_weights_changed_between_the_passes(cuda):
+    """The backward pass multiplies what the forward pass did, whatever has become of the weights since; the norms' weights say so."""
+    x, w, g = torch.randn(40, 256, device=cuda, requires_grad=True), torch.randn(64, 256, device=cuda, requires_grad=True), torch.randn(40, 64, device=cuda)
+    want = torch.autograd.grad(tab_nn.block_linear(x, w), (x, w), g)
+    y = tab_nn.block_linear(x, w)
+    with torch.no_grad():
+        w.mul_(3)
+    got = torch.autograd.grad(y, (x, w), g)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    p = torch.rand(256, device=cuda, requires_grad=True)
+    h = tab_nn.residual_norm(x, pre_weight=p)[1]
+    with torch.no_grad():
+        p.mul_(3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        h.sum().backward()

@@ -262,3 +262,46 @@ def test_one_gradient_alone(cuda, shape, only):
         grads.append(torch.autograd.grad(out, leaves[only], (gr.to(cuda), gh.to(cuda)))[0])
     size = float(grads[0].abs().max()) + 30 * (1 if only in ("y", "residual") else shape[0] ** 0.5)
     assert float((grads[0] - grads[1]).abs().max()) <= size * (96 + 4 * shape[0] ** 0.5) * 2.0 ** -24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(9, 100), (700, 1032), (500, 4096), (350, 8192)])
+@pytest.mark.parametrize("kind", ["rms", "layer"])
+@pytest.mark.parametrize("gate", [None, "token", "channel"])
+def test_one_output_alone(cuda, shape, kind, gate):
+    """Gradients of r alone and of h alone add up to those of both (fp32 roundings as counted above, for each of the three)."""
+    t, gr, gh = make(9, shape, "fp32", "fp32", kind, gate, True, True, True)
+    dev = {k: None if v is None else v.to(cuda).requires_grad_() for k, v in t.items() if not k.endswith("bias")}      # (centred norms without shifts, too)
+    leaves = [v for v in dev.values() if v is not None]
+    out = tab_nn.residual_norm(**dev, kind=kind)
+    gr, gh = gr.to(cuda), gh.to(cuda)
+    parts = [torch.autograd.grad(o, leaves, g, retain_graph=True, allow_unused=True) for o, g in zip(out, (gr, gh))]
+    both = torch.autograd.grad(out, leaves, (gr, gh))
+    for a, b, c, leaf in zip(*parts, both, leaves):
+        total = sum(v for v in (a, b) if v is not None)
+        size = float(c.abs().max()) + 30 * (1 if leaf.shape == c.new_empty(shape).shape else max(shape[0], shape[1] if leaf.shape[-1] == 1 else 1) ** 0.5)
+        assert float((total - c).abs().max()) <= 3 * size * (96 + 4 * max(shape) ** 0.5) * 2.0 ** -24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(6, 200), (6, 1032), (400, 4096)])
+@pytest.mark.parametrize("format", ["e4m3", "e5m2"])
+def test_residual_norm_quantized_non_finite(cuda, shape, format):
+    """A NaN voids its row; an infinite weight makes its column infinite (NaN in e4m3) and leaves the other values of the block as they are."""
+    y, w = torch.randn(*shape, device=cuda), torch.rand(shape[1], device=cuda) + 0.5
+    f8 = ref.FORMATS[format][0]
+    _, q0, s0 = TAB.residual_norm(y, pre_weight=w, quantize=f8)
+    bad = y.clone()
+    bad[2, 3] = float("nan")
+    _, q, s = TAB.residual_norm(bad, pre_weight=w, quantize=f8)
+    keep = [i for i in range(shape[0]) if i != 2]
+    bytes_of = lambda t: t.contiguous().view(torch.uint8)
+    assert q[2].float().isnan().all() and torch.equal(bytes_of(q[keep]), bytes_of(q0[keep])) and torch.equal(bytes_of(s[keep]), bytes_of(s0[keep]))
+    w[5] = 0
+    _, q0, s0 = TAB.residual_norm(y, pre_weight=w, quantize=f8)
+    w[5] = float("inf")
+    _, q, s = TAB.residual_norm(y, pre_weight=w, quantize=f8)
+    column = q[:, 5].float()
+    assert (column.isnan() if format == "e4m3" else column.isinf()).all()
+    others = [i for i in range(shape[1]) if i != 5]
+    assert torch.equal(bytes_of(s), bytes_of(s0)) and torch.equal(bytes_of(q)[:, others], bytes_of(q0)[:, others])
