@@ -411,8 +411,9 @@ int tab_quantize_blocks_launch(const void* x, int type, long long ldx, long long
     if ((M > 1 && (ldx < K || (q && ldq < K))) || (qt && K > 1 && ldqt < M)) return TAB_E_BAD_ARGUMENT;
     if ((q && (square ? MB > 1 && lds < KB : KB > 1 && lds < M)) || (qt && (square ? KB > 1 && ldst < MB : MB > 1 && ldst < K))) return TAB_E_BAD_ARGUMENT;
     if (misaligned(x, (uintptr_t)type_bytes(type) - 1)) return TAB_E_ALIGNMENT;
-    // pitches of single rows are of no account; beyond 2^31 rows or 2^40 elements between two of them the index arithmetic ends
-    if (M >= (1LL << 31) || (M > 1 && (ldx >= (1LL << 40) || ldq >= (1LL << 40))) || (K > 1 && ldqt >= (1LL << 40)) || (q && lds >= (1LL << 40)) || (qt && ldst >= (1LL << 40))) return TAB_E_TOO_LARGE;
+    // pitches of single rows are of no account; beyond 2^31 rows, as many elements of a row (rounded up to two blocks) or 2^40 between two rows the
+    // index arithmetic ends
+    if (M >= (1LL << 31) || K > 0x7FFFFF00 || (M > 1 && (ldx >= (1LL << 40) || ldq >= (1LL << 40))) || (K > 1 && ldqt >= (1LL << 40)) || (q && lds >= (1LL << 40)) || (qt && ldst >= (1LL << 40))) return TAB_E_TOO_LARGE;
     QuantBlocksParams p = {x, M > 1 ? ldx : 0, M, K, format, static_cast<uint8_t*>(q), M > 1 ? ldq : 0, q ? s : nullptr, lds,
                            static_cast<uint8_t*>(qt), K > 1 ? ldqt : 0, qt ? st : nullptr, ldst};
     return quantize_blocks_dispatch(p, type, square == 1, reinterpret_cast<cudaStream_t>(stream));

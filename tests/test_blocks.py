@@ -51,6 +51,15 @@ def test_matmul_blocks_refuses(over, code):
     assert _cabi.lib().tab_matmul_blocks_launch(*matmul_args(**over)) == code
 
 
+@pytest.mark.parametrize("K", [2 ** 31 - 1, 2 ** 31 - 255])
+@pytest.mark.parametrize("square", [0, 1])
+def test_quantize_blocks_refuses_rows_beyond_its_indexes(K, square):
+    """Columns are counted in 32 bits, two blocks at a time."""
+    over = dict(K=K, M=1, lds=1 << 25, square=square)
+    assert _cabi.lib().tab_quantize_blocks_launch(*quantize_args(**over)) == -5
+    assert _cabi.lib().tab_quantize_blocks_launch(*quantize_args(**over, qt=BASE, st=BASE, ldqt=16, ldst=1 << 31)) == -5
+
+
 def test_operators_refuse_host_tensors():
     x = torch.zeros(2, 128)
     with pytest.raises(RuntimeError, match="CUDA tensor"):
