@@ -206,7 +206,7 @@ int type_of(const Tensor& t) {
 }
 int type_of(at::ScalarType s) { return s == at::kFloat ? TAB_FP32 : s == at::kBFloat16 ? TAB_BF16 : s == at::kHalf ? TAB_FP16 : -1; }
 int format_of(at::ScalarType s) { return s == at::kFloat8_e4m3fn ? TAB_E4M3 : s == at::kFloat8_e5m2 ? TAB_E5M2 : -1; }
-bool on_cuda(const Tensor& t) { return t.defined() && t.is_cuda(); }
+bool on_cuda(const Tensor& t) { return t.defined() && t.is_cuda() && !t.is_neg(); }      // (a negated view's memory is not its values)
 int64_t blocks(int64_t n) { return (n + 127) / 128; }
 
 // Leading dimensions that are one axis of evenly spaced rows without gaps in them, none of them empty.
@@ -348,6 +348,7 @@ void differentiable_once(torch::autograd::variable_list& grads) {
 }
 Tensor even_rows(const Tensor& g) {
     Rows r;
+    if (g.defined() && g.is_neg()) return g.resolve_neg().contiguous();
     return !g.defined() || g.numel() == 0 || r.of(g) ? g : g.contiguous();
 }
 
@@ -405,7 +406,7 @@ struct Norm {
         a.y = y.data_ptr(); a.ldy = r.pitch; a.type = type_of(y); a.layer = (int)layer; a.alpha = (float)alpha; a.eps = (float)eps; a.M = r.M; a.C = (int)r.K;
         Rows q;
         if (x.defined()) {
-            if (!x.is_cuda() || x.device() != y.device() || x.scalar_type() != y.scalar_type() || x.sizes() != y.sizes() || !q.of(x)) return false;
+            if (!on_cuda(x) || x.device() != y.device() || x.scalar_type() != y.scalar_type() || x.sizes() != y.sizes() || !q.of(x)) return false;
             a.x = x.data_ptr(); a.ldx = q.pitch;
         }
         int ptype = -1;
@@ -413,7 +414,7 @@ struct Norm {
         for (const auto& w : weights) {
             if (!w.t.defined()) continue;
             const int type = type_of(w.t);
-            if (!w.t.is_cuda() || w.t.device() != y.device() || (type != TAB_FP32 && type != a.type) || w.t.dim() != 1 || w.t.size(0) != r.K || !w.t.is_contiguous() ||
+            if (!on_cuda(w.t) || w.t.device() != y.device() || (type != TAB_FP32 && type != a.type) || w.t.dim() != 1 || w.t.size(0) != r.K || !w.t.is_contiguous() ||
                 (ptype >= 0 && ptype != type)) return false;
             *w.p = w.t.data_ptr();
             a.ptype = ptype = type;
@@ -421,7 +422,7 @@ struct Norm {
         if ((a.b1 && !a.w1) || (a.b2 && !a.w2) || (!layer && (a.b1 || a.b2))) return false;
         if (gate.defined()) {
             a.gtype = type_of(gate);
-            if (!gate.is_cuda() || gate.device() != y.device() || (a.gtype != TAB_FP32 && a.gtype != a.type)) return false;
+            if (!on_cuda(gate) || gate.device() != y.device() || (a.gtype != TAB_FP32 && a.gtype != a.type)) return false;
             a.gate = gate.data_ptr();
             if (gate.dim() == 1 && gate.size(0) == r.K && (gate.is_contiguous() || r.K == 1)) {
                 a.gkind = TAB_GATE_CHANNEL;

@@ -194,6 +194,7 @@ class TABConv2d(torch.nn.Module):
 
 def _even_rows(g):
     """A gradient as autograd hands it over (expanded, transposed, ...) with the rows the operators take."""
+    g = g.resolve_neg()
     try:
         ops._rows(g, "grad")
         return g

@@ -431,6 +431,8 @@ def _on_device(t, name, device, types, what):
         raise RuntimeError("%s must be %s, not %s" % (name, what, t.dtype))
     if device is not None and t.device != device:
         raise RuntimeError("%s must be on %s" % (name, device))
+    if t.is_neg():
+        raise RuntimeError("%s must not be a negated view (resolve_neg makes a tensor of it)" % name)
 
 
 def _rows(t, name):

@@ -571,3 +571,22 @@ def test_weights_changed_between_the_passes(cuda):
         p.mul_(3)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         h.sum().backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_negated_views(cuda, monkeypatch, native):
+    """A view whose memory holds the negatives of its values is refused; as a gradient it is resolved."""
+    if not native:
+        monkeypatch.setattr(TAB.ops, "_native", False)
+    x, w, p = torch.randn(5, 256, device=cuda), torch.randn(40, 256, device=cuda), torch.rand(256, device=cuda)
+    n = torch._neg_view(x)
+    for call in (lambda: TAB.quantize_blocks(n), lambda: TAB.quantize_blocks2d(n), lambda: TAB.residual_norm(n, pre_weight=p), lambda: TAB.residual_norm(x, n),
+                 lambda: TAB.residual_norm(x, pre_weight=torch._neg_view(p)), lambda: TAB.residual_norm(x, gate=n), lambda: tab_nn.block_linear(x, torch._neg_view(w))):
+        with pytest.raises(RuntimeError, match="negated"):
+            call()
+    leaves = [x.requires_grad_(), w.requires_grad_(), p.requires_grad_()]
+    g, gh = torch.randn(5, 40, device=cuda), torch.randn(5, 256, device=cuda)
+    for of, grad, result in ((leaves[:2], g, lambda: tab_nn.block_linear(x, w)), (leaves[::2], gh, lambda: tab_nn.residual_norm(x, pre_weight=p)[1])):
+        got, want = (torch.autograd.grad(result(), of, v) for v in (torch._neg_view(grad), -grad))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
