@@ -352,6 +352,15 @@ Tensor even_rows(const Tensor& g) {
     return !g.defined() || g.numel() == 0 || r.of(g) ? g : g.contiguous();
 }
 
+// Kept values as matmul_any takes them: hooks on saved tensors (which keep them on the host, say) may hand them back without the bytes between rows.
+Tensor aligned_rows(const Tensor& q) {
+    Rows r;
+    if (!q.defined() || !r.of(q) || ((r.M == 1 || r.pitch % 16 == 0) && reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0)) return q;
+    Tensor o = new_blocks(q, q.sizes(), r.K, q.scalar_type());
+    o.view(at::kByte).copy_(q.view(at::kByte));
+    return o;
+}
+
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -376,8 +385,8 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
         const Tensor g = even_rows(grads[0].detach());
         Quantized q;
         bool ok = quantize_any(g, (at::ScalarType)types[2], need_w, false, q);
-        if (ok && need_x) ok = matmul_any(q.q, q.s, saved[2], saved[3], (at::ScalarType)types[0], out[0]);
-        if (ok && need_w) ok = matmul_any(q.qt, q.st, saved[0], saved[1], (at::ScalarType)types[1], out[1]);
+        if (ok && need_x) ok = matmul_any(q.q, q.s, aligned_rows(saved[2]), saved[3], (at::ScalarType)types[0], out[0]);
+        if (ok && need_w) ok = matmul_any(q.qt, q.st, aligned_rows(saved[0]), saved[1], (at::ScalarType)types[1], out[1]);
         TORCH_CHECK(ok, "block_linear: a launch of the backward pass failed [cudaError ", tab_last_cuda_error(), "]");
         differentiable_once(out);
         return out;

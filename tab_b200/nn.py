@@ -225,8 +225,8 @@ class _BlockLinear(torch.autograd.Function):
     def backward(ctx, grad):
         xt, xts, wt, wts = ctx.saved_tensors
         g = ops.quantize_blocks(_even_rows(grad.detach()), ctx.grad_dtype, columns=xt is not None)
-        dx = None if wt is None else ops.matmul_blocks(*g[:2], wt, wts, out_dtype=ctx.types[0])
-        dw = None if xt is None else ops.matmul_blocks(*g[2:], xt, xts, out_dtype=ctx.types[1])
+        dx = None if wt is None else ops.matmul_blocks(*g[:2], ops._aligned_rows(wt), wts, out_dtype=ctx.types[0])
+        dw = None if xt is None else ops.matmul_blocks(*g[2:], ops._aligned_rows(xt), xts, out_dtype=ctx.types[1])
         return *_differentiable_once((dx, dw)), None, None
 
 

@@ -462,6 +462,16 @@ def _new_blocks(shape, rows, n, dtype, device):
     return held[:, :n].view(shape)
 
 
+def _aligned_rows(q):
+    """8-bit values with every row starting on 16 bytes: ``q`` itself, or a copy of one that was copied without the bytes between its rows."""
+    M, K, ld = _rows(q, "values")
+    if q.numel() == 0 or (q.data_ptr() % 16 == 0 and (M == 1 or ld % 16 == 0)):
+        return q
+    new = _new_blocks(tuple(q.shape), M, K, q.dtype, q.device)
+    new.view(torch.uint8).copy_(q.view(torch.uint8))
+    return new
+
+
 def _new_scales(shape, rows, n, device):
     """Scales ``shape`` (``rows`` x ``n``) that lie block by block: a quantiser's CTA, which has one block of many rows, writes them side by
     side, and so the product reads them."""

@@ -1,4 +1,6 @@
 """8-bit block quantisers and the block-scaled product: what is refused (no GPU), and the results against 64-bit references."""
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -590,3 +592,17 @@ def test_negated_views(cuda, monkeypatch, native):
     for of, grad, result in ((leaves[:2], g, lambda: tab_nn.block_linear(x, w)), (leaves[::2], gh, lambda: tab_nn.residual_norm(x, pre_weight=p)[1])):
         got, want = (torch.autograd.grad(result(), of, v) for v in (torch._neg_view(grad), -grad))
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_tensors_kept_on_the_host(cuda, monkeypatch, native):
+    """What the forward passes keep may be copied to the host and back, where rows of odd lengths lose the bytes between them."""
+    if not native:
+        monkeypatch.setattr(TAB.ops, "_native", False)
+    x, w, p, g = torch.randn(37, 100, device=cuda, requires_grad=True), torch.randn(51, 100, device=cuda, requires_grad=True), torch.rand(100, device=cuda, requires_grad=True), torch.randn(37, 51, device=cuda)
+    def grads(outside):
+        with outside:
+            y = tab_nn.block_linear(tab_nn.residual_norm(x, x, pre_weight=p, gate=x)[1], w)
+        return torch.autograd.grad(y, (x, w, p), g)
+    assert all(torch.equal(a, b) for a, b in zip(grads(contextlib.nullcontext()), grads(torch.autograd.graph.save_on_cpu())))
