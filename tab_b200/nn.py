@@ -253,8 +253,15 @@ class BlockLinear(torch.nn.Module):
             raise ValueError("Wq must be [N, K] and Ws [ceil(N/128) or N, ceil(K/128)]")
         self.N, self.K = (int(v) for v in Wq.shape)
         self.out_dtype = out_dtype
-        self.register_buffer("Wq", Wq)
+        self.register_buffer("Wq", ops._aligned_rows(Wq) if Wq.dtype in ops._FORMATS else Wq)
         self.register_buffer("Ws", Ws)
+
+    def _apply(self, fn, recurse=True):
+        # As bytes: half() and the like are for values, which these only become with their scales; a copy may lose the rows' starts.
+        super()._apply(lambda t: fn(t.view(torch.uint8)).view(t.dtype) if t.dtype.itemsize == 1 else fn(t), recurse)
+        if self.Wq.dtype in ops._FORMATS:
+            self.Wq = ops._aligned_rows(self.Wq)
+        return self
 
     @classmethod
     def from_float(cls, weight, dtype=torch.float8_e4m3fn, out_dtype=torch.bfloat16):

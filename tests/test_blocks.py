@@ -1,5 +1,6 @@
 """8-bit block quantisers and the block-scaled product: what is refused (no GPU), and the results against 64-bit references."""
 import contextlib
+import copy
 
 import numpy as np
 import pytest
@@ -441,6 +442,27 @@ def test_second_derivatives_are_refused(cuda, monkeypatch, native):
         g, = torch.autograd.grad(y.sum(), x, create_graph=True)
         with pytest.raises(RuntimeError, match="differentiable"):
             g.sum().backward()
+
+
+@pytest.mark.parametrize("K", [100, 256])
+def test_block_linear_module_on_the_host(K):
+    """Changes of type leave 8-bit values and scales as they are, from tensors without gaps between rows too, and rows start on 16 bytes."""
+    wq, ws = torch.randint(0, 127, (40, K), dtype=torch.uint8), torch.randint(100, 140, (1, -(-K // 128)), dtype=torch.uint8)
+    m = tab_nn.BlockLinear(wq.view(torch.float8_e4m3fn), ws.view(torch.float8_e8m0fnu))
+    for change in (lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: torch.nn.Sequential(m).double()[0], lambda m: m.cpu(), copy.deepcopy):
+        m = change(m)
+        assert m.Wq.dtype == torch.float8_e4m3fn and m.Ws.dtype == torch.float8_e8m0fnu and m.Wq.stride(0) % 16 == 0 and m.Wq.data_ptr() % 16 == 0
+        assert torch.equal(m.Wq.view(torch.uint8), wq) and torch.equal(m.Ws.view(torch.uint8), ws)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K", [100, 256])
+def test_block_linear_module_moves(cuda, K):
+    w, x = torch.randn(70, K, device=cuda), torch.randn(9, K, device=cuda)
+    m = tab_nn.BlockLinear.from_float(w)
+    want = m(x)
+    m = torch.nn.Sequential(m).half().cpu().cuda()[0]
+    assert want.dtype == torch.bfloat16 and torch.equal(m(x), want) and torch.equal(tab_nn.BlockLinear(m.Wq.contiguous(), m.Ws)(x), want)
 
 
 # ---- together, as they are used ---------------------------------------------------------------------------------------
