@@ -236,8 +236,10 @@ def block_linear(x, weight, out_dtype=None, grad_dtype=torch.float8_e4m3fn):
 
     Its gradients are products of the same kind, with the gradient ``g`` of the result rounded to ``grad_dtype``: ``g`` (along its rows) times the
     rounded weights for ``x``, and ``g`` and ``x`` (both along their columns, i.e. over the rows that this product sums) for ``weight``, in the
-    types of ``x`` and ``weight``.  The rounding itself counts as the identity.  For the backward pass 8-bit copies are kept, not ``x`` and ``weight``."""
+    types of ``x`` and ``weight``.  None of the sums may be longer than 2^24.  The rounding itself counts as the identity.  For the backward pass 8-bit copies are kept, not ``x`` and ``weight``."""
     out_dtype = x.dtype if out_dtype is None else out_dtype
+    if max(x.shape[:-1].numel(), 0, *weight.shape) > 1 << 24:
+        raise RuntimeError("block_linear: products sum at most 2^24 elements; the gradients' sums run over the rows of x and of weight")
     y = ops._try("block_linear", x, weight, out_dtype, grad_dtype)
     return _BlockLinear.apply(x, weight, out_dtype, grad_dtype) if y is None else y
 

@@ -63,6 +63,13 @@ def test_quantize_blocks_refuses_rows_beyond_its_indexes(K, square):
     assert _cabi.lib().tab_quantize_blocks_launch(*quantize_args(**over, qt=BASE, st=BASE, ldqt=16, ldst=1 << 31)) == -5
 
 
+@pytest.mark.parametrize("x, w", [((2 ** 24 + 1, 2), (3, 2)), ((4096, 4097, 2), (3, 2)), ((3, 2), (2 ** 24 + 1, 2)), ((1, 2 ** 24 + 1), (1, 2 ** 24 + 1))])
+def test_block_linear_refuses_longer_sums(x, w):
+    """Before the forward pass, not in the backward pass that would need them."""
+    with pytest.raises(RuntimeError, match="2\\^24"):
+        tab_nn.block_linear(torch.zeros(1).expand(x), torch.zeros(1).expand(w))
+
+
 def test_operators_refuse_host_tensors():
     x = torch.zeros(2, 128)
     with pytest.raises(RuntimeError, match="CUDA tensor"):
@@ -628,3 +635,36 @@ def test_tensors_kept_on_the_host(cuda, monkeypatch, native):
             y = tab_nn.block_linear(tab_nn.residual_norm(x, x, pre_weight=p, gate=x)[1], w)
         return torch.autograd.grad(y, (x, w, p), g)
     assert all(torch.equal(a, b) for a, b in zip(grads(contextlib.nullcontext()), grads(torch.autograd.graph.save_on_cpu())))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [2, 40, 200, 2304])
+def test_matmul_blocks_values_behind_the_sum(cuda, M):
+    """Sums that end inside a block, and inside sixteen bytes, with NaN and live values right behind them in memory."""
+    rng = np.random.default_rng(M)
+    N, K, end = (1300 if M > 1000 else 300), 512, 401
+    a, b = random_blocks(rng, M, K, "e4m3", False, True), random_blocks(rng, N, K, "e4m3", True, True)
+    (qa, sa), (qb, sb) = device_blocks(cuda, *a, "e4m3"), device_blocks(cuda, *b, "e4m3")
+    va, vb = ref.values(*a, "e4m3")[:, 128:end], ref.values(*b, "e4m3")[:, 128:end]
+    for q in (qa, qb):
+        q.view(torch.uint8)[:, end::2] = 0x7F
+    y = TAB.matmul_blocks(qa[:, 128:end], sa[:, 1:4], qb[:, 128:end], sb[:, 1:4], out_dtype=torch.float32)
+    assert np.array_equal(y.cpu().numpy(), va @ vb.T)
+
+
+@pytest.mark.gpu
+def test_the_same_leaf_twice(cuda):
+    """One tensor in several places has the sum of their gradients (fp32, of terms below 2^6: roundings of three sums)."""
+    x, p = torch.randn(33, 200, device=cuda, requires_grad=True), torch.rand(200, device=cuda, requires_grad=True)
+    gr, gh = torch.randn(33, 200, device=cuda), torch.randn(33, 200, device=cuda)
+    one = torch.autograd.grad(tab_nn.residual_norm(x, x, pre_weight=p, post_weight=p, gate=x), (x, p), (gr, gh))
+    xs, ps = [x.detach().clone().requires_grad_() for _ in range(3)], [p.detach().clone().requires_grad_() for _ in range(2)]
+    each = torch.autograd.grad(tab_nn.residual_norm(xs[0], xs[1], pre_weight=ps[0], post_weight=ps[1], gate=xs[2]), xs + ps, (gr, gh))
+    for got, parts in zip(one, (each[:3], each[3:])):
+        size = sum(t.abs() for t in parts)
+        assert bool(((got - sum(parts)).abs() <= size * 4 * 2.0 ** -24).all())
+    w = torch.randn(200, 200, device=cuda, requires_grad=True)
+    both, = torch.autograd.grad(tab_nn.block_linear(w, w), w, torch.ones(200, 200, device=cuda))
+    ws = [w.detach().clone().requires_grad_() for _ in range(2)]
+    parts = torch.autograd.grad(tab_nn.block_linear(*ws), ws, torch.ones(200, 200, device=cuda))
+    assert torch.equal(both, parts[0] + parts[1])
