@@ -65,14 +65,19 @@ struct ScaleLoader {
         if (layout == 1) {
             const int row = row0 + 4 * lane, n = o.rows - row;
             const uint8_t* s = o.s + row + (long long)kb * o.sk;
+            if (n >= 4) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                if (kb + i >= kb1 || n <= 0) continue;
-                if (n >= 4) {
-                    w[i] = *reinterpret_cast<const uint32_t*>(s + i * o.sk);
-                } else {
-                    for (int j = 0; j < n; j++) w[i] = (w[i] & ~(0xFFu << (8 * j))) | (uint32_t)s[i * o.sk + j] << (8 * j);
+                for (int i = 0; i < 16; i++) if (kb + i < kb1) w[i] = *reinterpret_cast<const uint32_t*>(s + i * o.sk);
+            } else if (n > 0) {                                            // the last one to three rows: all loads before the first of them is used
+                uint32_t two[16], one[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    two[i] = one[i] = 0x7F7Fu;
+                    if (kb + i < kb1 && n >= 2) two[i] = *reinterpret_cast<const uint16_t*>(s + i * o.sk);
+                    if (kb + i < kb1 && n != 2) one[i] = s[i * o.sk + n - 1] | 0x7F00u;
                 }
+#pragma unroll
+                for (int i = 0; i < 16; i++) w[i] = n == 1 ? one[i] | 0x7F7F0000u : two[i] | one[i] << 16;
             }
             return;
         }
