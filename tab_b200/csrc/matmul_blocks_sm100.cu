@@ -47,7 +47,8 @@ __device__ __forceinline__ float ld_cluster_f32(uint32_t addr, uint32_t rank) {
 // The scales of 16 blocks from kb on of the 128 rows from row0 on, brought from memory by a warp (load), and written to shared memory as
 // the tensor memory wants them, four blocks a time (store).  127 = 2^0 stands where there is no block or row; only blocks below kb1
 // are read.  A load takes longer than the MMAs of four blocks when the operands' copies fill the memory system, hence 16 at a time.
-//   layout 1     block by block, as the quantiser writes them (sr == 1): lane l holds rows 4l .. 4l+3, a word for each block
+//   layout 1     block by block, as the quantiser writes them (sr == 1): lane l holds rows 4l .. 4l+3, a word for each block (for the last
+//                one to three rows too: their bytes one by one, or block after block, 511x777x4000 18.6 us, this way 11.6)
 //   layout 16, 4 row by row (sk == 1), 16 or 4 scales of a row one aligned vector or word; 0: bytes of any strides; a square's scale serves
 //                all rows.  Lane l holds rows l, l + 32, l + 64, l + 96, a word for four blocks.
 struct ScaleLoader {
@@ -55,7 +56,7 @@ struct ScaleLoader {
     uint32_t w[16];
     __device__ __forceinline__ ScaleLoader(const BlocksOperand& o, int kb0) {
         const uintptr_t at = reinterpret_cast<uintptr_t>(o.s);
-        if (o.shift == 0 && o.sr == 1 && (at & 3) == 0 && o.sk % 4 == 0) layout = 1;
+        if (o.shift == 0 && o.sr == 1 && (at & 3) == 0 && o.sk % 4 == 0 && o.sk >= ((long long)o.rows + 3) / 4 * 4) layout = 1;
         else if (o.sk != 1) layout = 0;
         else layout = ((at | (uintptr_t)o.sr | (uintptr_t)kb0) & 15) == 0 ? 16 : ((at | (uintptr_t)o.sr | (uintptr_t)kb0) & 3) == 0 ? 4 : 0;
     }
@@ -65,20 +66,21 @@ struct ScaleLoader {
         if (layout == 1) {
             const int row = row0 + 4 * lane, n = o.rows - row;
             const uint8_t* s = o.s + row + (long long)kb * o.sk;
-            if (n >= 4) {
+            if (n <= 0) return;
+            // A word that holds the last one to three rows reaches into the bytes before the next block's, and is cut to size; behind the last
+            // block there need be none.
+            const int whole = n >= 4 ? kb1 : kb1 - 1;
 #pragma unroll
-                for (int i = 0; i < 16; i++) if (kb + i < kb1) w[i] = *reinterpret_cast<const uint32_t*>(s + i * o.sk);
-            } else if (n > 0) {                                            // the last one to three rows: all loads before the first of them is used
-                uint32_t two[16], one[16];
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    two[i] = one[i] = 0x7F7Fu;
-                    if (kb + i < kb1 && n >= 2) two[i] = *reinterpret_cast<const uint16_t*>(s + i * o.sk);
-                    if (kb + i < kb1 && n != 2) one[i] = s[i * o.sk + n - 1] | 0x7F00u;
-                }
-#pragma unroll
-                for (int i = 0; i < 16; i++) w[i] = n == 1 ? one[i] | 0x7F7F0000u : two[i] | one[i] << 16;
+            for (int i = 0; i < 16; i++) if (kb + i < whole) w[i] = *reinterpret_cast<const uint32_t*>(s + i * o.sk);
+            if (n >= 4) return;
+            uint32_t end = 0x7F7F7F7Fu;
+            if (kb1 - kb <= 16) {
+                const uint8_t* e = o.s + row + (long long)whole * o.sk;
+                end = (uint32_t)e[0] | (uint32_t)(n > 1 ? e[1] : 127) << 8 | (uint32_t)(n > 2 ? e[2] : 127) << 16;
             }
+            const uint32_t keep = 0xFFFFFFu >> (8 * (3 - n));
+#pragma unroll
+            for (int i = 0; i < 16; i++) w[i] = ((kb + i == whole ? end : w[i]) & keep) | (0x7F7F7F7Fu & ~keep);
             return;
         }
 #pragma unroll

@@ -668,3 +668,17 @@ def test_the_same_leaf_twice(cuda):
     ws = [w.detach().clone().requires_grad_() for _ in range(2)]
     parts = torch.autograd.grad(tab_nn.block_linear(*ws), ws, torch.ones(200, 200, device=cuda))
     assert torch.equal(both, parts[0] + parts[1])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M, N, K", [(3, 130, 2300), (41, 130, 2300), (133, 299, 2300), (2303, 1301, 2300)])
+def test_matmul_blocks_scales_shared_by_blocks(cuda, M, N, K):
+    """One scale for all blocks of a row, and scales block by block without a gap behind the last row: exact, as in test_matmul_blocks_exact."""
+    rng = np.random.default_rng(M)
+    a, b = random_blocks(rng, M, K, "e4m3", False, True), random_blocks(rng, N, K, "e4m3", False, True)
+    (qa, sa), (qb, sb) = device_blocks(cuda, *a, "e4m3"), device_blocks(cuda, *b, "e4m3")
+    f64 = lambda q, s: torch.from_numpy(ref.values(q, s, "e4m3")).to(cuda)
+    row = sa.view(torch.uint8)[:, 3].contiguous()[:, None].expand(sa.shape).view(torch.float8_e8m0fnu)
+    close = sb.view(torch.uint8).t().contiguous().t().view(torch.float8_e8m0fnu)
+    want = f64(a[0], np.repeat(a[1][:, 3:4], a[1].shape[1], 1)) @ f64(*b).t()
+    assert torch.equal(TAB.matmul_blocks(qa, row, qb, close, out_dtype=torch.float32).double(), want)
