@@ -299,7 +299,7 @@ enum { TAB_E4M3 = 0, TAB_E5M2 = 1 };                   /* formats of 8-bit float
  *                 qt [K][M], pitch ldqt, the scale of column k, block j at st[j * ldst + k].
  *   square == 1   blocks of 128 x 128: q [M][K], s [ceil(M/128)][ceil(K/128)], pitch lds, and / or their transposes qt [K][M],
  *                 st [ceil(K/128)][ceil(M/128)], pitch ldst (either pair may be NULL).
- * The last block of an axis may be short.  Bytes between rows are not written.
+ * The last block of an axis may be short.  Bytes between rows are not written.  M < 2^31, K <= 2^31 - 256.
  */
 int tab_quantize_blocks_launch(const void* x, int type, long long ldx, long long M, int K, int format, int square,
                                void* q, long long ldq, uint8_t* s, long long lds, void* qt, long long ldqt, uint8_t* st, long long ldst,
