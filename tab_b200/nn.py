@@ -240,6 +240,8 @@ def block_linear(x, weight, out_dtype=None, grad_dtype=torch.float8_e4m3fn):
     out_dtype = x.dtype if out_dtype is None else out_dtype
     if max(x.shape[:-1].numel(), 0, *weight.shape) > 1 << 24:
         raise RuntimeError("block_linear: products sum at most 2^24 elements; the gradients' sums run over the rows of x and of weight")
+    if grad_dtype not in ops._FORMATS or out_dtype not in ops._TYPES:
+        raise RuntimeError("block_linear: grad_dtype must be torch.float8_e4m3fn or torch.float8_e5m2, out_dtype torch.float32, torch.bfloat16 or torch.float16")
     y = ops._try("block_linear", x, weight, out_dtype, grad_dtype)
     return _BlockLinear.apply(x, weight, out_dtype, grad_dtype) if y is None else y
 
@@ -312,6 +314,8 @@ def residual_norm(y, residual=None, pre_weight=None, pre_bias=None, post_weight=
                   kind="rms", eps=1e-6):
     """``ops.residual_norm`` with gradients: returns ``(r, h)``.  Gradients go to ``y``, ``residual``, the weights, the biases and the gate;
     that of a weight or of a gate ``[C]`` is summed over the rows in a fixed order, so that the same inputs give the same bits."""
+    if isinstance(residual_scale, torch.Tensor) and residual_scale.requires_grad:
+        raise RuntimeError("residual_scale is a number without a gradient; a learned factor is a gate")
     done = ops._try("residual_norm_grad", y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps)
     if done is not None:
         return done

@@ -70,6 +70,13 @@ def test_block_linear_refuses_longer_sums(x, w):
         tab_nn.block_linear(torch.zeros(1).expand(x), torch.zeros(1).expand(w))
 
 
+def test_block_linear_refuses_types_before_the_backward_pass():
+    x = torch.zeros(2, 128)
+    for over in (dict(grad_dtype=torch.float8_e4m3fnuz), dict(grad_dtype=torch.bfloat16), dict(out_dtype=torch.float64)):
+        with pytest.raises(RuntimeError, match="grad_dtype must be"):
+            tab_nn.block_linear(x, x, **over)
+
+
 def test_operators_refuse_host_tensors():
     x = torch.zeros(2, 128)
     with pytest.raises(RuntimeError, match="CUDA tensor"):

@@ -44,6 +44,12 @@ def test_residual_norm_backward_refuses(over, f, code):
     assert _cabi.lib().tab_residual_norm_backward_launch(ctypes.byref(b), None) == code
 
 
+def test_learned_factor_of_the_residual_is_refused():
+    x = torch.zeros(2, 128)
+    with pytest.raises(RuntimeError, match="residual_scale"):
+        tab_nn.residual_norm(x, x, pre_weight=x[0], residual_scale=torch.ones((), requires_grad=True))
+
+
 def test_workspace_and_host_tensors():
     l = _cabi.lib()
     assert l.tab_residual_norm_workspace_bytes(0, 5) == 0 and l.tab_residual_norm_workspace_bytes(5, 16385) == 0
