@@ -83,33 +83,40 @@ struct ScaleLoader {
             for (int i = 0; i < 16; i++) w[i] = ((kb + i == whole ? end : w[i]) & keep) | (0x7F7F7F7Fu & ~keep);
             return;
         }
+        const int row = row0 + (o.shift ? 0 : lane), left = kb1 - kb, whole = layout >= 4 ? min(left >> 2, 4) : 0;      // words of four blocks that there are
+        const uint8_t* s = o.s + (long long)(row >> o.shift) * o.sr + (long long)kb * o.sk;
+        const long long step = 32 * o.sr;
+        if (layout == 16 && whole == 4) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int row = o.shift ? row0 : row0 + i * 32 + lane;
-            if (i > 0 && o.shift) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) w[4 * i + j] = w[j];
-                continue;
-            }
-            if (row >= o.rows) continue;
-            const uint8_t* s = o.s + (long long)(row >> o.shift) * o.sr + (long long)kb * o.sk;
-            if (layout == 16 && kb + 16 <= kb1) {
-                const uint4 u = *reinterpret_cast<const uint4*>(s);
+            for (int i = 0; i < 4; i++) {
+                if ((i > 0 && o.shift) || row + 32 * i >= o.rows) continue;
+                const uint4 u = *reinterpret_cast<const uint4*>(s + i * step);
                 w[4 * i] = u.x; w[4 * i + 1] = u.y; w[4 * i + 2] = u.z; w[4 * i + 3] = u.w;
-                continue;
             }
+        } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                if (layout >= 4 && kb + 4 * j + 4 <= kb1) {
-                    w[4 * i + j] = reinterpret_cast<const uint32_t*>(s)[j];
-                } else if (kb + 4 * j < kb1) {
-                    uint32_t v = 0;
+            for (int i = 0; i < 4; i++)
 #pragma unroll
-                    for (int b = 0; b < 4; b++) v |= (kb + 4 * j + b < kb1 ? (uint32_t)s[(4 * j + b) * o.sk] : 127u) << (8 * b);
-                    w[4 * i + j] = v;
+                for (int j = 0; j < 4; j++)
+                    if (j < whole && !(i > 0 && o.shift) && row + 32 * i < o.rows) w[4 * i + j] = reinterpret_cast<const uint32_t*>(s + i * step)[j];
+            if (4 * whole < min(left, 16)) {                               // byte by byte
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if ((i > 0 && o.shift) || row + 32 * i >= o.rows) continue;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        if (j < whole || 4 * j >= left) continue;
+                        uint32_t v = 0;
+#pragma unroll
+                        for (int b = 0; b < 4; b++) v |= (4 * j + b < left ? (uint32_t)s[i * step + (4 * j + b) * o.sk] : 127u) << (8 * b);
+                        w[4 * i + j] = v;
+                    }
                 }
             }
         }
+        if (o.shift)
+#pragma unroll
+            for (int i = 4; i < 16; i++) w[i] = w[i & 3];
     }
     // The words of blocks 4j .. 4j+3: row r at at + (r % 32) * 16 + (r / 32) * 4.
     __device__ __forceinline__ void store(uint32_t at, int j, int lane) const {
