@@ -584,16 +584,18 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 }
 
 static constexpr int VMOST = 8;                          // rows of a
-static constexpr int VAHEAD = 2;                         // blocks of the sum a warp has under way
 
 // At most eight rows of a against all of b: every weight is read once and multiplied so few times that nothing but the reading counts,
 // so there is no pipeline through shared and tensor memory, whose start and end cost more than the reading of a few megabytes.  A warp
 // takes 16 rows of b and a share of the sum straight into registers, 16 bytes a lane, and multiplies in fp16, which holds every 8-bit
 // float, with fp32 sums (the sum's order is free as long as both operands agree, so a lane's 16 neighbours serve four MMAs).  A block's
-// sum is added under its scales; the warps' sums are added in their order.  Cold weights: 1x4096x4096 6.1 us (the tile kernel 8.4), 1x8192x8192
-// 16.4 (15.1), 1x1024x4096 4.4 (6.4), 1x512x512 2.1 (4.3); up to 64 rows this way were slower from 16 on (24x4096x4096 10.8, 8.3).
-template <int FA, int FB>
-__global__ void __launch_bounds__(256, 2) matmul_blocks_rows_kernel(BlocksOperand A, BlocksOperand B, void* y, long long ldy, int type, int K, int per) {
+// sum is added under its scales; the warps' sums are added in their order.  CTAS on an SM: two with two blocks of the sum under way in each warp
+// while that is all of b, else four with one, which leave fewer SMs idle at the end (cold weights, us, two / four): 1x1024x4096 4.1 / 5.4,
+// 1x4096x4096 5.8 / 6.4 (the tile kernel 7.3), 1x8192x8192 16.1 / 14.7 (19.4), 1x32000x4096 28.5 / 24.8 (5.3 TB/s; 26.2), 1x6000x2000 9.3 / 7.2.
+// Up to 64 rows of a this way were slower from 16 on (24x4096x4096 10.8, 8.3).
+template <int FA, int FB, int CTAS>
+__global__ void __launch_bounds__(256, CTAS) matmul_blocks_rows_kernel(BlocksOperand A, BlocksOperand B, void* y, long long ldy, int type, int K, int per) {
+    constexpr int VAHEAD = 4 / CTAS;                                       // blocks of the sum a warp has under way
     __shared__ float part[8][16][9];
     pdl_wait();
     pdl_launch_dependents();
@@ -652,7 +654,7 @@ __global__ void __launch_bounds__(256, 2) matmul_blocks_rows_kernel(BlocksOperan
         kb += N;
     };
     while (kb + VAHEAD <= whole) several(std::integral_constant<int, VAHEAD>());
-    while (kb < whole) several(std::integral_constant<int, 1>());
+    if (VAHEAD > 1) while (kb < whole) several(std::integral_constant<int, 1>());
     if (kb < kb1) {                                                        // the row's last, short block
         uint4 w[2][2], v[2];
         int sb[2], sa[2];
@@ -811,7 +813,9 @@ static int launch_rows(const MatmulBlocksParams& p, cudaStream_t stream) {
     const int warps = 8;
     const int per = (KB + warps - 1) / warps;
     g_last.kind = 1;
-#define TAB_MR(FA, FB) launch_pdl(matmul_blocks_rows_kernel<FA, FB>, dim3(grid), dim3(32 * warps), 0, stream, p.a, p.b, p.y, p.ldy, p.type, p.K, per)
+    const bool one_round = (long long)grid <= 2LL * blocks_sms();
+#define TAB_MR(FA, FB) (one_round ? launch_pdl(matmul_blocks_rows_kernel<FA, FB, 2>, dim3(grid), dim3(32 * warps), 0, stream, p.a, p.b, p.y, p.ldy, p.type, p.K, per) \
+                                  : launch_pdl(matmul_blocks_rows_kernel<FA, FB, 4>, dim3(grid), dim3(32 * warps), 0, stream, p.a, p.b, p.y, p.ldy, p.type, p.K, per))
     if (p.a.format == TAB_E5M2) return p.b.format == TAB_E5M2 ? TAB_MR(TAB_E5M2, TAB_E5M2) : TAB_MR(TAB_E5M2, TAB_E4M3);
     return p.b.format == TAB_E5M2 ? TAB_MR(TAB_E4M3, TAB_E5M2) : TAB_MR(TAB_E4M3, TAB_E4M3);
 #undef TAB_MR

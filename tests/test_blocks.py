@@ -689,3 +689,15 @@ def test_matmul_blocks_scales_shared_by_blocks(cuda, M, N, K):
     close = sb.view(torch.uint8).t().contiguous().t().view(torch.float8_e8m0fnu)
     want = f64(a[0], np.repeat(a[1][:, 3:4], a[1].shape[1], 1)) @ f64(*b).t()
     assert torch.equal(TAB.matmul_blocks(qa, row, qb, close, out_dtype=torch.float32).double(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("formats", [("e4m3", "e4m3"), ("e5m2", "e4m3"), ("e4m3", "e5m2"), ("e5m2", "e5m2")])
+@pytest.mark.parametrize("M, N, K", [(1, 6000, 2000), (8, 4753, 1100), (3, 16390, 200), (5, 20001, 16)])
+def test_matmul_blocks_few_rows_many_columns(cuda, M, N, K, formats):
+    """More columns than the SMs take at once: exact, as in test_matmul_blocks_exact."""
+    rng = np.random.default_rng(N)
+    fa, fb = formats
+    a, b = random_blocks(rng, M, K, fa, False, True), random_blocks(rng, N, K, fb, True, True)
+    y = TAB.matmul_blocks(*device_blocks(cuda, *a, fa), *device_blocks(cuda, *b, fb), out_dtype=torch.float32)
+    assert np.array_equal(y.cpu().numpy(), ref.values(*a, fa) @ ref.values(*b, fb).T)
