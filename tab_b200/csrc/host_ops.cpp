@@ -209,27 +209,43 @@ int format_of(at::ScalarType s) { return s == at::kFloat8_e4m3fn ? TAB_E4M3 : s 
 bool on_cuda(const Tensor& t) { return t.defined() && t.is_cuda() && !t.is_neg(); }      // (a negated view's memory is not its values)
 int64_t blocks(int64_t n) { return (n + 127) / 128; }
 
+// The dimensions before the last one as one axis: its length and the distance of its places, which stays as it is where there is at most one.  A
+// distance of 0 (a broadcast dimension) is one like any other, hence the word of its own for having met a dimension.
+bool leading_axis(const Tensor& t, int64_t& length, int64_t& distance) {
+    bool met = false;
+    int64_t step = 0;                                                      // what the next (outer) dimension must be apart
+    const auto sizes = t.sizes(), strides = t.strides();
+    length = 1;
+    for (int64_t i = t.dim() - 2; i >= 0; i--) {
+        const int64_t size = sizes[i], stride = strides[i];
+        if (size == 1) continue;
+        if (!met) distance = stride;
+        else if (stride != step) return false;
+        met = true;
+        step = stride * size;
+        length *= size;
+    }
+    return true;
+}
+
 // Leading dimensions that are one axis of evenly spaced rows without gaps in them, none of them empty.
 struct Rows {
     int64_t M = 1, K = 0, pitch = 0;
     bool of(const Tensor& t) {
         const int64_t d = t.dim();
         if (d == 0 || t.numel() == 0) return false;
-        const auto sizes = t.sizes(), strides = t.strides();
-        K = sizes[d - 1];
-        if (K > 1 && strides[d - 1] != 1) return false;
+        K = t.sizes()[d - 1];
+        if (K > 1 && t.strides()[d - 1] != 1) return false;
         pitch = K;
-        int64_t step = 0;                                                  // stride that the next (outer) dimension must have
-        for (int64_t i = d - 2; i >= 0; i--) {
-            if (sizes[i] == 1) continue;
-            if (step == 0) pitch = strides[i];
-            else if (strides[i] != step) return false;
-            step = strides[i] * sizes[i];
-            M *= sizes[i];
-        }
-        return pitch >= K && M < (1LL << 31) && K < (1LL << 31) - 256;
+        return leading_axis(t, M, pitch) && pitch >= K && M < (1LL << 31) && K < (1LL << 31) - 256;
     }
 };
+
+// Rows::of for the tests, which need no device: (rows, row length, pitch), or None for what it does not take.
+py::object row_layout(const Tensor& t) {
+    Rows r;
+    return r.of(t) ? py::object(py::make_tuple(r.M, r.K, r.pitch)) : py::none();
+}
 
 // An uninitialised tensor, past the dispatcher (two or three of them are most of what a small call costs the host).
 Tensor fresh(const Tensor& like, at::IntArrayRef size, at::IntArrayRef strides, at::ScalarType dtype) {
@@ -567,6 +583,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("layer", &layer);
     m.def("pack_weights", &pack_weights);
     m.def("conv2d_packed4", &conv2d_packed4);
+    m.def("row_layout", &row_layout);
     m.def("quantize_blocks", &quantize_blocks);
     m.def("quantize_blocks2d", &quantize_blocks2d);
     m.def("matmul_blocks", &matmul_blocks);

@@ -291,6 +291,7 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps):
         y = _even_rows(y)
         residual = None if residual is None else _even_rows(residual)
+        gate = gate if gate is None or gate.dim() < 2 else _even_rows(gate)
         (r, h), stats = ops._residual_norm(y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps, stats=True)
         ctx.set_materialize_grads(False)
         ctx.has_residual, ctx.args = residual is not None, (residual_scale, kind, eps)

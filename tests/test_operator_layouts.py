@@ -1,0 +1,86 @@
+"""Layouts of the tensors that the 8-bit block operators and the residual stream are given: broadcast dimensions, far sizes, what hooks hand back."""
+import itertools
+
+import pytest
+import torch
+
+import tab_b200 as TAB
+from tab_b200 import nn as tab_nn
+
+
+def layouts():
+    """Views of one buffer with every mix of broadcast, single, packed and spaced dimensions before a row of 1 or 8."""
+    buffer = torch.zeros(1 << 14)
+    for K, sizes in itertools.product((1, 8), itertools.product((1, 2, 3), repeat=3)):
+        for strides in itertools.product((0, 1, K, 3 * K, 9 * K, 64), repeat=3):
+            yield buffer.as_strided((*sizes, K), (*strides, 1))
+
+
+def test_both_bodies_take_the_same_rows():
+    """Which tensors are evenly spaced rows, and what their pitch is: the native bodies and those behind them agree, and what they say holds for every row."""
+    host = TAB.ops._host()
+    assert host, "the native bodies are not built"
+    taken = 0
+    for t in layouts():
+        try:
+            want = TAB.ops._rows(t, "t")
+        except RuntimeError:
+            want = None
+        assert host.row_layout(t) == want, (tuple(t.shape), t.stride())
+        if want is not None:
+            M, K, pitch = want
+            offsets = sorted(sum(i * s for i, s in zip(at, t.stride())) for at in itertools.product(*(range(n) for n in t.shape[:-1])))
+            assert offsets == [i * pitch for i in range(M)]
+            taken += 1
+    assert taken > 100
+
+
+@pytest.mark.parametrize("view", [lambda t: t[:, None].expand(4, 256, 512), lambda t: t[:, None, :1].expand(4, 256, 1), lambda t: t[:, None, None].expand(4, 3, 5, 512)])
+def test_broadcast_rows_are_no_even_rows(view):
+    t = view(torch.zeros(4, 512))
+    assert TAB.ops._host().row_layout(t) is None and TAB.ops._host().row_layout(t.contiguous()) is not None
+    with pytest.raises(RuntimeError, match="rows"):
+        TAB.ops._rows(t, "t")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("dim", [0, 1, (0, 1)])
+def test_gradients_of_sums_over_tokens(cuda, monkeypatch, native, dim):
+    """Autograd hands such a gradient over with broadcast dimensions: the same as from a contiguous one."""
+    if not native:
+        monkeypatch.setattr(TAB.ops, "_native", False)
+    x, w, p = torch.randn(3, 40, 256, device=cuda, requires_grad=True), torch.randn(96, 256, device=cuda, requires_grad=True), torch.rand(256, device=cuda, requires_grad=True)
+    for of, result in (((x, w), lambda: tab_nn.block_linear(x, w)), ((x, p), lambda: tab_nn.residual_norm(x, pre_weight=p)[1]), ((x,), lambda: tab_nn.residual_norm(x, x)[0])):
+        g = torch.randn_like(result().sum(dim))
+        y = result()
+        got = torch.autograd.grad(y.sum(dim), of, g)
+        full = g.expand_as(y) if dim != 1 else g[:, None].expand_as(y)
+        want = torch.autograd.grad(result(), of, full.contiguous())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+def test_tensors_broadcast_over_tokens(cuda, monkeypatch, native):
+    """One row (or one number) of each sequence for all of its tokens: refused where the kernels would need rows of their own, laid out in the
+    differentiable forms, which say the same as for contiguous tensors."""
+    if not native:
+        monkeypatch.setattr(TAB.ops, "_native", False)
+    B, S, C = 3, 40, 256
+    y, p, w = torch.randn(B, S, C, device=cuda), torch.rand(C, device=cuda), torch.randn(64, C, device=cuda)
+    one, number = torch.randn(B, 1, C, device=cuda), torch.randn(B, 1, 1, device=cuda)
+    wide, narrow = one.expand(B, S, C), number.expand(B, S, 1)
+    for call in (lambda: TAB.quantize_blocks(wide), lambda: TAB.residual_norm(wide, pre_weight=p), lambda: TAB.residual_norm(y, wide, pre_weight=p),
+                 lambda: TAB.residual_norm(y, gate=wide), lambda: TAB.residual_norm(y, gate=narrow)):
+        with pytest.raises(RuntimeError, match="rows"):
+            call()
+    for make in (lambda t: t, torch.Tensor.contiguous):
+        leaves = [t.clone().requires_grad_() for t in (y, one, number, w)]
+        full, token = make(leaves[1].expand(B, S, C)), make(leaves[2].expand(B, S, 1))
+        out = [tab_nn.block_linear(full, leaves[3]), tab_nn.residual_norm(full, leaves[0], pre_weight=p)[1], *tab_nn.residual_norm(leaves[0], full, pre_weight=p, gate=full),
+               tab_nn.residual_norm(leaves[0], full, gate=token)[0]]
+        grads = torch.autograd.grad(out, leaves, [torch.ones_like(t) for t in out])
+        if make is torch.Tensor.contiguous:
+            assert all(torch.equal(a, b) for a, b in zip(kept, [*out, *grads]))
+        kept = [*out, *grads]
