@@ -319,22 +319,24 @@ struct Operand {
     int share = 1;
     int64_t sr = 0, sk = 0;
     bool of(const Tensor& q, const Tensor& s) {
-        if (!on_cuda(q) || !on_cuda(s) || s.device() != q.device() || format_of(q.scalar_type()) < 0 || s.scalar_type() != at::kFloat8_e8m0fnu || !r.of(q)) return false;
+        return on_cuda(q) && on_cuda(s) && s.device() == q.device() && format_of(q.scalar_type()) >= 0 && s.scalar_type() == at::kFloat8_e8m0fnu && r.of(q) && scales(s);
+    }
+    // The scales of r's values.
+    bool scales(const Tensor& s) {
         if (s.dim() == 0 || s.size(-1) != blocks(r.K)) return false;
         sk = s.stride(-1);
-        int64_t rows = 1, step = 0;                                        // leading dimensions that are one axis of even strides
-        for (int64_t i = s.dim() - 2; i >= 0; i--) {
-            if (s.size(i) == 1) continue;
-            if (step == 0) sr = s.stride(i);
-            else if (s.stride(i) != step) return false;
-            step = s.stride(i) * s.size(i);
-            rows *= s.size(i);
-        }
+        int64_t rows = 1;
+        if (!leading_axis(s, rows, sr)) return false;
         if (rows != r.M && rows != blocks(r.M)) return false;
         share = rows == r.M ? 1 : 128;
         return true;
     }
 };
+// Operand::scales for the tests, which need no device: (rows to a scale, distance of rows, of blocks), or None for what it does not take.
+py::object scale_layout(const Tensor& q, const Tensor& s) {
+    Operand o;
+    return o.r.of(q) && o.scales(s) ? py::object(py::make_tuple(o.share, o.sr, o.sk)) : py::none();
+}
 bool matmul_any(const Tensor& a, const Tensor& as, const Tensor& b, const Tensor& bs, at::ScalarType dtype, Tensor& y) {
     Operand A, B;
     const int type = type_of(dtype);
@@ -584,6 +586,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("pack_weights", &pack_weights);
     m.def("conv2d_packed4", &conv2d_packed4);
     m.def("row_layout", &row_layout);
+    m.def("scale_layout", &scale_layout);
     m.def("quantize_blocks", &quantize_blocks);
     m.def("quantize_blocks2d", &quantize_blocks2d);
     m.def("matmul_blocks", &matmul_blocks);

@@ -43,6 +43,39 @@ def test_broadcast_rows_are_no_even_rows(view):
         TAB.ops._rows(t, "t")
 
 
+def test_both_bodies_take_the_same_scales(monkeypatch):
+    """Scales of any even strides, those of broadcast rows among them: the native body and the one behind it agree, and what they say holds for every scale."""
+    monkeypatch.setattr(TAB.ops, "_on_device", lambda *_: None)
+    buffer, taken, shared = torch.zeros(4096, dtype=torch.uint8).view(torch.float8_e8m0fnu), 0, 0
+    for KB, sizes, wide in itertools.product((1, 2), itertools.product((1, 2, 3), repeat=2), (False, True)):
+        lead = (128 * sizes[0] * sizes[1] - 1,) if wide else sizes         # values: a row for each scale, or 128 rows
+        q = torch.zeros(*lead, 128 * KB, dtype=torch.uint8).view(torch.float8_e4m3fn)
+        for strides in itertools.product((0, 1, 2, 3, 4, 8, 12), (0, 1, 2, 4), (0, 1, 16)):
+            s = buffer.as_strided((*sizes, KB), strides)
+            try:
+                want = TAB.ops._operand(q, s, "a", None)[0][4:]
+            except RuntimeError:
+                want = None
+            got = TAB.ops._host().scale_layout(q, s)
+            assert (got is None) == (want is None), (tuple(s.shape), s.stride())
+            if got is None:
+                continue
+            flat = [sum(i * n for i, n in zip(at, strides)) for at in itertools.product(range(sizes[0]), range(sizes[1]))]
+            for share, sr, sk in (got, want):
+                assert share == (1 if q.numel() // (128 * KB) == len(flat) else 128) and (KB == 1 or sk == strides[2])
+                assert len(flat) == 1 or flat == [i * sr for i in range(len(flat))], (tuple(s.shape), s.stride())
+            taken += 1
+            shared += share == 128
+    assert taken > 100 and shared > 20
+
+
+def test_scales_broadcast_along_one_of_two_dimensions():
+    q, s = torch.zeros(5, 64, 256, dtype=torch.uint8).view(torch.float8_e4m3fn), torch.zeros(5, 1, 2, dtype=torch.uint8)
+    layout = TAB.ops._host().scale_layout
+    assert layout(q, s.expand(5, 64, 2)) is None and layout(q, s.expand(5, 64, 2).contiguous()) == (1, 2, 1)
+    assert layout(q, s[:1, :, :1].expand(5, 64, 2)) == (1, 0, 0)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("native", [True, False])
 @pytest.mark.parametrize("dim", [0, 1, (0, 1)])
@@ -84,3 +117,18 @@ def test_tensors_broadcast_over_tokens(cuda, monkeypatch, native):
         if make is torch.Tensor.contiguous:
             assert all(torch.equal(a, b) for a, b in zip(kept, [*out, *grads]))
         kept = [*out, *grads]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("B, S", [(2, 3), (5, 64), (9, 128)])
+def test_products_with_broadcast_scales(cuda, monkeypatch, native, B, S):
+    """One row of scales for a sequence: refused, since its rows are not evenly spaced; one for everything is taken.  (The product as of laid-out scales.)"""
+    if not native:
+        monkeypatch.setattr(TAB.ops, "_native", False)
+    a, b = TAB.quantize_blocks(torch.randn(B, S, 256, device=cuda)), TAB.quantize_blocks(torch.randn(70, 256, device=cuda))
+    one = a[1][:, :1].expand(B, S, 2)
+    with pytest.raises(RuntimeError, match="rows"):
+        TAB.matmul_blocks(a[0], one, *b)
+    for same in (a[1][:1, :1].expand(B, S, 2), a[1][:1, :1, :1].expand(B, S, 2)):
+        assert torch.equal(TAB.matmul_blocks(a[0], same, *b), TAB.matmul_blocks(a[0], same.contiguous(), *b))
