@@ -435,6 +435,12 @@ def _on_device(t, name, device, types, what):
         raise RuntimeError("%s must not be a negated view (resolve_neg makes a tensor of it)" % name)
 
 
+def _counted(rows, length, name):
+    """The kernels count rows and the elements of a row in 32 bits, and the C ABI's parameters would drop what lies above them."""
+    if rows >= 1 << 31 or length >= 1 << 31:
+        raise RuntimeError("%s must have less than 2^31 rows, of less than 2^31 elements" % name)
+
+
 def _rows(t, name):
     """``(rows, row length, pitch)`` of a tensor whose leading dimensions are one axis of evenly spaced rows without gaps in them."""
     if t.dim() == 0:
@@ -443,6 +449,7 @@ def _rows(t, name):
     M = t[..., 0].numel() if K else int(torch.Size(t.shape[:-1]).numel())
     if M == 0 or K == 0:
         return M, K, K
+    _counted(M, K, name)
     if K > 1 and t.stride(-1) != 1:
         raise RuntimeError("%s must have contiguous rows" % name)
     try:
@@ -494,7 +501,7 @@ def quantize_blocks(x, dtype=torch.float8_e4m3fn, columns=False):
     ``columns``: also ``(qt, st)``, from the same reading of ``x``: its transpose ``[K, rows]`` with blocks along the rows of ``x``,
     ``st`` ``[K, ceil(rows/128)]`` - what a product that sums over the rows takes (the gradient of a dense layer's weights).
 
-    Rows of ``q`` and ``qt`` start on 16 bytes, as ``matmul_blocks`` wants them; the scales lie block by block in memory, the form it reads
+    At most 2^31 - 1 rows (of 2^31 - 256 elements).  Rows of ``q`` and ``qt`` start on 16 bytes, as ``matmul_blocks`` wants them; the scales lie block by block in memory, the form it reads
     fastest."""
     done = _try("quantize_blocks", x, dtype, columns)
     if done is not None:
@@ -572,6 +579,9 @@ def matmul_blocks(a, a_scales, b, b_scales, out_dtype=torch.bfloat16):
     (pa, M, K), (pb, N, KB) = _operand(a, a_scales, "a", None), _operand(b, b_scales, "b", a.device)
     if b.dim() != 2 or KB != K:
         raise RuntimeError("b must be [N, %d]" % K)
+    if K == 0:
+        _counted(M, 0, "a")
+        _counted(N, 0, "b")
     with torch.cuda.device(a.device):
         y = torch.empty((*a.shape[:-1], N), dtype=out_dtype, device=a.device)
         rc = _cabi.lib().tab_matmul_blocks_launch(*pa, *pb, y.data_ptr(), _TYPES[out_dtype], N, M, N, K, _stream_ptr(a.device))

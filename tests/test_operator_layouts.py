@@ -76,6 +76,34 @@ def test_scales_broadcast_along_one_of_two_dimensions():
     assert layout(q, s[:1, :, :1].expand(5, 64, 2)) == (1, 0, 0)
 
 
+FAR = 1 << 32                                                              # what 32 bits take for 0
+
+
+@pytest.mark.parametrize("shape", [(1 << 31,), (FAR,), (FAR + 5,), (1, FAR + 5), (FAR, 1), (FAR + 5, 1), (1 << 16, 1 << 16, 2)])
+def test_rows_beyond_32_bits_are_refused(monkeypatch, shape):
+    """Before a size meets a 32-bit parameter: neither rows nor elements of a row may be 2^31 or more.  (Meta tensors: shapes without memory.)"""
+    monkeypatch.setattr(TAB.ops, "_on_device", lambda *_: None)
+    x, q = torch.empty(shape, dtype=torch.bfloat16, device="meta"), torch.empty(shape, dtype=torch.float8_e4m3fn, device="meta")
+    s = torch.empty((*shape[:-1], -(-shape[-1] // 128)), dtype=torch.float8_e8m0fnu, device="meta")
+    few = torch.empty((1, shape[-1]), dtype=torch.float8_e4m3fn, device="meta"), torch.empty((1, s.shape[-1]), dtype=torch.float8_e8m0fnu, device="meta")
+    two = (lambda t: t) if len(shape) == 2 else (lambda t: t.view(-1, t.shape[-1]))
+    w = torch.empty(shape[-1], device="meta")
+    for call in (lambda: TAB.ops._rows(x, "x"), lambda: TAB.quantize_blocks(x), lambda: TAB.quantize_blocks2d(two(x)), lambda: TAB.matmul_blocks(q, s, *few), lambda: TAB.matmul_blocks(*few, two(q), two(s)),
+                 lambda: TAB.residual_norm(x, pre_weight=w), lambda: TAB.ops._norm_args(x, None, w, None, None, None, None, 1.0, "rms", 1e-6)):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            call()
+
+
+def test_empty_sums_of_many_rows_are_refused(monkeypatch):
+    """An empty sum is a result of zeros, however many rows the operands have; results of no rows stay what they are."""
+    monkeypatch.setattr(TAB.ops, "_on_device", lambda *_: None)
+    blocks = lambda *shape: (torch.empty(shape, dtype=torch.float8_e4m3fn, device="meta"), torch.empty((*shape[:-1], -(-shape[-1] // 128)), dtype=torch.float8_e8m0fnu, device="meta"))
+    for a, b in ((blocks(FAR, 0), blocks(3, 0)), (blocks(3, 0), blocks(FAR, 0)), (blocks(1 << 16, 1 << 16, 0), blocks(3, 0)), (blocks(FAR + 7, 0), blocks(1, 0))):
+        with pytest.raises(RuntimeError, match="2\\^31"):
+            TAB.matmul_blocks(*a, *b)
+    assert TAB.ops._rows(torch.empty(0, FAR, device="meta"), "t") == (0, FAR, FAR)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("native", [True, False])
 @pytest.mark.parametrize("dim", [0, 1, (0, 1)])
@@ -132,3 +160,18 @@ def test_products_with_broadcast_scales(cuda, monkeypatch, native, B, S):
         TAB.matmul_blocks(a[0], one, *b)
     for same in (a[1][:1, :1].expand(B, S, 2), a[1][:1, :1, :1].expand(B, S, 2)):
         assert torch.equal(TAB.matmul_blocks(a[0], same, *b), TAB.matmul_blocks(a[0], same.contiguous(), *b))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [FAR, FAR + 300])
+def test_a_flat_tensor_beyond_32_bits(cuda, n):
+    """A flat vector of 2^32 elements and more has no place in 32-bit sizes and is refused; the same memory as rows is taken."""
+    x = torch.zeros(n, dtype=torch.float8_e4m3fn, device=cuda)
+    s = torch.full((-(-n // 128),), 127, dtype=torch.uint8, device=cuda).view(torch.float8_e8m0fnu)
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        TAB.matmul_blocks(x, s, x[None], s[None])
+    column, one = x[:, None], s.new_empty(0).set_(s.untyped_storage(), 0, (n, 1), (0, 1))
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        TAB.matmul_blocks(TAB.ops._new_blocks((2, 1), 2, 1, x.dtype, cuda), s[:2, None], column, one)
+    with pytest.raises(RuntimeError, match="2\\^31"):
+        TAB.quantize_blocks(torch.empty(n, dtype=torch.bfloat16, device=cuda), columns=True)
