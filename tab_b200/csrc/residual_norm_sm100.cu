@@ -291,11 +291,11 @@ __global__ void __launch_bounds__(THREADS, forward_threads(LAYER, FAST) / THREAD
                 for (int i = 0; i < NV; i++)
                     if (mine[i]) store_pairs<TYPE>(p.h, m * p.ldh + (i * THREADS + g) * 8, v[i], false);
             } else {
-                // The larger magnitudes, which fmaxf takes past NaN; rows with an infinity are looked at again.
+                // The larger magnitudes, which fmaxf takes past NaN, from 0 on, so that eight NaN leave 0; rows with an infinity are looked at again.
                 float a[NV], most = 0.f;
 #pragma unroll
                 for (int i = 0; i < NV; i++) {
-                    a[i] = fmaxf(fmaxf(fmaxf(fabsf(v[i][0].x), fabsf(v[i][0].y)), fmaxf(fabsf(v[i][1].x), fabsf(v[i][1].y))),
+                    a[i] = fmaxf(fmaxf(fmaxf(fmaxf(0.f, fabsf(v[i][0].x)), fabsf(v[i][0].y)), fmaxf(fabsf(v[i][1].x), fabsf(v[i][1].y))),
                                  fmaxf(fmaxf(fabsf(v[i][2].x), fabsf(v[i][2].y)), fmaxf(fabsf(v[i][3].x), fabsf(v[i][3].y))));
                     most = fmaxf(most, a[i]);
                 }
