@@ -522,12 +522,18 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
         const auto v = ctx->get_saved_variables();
-        const Tensor &y = v[0], &r = v[1], &st = v[2], &w2 = v[3], &b2 = v[4], &w1 = v[5], &b1 = v[6], &gate = v[7];
-        const bool plain = !r.defined(), residual = ctx->saved_data["residual"].toBool();
+        const Tensor &w2 = v[3], &b2 = v[4], &w1 = v[5], &b1 = v[6];
+        const bool plain = !v[1].defined(), residual = ctx->saved_data["residual"].toBool();
         variable_list out(10);
         const Tensor gr = plain ? Tensor() : even_rows(grads[0].defined() ? grads[0].detach() : grads[0]);
         const Tensor gh = w2.defined() ? even_rows(grads.back().defined() ? grads.back().detach() : grads.back()) : Tensor();
         if (!gr.defined() && !gh.defined()) return out;
+        // Hooks on kept tensors may hand them back with other strides; in another type, shape or place they are not what the gradients belong to.
+        const Tensor y = even_rows(v[0]), r = even_rows(v[1]), st = v[2].contiguous(), gate = v[7].defined() && v[7].dim() > 1 ? even_rows(v[7]) : v[7];
+        auto fits = [&](const Tensor& t) { return !t.defined() || (on_cuda(t) && t.device() == y.device() && t.scalar_type() == y.scalar_type() && t.sizes() == y.sizes()); };
+        TORCH_CHECK(fits(y) && fits(r) && fits(gr) && fits(gh) && on_cuda(st) && st.device() == y.device() && st.scalar_type() == at::kFloat && y.dim() > 0 &&
+                        st.numel() * y.size(-1) == 4 * y.numel() && reinterpret_cast<uintptr_t>(st.data_ptr()) % 16 == 0,
+                    "residual_norm: the backward pass needs the kept tensors in the type, shape and place in which the forward pass kept them");
         Norm n;
         bool ok = n.of(y, Tensor(), w2, b2, w1, b1, gate, ctx->saved_data["alpha"].toDouble(), ctx->saved_data["layer"].toInt(), ctx->saved_data["eps"].toDouble());
         if (ok) {
@@ -535,7 +541,8 @@ struct ResidualNorm : torch::autograd::Function<ResidualNorm> {
             tab_norm_backward_t b = {};
             Rows q;
             n.a.r = const_cast<void*>(static_cast<const void*>((plain ? y : r).data_ptr()));
-            n.a.ldr = plain ? n.r.pitch : n.r.K;
+            n.a.ldr = n.r.pitch;
+            if (!plain) { ok = q.of(r); n.a.ldr = q.pitch; q = Rows(); }
             n.a.stats = st.data_ptr<float>();
             b.f = n.a;
             if (gr.defined()) { ok = ok && q.of(gr); b.gr = gr.data_ptr(); b.ldgr = q.pitch; }

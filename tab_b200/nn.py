@@ -202,6 +202,11 @@ def _even_rows(g):
         return g.contiguous()
 
 
+def _even_gate(gate):
+    """The same for a gate with rows (that of channels is a vector)."""
+    return gate if gate is None or gate.dim() < 2 else _even_rows(gate)
+
+
 def _differentiable_once(grads):
     """Gradients of gradients are refused when somebody asks for them, not before."""
     if not torch.is_grad_enabled():
@@ -291,7 +296,7 @@ class _ResidualNorm(torch.autograd.Function):
     def forward(ctx, y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps):
         y = _even_rows(y)
         residual = None if residual is None else _even_rows(residual)
-        gate = gate if gate is None or gate.dim() < 2 else _even_rows(gate)
+        gate = _even_gate(gate)
         (r, h), stats = ops._residual_norm(y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps, stats=True)
         ctx.set_materialize_grads(False)
         ctx.has_residual, ctx.args = residual is not None, (residual_scale, kind, eps)
@@ -307,7 +312,9 @@ class _ResidualNorm(torch.autograd.Function):
         if (gr is None and gh is None) or not wanted:
             return (None,) * 10
         gr, gh = (None if g is None else _even_rows(g.detach()) for g in (gr, gh))
-        out = ops.residual_norm_backward(gr, gh, y, y if ctx.plain else r, stats, ctx.has_residual, *weights, *ctx.args, wanted)
+        # hooks on kept tensors may hand them back with other strides
+        y, r, weights[-1] = _even_rows(y), None if ctx.plain else _even_rows(r), _even_gate(weights[-1])
+        out = ops.residual_norm_backward(gr, gh, y, y if ctx.plain else r, stats.contiguous(), ctx.has_residual, *weights, *ctx.args, wanted)
         return *_differentiable_once(tuple(out.get(n) for n in _NORM_TENSORS)), None, None, None
 
 

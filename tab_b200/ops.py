@@ -687,6 +687,14 @@ def residual_norm_backward(grad_r, grad_h, y, r, stats, has_residual, pre_weight
     """Gradients of ``residual_norm`` for those of ``r`` and ``h`` (either may be ``None``), from the kept ``y``, ``r`` and statistics.  ``wanted``: names
     among y, residual, gate, pre_weight, pre_bias, post_weight, post_bias; returns a dict of those that the arguments have."""
     a, M, C = _norm_args(y, None, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps)
+    for name, t in (("r", r), ("grad_r", grad_r), ("grad_h", grad_h)):
+        if t is not None:
+            _on_device(t, name, y.device, (y.dtype,), str(y.dtype))
+            if t.shape != y.shape:
+                raise RuntimeError("%s must have the shape of y" % name)
+    _on_device(stats, "stats", y.device, (torch.float32,), "float32")
+    if tuple(stats.shape) != (M, 4) or not stats.is_contiguous():
+        raise RuntimeError("stats must be contiguous, [%d, 4]" % M)
     b = _cabi.NormBackwardArgs()
     a.r, a.ldr, a.stats = r.data_ptr(), _rows(r, "r")[2], stats.data_ptr()
     b.f = a

@@ -175,3 +175,51 @@ def test_a_flat_tensor_beyond_32_bits(cuda, n):
         TAB.matmul_blocks(TAB.ops._new_blocks((2, 1), 2, 1, x.dtype, cuda), s[:2, None], column, one)
     with pytest.raises(RuntimeError, match="2\\^31"):
         TAB.quantize_blocks(torch.empty(n, dtype=torch.bfloat16, device=cuda), columns=True)
+
+
+def wider(t):
+    """The same values, rows farther apart."""
+    if t.dim() < 2:
+        return t
+    return torch.cat([t, torch.full_like(t, 7)], -1)[..., :t.shape[-1]]
+
+
+def turned(t):
+    """The same values, the last two dimensions the other way round in memory."""
+    return t if t.dim() < 2 else t.transpose(-1, -2).contiguous().transpose(-1, -2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("unpack", [wider, turned])
+@pytest.mark.parametrize("shape", [(37, 100), (400, 1032), (2, 3, 64)])
+def test_kept_tensors_that_come_back_with_other_strides(cuda, monkeypatch, native, unpack, shape):
+    if not native:
+        monkeypatch.setattr(TAB.ops, "_native", False)
+    x, y = (torch.randn(*shape, device=cuda, requires_grad=True) for _ in range(2))
+    p, g = torch.rand(shape[-1], device=cuda, requires_grad=True), torch.rand(shape[-1], device=cuda, requires_grad=True)
+    grads = []
+    for hook in (None, unpack):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, hook or (lambda t: t)):
+            out = [*tab_nn.residual_norm(y, x, pre_weight=p, post_weight=p, gate=g), tab_nn.residual_norm(y, pre_weight=p)[1], tab_nn.residual_norm(y, gate=x)[0]]
+        grads.append(torch.autograd.grad(out, (x, y, p, g), [torch.ones_like(t) * i for i, t in enumerate(out, 1)]))
+    # rows farther apart may be worked by another kernel than packed ones: up to fp32 roundings of sums of a row, and over the rows
+    for a, b in zip(*grads):
+        assert float((a - b).abs().max()) <= (float(b.abs().max()) + 30) * (96 + 4 * b.numel() ** 0.5) * 2.0 ** -24
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("native", [True, False])
+@pytest.mark.parametrize("unpack", [lambda t: t.half(), lambda t: t.half() if t.dim() == 2 and t.shape[-1] > 4 else t, lambda t: t.cpu(), lambda t: t[..., :-1] if t.dim() == 2 else t,
+                                    lambda t: t.double() if t.shape[-1:] == (4,) else t, lambda t: t[:5] if t.dim() == 2 else t])
+def test_kept_tensors_that_come_back_as_others_are_refused(cuda, monkeypatch, native, unpack):
+    if not native:
+        monkeypatch.setattr(TAB.ops, "_native", False)
+    x, y, p = torch.randn(37, 96, device=cuda, requires_grad=True), torch.randn(37, 96, device=cuda), torch.rand(96, device=cuda)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        out = tab_nn.residual_norm(y, x, pre_weight=p)
+        plain = tab_nn.residual_norm(x, pre_weight=p)[1]
+    for result in (out[0].sum() + out[1].sum(), plain.sum()):
+        with pytest.raises(RuntimeError):
+            result.backward()
+    torch.cuda.synchronize()
