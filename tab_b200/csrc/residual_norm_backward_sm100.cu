@@ -426,7 +426,19 @@ static long long norm_parts(long long M, int C) {
     const long long most = 148LL * G * (C <= 2048 ? 4 : C <= 4096 ? 2 : 1), wanted = std::min(most, std::min(M, std::max(148LL * G, M / 4)));
     return (wanted + G - 1) / G * G;
 }
-size_t residual_norm_partial_bytes(long long M, int C) { return (size_t)std::max(norm_parts(M, C), std::min<long long>(M, NORM_CTAS)) * 5 * (size_t)C * sizeof(float); }
+// The most CTAs of the stream kernel, each of which sums its rows on its own: what an SM holds by registers of those the row's length chooses
+// (norm_backward_sizes), and some rows for each.  0: rows that it does not take.
+static int stream_rows(int C) { return C <= 2048 ? 4 : 2; }
+static long long stream_parts(long long M, int C, bool layer) {
+    if (C <= 256 || C > 8192) return 0;
+    const int wide = C <= 512 ? 512 : C <= 1024 ? 1024 : C <= 2048 ? 2048 : C <= 4096 ? 4096 : 8192, each = layer ? std::max(1, 4096 / wide) : 8192 / wide;
+    return std::min({M, 148LL * each, std::max(148LL, M / stream_rows(C))});
+}
+// Neither the kernel nor the number of sums is known here: room for whichever needs most.
+size_t residual_norm_partial_bytes(long long M, int C) {
+    const long long rows = std::max({norm_parts(M, C) * NORM_SUMS<true>, stream_parts(M, C, true) * NORM_SUMS<true>, stream_parts(M, C, false) * NORM_SUMS<false>});
+    return (size_t)rows * (size_t)C * sizeof(float);
+}
 static bool wants_sums(const NormBackwardParams& b) { return b.dw1 || b.db1 || b.dw2 || b.db2 || (b.f.gkind == TAB_GATE_CHANNEL && b.dgate); }
 static int backward_flags(const NormBackwardParams& b, int type) {
     const int s = type_bytes(type);
@@ -460,13 +472,13 @@ static int launch_norm_backward_stream_as(NormBackwardParams b, cudaStream_t str
     // Below two rows an SM the general kernel is as fast (148x4096 8.9 us, this one 10.3; 296: 11.6 / 12.2; 444: 14.2 / 13.9; 2048: 72 / 26); a
     // CTA has some rows to itself, since its sums are as many bytes as some of them (us at 592x4096 / 2048x1024: 1 row 14.5 / 18.1, 4 rows 16.4 / 15.6).
     if (p.M < 2LL * blocks_sms()) return TAB_E_TOO_LARGE;
-    const StreamPlan pl = stream_plan<kernel>(backward_threads(NV, LAYER) / THREADS, p.M, p.C <= 2048 ? 4 : 2, 4 * (size_t)p.C * type_bytes(TYPE), (p.gkind == TAB_GATE_CHANNEL ? 12 : 8) * (size_t)p.C);
+    const StreamPlan pl = stream_plan<kernel>(backward_threads(NV, LAYER) / THREADS, p.M, stream_rows(p.C), 4 * (size_t)p.C * type_bytes(TYPE), (p.gkind == TAB_GATE_CHANNEL ? 12 : 8) * (size_t)p.C);
     if (!pl.stages) return TAB_E_TOO_LARGE;
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
     const bool sums = wants_sums(b);
     if (!sums) b.partial = nullptr;
-    const int ctas = (int)std::min<long long>(p.M, pl.ctas);
+    const int ctas = (int)std::min<long long>(stream_parts(p.M, p.C, LAYER), pl.ctas);
     const int rc = launch_pdl(kernel, dim3((unsigned)ctas), dim3(THREADS), pl.smem, stream, b, pl.stages, status);
     return rc != TAB_OK || !sums ? rc : launch_norm_sums(b, ctas, stream);
 }
