@@ -398,7 +398,8 @@ struct BlockLinear : torch::autograd::Function<BlockLinear> {
         const auto saved = ctx->get_saved_variables();
         const auto types = ctx->saved_data["types"].toIntVector();
         variable_list out(6);
-        const bool need_w = saved[0].defined(), need_x = saved[2].defined();
+        // what this pass is asked for, of what was kept for any
+        const bool need_w = saved[0].defined() && ctx->needs_input_grad(1), need_x = saved[2].defined() && ctx->needs_input_grad(0);
         if (!grads[0].defined() || (!need_x && !need_w)) return out;
         const Tensor g = even_rows(grads[0].detach());
         Quantized q;
