@@ -38,8 +38,10 @@ def _try(name, *args):
     host = _host()
     if not host:
         return None
+    if not hasattr(host, name):
+        raise RuntimeError("tab_b200._host has no %s: it was built from older sources (python -m tab_b200.build)" % name)
     try:
-        return getattr(host, name, lambda *_: None)(*args)
+        return getattr(host, name)(*args)
     except TypeError:
         return None
 

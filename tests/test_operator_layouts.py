@@ -1,5 +1,6 @@
 """Layouts of the tensors that the 8-bit block operators and the residual stream are given: broadcast dimensions, far sizes, what hooks hand back."""
 import itertools
+import types
 
 import pytest
 import torch
@@ -102,6 +103,14 @@ def test_empty_sums_of_many_rows_are_refused(monkeypatch):
         with pytest.raises(RuntimeError, match="2\\^31"):
             TAB.matmul_blocks(*a, *b)
     assert TAB.ops._rows(torch.empty(0, FAR, device="meta"), "t") == (0, FAR, FAR)
+
+
+def test_an_older_extension_is_named(monkeypatch):
+    """A native body that is not there: the extension is older than the sources, and the slow body behind it does not stand in without a word."""
+    monkeypatch.setattr(TAB.ops, "_native", types.SimpleNamespace(quantize=lambda *_: None))
+    assert TAB.ops._try("quantize") is None
+    with pytest.raises(RuntimeError, match="older"):
+        TAB.quantize_blocks(torch.zeros(2, 128))
 
 
 @pytest.mark.gpu
