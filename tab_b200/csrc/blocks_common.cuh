@@ -151,16 +151,9 @@ __device__ __forceinline__ uint32_t finite_bits(float v) {
     const uint32_t b = __float_as_uint(v) & 0x7FFFFFFFu;
     return b < 0x7F800000u ? b : 0u;
 }
-// Least e with amax <= F * 2^e for F = 1.75 * 2^8 (e4m3) or 1.75 * 2^15 (e5m2), from the bits of amax = m * 2^k: k - 8 (k - 15), one
-// more where m > 1.75.  At least -127, the least exponent an e8m0 byte holds (which subnormal maxima fall below); 0 for a block of
-// zeros.
-__device__ __forceinline__ int scale_exponent(uint32_t amax_bits, int format) {
-    const int k = (int)(amax_bits >> 23) - 127;
-    const int e = k - (format == TAB_E5M2 ? 15 : 8) + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
-    return amax_bits == 0 ? 0 : max(e, -127);
-}
-// e + 127 of the block's scale 2^e from the bits of its largest magnitude m * 2^k: k - 8 (e5m2: k - 15), one more where m > 1.75, which
-// the addition carries into the exponent; at least 0; 127 for a block of zeros.
+// e + 127 of the block's scale 2^e, e the least with amax <= F * 2^e for F = 1.75 * 2^8 (e4m3) or 1.75 * 2^15 (e5m2), from the bits of amax = m * 2^k:
+// k - 8 (k - 15), one more where m > 1.75, which the addition carries into the exponent; at least 0, the least a byte holds (which subnormal
+// maxima fall below); 127 for a block of zeros.
 template <int FORMAT>
 __device__ __forceinline__ uint32_t scale_byte(uint32_t bits) {
     const int b = (int)((bits + 0x1FFFFFu) >> 23) - (FORMAT == TAB_E5M2 ? 15 : 8);

@@ -198,10 +198,10 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
     using T = typename ElemOf<TYPE>::type;
     extern __shared__ uint8_t raw[];
     constexpr int STAGE = KS * (128 + BN) * 128;                           // KS blocks: their rows of R, then their rows of C
-    constexpr int CG = (BN + 127) / 128;                                   // groups of 128 rows of C
-    constexpr int SFB = 512 * (1 + CG);                                    // bytes of four blocks' scales; a slot holds four of them
+    static_assert(BN <= 128, "the scales of 128 rows on either side");
+    constexpr int SFB = 1024;                                              // bytes of four blocks' scales; a slot holds four of them
     constexpr int SFCOL = BN < 32 ? 32 : BN;                               // first tensor-memory column of the scales: two slots
-    constexpr int TCOLS = SFCOL + 8 * (1 + CG) <= 64 ? 64 : SFCOL + 8 * (1 + CG) <= 128 ? 128 : SFCOL + 8 * (1 + CG) <= 256 ? 256 : 512;
+    constexpr int TCOLS = SFCOL + 16 <= 64 ? 64 : SFCOL + 16 <= 128 ? 128 : 256;
     __shared__ __align__(8) uint64_t bars[16 + 2 * SF_SLOTS + 1];
     __shared__ __align__(512) uint8_t sf[SF_SLOTS * 4 * SFB];
     __shared__ uint32_t tslot;
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
         const uint32_t idesc = umma_idesc_f8(128, BN, R.format == TAB_E5M2, C.format == TAB_E5M2);
         for (int kb = kb0, g = 0; kb < kb1; kb += KS, g++) {
             const int s = g % nst, at = kb - kb0, q = at >> 4, slot = q % SF_SLOTS;
-            const uint32_t sfcol = tmem + SFCOL + ((at >> 2) & 1) * 4 * (1 + CG);
+            const uint32_t sfcol = tmem + SFCOL + ((at >> 2) & 1) * 8;
             if ((at & 15) == 0) {
                 if (!mbar_wait_warp(sfFull + 8 * slot, (q / SF_SLOTS) & 1)) { expire(32); break; }
                 tc_fence_after();
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
             if (elect_one()) {
                 if ((at & 3) == 0) {
 #pragma unroll
-                    for (int i = 0; i < 1 + CG; i++) tmem_copy_scales(sfcol + 4 * i, sSF + (slot * 4 + ((at >> 2) & 3)) * SFB + 512 * i);
+                    for (int i = 0; i < 2; i++) tmem_copy_scales(sfcol + 4 * i, sSF + (slot * 4 + ((at >> 2) & 3)) * SFB + 512 * i);
                     if ((at & 12) == 12 || kb + 4 >= kb1) umma_commit(sfEmpty + 8 * slot);
                 }
 #pragma unroll
@@ -278,7 +278,6 @@ __global__ void __launch_bounds__(TT) matmul_blocks_tile_kernel(const __grid_con
     } else if (warp == 2) {
         ScaleLoader r(R, kb0), c(C, kb0);
         for (int kb = kb0, q = 0; kb < kb1; kb += 16, q++) {
-            static_assert(CG == 1, "one group of 128 rows on either side");
             r.load(R, r0, kb, kb1, lane);
             c.load(C, c0, kb, kb1, lane);
             const int slot = q % SF_SLOTS;
@@ -864,7 +863,9 @@ int matmul_blocks_dispatch(const MatmulBlocksParams& p, cudaStream_t stream) {
     int* status = device_status_word();
     if (stalled(status)) return TAB_E_STALLED;
     const int sms = blocks_sms();
-    // pairs from two rounds of 128 x 128 tiles on: 1536x4096x1024 (384 of them) 15.8, single CTAs 17.1; 4096x1024x1024 (256) 12.4 / 9.9
+    // pairs from two rounds of 128 x 128 tiles on: 1536x4096x1024 (384 of them) 15.8, single CTAs 17.1; 4096x1024x1024 (256) 12.4 / 9.9; 129x20000x4096
+    // 41 / 47, 200x40000x4096 57 / 81.  The count alone decides, so 65 to 128 rows against more than 37888 columns take them too, whose tiles are half
+    // padding then: 100x40000x4096 57 / 53, 128x65536x4096 76 / 65, 128x40000x512 22 / 16.
     const long long tiles128 = ((long long)p.a.rows + 127) / 128 * (((long long)p.b.rows + 127) / 128);
     const int pairs = matmul_pairs();
     bool few = p.a.rows <= VMOST, pair = pairs > 0 && p.a.rows > 64 && tiles128 > 2LL * sms;

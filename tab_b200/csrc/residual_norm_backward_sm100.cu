@@ -142,6 +142,10 @@ __global__ void __launch_bounds__(GT < 128 ? 128 : GT) residual_norm_backward_ke
 }
 
 // ---- many rows -------------------------------------------------------------------------------------------------------------------
+// CTAs that stay and a ring of rows as in the forward pass.  The weights and the gate of channels lie in shared memory as fp32; the registers hold the
+// sums over rows of a thread's NV times eight columns.  Rows of 257 to 8192 elements as there, if shared memory holds two of them: 16-bit types always,
+// fp32 up to 5256 elements with a gate of channels and 5784 without (4096x5248 92 us, 5.6 TB/s; 4096x5264 by the kernel above 150).  Beyond, that
+// kernel's registers spill: us at 2048x8192 fp32 99, 2048x16384 bf16 235 (1.7 TB/s), centred 380, fp32 362 (2.2 TB/s).
 // us with weights, gate, residual, bf16: 8192x4096 71 with the sums' launch (403 MB: 5.7 TB/s), 4096x8192 75; centred 130 (five sums over rows leave one
 // CTA of 512 threads on an SM).  One vector a thread and twice the warps: 90.
 // What a row's sums are needed for is read from the ring again behind the meeting instead of being kept: registers are what the sums

@@ -97,11 +97,8 @@ __device__ __forceinline__ void row_sums(float (&v)[N], float (*exchange)[32][N]
     bank ^= 1;
 }
 
-// ---- many rows ------------------------------------------------------------------------------------------------------------------
-// The same with CTAs that stay: rows come by bulk copies into a ring in shared memory, a few rows ahead, so that the memory is asked for the
-// next rows while the threads meet over this one; a thread keeps its eight columns' weights (forward) or their sums (backward) in
-// registers from row to row, so that weights are read once a CTA and not once a row.  Rows and their pitches are multiples of 16 bytes
-// and eight elements here; the kernels above take everything else.
+// ---- what the kernels for many rows share ---------------------------------------------------------------------------------------
+// A row's copy into shared memory, counted on a barrier; address and size are multiples of 16 bytes.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t mbar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(mbar) : "memory");
 }
