@@ -320,7 +320,8 @@ class _ResidualNorm(torch.autograd.Function):
 
 def residual_norm(y, residual=None, pre_weight=None, pre_bias=None, post_weight=None, post_bias=None, gate=None, residual_scale=1.0,
                   kind="rms", eps=1e-6):
-    """``ops.residual_norm`` with gradients: returns ``(r, h)``.  Gradients go to ``y``, ``residual``, the weights, the biases and the gate;
+    """``ops.residual_norm`` with gradients: returns ``(r, h)``.  ``y``, ``residual`` and a gate with rows may have any strides (others than evenly
+    spaced rows are copied).  Gradients go to ``y``, ``residual``, the weights, the biases and the gate;
     that of a weight or of a gate ``[C]`` is summed over the rows in a fixed order, so that the same inputs give the same bits."""
     if isinstance(residual_scale, torch.Tensor) and residual_scale.requires_grad:
         raise RuntimeError("residual_scale is a number without a gradient; a learned factor is a gate")

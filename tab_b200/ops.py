@@ -649,7 +649,8 @@ def residual_norm(y, residual=None, pre_weight=None, pre_bias=None, post_weight=
     Returns ``(r, h)``, or with ``quantize`` (``torch.float8_e4m3fn`` or ``torch.float8_e5m2``) ``(r, q, s)``: ``h`` as ``quantize_blocks`` would
     give it from fp32, for ``matmul_blocks``.  Without residual, post norm and gate, ``r`` is ``y``.
     ``kind``: ``"rms"``, v / sqrt(mean(v^2) + eps), or ``"layer"``, (v - mean) / sqrt(var + eps), which alone takes biases.
-    ``gate``: ``[C]``, one for each row (``[..., 1]``), or of ``y``'s shape.  Weights and gate are fp32 or of ``y``'s type.  C <= 16384.
+    ``gate``: ``[C]``, one for each row (``[..., 1]``), or of ``y``'s shape.  Weights and gate are fp32 or of ``y``'s type.  C <= 16384.  Tensors with
+    rows have evenly spaced ones (``[B, 1, C]`` expanded over tokens has not).
     ``tab_b200.nn.residual_norm`` is the differentiable form."""
     done = _try("residual_norm", y, residual, pre_weight, pre_bias, post_weight, post_bias, gate, residual_scale, kind, eps, quantize)
     if done is not None:
